@@ -471,6 +471,64 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
                      size_t workspace_bytes, int* status);
 
 /*
+ * Softmax over a vocabulary: a table of `vocab` rows y_j that features x_i are scored against,
+ *   z_ij = <x_i, y_j> / T,   lse_i = log sum_j exp(z_ij),   p_ij = exp(z_ij - lse_i),
+ * without storing the rows x vocab scores.  One tile pass leaves 16 bytes per row and half column tile (and 8 bytes per
+ * row and 32 columns when alternatives are asked for), a row kernel finishes.  The reference has no such operators.
+ *
+ * Operands: x [rows, d], table [vocab, d], both MECLIP_BF16 or both MECLIP_F16, d and pitches multiples of 8, 16-byte
+ * aligned (meclip_normalize_fwd with normalize = 0 makes bf16 ones of anything).  Scores must be finite; a row whose
+ * scores are not numbers gives NaN for that row.  tokens, teacher_tokens: int64 [rows, per_row], contiguous, 0 <=
+ * per_row <= 256.  A negative token is absent (padding); one behind the table gives NaN.  workspace: 256-byte aligned,
+ * meclip_vocab_workspace_bytes / meclip_vocab_grad_workspace_bytes.
+ *
+ *   meclip_token_log_probs  log_probs [rows, per_row] = z - lse (0 for an absent token); entropy [rows] =
+ *                           lse - sum_j p z (may be NULL); the top_k (<= 32, <= vocab) best tokens of each row and
+ *                           their log probabilities, larger first and the lower token first among equals (decided on
+ *                           fp64 dot products).  row_lse [rows] (base 2) and token_scores [rows, per_row] are saved for
+ *                           the gradient; NULL when there will be none.
+ *   meclip_token_log_probs_grad  dx = dz Y / T, dtable = dz^T X / T for
+ *                           dz_ij = sum_k g_ik ([j = token_ik] - p_ij) - h_i p_ij (log p_ij + entropy_i),
+ *                           g = grad_log_probs, h = grad_entropy (either may be NULL: zero).
+ *   meclip_distill          KL(q || p) per row for a teacher that is known by its top logits: q = softmax of
+ *                           teacher_logits / teacher_temperature (teacher_dtype, [rows, per_row]) over the row's
+ *                           entries that are present (token >= 0 and logit > -inf).  A row without one has loss 0,
+ *                           row_has 0 and no gradient.  Entries that name the same token add up.
+ *                           loss = sum of row_loss, times inv_count = 1 / (rows with an entry) when `mean` is set
+ *                           (both NULL: only row_loss is wanted); no row at all: loss 0.
+ *   meclip_distill_grad     dz_ij = w_i (p_ij - q_ij), w_i = grad_out (one scalar, or [rows] with grad_per_row) times
+ *                           inv_count (NULL: 1).  The teacher gets no gradient.
+ * The gradients read bf16 operands; x_f16 / table_f16 (NULL otherwise) are the fp16 operands of a forward that ran on
+ * those, and the scores are formed from them again.  Coefficients are rounded to bf16 once, as in meclip_grad; output
+ * modes, blocking and side streams are those of meclip_grad, without atomics.  Either output may be NULL.
+ */
+size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
+size_t meclip_vocab_grad_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
+int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
+                           int64_t ldx, int64_t ldt, float temperature, const int64_t* tokens, int64_t per_row,
+                           float* log_probs, float* entropy, int top_k, float* top_log_probs, int64_t* top_tokens,
+                           float* row_lse, float* token_scores, void* workspace, size_t workspace_bytes, int* status,
+                           void* stream);
+int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16,
+                                int64_t rows, int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16,
+                                int64_t ldt_f16, float temperature, const int64_t* tokens, int64_t per_row,
+                                const float* row_lse, const float* entropy, const float* token_scores,
+                                const float* grad_log_probs, const float* grad_entropy, void* dx, int dx_mode, int64_t lddx,
+                                void* dtable, int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes,
+                                int* status, void* stream);
+int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
+                   int64_t ldt, float temperature, const int64_t* teacher_tokens, const void* teacher_logits,
+                   int teacher_dtype, int64_t per_row, float teacher_temperature, int mean, float* row_loss, float* row_has,
+                   float* loss, float* inv_count, float* row_lse, float* token_scores, float* teacher_probs,
+                   void* workspace, size_t workspace_bytes, int* status, void* stream);
+int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16, int64_t rows,
+                        int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16, int64_t ldt_f16,
+                        float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
+                        const float* token_scores, const float* teacher_probs, const float* row_has, const float* grad_out,
+                        int grad_per_row, const float* inv_count, void* dx, int dx_mode, int64_t lddx, void* dtable,
+                        int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes, int* status, void* stream);
+
+/*
  * Test hook: C (m x n, fp32, ldc) = A * B^T-style contraction through the same
  * tcgen05 mainloop the loss kernels use.  a_mn_major == 0: A is m x k row-major
  * (K contiguous); 1: A is stored k x m row-major (M contiguous).  Same for B

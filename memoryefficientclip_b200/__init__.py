@@ -10,8 +10,10 @@ from .clip_loss import (MemoryEfficientCLIPLoss, MemoryEfficientCLIPLossNormed, 
 from .lit_loss import (MemoryEfficientLiTLoss, MemoryEfficientLiTLossNormed, StableMemoryEfficientLiTLoss,
                        StableMemoryEfficientLiTLossNormed)
 from .siglip_loss import MemoryEfficientSigLIPLoss, MemoryEfficientSigLIPLossFn
+from .vocabulary import MemoryEfficientDistillLoss, MemoryEfficientDistillLossFn, TokenLogProbs, token_log_probs
 
 __all__ = [
+    "MemoryEfficientDistillLoss", "MemoryEfficientDistillLossFn", "TokenLogProbs", "token_log_probs",
     "MemoryEfficientSigLIPLoss", "MemoryEfficientSigLIPLossFn",
     "MemoryEfficientCLIPLoss", "MemoryEfficientCLIPLossNormed", "StableMemoryEfficientCLIPLoss",
     "StableMemoryEfficientCLIPLossNormed", "MemoryEfficientLiTLoss", "MemoryEfficientLiTLossNormed",

@@ -105,6 +105,22 @@ SIGNATURES = {
                                     c_void_p, c_size_t, c_void_p, c_void_p, c_void_p]),
     "meclip_step_backward": (c_int, [c_int, c_void_p, c_size_t, c_int64, c_int64, c_int, c_float, c_void_p, c_float,
                                      c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_vocab_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "meclip_vocab_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "meclip_token_log_probs": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+                                       c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_token_log_probs_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                            c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p,
+                                            c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int,
+                                            c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_distill": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
+                               c_void_p, c_int, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_distill_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                    c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
+                                    c_void_p, c_size_t, c_void_p, c_void_p]),
     "meclip_debug_gemm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64,
                                   c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
 }

@@ -1,4 +1,4 @@
-// The three epilogues of the tile kernels, shared by the single-CTA and the CTA-pair kernel.
+// The five epilogues of the tile kernels, shared by the single-CTA and the CTA-pair kernel.
 // Eight warps (two per TMEM lane quadrant) work on one 128-row accumulator: warp quadrant
 // q = warp % 4 owns rows 32q..32q+31, warp group wg = 0/1 owns the first / second half of the
 // tile's columns.  One thread = one row (tcgen05.ld 32x32b), 32 columns per load.
@@ -77,6 +77,86 @@ __device__ __forceinline__ void coef_chunk(const uint32_t (&v)[32], float fmul, 
         gv[c + 1] = coef_value<SIG>(__uint_as_float(v[c + 1]), fmul, fadd) * (inv_r + ic.y);
         gv[c + 2] = coef_value<SIG>(__uint_as_float(v[c + 2]), fmul, fadd) * (inv_r + ic.z);
         gv[c + 3] = coef_value<SIG>(__uint_as_float(v[c + 3]), fmul, fadd) * (inv_r + ic.w);
+    }
+}
+
+// One 32-column chunk of the vocabulary statistics of a row.  Everything is relative to the chunk's own maximum:
+// u_c = S_c fmul - cm <= 0 (up to the rounding of cm), l = sum 2^u, t = sum 2^u u; nv of the 32 columns exist.
+// With CAND also the column of the best and a lower bound of the second best's distance: the two smallest of the
+// integers |u| bits (low five cleared) | column.  Non-negative floats order like their bits and the low bits break
+// ties towards the lower column, so that is one logic operation and three integer minima / maxima per element.
+template <bool CAND>
+__device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul, int nv, float& cm, float& l, float& t,
+                                            uint32_t& second) {
+    float l0 = 0.f, l1 = 0.f, t0 = 0.f, t1 = 0.f;
+    uint32_t n1 = 0x7fffffffu, n2 = 0x7fffffffu;
+    if (nv >= 32) {
+        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]), m2 = __uint_as_float(v[2]), m3 = __uint_as_float(v[3]);
+#pragma unroll
+        for (int c = 4; c < 32; c += 4) {
+            m0 = fmaxf(m0, __uint_as_float(v[c]));
+            m1 = fmaxf(m1, __uint_as_float(v[c + 1]));
+            m2 = fmaxf(m2, __uint_as_float(v[c + 2]));
+            m3 = fmaxf(m3, __uint_as_float(v[c + 3]));
+        }
+        cm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * fmul;
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+            const float ua = fmaf(__uint_as_float(v[c]), fmul, -cm), ub = fmaf(__uint_as_float(v[c + 1]), fmul, -cm);
+            const float ea = ex2_approx(ua), eb = ex2_approx(ub);
+            l0 += ea; l1 += eb;
+            t0 = fmaf(ea, ua, t0); t1 = fmaf(eb, ub, t1);
+            if (CAND) {
+                const uint32_t ka = (__float_as_uint(ua) & 0x7fffffe0u) | (uint32_t)c;
+                const uint32_t kb = (__float_as_uint(ub) & 0x7fffffe0u) | (uint32_t)(c + 1);
+                n2 = min(n2, max(n1, ka)); n1 = min(n1, ka);
+                n2 = min(n2, max(n1, kb)); n1 = min(n1, kb);
+            }
+        }
+    } else {
+        float m = __uint_as_float(v[0]);           // nv >= 1: column 0 exists
+#pragma unroll
+        for (int c = 1; c < 32; ++c)
+            if (c < nv) m = fmaxf(m, __uint_as_float(v[c]));
+        cm = m * fmul;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+            if (c < nv) {
+                const float u = fmaf(__uint_as_float(v[c]), fmul, -cm);
+                const float e = ex2_approx(u);
+                l0 += e;
+                t0 = fmaf(e, u, t0);
+                if (CAND) {
+                    const uint32_t k = (__float_as_uint(u) & 0x7fffffe0u) | (uint32_t)c;
+                    n2 = min(n2, max(n1, k)); n1 = min(n1, k);
+                }
+            }
+        }
+    }
+    l = l0 + l1;
+    t = t0 + t1;
+    second = (n2 & ~31u) | (n1 & 31u);
+}
+
+// Joins {maximum m2, sum l2, moment t2} to {m, l, t}: the sums are rescaled to the larger maximum and the exponents
+// inside the moment shift with it.  An empty side has a finite m of -1e30 and l = t = 0, so no infinities meet.
+__device__ __forceinline__ void stats_join(float& m, float& l, float& t, float m2, float l2, float t2) {
+    const float mn = fmaxf(m, m2);
+    const float a = m - mn, b = m2 - mn;
+    const float fa = ex2_approx(a), fb = ex2_approx(b);
+    t = fa * fmaf(a, l, t) + fb * fmaf(b, l2, t2);
+    l = fa * l + fb * l2;
+    m = mn;
+}
+static constexpr float STATS_EMPTY = -1e30f;
+
+// Coefficients of a chunk over a vocabulary: 2^u (a + b u), u = log2 of the row's softmax.
+__device__ __forceinline__ void vocab_chunk(const uint32_t (&v)[32], float fmul, float lse, float a, float b,
+                                            float (&gv)[32]) {
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+        const float u = fmaf(__uint_as_float(v[c]), fmul, -lse);
+        gv[c] = ex2_approx(u) * fmaf(b, u, a);
     }
 }
 
@@ -163,7 +243,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
     const int jd = (jd_ll >= 0 && jd_ll < p.bn && n0 + jd_ll < p.n && rvalid) ? (int)jd_ll : -1;
     // this warp group's share of the columns, in units of 32 (SUMS, OUT) or 64 (COEF) columns
     // tile_bn differs from p.bn only for the narrower last column tile of a contraction (EPI_OUT)
-    const int units = (EPI == EPI_COEF) ? (p.bn >> 6) : (EPI == EPI_OUT ? (tile_bn >> 5) : (p.bn >> 5));
+    const int units = epi_is_coef(EPI) ? (p.bn >> 6) : (EPI == EPI_OUT ? (tile_bn >> 5) : (p.bn >> 5));
     const int u_split = EPI_WARPS == 8 ? (units + 1) >> 1 : units;
     const int u_begin = wg == 0 ? 0 : u_split;
     const int u_end = wg == 0 ? u_split : units;
@@ -243,23 +323,35 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         if (jd >= 0 && (jd >> 5) >= u_begin && (jd >> 5) < u_end) p.diag[grow] = sdiag;
         // deterministic mode: one slot per tile, so the column partials are handed in after every tile
         if (want_cols && p.col_part != nullptr) flush_column_sums(p, tail, st, warp, lane);
-    } else if (EPI == EPI_COEF) {
+    } else if (epi_is_coef(EPI)) {
         // g / c_j for the tile's columns, staged once per tile for all eight warps
-        named_bar_sync(1, EPI_THREADS);            // previous tile's readers of icol are done
-        for (int j = et; j < p.bn; j += EPI_THREADS) {
-            float v = 0.f;
-            if (p.c != nullptr && n0 + j < p.n) v = p.coef * st.gscale / __ldg(p.c + n0 + j);
-            tail->icol[j] = v;
+        constexpr bool VOCAB = EPI == EPI_VCOEF;   // softmax over a vocabulary: row factors only, no diagonal
+        if (!VOCAB) {
+            named_bar_sync(1, EPI_THREADS);        // previous tile's readers of icol are done
+            for (int j = et; j < p.bn; j += EPI_THREADS) {
+                float v = 0.f;
+                if (p.c != nullptr && n0 + j < p.n) v = p.coef * st.gscale / __ldg(p.c + n0 + j);
+                tail->icol[j] = v;
+            }
         }
         // row factor: g / r_i for the softmax losses, plain g when there are no row sums (sigmoid loss)
-        const float inv_r = !rvalid ? 0.f : (p.r != nullptr ? p.coef * st.gscale / __ldg(p.r + grow) : p.coef * st.gscale);
-        named_bar_sync(1, EPI_THREADS);
+        const float inv_r = (VOCAB || !rvalid) ? 0.f : (p.r != nullptr ? p.coef * st.gscale / __ldg(p.r + grow) : p.coef * st.gscale);
+        float v_lse = 1e30f, v_a = 0.f, v_b = 0.f;          // a row past the edge: 2^-huge = 0
+        if (VOCAB) {
+            if (rvalid) {
+                v_lse = __ldg(p.row_lse + grow);
+                v_a = __ldg(p.row_a + grow);
+                if (p.row_b != nullptr) v_b = __ldg(p.row_b + grow);
+            }
+        } else {
+            named_bar_sync(1, EPI_THREADS);
+        }
         // Each warp turns 32 rows x 64 columns into a 128-byte-swizzled shared tile and one lane
         // TMA-stores it (full 128-byte lines; rows and chunks outside the panel are clipped by the
         // tensor map).
         const float dsub = p.dcoef * st.gscale;
-        const bool diag_here = __any_sync(0xffffffffu, jd >= 0);
-        const bool want_sg = p.sg_acc != nullptr;      // sum of G_ij * S_ij for the temperature gradient
+        const bool diag_here = !VOCAB && __any_sync(0xffffffffu, jd >= 0);
+        const bool want_sg = !VOCAB && p.sg_acc != nullptr;      // sum of G_ij * S_ij for the temperature gradient
         float sg = 0.f, sg1 = 0.f;
         uint8_t* buf = tail->scratch + (size_t)(warp - 2) * STORE_BUF_BYTES;
         for (int u = u_begin; u < u_end; ++u) {
@@ -275,7 +367,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
                 tmem_ld32(taddr + ch * 32, v);
                 tmem_ld_wait();
                 float gv[32];
-                if (p.sigmoid) coef_chunk<true>(v, st.fmul, st.fadd, inv_r, &tail->icol[ch * 32], gv);
+                if (VOCAB) vocab_chunk(v, st.fmul, v_lse, v_a, v_b, gv);
+                else if (p.sigmoid) coef_chunk<true>(v, st.fmul, st.fadd, inv_r, &tail->icol[ch * 32], gv);
                 else           coef_chunk<false>(v, st.fmul, st.fadd, inv_r, &tail->icol[ch * 32], gv);
                 if (diag_here) {      // warp-uniform: only tiles that cross the diagonal pay for the correction
                     const int jdc = (jd >= 0 && (jd >> 5) == ch) ? (jd & 31) : -1;
@@ -329,6 +422,31 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             }
             if (lane == 0) { atomicAdd(p.sg_acc, sg); atomicAdd(p.sg_acc + 1, sg1); }
         }
+    } else if (EPI == EPI_STATS) {
+        float m = STATS_EMPTY, l = 0.f, t = 0.f;
+        const bool cand = p.chunk_max != nullptr;
+        for (int ch = u_begin; ch < u_end; ++ch) {
+            uint32_t v[32];
+            tmem_ld32(taddr + ch * 32, v);
+            tmem_ld_wait();
+            const int col0 = n0 + ch * 32;
+            const int nv = p.n - col0;
+            if (nv > 0) {                      // the same for the whole warp
+                float cm, cl, ct;
+                uint32_t second;
+                if (cand) stats_chunk<true>(v, st.fmul, nv, cm, cl, ct, second);
+                else      stats_chunk<false>(v, st.fmul, nv, cm, cl, ct, second);
+                stats_join(m, l, t, cm, cl, ct);
+                if (cand && rvalid) {
+                    const long long at = (long long)grow * p.chunk_ld + (col0 >> 5);
+                    p.chunk_max[at] = cm;
+                    p.chunk_second[at] = second;
+                }
+            }
+        }
+        tc_fence_before();
+        release();
+        if (rvalid) p.stats[(long long)grow * p.stats_ld + 2 * (n0 / p.bn) + wg] = make_float4(m, l, t, 0.f);
     } else {   // EPI_OUT
         // Wide tiles (two MMAs per K step, see GemmParams::wide): the first MMA's 256 accumulator columns hold the
         // first 128 B rows of CTA 0 and of CTA 1, the second MMA's columns (from TMEM column 256) the remaining rows
@@ -403,7 +521,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
 // (Pending column sums are flushed by the kernels, which know whether the tile loop ended cleanly.)
 template <int EPI>
 __device__ __forceinline__ void epilogue_drain(const EpiState& st, int lane) {
-    if (EPI == EPI_COEF && lane == 0 && st.stores_in_flight > 0) {
+    if (epi_is_coef(EPI) && lane == 0 && st.stores_in_flight > 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 }

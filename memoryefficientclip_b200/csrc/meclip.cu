@@ -706,6 +706,8 @@ struct Operand {
     long long blocked_rows_alloc = 0;
     // fp32 elements, multiplied as tf32 (K-major, sums and coefficient passes only; A and B together)
     bool f32 = false;
+    // fp16 elements instead of bf16 ones (vocabulary passes only; A and B together: one MMA takes one type)
+    bool f16 = false;
 };
 
 template <int EPI, bool A_MN, bool B_MN>
@@ -781,10 +783,14 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     if (m < 1 || n < 1 || k < 1) return fail(MECLIP_EINVAL, "gemm extents must be >= 1 (m=%lld n=%lld k=%lld)", m, n, k);
     if (m > 0x7fffffffLL || n > 0x7fffffffLL || k > 0x7fffffffLL) return fail(MECLIP_EINVAL, "gemm extent exceeds 2^31");
     const bool wide = bn > MAX_BN;      // two MMAs per K step, CTA-pair kernel, plain contraction only
-    if (bn < 32 || bn > 2 * MAX_BN || bn % 32 != 0 || ((b.mn_major || epi == EPI_COEF || wide) && bn % 64 != 0) ||
+    if (bn < 32 || bn > 2 * MAX_BN || bn % 32 != 0 || ((b.mn_major || epi_is_coef(epi) || epi == EPI_STATS || wide) && bn % 64 != 0) ||
         (wide && (epi != EPI_OUT || b.mn_major || g_trace_buf != nullptr || pair_mode() == 0)))
         return fail(MECLIP_EINVAL, "tile width %d not supported", bn);
     const bool f32 = a.f32;
+    if (a.f16 != b.f16 || (a.f16 && (f32 || (epi != EPI_STATS && epi != EPI_VCOEF))))
+        return fail(MECLIP_EINVAL, "fp16 operands: vocabulary passes only, A and B together");
+    // bits 7 and 10 of the instruction descriptor say bf16; cleared they say fp16
+    const uint32_t idesc_keep = a.f16 ? ~((1u << 7) | (1u << 10)) : ~0u;
     if (f32) {
         // fp32 operands read as tf32: the CTA-pair kernel with K-major A and B, 32 elements per K step
         if (!b.f32 || a.mn_major || b.mn_major || a.blocked_rows_alloc > 0 || epi == EPI_OUT || wide || bn % 64 != 0 ||
@@ -812,11 +818,12 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     const int pmode = pair_mode();
     const bool pair = !b.mn_major && bn % 64 == 0 && g_trace_buf == nullptr &&      // the in-kernel trace is a single-CTA hook
                       (f32 || wide || pmode == 1 || ((pmode == 2 || pmode < 0) && epi == EPI_OUT && bn == 256) ||
-                       (pmode < 0 && epi != EPI_OUT && bn == 256 && k >= PAIR_MIN_K));
+                       (pmode < 0 && epi != EPI_OUT && bn == 256 && k >= PAIR_MIN_K)) &&
+                      !(m <= BM && (epi == EPI_STATS || epi == EPI_VCOEF));     // half of every pair would have no rows
     if (b.mn_major) rc = make_tmap(&tb, b.ptr, n, k, b.ld, 64, BK);
     else            rc = make_tmap(&tb, b.ptr, k, n, b.ld, bk, pair ? bn / 2 : bn, f32);
     if (rc) return rc;
-    if (epi == EPI_COEF) {
+    if (epi_is_coef(epi)) {
         if (panel == nullptr || !aligned16(panel) || panel_rows_alloc < m) return fail(MECLIP_EINVAL, "coefficient panel misaligned");
         rc = make_tmap_blocked(&tc, panel, m, (n + 63) / 64, panel_rows_alloc, 32, panel_chunks_alloc);   // one warp's 32 rows x 64 columns per store
         if (rc) return rc;
@@ -844,7 +851,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         const long long per_sm = (long long)p.num_m_tiles * p.num_n_tiles / sm_count();
         p.strip_len = per_sm >= 64 ? 16 : per_sm >= 32 ? 8 : per_sm >= 16 ? 4 : per_sm >= 8 ? 2 : 1;
     }
-    p.idesc = umma_idesc_bf16(BM, bn, a.mn_major ? 1 : 0, b.mn_major ? 1 : 0);
+    p.idesc = umma_idesc_bf16(BM, bn, a.mn_major ? 1 : 0, b.mn_major ? 1 : 0) & idesc_keep;
     p.bn_last = bn;
     p.idesc_last = p.idesc;
     if (epi == EPI_OUT) {      // narrower last column tile: only as many 32-column chunks as hold valid columns
@@ -881,9 +888,9 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     if (pair) {
         const int amn = a.mn_major ? 1 : 0;
         p.wide = wide ? 1 : 0;
-        p.idesc = umma_idesc_bf16(PAIR_BM, bn < MAX_BN ? bn : MAX_BN, amn, 0);
+        p.idesc = umma_idesc_bf16(PAIR_BM, bn < MAX_BN ? bn : MAX_BN, amn, 0) & idesc_keep;
         p.idesc2 = wide ? umma_idesc_bf16(PAIR_BM, bn - MAX_BN, amn, 0) : 0u;
-        p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last < MAX_BN ? p.bn_last : MAX_BN, amn, 0);
+        p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last < MAX_BN ? p.bn_last : MAX_BN, amn, 0) & idesc_keep;
         p.idesc2_last = p.bn_last > MAX_BN ? umma_idesc_bf16(PAIR_BM, p.bn_last - MAX_BN, amn, 0) : 0u;
         p.stage_bytes = A_STAGE_BYTES + (bn / 2) * BK * 2;
         stages = (SMEM_LIMIT - 1024 - tail_bytes(epi)) / p.stage_bytes;
@@ -898,6 +905,8 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         }
         if (epi == EPI_SUMS) return launch_pair_t<EPI_SUMS, 0>(ta, tb, tc, p, pair_smem, stream);
         if (epi == EPI_COEF) return launch_pair_t<EPI_COEF, 0>(ta, tb, tc, p, pair_smem, stream);
+        if (epi == EPI_STATS) return launch_pair_t<EPI_STATS, 0>(ta, tb, tc, p, pair_smem, stream);
+        if (epi == EPI_VCOEF) return launch_pair_t<EPI_VCOEF, 0>(ta, tb, tc, p, pair_smem, stream);
         if (epi == EPI_OUT) return a.mn_major ? launch_pair_t<EPI_OUT, 1>(ta, tb, tc, p, pair_smem, stream)
                                               : launch_pair_t<EPI_OUT, 0>(ta, tb, tc, p, pair_smem, stream);
         return fail(MECLIP_EINVAL, "unknown epilogue %d", epi);
@@ -913,6 +922,8 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     }
     if (epi == EPI_SUMS) return launch_gemm_t<EPI_SUMS, false, false>(ta, tb, tc, p, smem_bytes, stream);
     if (epi == EPI_COEF) return launch_gemm_t<EPI_COEF, false, false>(ta, tb, tc, p, smem_bytes, stream);
+    if (epi == EPI_STATS) return launch_gemm_t<EPI_STATS, false, false>(ta, tb, tc, p, smem_bytes, stream);
+    if (epi == EPI_VCOEF) return launch_gemm_t<EPI_VCOEF, false, false>(ta, tb, tc, p, smem_bytes, stream);
     MECLIP_DISPATCH(EPI_OUT)
 #undef MECLIP_DISPATCH
     return fail(MECLIP_EINVAL, "unknown epilogue %d", epi);
@@ -1121,6 +1132,8 @@ operand_f32_kernel(const float* __restrict__ x, long long ldx, long long rows, i
 }
 
 }  // namespace meclip
+
+#include "vocab_kernels.cuh"
 
 using namespace meclip;
 
@@ -1480,7 +1493,9 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                      cudaStream_t s0, bool overlap, bool transposed_copies, float* sg_acc = nullptr,
                      float logit_scale = 0.f, float logit_bias = 0.f, int64_t n_extra = 0, bool plain_e = false,
                      const DeviceScalars& ds = DeviceScalars(), bool honour_overrides = true,
-                     const float* x_f32 = nullptr, int64_t ldxf = 0, const float* y_f32 = nullptr, int64_t ldyf = 0) {
+                     const float* x_f32 = nullptr, int64_t ldxf = 0, const float* y_f32 = nullptr, int64_t ldyf = 0,
+                     const VocabGrad* vg = nullptr) {
+    // vg: the coefficients of a softmax over a vocabulary (with kind MECLIP_SIGLIP: no sums of rows and columns)
     // x_f32 / y_f32: optional fp32 copies of the operands; the coefficient pass then forms S from them with tf32
     // MMAs (the contractions keep the bf16 operands)
     NvtxRange range("meclip_grad");
@@ -1608,7 +1623,21 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     b = Operand{y_f32 + c0 * ldyf, ldyf, false, 0, true};
                 }
                 t_tag = TAG_COEF;
-                rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
+                if (vg != nullptr) {
+                    p.sigmoid = 0;
+                    p.fmul = 1.4426950408889634f / temperature;
+                    p.row_lse = vg->row_lse + r0;
+                    p.row_a = vg->row_a + r0;
+                    p.row_b = vg->row_b != nullptr ? vg->row_b + r0 : nullptr;
+                    if (vg->x_f16 != nullptr) {
+                        a = Operand{vg->x_f16 + r0 * vg->ldx_f16, vg->ldx_f16, false, 0, false, true};
+                        b = Operand{vg->y_f16 + c0 * vg->ldy_f16, vg->ldy_f16, false, 0, false, true};
+                    }
+                    rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, cols, gpanel[gb], plan.row_block, s0);
+                } else {
+                    rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
+                }
                 if (rc) return rc;
             }
             if (overlap) {
@@ -2321,3 +2350,5 @@ int meclip_debug_gemm(const void* a_bf16, int64_t lda, int a_mn_major, const voi
 }
 
 }  // extern "C"
+
+#include "vocab_abi.cuh"

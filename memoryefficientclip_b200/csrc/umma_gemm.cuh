@@ -1,11 +1,14 @@
 // Persistent, warp-specialised tcgen05 GEMM mainloop shared by every tile kernel
-// of the loss path, with three epilogues:
+// of the loss path, with five epilogues:
 //
 //   EPI_SUMS  S = X Y^T tile -> E = exp2(k S - k) -> row sums, column sums, diagonal
 //   EPI_COEF  S tile -> E -> G = E (g/r_i + g/c_j) - [i==j] g -> bf16 panel, TMA-stored in a
 //             column-blocked layout [64-column chunk][row][64] so that every later tile load of
 //             the panel (as G or as G^T) is one contiguous run of memory
 //   EPI_OUT   plain contraction -> (+ fp32 partial) -> fp32 / bf16 store
+//   EPI_STATS S tile -> per row and half tile: maximum, sum of exponentials and their first moment, and for each
+//             32 columns the maximum with the distance to the second best (softmax over a vocabulary)
+//   EPI_VCOEF EPI_COEF for a vocabulary: G = p (a_i + b_i log2 p), p = 2^(S fmul - lse_i), into the same panel
 //
 // One CTA per SM, 320 threads:
 //   warp 0      tile scheduler + TMA producer (one lane): global -> 128B-swizzled shared tiles
@@ -49,7 +52,8 @@ static_assert(!MECLIP_STRIPS || EPI_WARPS == 8, "strip accumulators need 8 epilo
 static constexpr int SMEM_LIMIT = 232448; // 227 KiB: most dynamic shared memory one CTA can have
 static constexpr int STORE_BUF_BYTES = 32 * 128;   // one warp's 32 rows x 64 bf16 staging tile
 
-enum { EPI_SUMS = 0, EPI_COEF = 1, EPI_OUT = 2 };
+enum { EPI_SUMS = 0, EPI_COEF = 1, EPI_OUT = 2, EPI_STATS = 3, EPI_VCOEF = 4 };
+__host__ __device__ constexpr bool epi_is_coef(int epi) { return epi == EPI_COEF || epi == EPI_VCOEF; }
 
 struct GemmParams {
     int m, n, k;              // valid extents of the problem
@@ -129,6 +133,20 @@ struct GemmParams {
     // Records of 3 words start at trace[2]; role r owns records [r*cap/3, (r+1)*cap/3); unused ones stay zero.
     unsigned long long* trace;
     unsigned int trace_capacity;
+    // EPI_STATS: every (row, warp group of a column tile) stores {maximum of S fmul, sum 2^(S fmul - maximum), sum of
+    // the same times its exponent, 0} in stats[row * stats_ld + 2 * column tile + group].  With top alternatives wanted
+    // (chunk_max set) every (row, 32-column chunk) also stores the chunk's maximum of S fmul and, as one word, the
+    // distance of its second best (fp32 bits, low five cleared, so never too large) | the column of its best.
+    float4* stats;
+    long long stats_ld;
+    float* chunk_max;
+    uint32_t* chunk_second;
+    long long chunk_ld;
+    // EPI_VCOEF: u = S fmul - row_lse[i] = log2 p_ij, G_ij = 2^u (row_a[i] + row_b[i] u);
+    // no diagonal, no column factors; row_b may be null
+    const float* row_lse;
+    const float* row_a;
+    const float* row_b;
 };
 
 enum { TR_LOAD_BEGIN = 1, TR_LOAD_END = 2, TR_MMA_BEGIN = 10, TR_MMA_FIRST_DATA = 11, TR_MMA_END = 12,
@@ -167,8 +185,8 @@ struct SharedTail {
 
 __host__ __device__ constexpr int tail_bytes(int epi) {
     // the scratch union is the first member; kernels that do not need all of it start the tail later
-    return (int)sizeof(SharedTail) - (epi == EPI_COEF ? 0 : epi == EPI_SUMS ? 4 * 2 * STORE_BUF_BYTES - 4 * MAX_BN * 4
-                                                                            : 4 * 2 * STORE_BUF_BYTES);
+    return (int)sizeof(SharedTail) - (epi_is_coef(epi) ? 0 : epi == EPI_SUMS ? 4 * 2 * STORE_BUF_BYTES - 4 * MAX_BN * 4
+                                                                            : 4 * 2 * STORE_BUF_BYTES);   // OUT, STATS
 }
 
 template <int HALF>
@@ -279,7 +297,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
         fence_barrier_init();
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
-        if (EPI == EPI_COEF) tma_prefetch_desc(&tmap_c);
+        if (epi_is_coef(EPI)) tma_prefetch_desc(&tmap_c);
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(&tail->tmem_base), TMEM_COLS);

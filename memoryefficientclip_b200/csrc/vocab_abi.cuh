@@ -1,0 +1,295 @@
+// Host side of the vocabulary softmax: meclip_token_log_probs, meclip_distill and their gradients (include/meclip.h).
+#pragma once
+
+namespace meclip {
+
+// Rows handled by one tile pass: the partial results (1/8 byte per score, 3/8 with alternatives) stay a bounded
+// workspace however many rows there are, and 16384 rows fill the GPU many times over.
+static constexpr long long VOCAB_ROW_BLOCK = 16384;
+
+// Column-tile width of the statistics pass: the fewest waves x width over the SMs, wider on ties.  The narrower tiles
+// only win when few rows leave SMs without a tile (see pick_contraction_bn for what a narrow tile costs per column).
+static int pick_stats_bn(long long rows, long long vocab) {
+    const int cand[4] = {256, 192, 128, 64};
+    const double cost_per_col[4] = {1.0, 1.07, 1.2, 1.5};
+    int best = 256;
+    double best_t = 0.0;
+    for (int i = 0; i < 4; ++i) {
+        const long long tiles = ((rows + BM - 1) / BM) * ((vocab + cand[i] - 1) / cand[i]);
+        const double t = (double)((tiles + sm_count() - 1) / sm_count()) * cand[i] * cost_per_col[i];
+        if (i == 0 || t < best_t) { best_t = t; best = cand[i]; }
+    }
+    return best;
+}
+
+struct VocabPlan {
+    long long row_block, slots, chunks, chunk_ld;
+    int bn;
+    size_t stats_bytes, chunk_bytes, total;
+};
+static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
+    VocabPlan v;
+    v.row_block = rows < VOCAB_ROW_BLOCK ? rows : VOCAB_ROW_BLOCK;
+    v.bn = pick_stats_bn(v.row_block, vocab);
+    v.slots = 2 * ((vocab + v.bn - 1) / v.bn);
+    v.chunks = (vocab + 31) / 32;
+    v.chunk_ld = (long long)round_up((size_t)v.chunks, 4);
+    v.stats_bytes = round_up((size_t)v.row_block * v.slots * 16, 256);
+    v.chunk_bytes = top_k > 0 ? round_up((size_t)v.row_block * v.chunk_ld * 4, 256) : 0;
+    v.total = v.stats_bytes + 2 * v.chunk_bytes;
+    return v;
+}
+
+template <int G, bool DISTILL>
+static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
+    const int per_block = VOCAB_THREADS / G;
+    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap, G / 32);
+    const unsigned grid = (unsigned)((p.rows + per_block - 1) / per_block);
+    const double bytes = (double)p.rows * (16.0 * p.slots + (p.top_k > 0 ? 8.0 * p.chunks : 0.0) +
+                                           2.0 * p.d * (1 + p.k + p.top_k));
+    ScopedTiming timing(s, TAG_ROW, bytes);
+    if (f16) {
+        auto kern = vocab_rows_kernel<G, __half, DISTILL>;
+        if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
+    } else {
+        auto kern = vocab_rows_kernel<G, __nv_bfloat16, DISTILL>;
+        if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
+    }
+    MECLIP_CUDA(cudaGetLastError());
+    return MECLIP_OK;
+}
+
+// What both forwards ask of their operands.
+static int check_vocab(const char* what, const void* x, const void* table, int dtype, int64_t rows, int64_t vocab,
+                       int64_t d, int64_t ldx, int64_t ldt, float temperature, const void* tokens, int64_t k) {
+    if (x == nullptr || table == nullptr || (tokens == nullptr && k > 0)) return fail(MECLIP_EINVAL, "%s: null pointer", what);
+    if (dtype != MECLIP_BF16 && dtype != MECLIP_F16) return fail(MECLIP_EINVAL, "%s: operands are bf16 or fp16", what);
+    if (rows < 1 || vocab < 1 || rows > 0x7fffffffLL || vocab > 0x7fffffffLL || d < 8 || d % 8 != 0 || d > 0x7fffffffLL ||
+        ldx < d || ldt < d || ldx % 8 != 0 || ldt % 8 != 0 || !aligned16(x) || !aligned16(table))
+        return fail(MECLIP_EINVAL, "%s: need rows, vocab in [1, 2^31), d and pitches multiples of 8, 16-byte alignment", what);
+    if (!(temperature > 0.f) || std::isinf(temperature)) return fail(MECLIP_EINVAL, "%s: temperature must be positive", what);
+    if (k < 0 || k > VOCAB_MAX_ENTRIES) return fail(MECLIP_EINVAL, "%s: at most %d entries per row", what, VOCAB_MAX_ENTRIES);
+    return MECLIP_OK;
+}
+
+// Statistics pass and row kernel over blocks of rows.  `r` holds the per-row arguments of the whole problem.
+template <bool DISTILL>
+static int vocab_forward(VocabRows r, int dtype, void* workspace, size_t workspace_bytes, int* status, cudaStream_t s) {
+    int rc = check_device();
+    if (rc) return rc;
+    const long long rows = r.rows;
+    const VocabPlan plan = plan_vocab(rows, r.vocab, r.top_k);
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+        return fail(MECLIP_EINVAL, "vocabulary pass: the workspace must be 256-byte aligned");
+    if (workspace_bytes < plan.total) return fail(MECLIP_ENOSPC, "vocabulary pass: workspace %zu < %zu bytes", workspace_bytes, plan.total);
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    r.stats = reinterpret_cast<const float4*>(ws);
+    r.slots = (int)plan.slots;
+    r.stats_ld = plan.slots;
+    r.chunk_max = r.top_k > 0 ? reinterpret_cast<const float*>(ws + plan.stats_bytes) : nullptr;
+    r.chunk_second = r.top_k > 0 ? reinterpret_cast<const uint32_t*>(ws + plan.stats_bytes + plan.chunk_bytes) : nullptr;
+    r.chunks = (int)plan.chunks;
+    r.chunk_ld = plan.chunk_ld;
+    r.list_cap = r.top_k > 0 ? 32 * r.top_k + 64 : 0;
+    for (long long r0 = 0; r0 < rows; r0 += plan.row_block) {
+        VocabRows b = r;
+        b.rows = rows - r0 < plan.row_block ? rows - r0 : plan.row_block;
+        b.x = reinterpret_cast<const uint16_t*>(r.x) + r0 * r.ldx;
+        if (r.tokens != nullptr) b.tokens = r.tokens + r0 * r.k;
+        if (r.row_lse != nullptr) b.row_lse = r.row_lse + r0;
+        if (r.entropy != nullptr) b.entropy = r.entropy + r0;
+        if (r.token_s2 != nullptr) b.token_s2 = r.token_s2 + r0 * r.k;
+        if (r.log_probs != nullptr) b.log_probs = r.log_probs + r0 * r.k;
+        if (r.top_k > 0) { b.top_log_probs = r.top_log_probs + r0 * r.top_k; b.top_tokens = r.top_tokens + r0 * r.top_k; }
+        if (DISTILL) {
+            b.teacher_logits = reinterpret_cast<const uint8_t*>(r.teacher_logits) + (size_t)r0 * r.k * (r.teacher_dtype == MECLIP_F32 ? 4 : 2);
+            b.teacher_probs = r.teacher_probs + r0 * r.k;
+            b.row_loss = r.row_loss + r0;
+            b.row_has = r.row_has + r0;
+        }
+        GemmParams p;
+        std::memset(&p, 0, sizeof(p));
+        p.fmul = r.fmul;
+        p.stats = const_cast<float4*>(r.stats);
+        p.stats_ld = r.stats_ld;
+        p.chunk_max = const_cast<float*>(r.chunk_max);
+        p.chunk_second = const_cast<uint32_t*>(r.chunk_second);
+        p.chunk_ld = r.chunk_ld;
+        p.status = status;
+        const bool f16 = dtype == MECLIP_F16;
+        Operand a{b.x, r.ldx, false, 0, false, f16}, t{r.y, r.ldy, false, 0, false, f16};
+        t_tag = TAG_SUMS;
+        rc = launch_gemm(EPI_STATS, a, t, b.rows, r.vocab, r.d, plan.bn, p, s);
+        if (rc) return rc;
+        // a few rows: a block each; many: a warp each
+        if (b.rows <= 2 * sm_count()) rc = launch_vocab_rows_t<256, DISTILL>(b, f16, s);
+        else                          rc = launch_vocab_rows_t<32, DISTILL>(b, f16, s);
+        if (rc) return rc;
+    }
+    return MECLIP_OK;
+}
+
+struct VocabGradPlan { size_t rows_bytes, grad_bytes; bool transposed; };
+static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long d) {
+    VocabGradPlan g;
+    g.rows_bytes = round_up((size_t)rows * 4, 256);
+    // transposed copies of the operands and side streams pay for themselves when the contractions are long
+    g.transposed = rows >= 1024 && transposes_allowed();
+    g.grad_bytes = plan_grad(rows, vocab, d, g.transposed).total();
+    return g;
+}
+
+static int vocab_grad(VocabGrad vg, const void* x_bf16, const void* t_bf16, int64_t rows, int64_t vocab, int64_t d,
+                      int64_t ldx, int64_t ldt, float temperature, void* dx, int dx_mode, int64_t lddx, void* dt,
+                      int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
+    return grad_impl(MECLIP_SIGLIP, x_bf16, t_bf16, rows, vocab, d, ldx, ldt, temperature, 0, 0, nullptr, nullptr, nullptr,
+                     1.f, dx, dx_mode, lddx, dt, dt_mode, lddt, ws + 2 * plan.rows_bytes, plan.grad_bytes, status, s,
+                     plan.transposed && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false, DeviceScalars(),
+                     true, nullptr, 0, nullptr, 0, &vg);
+}
+
+static int check_vocab_grad(const char* what, const void* x16, const void* t16, int64_t ldx16, int64_t ldt16, int64_t d,
+                            const void* ws, size_t ws_bytes, const VocabGradPlan& plan) {
+    if ((x16 == nullptr) != (t16 == nullptr) ||
+        (x16 != nullptr && (ldx16 < d || ldt16 < d || ldx16 % 8 != 0 || ldt16 % 8 != 0 || !aligned16(x16) || !aligned16(t16))))
+        return fail(MECLIP_EINVAL, "%s: fp16 operands come as a pair, 16-byte aligned with pitches multiples of 8", what);
+    if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(MECLIP_EINVAL, "%s: workspace must be 256-byte aligned", what);
+    if (ws_bytes < 2 * plan.rows_bytes + plan.grad_bytes)
+        return fail(MECLIP_ENOSPC, "%s: workspace %zu < %zu bytes", what, ws_bytes, 2 * plan.rows_bytes + plan.grad_bytes);
+    return MECLIP_OK;
+}
+
+}  // namespace meclip
+
+extern "C" {
+
+size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
+    if (rows < 1 || vocab < 1 || top_k < 0) return 0;
+    return plan_vocab(rows, vocab, top_k).total;
+}
+
+size_t meclip_vocab_grad_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
+    if (rows < 1 || vocab < 1 || d < 1) return 0;
+    const VocabGradPlan g = plan_vocab_grad(rows, vocab, d);
+    return 2 * g.rows_bytes + g.grad_bytes;
+}
+
+int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
+                           int64_t ldx, int64_t ldt, float temperature, const int64_t* tokens, int64_t per_row,
+                           float* log_probs, float* entropy, int top_k, float* top_log_probs, int64_t* top_tokens,
+                           float* row_lse, float* token_scores, void* workspace, size_t workspace_bytes, int* status,
+                           void* stream) {
+    NvtxRange range("meclip_token_log_probs");
+    int rc = check_vocab("token_log_probs", x, table, dtype, rows, vocab, d, ldx, ldt, temperature, tokens, per_row);
+    if (rc) return rc;
+    if (per_row > 0 && log_probs == nullptr) return fail(MECLIP_EINVAL, "token_log_probs: log_probs is null");
+    if (top_k < 0 || top_k > VOCAB_MAX_TOP || top_k > vocab)
+        return fail(MECLIP_EINVAL, "token_log_probs: top_k must be in [0, min(%d, vocab)]", VOCAB_MAX_TOP);
+    if (top_k > 0 && (top_log_probs == nullptr || top_tokens == nullptr)) return fail(MECLIP_EINVAL, "token_log_probs: top outputs are null");
+    VocabRows r;
+    std::memset(&r, 0, sizeof(r));
+    r.x = x; r.y = table; r.ldx = ldx; r.ldy = ldt; r.d = (int)d; r.rows = rows; r.vocab = vocab;
+    r.fmul = 1.4426950408889634f / temperature;
+    r.tokens = reinterpret_cast<const long long*>(tokens); r.k = (int)per_row;
+    r.row_lse = row_lse; r.entropy = entropy; r.token_s2 = token_scores; r.log_probs = log_probs;
+    r.top_k = top_k; r.top_log_probs = top_log_probs; r.top_tokens = reinterpret_cast<long long*>(top_tokens);
+    return vocab_forward<false>(r, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
+}
+
+int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16,
+                                int64_t rows, int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16,
+                                int64_t ldt_f16, float temperature, const int64_t* tokens, int64_t per_row,
+                                const float* row_lse, const float* entropy, const float* token_scores,
+                                const float* grad_log_probs, const float* grad_entropy, void* dx, int dx_mode, int64_t lddx,
+                                void* dtable, int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes,
+                                int* status, void* stream) {
+    NvtxRange range("meclip_token_log_probs_grad");
+    int rc = check_vocab("token_log_probs_grad", x_bf16, table_bf16, MECLIP_BF16, rows, vocab, d, ldx, ldt, temperature, tokens, per_row);
+    if (rc) return rc;
+    if (row_lse == nullptr || (per_row > 0 && token_scores == nullptr) || (grad_entropy != nullptr && entropy == nullptr))
+        return fail(MECLIP_EINVAL, "token_log_probs_grad: null pointer");
+    const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
+    rc = check_vocab_grad("token_log_probs_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
+    if (rc) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    float* row_a = reinterpret_cast<float*>(ws);
+    float* row_b = grad_entropy != nullptr ? reinterpret_cast<float*>(ws + plan.rows_bytes) : nullptr;
+    const int wpb = ROW_KERNEL_THREADS / 32;
+    {
+        ScopedTiming timing(s, TAG_ROW, (double)rows * (12.0 * per_row + 16.0));
+        token_grad_rows_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
+            grad_log_probs, grad_entropy, entropy, reinterpret_cast<const long long*>(tokens), (int)per_row, rows, vocab,
+            1.f / temperature, row_a, row_b);
+        MECLIP_CUDA(cudaGetLastError());
+    }
+    VocabGrad vg{row_lse, row_a, row_b, reinterpret_cast<const long long*>(tokens), token_scores, (int)per_row,
+                 grad_log_probs, nullptr, 1.f / temperature, (const __nv_bfloat16*)x_f16, ldx_f16,
+                 (const __nv_bfloat16*)table_f16, ldt_f16};
+    return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
+                      lddt, ws, plan, status, s);
+}
+
+int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
+                   int64_t ldt, float temperature, const int64_t* teacher_tokens, const void* teacher_logits,
+                   int teacher_dtype, int64_t per_row, float teacher_temperature, int mean, float* row_loss, float* row_has,
+                   float* loss, float* inv_count, float* row_lse, float* token_scores, float* teacher_probs,
+                   void* workspace, size_t workspace_bytes, int* status, void* stream) {
+    NvtxRange range("meclip_distill");
+    int rc = check_vocab("distill", x, table, dtype, rows, vocab, d, ldx, ldt, temperature, teacher_tokens, per_row);
+    if (rc) return rc;
+    if (per_row < 1) return fail(MECLIP_EINVAL, "distill: at least one teacher entry per row");
+    if (teacher_logits == nullptr || row_loss == nullptr || row_has == nullptr || row_lse == nullptr || token_scores == nullptr ||
+        teacher_probs == nullptr || (loss == nullptr) != (inv_count == nullptr))
+        return fail(MECLIP_EINVAL, "distill: null pointer");
+    if (teacher_dtype != MECLIP_BF16 && teacher_dtype != MECLIP_F32 && teacher_dtype != MECLIP_F16)
+        return fail(MECLIP_EINVAL, "distill: bad teacher dtype %d", teacher_dtype);
+    if (!(teacher_temperature > 0.f) || std::isinf(teacher_temperature)) return fail(MECLIP_EINVAL, "distill: teacher temperature must be positive");
+    VocabRows r;
+    std::memset(&r, 0, sizeof(r));
+    r.x = x; r.y = table; r.ldx = ldx; r.ldy = ldt; r.d = (int)d; r.rows = rows; r.vocab = vocab;
+    r.fmul = 1.4426950408889634f / temperature;
+    r.tokens = reinterpret_cast<const long long*>(teacher_tokens); r.k = (int)per_row;
+    r.row_lse = row_lse; r.token_s2 = token_scores;
+    r.teacher_logits = teacher_logits; r.teacher_dtype = teacher_dtype; r.inv_teacher_t = 1.f / teacher_temperature;
+    r.teacher_probs = teacher_probs; r.row_loss = row_loss; r.row_has = row_has;
+    rc = vocab_forward<true>(r, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
+    if (rc || loss == nullptr) return rc;
+    ScopedTiming timing((cudaStream_t)stream, TAG_ROW, 8.0 * (double)rows);
+    distill_reduce_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_loss, row_has, rows, mean, loss, inv_count);
+    MECLIP_CUDA(cudaGetLastError());
+    return MECLIP_OK;
+}
+
+int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16, int64_t rows,
+                        int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16, int64_t ldt_f16,
+                        float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
+                        const float* token_scores, const float* teacher_probs, const float* row_has, const float* grad_out,
+                        int grad_per_row, const float* inv_count, void* dx, int dx_mode, int64_t lddx, void* dtable,
+                        int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes, int* status, void* stream) {
+    NvtxRange range("meclip_distill_grad");
+    int rc = check_vocab("distill_grad", x_bf16, table_bf16, MECLIP_BF16, rows, vocab, d, ldx, ldt, temperature, teacher_tokens, per_row);
+    if (rc) return rc;
+    if (per_row < 1 || row_lse == nullptr || token_scores == nullptr || teacher_probs == nullptr || row_has == nullptr || grad_out == nullptr)
+        return fail(MECLIP_EINVAL, "distill_grad: null pointer");
+    const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
+    rc = check_vocab_grad("distill_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
+    if (rc) return rc;
+    cudaStream_t s = (cudaStream_t)stream;
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    float* row_a = reinterpret_cast<float*>(ws);
+    {
+        ScopedTiming timing(s, TAG_ROW, (double)rows * 12.0);
+        distill_grad_rows_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, s>>>(grad_out, grad_per_row, inv_count, row_has, rows,
+                                                                               1.f / temperature, row_a);
+        MECLIP_CUDA(cudaGetLastError());
+    }
+    VocabGrad vg{row_lse, row_a, nullptr, reinterpret_cast<const long long*>(teacher_tokens), token_scores, (int)per_row,
+                 teacher_probs, row_a, -1.f, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16};
+    return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
+                      lddt, ws, plan, status, s);
+}
+
+}  // extern "C"

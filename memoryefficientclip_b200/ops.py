@@ -716,3 +716,113 @@ def ring_grad(call: RingCall, kind, temperature, row_sum, col_sum_all, grad_out,
         if t_ is not None:
             t_.record_stream(call.copy_stream)
     return dx, dy
+
+
+# ---- softmax over a vocabulary ------------------------------------------------------------------------------
+def vocab_operands(x: torch.Tensor, table: torch.Tensor):
+    """(x, table) as the vocabulary passes read them: both fp16 if both inputs are, else both bf16 (fp32 inputs are
+    rounded, as everywhere in this package); rows of padded(d) columns, 16-byte aligned."""
+    if x.dtype == torch.float16 and table.dtype == torch.float16:
+        return _as_f16_operand(x), _as_f16_operand(table)
+    return as_operand(x), as_operand(table)
+
+
+def _as_f16_operand(x: torch.Tensor) -> torch.Tensor:
+    _check_matrix(x, "operand")
+    if x.shape[1] % 8 == 0 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    out = torch.zeros(x.shape[0], padded(x.shape[1]), dtype=torch.float16, device=x.device)
+    out[:, :x.shape[1]] = x
+    return out
+
+
+def _vocab_workspace(rows, vocab, top_k, device):
+    n = _lib.load().meclip_vocab_workspace_bytes(rows, vocab, top_k)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def token_log_probs(x, table, tokens, temperature, top_k=0, want_entropy=True, save=False, status=None):
+    """(log_probs, entropy, top_log_probs, top_tokens, row_lse, token_scores) of operands from vocab_operands; tokens
+    int64 [rows, per_row].  What is not asked for is None (meclip_token_log_probs)."""
+    rows, d = x.shape
+    vocab, per_row, dev = table.shape[0], tokens.shape[1], x.device
+
+    def new(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device=dev)
+
+    lp = new(rows, per_row)
+    entropy = new(rows) if want_entropy else None
+    top_lp, top = (new(rows, top_k), new(rows, top_k, dtype=torch.int64)) if top_k else (None, None)
+    lse, scores = (new(rows), new(rows, per_row)) if save else (None, None)
+    with _on_device(dev):
+        ws = _vocab_workspace(rows, vocab, top_k, dev)
+        _lib.check(_lib.load().meclip_token_log_probs(
+            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0),
+            float(temperature), tokens.data_ptr(), per_row, lp.data_ptr(), _ptr(entropy), top_k, _ptr(top_lp), _ptr(top),
+            _ptr(lse), _ptr(scores), ws.data_ptr(), ws.numel(), _ptr(status), _stream(x)))
+    return lp, entropy, top_lp, top, lse, scores
+
+
+class _VocabGrads:
+    """What both gradients share: bf16 operands beside fp16 ones, the outputs, the workspace."""
+
+    def __init__(self, x, table, need_dx, need_dtable, dx_dtype, dtable_dtype):
+        rows, d = x.shape
+        vocab, dev = table.shape[0], x.device
+        f16 = x.dtype == torch.float16
+        self.x16, self.t16 = (x, table) if f16 else (None, None)
+        # the contractions run on bf16 operands: a coefficient can be far below fp16's smallest number
+        self.x, self.t = (normalize_fwd(x, False)[0], normalize_fwd(table, False)[0]) if f16 else (x, table)
+        self.dx = torch.empty(rows, d, dtype=dx_dtype, device=dev) if need_dx else None
+        self.dt = torch.empty(vocab, d, dtype=dtable_dtype, device=dev) if need_dtable else None
+        n = _lib.load().meclip_vocab_grad_workspace_bytes(rows, vocab, d)
+        self.ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        self.head = (self.x.data_ptr(), self.t.data_ptr(), _ptr(self.x16), _ptr(self.t16), rows, vocab, d,
+                     self.x.stride(0), self.t.stride(0), x.stride(0) if f16 else 0, table.stride(0) if f16 else 0)
+        self.tail = (_ptr(self.dx), _MODE[dx_dtype], d, _ptr(self.dt), _MODE[dtable_dtype], d, self.ws.data_ptr(),
+                     self.ws.numel())
+
+
+def token_log_probs_grad(x, table, tokens, temperature, row_lse, entropy, token_scores, grad_log_probs, grad_entropy,
+                         dx_dtype, dtable_dtype, need_dx=True, need_dtable=True, status=None):
+    """(dx, dtable) for the operands of token_log_probs (meclip_token_log_probs_grad); dtypes fp32 or bf16."""
+    with _on_device(x.device):
+        g = _VocabGrads(x, table, need_dx, need_dtable, dx_dtype, dtable_dtype)
+        _lib.check(_lib.load().meclip_token_log_probs_grad(
+            *g.head, float(temperature), tokens.data_ptr(), tokens.shape[1], row_lse.data_ptr(), _ptr(entropy),
+            _ptr(token_scores), _ptr(grad_log_probs), _ptr(grad_entropy), *g.tail, _ptr(status), _stream(x)))
+    return g.dx, g.dt
+
+
+def distill_forward(x, table, teacher_tokens, teacher_logits, temperature, teacher_temperature, reduction, status=None):
+    """(result, saved): the loss of operands from vocab_operands, [rows] with reduction "none" and 0-dim otherwise, and
+    the tensors its gradient needs (meclip_distill)."""
+    rows, d = x.shape
+    vocab, per_row, dev = table.shape[0], teacher_tokens.shape[1], x.device
+    row_loss, row_has, lse = torch.empty(3, rows, dtype=torch.float32, device=dev).unbind(0)
+    scores, probs = torch.empty(2, rows, per_row, dtype=torch.float32, device=dev).unbind(0)
+    reduce = reduction != "none"
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduce else None
+    inv_count = torch.empty(1, dtype=torch.float32, device=dev) if reduce else None
+    with _on_device(dev):
+        ws = _vocab_workspace(rows, vocab, 0, dev)
+        _lib.check(_lib.load().meclip_distill(
+            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0),
+            float(temperature), teacher_tokens.data_ptr(), teacher_logits.data_ptr(), _DT[teacher_logits.dtype], per_row,
+            float(teacher_temperature), int(reduction == "mean"), row_loss.data_ptr(), row_has.data_ptr(), _ptr(loss),
+            _ptr(inv_count), lse.data_ptr(), scores.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), _ptr(status),
+            _stream(x)))
+    return (loss if reduce else row_loss), (lse, scores, probs, row_has, inv_count)
+
+
+def distill_backward(x, table, teacher_tokens, temperature, saved, grad_out, dx_dtype, dtable_dtype, need_dx=True,
+                     need_dtable=True, status=None):
+    """(dx, dtable) for the operands of distill_forward (meclip_distill_grad); grad_out fp32, one value or [rows]."""
+    lse, scores, probs, row_has, inv_count = saved
+    with _on_device(x.device):
+        g = _VocabGrads(x, table, need_dx, need_dtable, dx_dtype, dtable_dtype)
+        _lib.check(_lib.load().meclip_distill_grad(
+            *g.head, float(temperature), teacher_tokens.data_ptr(), teacher_tokens.shape[1], lse.data_ptr(),
+            scores.data_ptr(), probs.data_ptr(), row_has.data_ptr(), grad_out.data_ptr(), int(inv_count is None),
+            _ptr(inv_count), *g.tail, _ptr(status), _stream(x)))
+    return g.dx, g.dt

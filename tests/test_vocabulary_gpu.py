@@ -1,0 +1,339 @@
+"""Token log probabilities and distillation over a vocabulary against the 64-bit oracle (oracle/vocabulary.py, which
+derives the bounds from the roundings of the computation)."""
+import math
+
+import pytest
+import torch
+
+from oracle import vocabulary as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def _pair(n, v, d, dtype, seed, bump=8.0):
+    """Features that lean towards one row of the table each, and that row's index."""
+    g = torch.Generator().manual_seed(seed)
+    table = torch.randn(v, d, generator=g) / math.sqrt(d)
+    tokens = torch.randint(0, v, (n,), generator=g)
+    x = 2.0 * torch.randn(n, d, generator=g) + bump * table[tokens]
+    return x.to(dtype), table.to(dtype), tokens, g
+
+
+def _operands(x, table):
+    """What the kernels read of these inputs: fp16 pairs as they are, everything else as bf16."""
+    if x.dtype == table.dtype == torch.float16:
+        return x, table
+    return x.bfloat16(), table.bfloat16()
+
+
+def _inside(got, want, bound, what):
+    got = got.detach().double().cpu()
+    assert torch.isfinite(got).all(), what
+    worst = ((got - want).abs() / bound).max().item()
+    assert worst <= 1.0, f"{what}: {worst:.2f} of the bound"
+
+
+SHAPES = [            # rows, vocabulary, features
+    (1, 1, 8), (1, 33, 64), (1, 32768, 512), (3, 50, 100), (5, 257, 72), (127, 1000, 64), (128, 64, 128), (129, 4099, 512),
+    (300, 2049, 96), (297, 8191, 1152), (640, 777, 1024), (2000, 333, 30)]
+
+
+@pytest.mark.parametrize("n,v,d", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_scores_match_the_oracle(n, v, d, dtype):
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, d, dtype, n * 7 + v)
+    k = min(v, 7)
+    many = torch.randint(-2, v, (n, 5), generator=g)
+    many[:, 0] = tokens
+    xo, yo = _operands(x, table)
+    want = oracle.token_log_probs(xo, yo, many, 0.9, k)
+    got = token_log_probs(x.cuda(), table.cuda(), many.cuda(), temperature=0.9, top_k=k)
+    assert got.log_probs.shape == (n, 5) and got.top_tokens.dtype == torch.int64
+    _inside(got.log_probs, want["log_probs"], want["err_lp"][:, None], "log_probs")
+    _inside(got.entropy, want["entropy"], want["err_entropy"], "entropy")
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+    _inside(got.top_log_probs, want["top_log_probs"], want["err_lp"][:, None], "top_log_probs")
+    one = token_log_probs(x.cuda(), table.cuda(), tokens.int().cuda(), temperature=0.9)
+    assert one.log_probs.shape == (n,) and one.top_tokens is None
+    assert torch.equal(one.log_probs, got.log_probs[:, 0]) and torch.equal(one.entropy, got.entropy)
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 8, 31, 32])
+@pytest.mark.parametrize("n", [2, 400])
+def test_alternatives_that_are_close_or_equal(n, top_k):
+    """Best rows beside each other in one chunk of 32, repeated rows, and a row of zeros: ties go to the lower token."""
+    from memoryefficientclip_b200 import token_log_probs
+    v, d = 700, 64
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 5 + top_k, bump=0.0)
+    table[40:72] = (table[40] + 0.02 * torch.randn(32, d, generator=g).bfloat16())          # one direction, two chunks
+    table[300:340] = table[300]                                                             # equal rows
+    table[650:] = 0
+    x[0] = 0                                                                                # everything ties
+    x[1] = 6 * table[300]
+    if n > 2:
+        x[2:40] = 9 * table[40]
+        x[40:60] = -4 * table[100:120]
+    want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, top_k)
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=top_k)
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+    _inside(got.top_log_probs, want["top_log_probs"], want["err_lp"][:, None], "top_log_probs")
+
+
+def test_all_scores_low_and_far_apart():
+    """Scores of minus hundreds, and one row that holds all the probability."""
+    from memoryefficientclip_b200 import token_log_probs
+    g = torch.Generator().manual_seed(3)
+    table = (torch.randn(517, 64, generator=g) + 3.0).bfloat16()
+    x = (-3.0 + torch.randn(9, 64, generator=g)).bfloat16()
+    x[4] = 20 * table[11]
+    tokens = torch.full((9,), 11)
+    want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, 4)
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=4)
+    _inside(got.log_probs, want["log_probs"][:, 0], want["err_lp"], "log_probs")
+    _inside(got.entropy, want["entropy"], want["err_entropy"], "entropy")
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+
+
+def test_padding_and_tokens_behind_the_table():
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, _ = _pair(70, 300, 64, torch.bfloat16, 1)
+    tokens[3], tokens[5], tokens[8] = -1, 300, -100
+    x[9] = float("nan")
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=3)
+    lp = got.log_probs.cpu()
+    assert lp[3] == 0 and lp[8] == 0 and lp[5].isnan() and lp[9].isnan() and got.entropy[9].isnan()
+    keep = torch.tensor([i for i in range(70) if i not in (3, 5, 8, 9)])
+    want = oracle.token_log_probs(x[keep], table, tokens[keep][:, None], 1.0, 3)
+    _inside(lp[keep], want["log_probs"][:, 0], want["err_lp"], "the other rows")
+    assert torch.equal(got.top_tokens.cpu()[keep], want["top_tokens"])
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 40, 64), (5, 1000, 64), (130, 257, 100), (300, 4099, 512), (1100, 2051, 264),
+                                   (64, 9000, 96), (1500, 700, 1152)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_score_gradients(n, v, d, dtype):
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, d, dtype, n + v, bump=6.0)
+    many = torch.stack([tokens, torch.randint(-1, v, (n,), generator=g), tokens, torch.randint(-1, v, (n,), generator=g)], 1)
+    g_lp = torch.randn(n, 4, generator=g)
+    g_h = torch.randn(n, generator=g) * 0.3
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    got = token_log_probs(xg, yg, many.cuda(), temperature=1.3)
+    dx, dy = torch.autograd.grad([got.log_probs, got.entropy], [xg, yg], [g_lp.cuda(), g_h.cuda()])
+    assert dx.dtype == dtype and dy.dtype == dtype
+    xo, yo = _operands(x, table)
+    rounding = 2.0 ** -8 if dtype == torch.float16 else 0.0      # the contractions read bf16 operands
+    wx, wy, bx, by = oracle.token_log_probs_grad(xo, yo, many, 1.3, g_lp, g_h, (dtype, dtype), rounding)
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+
+
+def test_score_gradient_parts():
+    """Only log probabilities, only entropy, only one input, a frozen table; differences of the loss agree."""
+    from memoryefficientclip_b200 import token_log_probs
+    n, v, d = 40, 500, 64
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 11)
+    g_lp, g_h, zero = torch.randn(n, generator=g), torch.randn(n, generator=g), torch.zeros(n)
+    for a, b in ((g_lp, None), (None, g_h)):
+        xg, yg = x.cuda().requires_grad_(True), table.cuda()
+        out = token_log_probs(xg, yg, tokens.cuda())
+        out = out.log_probs if b is None else out.entropy
+        out.backward((a if b is None else b).cuda())
+        wx, _wy, bx, _by = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.0, (zero if a is None else a)[:, None],
+                                                       zero if b is None else b, (torch.bfloat16, torch.bfloat16))
+        _inside(xg.grad, wx, bx, "dx")
+    yg = table.cuda().requires_grad_(True)
+    token_log_probs(x.cuda(), yg, tokens.cuda()).log_probs.backward(g_lp.cuda())
+    _wx, wy, _bx, by = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.0, g_lp[:, None], zero,
+                                                   (torch.bfloat16, torch.bfloat16))
+    _inside(yg.grad, wy, by, "dtable")
+    # differences of the 64-bit sum along a direction against the oracle's gradient (which the kernels matched above)
+    def f(e):
+        r = oracle.token_log_probs(x.double() + e, table, tokens[:, None], 1.0)
+        return (r["log_probs"][:, 0] * g_lp.double()).sum() + (r["entropy"] * g_h.double()).sum()
+    wx, _, _, _ = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.0, g_lp[:, None], g_h, (torch.float64,) * 2)
+    way = torch.randn(n, d, generator=g).double()
+    slope = (f(1e-5 * way) - f(-1e-5 * way)) / 2e-5
+    assert abs(slope - (wx * way).sum()) <= 1e-6 * wx.norm() * way.norm()
+
+
+def _teacher(n, v, k, g, dtype=torch.float32):
+    t = torch.stack([torch.randperm(v, generator=g)[:k] if k <= v else torch.randint(0, v, (k,), generator=g)
+                     for _ in range(n)])
+    logits = (3 * torch.randn(n, k, generator=g)).to(dtype)
+    return t, logits
+
+
+@pytest.mark.parametrize("n,v,d,k", [(1, 9, 64, 1), (7, 300, 72, 5), (129, 4099, 512, 8), (310, 1000, 1152, 64),
+                                     (1200, 600, 128, 33), (33, 2000, 64, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_distillation(n, v, d, k, dtype, reduction):
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    x, table, _tokens, g = _pair(n, v, d, dtype, n + k)
+    t, logits = _teacher(n, v, k, g, torch.float32 if reduction == "mean" else dtype)
+    if n > 6:
+        t[1, k // 2:] = -1                       # short rows, with anything in the absent places
+        logits[1, k // 2:] = float("nan")
+        t[2] = -1                                # nothing left
+        logits[2] = float("inf")
+        logits[3] = float("-inf")                # named, but impossible: nothing left either
+        logits[4, :-1] = float("-inf")           # one entry left
+        logits[5, 0] = torch.finfo(logits.dtype).min
+    if k > 4:
+        t[0, 3] = t[0, 1]                        # the same token twice
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    mod = MemoryEfficientDistillLoss(0.8, normalized_inputs=True, teacher_temperature=1.7, reduction=reduction)
+    loss = mod(xg, yg, t.cuda(), logits.cuda())
+    xo, yo = _operands(x, table)
+    kl, has, err = oracle.distill(xo, yo, t, logits, 0.8, 1.7)
+    if reduction == "none":
+        go = torch.randn(n, generator=g)
+        weight = go
+        assert loss.shape == (n,)
+        _inside(loss, kl, err + 1e-30, "loss")
+    else:
+        go = torch.tensor(0.7)
+        count = has.sum().double() if reduction == "mean" else 1.0
+        weight = go.double() / count * torch.ones(n)
+        assert loss.shape == ()
+        _inside(loss, kl.sum() / count, err.sum() / count + 2 * oracle.ULP * kl.sum() / count, "loss")
+    dx, dy = torch.autograd.grad(loss, [xg, yg], go.cuda())
+    assert dx.dtype == dtype and dy.dtype == dtype
+    rounding = 2.0 ** -8 if dtype == torch.float16 else 0.0
+    wx, wy, bx, by = oracle.distill_grad(xo, yo, t, logits, 0.8, weight, (dtype, dtype), 1.7, rounding)
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+    if n > 6:
+        assert not dx[2:4].any()
+
+
+def test_distillation_without_any_teacher_entry():
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    x, table, _t, _g = _pair(20, 100, 64, torch.bfloat16, 2)
+    xg = x.cuda().requires_grad_(True)
+    loss = MemoryEfficientDistillLoss(1.0, True)(xg, table.cuda(), torch.full((20, 3), -1).cuda(), torch.zeros(20, 3).cuda())
+    loss.backward()
+    assert loss.item() == 0.0 and not xg.grad.any()
+    # a token behind the table is a mistake and shows
+    bad = MemoryEfficientDistillLoss(1.0, True)(xg, table.cuda(), torch.full((20, 3), 100).cuda(), torch.zeros(20, 3).cuda())
+    assert bad.isnan()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_of_two_towers(dtype):
+    """normalized_inputs=False: both sides are normalised inside; the gradients carry the Jacobian."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    n, d = 260, 96
+    g = torch.Generator().manual_seed(8)
+    img = torch.randn(n, d, generator=g).to(dtype)
+    txt = (img.float() + torch.randn(n, d, generator=g)).to(dtype)
+    t, logits = _teacher(n, n, 6, g)
+    t[:, 0] = torch.arange(n)
+    xg, yg = img.cuda().requires_grad_(True), txt.cuda().requires_grad_(True)
+    loss = MemoryEfficientDistillLoss(0.07)(xg, yg, t.cuda(), logits.cuda())
+    loss.backward()
+    a, b = img.double().requires_grad_(True), txt.double().requires_grad_(True)
+    z = torch.nn.functional.normalize(a, dim=1) @ torch.nn.functional.normalize(b, dim=1).T / 0.07
+    q = torch.softmax(logits.double(), 1)
+    ref = (torch.xlogy(q, q) - q * torch.log_softmax(z, 1).gather(1, t)).sum(1).mean()
+    ref.backward()
+    # the normalised operands are rounded to bf16 (2^-8 of each component; a cosine of 96 random roundings moves by
+    # 2^-8 sqrt(2 / 96 / 3) or so, over T): the package's usual bars for that
+    assert abs(loss.item() - ref.item()) <= 1e-3 * abs(ref.item())
+    for got, want in ((xg.grad, a.grad), (yg.grad, b.grad)):
+        got = got.double().cpu()
+        assert (got - want).norm() <= 1e-2 * want.norm()
+
+
+@pytest.mark.parametrize("make", ["strided", "offset", "transposed"])
+def test_layouts(make):
+    """Pitches, offsets and orders other than the plain ones."""
+    from memoryefficientclip_b200 import token_log_probs
+    n, v, d = 50, 333, 64
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 4)
+    if make == "strided":
+        xs = torch.zeros(n, d + 24, dtype=x.dtype).cuda()[:, :d].copy_(x)
+        ys = torch.zeros(2 * v, d, dtype=x.dtype).cuda()[::2].copy_(table)
+    elif make == "offset":
+        xs = torch.zeros(n * d + 3, dtype=x.dtype).cuda()[3:].view(n, d).copy_(x)
+        ys = torch.zeros(v, d + 5, dtype=x.dtype).cuda()[:, 5:].copy_(table)
+    else:
+        xs, ys = x.T.contiguous().cuda().T, table.T.contiguous().cuda().T
+    tk = torch.stack([tokens, tokens], 1).cuda()[:, 0]
+    plain = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=3)
+    got = token_log_probs(xs, ys, tk, top_k=3)
+    for a, b in zip(plain, got):
+        assert torch.equal(a, b)
+
+
+def test_many_row_blocks_and_panels():
+    """Rows over several coefficient blocks: the blocked backward puts every entry into its own panel."""
+    from memoryefficientclip_b200 import _lib, MemoryEfficientDistillLoss
+    n, v, d, k = 1300, 1500, 64, 9
+    x, table, _t, g = _pair(n, v, d, torch.bfloat16, 21)
+    t, logits = _teacher(n, v, k, g)
+    _lib.check(_lib.load().meclip_debug_set_blocking(256, 256 * 2 * 512))
+    try:
+        xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+        loss = MemoryEfficientDistillLoss(1.0, True)(xg, yg, t.cuda(), logits.cuda())
+        loss.backward()
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(_lib.load().meclip_debug_set_blocking(0, 0))
+    wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, 1.0, torch.full((n,), 1.0 / n), (torch.bfloat16,) * 2)
+    _inside(xg.grad, wx, bx, "dx")
+    _inside(yg.grad, wy, by, "dtable")
+
+
+def test_capture_streams_and_repeats():
+    """A captured step replays on new data; a side stream and repeats give the same bits."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss, token_log_probs
+    n, v, d, k = 1030, 2000, 256, 4
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 31)
+    t, logits = _teacher(n, v, k, g)
+    xg, yg, t, logits, tok = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True), t.cuda(), logits.cuda(), tokens.cuda()
+    mod = MemoryEfficientDistillLoss(1.0, True)
+
+    def step():
+        loss = mod(xg, yg, t, logits)
+        s = token_log_probs(xg, yg, tok, top_k=2)
+        dx, dy = torch.autograd.grad([loss, s.log_probs.sum(), s.entropy.sum()], [xg, yg])
+        return loss, s.log_probs, s.top_tokens, dx, dy
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            first = [o.detach().clone() for o in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, step()):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    x2, _, _, _ = _pair(n, v, d, torch.bfloat16, 32)
+    with torch.no_grad():
+        xg.copy_(x2)
+    graph.replay()
+    torch.cuda.synchronize()
+    replayed = [o.detach().clone() for o in out]
+    for a, b in zip(replayed, step()):
+        assert torch.equal(a, b)
+
+
+def test_entry_points_stay_inside_their_outputs():
+    """Rows behind the last one keep what was in them."""
+    from memoryefficientclip_b200 import ops
+    n, v, d = 37, 515, 64
+    x, table, tokens, _ = _pair(n, v, d, torch.bfloat16, 6)
+    guard = torch.full((n + 8, d), 7.0, dtype=torch.bfloat16, device="cuda")
+    guard[:n] = x.cuda()
+    with torch.no_grad():
+        a = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda()[:, None], 1.0, 2)
+        guard[n:] = float("nan")
+        b = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda()[:, None], 1.0, 2)
+    for p, q in zip(a[:4], b[:4]):
+        assert torch.equal(p, q)
+    ops.check_status()
