@@ -529,6 +529,21 @@ int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* 
                         int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes, int* status, void* stream);
 
 /*
+ * Rows of a table [vocab, d] (dtype: MECLIP_F32, MECLIP_BF16 or MECLIP_F16; any d >= 1, pitch and alignment) by token,
+ * and the table's gradient.  tokens: int64 [n], n may be 0.  The reference has no such operators.
+ *   meclip_embed       out[i] = scale * table[tokens[i]], rounded once; a negative token gives zeros, one behind the
+ *                      table NaN
+ *   meclip_embed_grad  dtable[v] = scale * sum over i with tokens[i] = v of grad[i], summed in fp32 in an order that
+ *                      depends on the tokens alone (no floating-point atomics); every row of dtable is written.  Tokens
+ *                      outside the table take no part.  workspace: meclip_embed_grad_workspace_bytes, 256-byte aligned.
+ */
+int meclip_embed(const int64_t* tokens, int64_t n, const void* table, int dtype, int64_t vocab, int64_t d, int64_t ldt,
+                 float scale, void* out, int64_t ldo, void* stream);
+size_t meclip_embed_grad_workspace_bytes(int64_t n, int64_t vocab, int64_t d);
+int meclip_embed_grad(const int64_t* tokens, int64_t n, const void* grad, int dtype, int64_t vocab, int64_t d, int64_t ldg,
+                      float scale, void* dtable, int64_t ldd, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Test hook: C (m x n, fp32, ldc) = A * B^T-style contraction through the same
  * tcgen05 mainloop the loss kernels use.  a_mn_major == 0: A is m x k row-major
  * (K contiguous); 1: A is stored k x m row-major (M contiguous).  Same for B

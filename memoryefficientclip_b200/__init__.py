@@ -7,6 +7,7 @@ raises if the library has not been built (there is no other implementation).
 """
 from .clip_loss import (MemoryEfficientCLIPLoss, MemoryEfficientCLIPLossNormed, StableMemoryEfficientCLIPLoss,
                         StableMemoryEfficientCLIPLossNormed)
+from .embedding import embed_tokens
 from .lit_loss import (MemoryEfficientLiTLoss, MemoryEfficientLiTLossNormed, StableMemoryEfficientLiTLoss,
                        StableMemoryEfficientLiTLossNormed)
 from .siglip_loss import MemoryEfficientSigLIPLoss, MemoryEfficientSigLIPLossFn
@@ -14,6 +15,7 @@ from .vocabulary import MemoryEfficientDistillLoss, MemoryEfficientDistillLossFn
 
 __all__ = [
     "MemoryEfficientDistillLoss", "MemoryEfficientDistillLossFn", "TokenLogProbs", "token_log_probs",
+    "embed_tokens",
     "MemoryEfficientSigLIPLoss", "MemoryEfficientSigLIPLossFn",
     "MemoryEfficientCLIPLoss", "MemoryEfficientCLIPLossNormed", "StableMemoryEfficientCLIPLoss",
     "StableMemoryEfficientCLIPLossNormed", "MemoryEfficientLiTLoss", "MemoryEfficientLiTLossNormed",

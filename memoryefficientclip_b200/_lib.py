@@ -121,6 +121,11 @@ SIGNATURES = {
                                     c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                     c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
                                     c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64,
+                             c_void_p]),
+    "meclip_embed_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "meclip_embed_grad": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64,
+                                  c_void_p, c_size_t, c_void_p]),
     "meclip_debug_gemm": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int64, c_int64, c_int64,
                                   c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
 }

@@ -2352,3 +2352,4 @@ int meclip_debug_gemm(const void* a_bf16, int64_t lda, int a_mn_major, const voi
 }  // extern "C"
 
 #include "vocab_abi.cuh"
+#include "embedding.cuh"

@@ -826,3 +826,28 @@ def distill_backward(x, table, teacher_tokens, temperature, saved, grad_out, dx_
             scores.data_ptr(), probs.data_ptr(), row_has.data_ptr(), grad_out.data_ptr(), int(inv_count is None),
             _ptr(inv_count), *g.tail, _ptr(status), _stream(x)))
     return g.dx, g.dt
+
+
+def embed(tokens: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
+    """scale * table[tokens] for int64 tokens [n] (meclip_embed)."""
+    n, (vocab, d) = tokens.shape[0], table.shape
+    tokens = tokens.contiguous()
+    out = torch.empty(n, d, dtype=table.dtype, device=table.device)
+    with _on_device(table.device):
+        _lib.check(_lib.load().meclip_embed(tokens.data_ptr(), n, table.data_ptr(), _DT[table.dtype], vocab, d,
+                                            max(table.stride(0), d), scale, out.data_ptr(), d, _stream(table)))
+    return out
+
+
+def embed_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
+    """[vocab, d] gradient of the table from grad [n, d] (meclip_embed_grad)."""
+    n, d = grad.shape
+    tokens, grad = tokens.contiguous(), grad if grad.stride(1) == 1 and grad.stride(0) >= d else grad.contiguous()
+    dt = torch.empty(vocab, d, dtype=grad.dtype, device=grad.device)
+    with _on_device(grad.device):
+        lib = _lib.load()
+        ws = torch.empty(lib.meclip_embed_grad_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=grad.device)
+        _lib.check(lib.meclip_embed_grad(tokens.data_ptr(), n, grad.data_ptr(), _DT[grad.dtype], vocab, d,
+                                         max(grad.stride(0), d), scale, dt.data_ptr(), d, ws.data_ptr(), ws.numel(),
+                                         _stream(grad)))
+    return dt
