@@ -3,10 +3,13 @@
 //   out_i = s table[t_i]          dtable_v = s sum_{i: t_i = v} g_i
 //
 // Both move each byte once; the sum has to be the same from run to run, so there are no floating-point atomics: the
-// positions are sorted by token (stable radix sort of (token, position) pairs), every row of the table then knows its
-// run of positions and adds their gradients in ascending order.  Runs of common tokens are thousands of positions long:
-// aligned chunks of 32, and of 1024, positions that lie inside one run are added up beforehand, each by its own warp,
-// so that the longest row of the table adds at most 4 x 31 + n / 1024 vectors instead of n.
+// positions are sorted by token (stable radix sort of (token, position) pairs) and added in ascending order.
+//   sort     few blocks, bound by latency; further blocks of the same launches clear the table's gradient meanwhile
+//   chunks   one warp per 32 sorted places and 256 columns adds what it finds; a run of one token that lies inside the
+//            chunk is a finished row, a run that goes on leaves a partial sum: in `head` if it fills the chunk from its
+//            first place on, in `tail` otherwise.  Every warp has the same work, however common a token is.
+//   level 2  32 chunks that lie inside one run, added up (the run of a common token is thousands of places long)
+//   join     runs over several chunks: tail + heads, whole level-2 sums in place of 32 heads
 #pragma once
 #include <cuda_fp16.h>
 
@@ -16,7 +19,7 @@ static constexpr int EMB_SORT_THREADS = 1024;
 static constexpr int EMB_MAX_BITS = 10;              // bits per sorting pass: 1024 bins, one per thread
 static constexpr int EMB_MAX_BLOCKS = 128;           // blocks of a sorting pass
 static constexpr long long EMB_ONE_BLOCK = 4096;     // up to here one block does all passes in one launch
-static constexpr int EMB_CHUNK = 32;                 // positions per first-level sum, first-level sums per second-level one
+static constexpr int EMB_CHUNK = 32;                 // places per chunk, chunks per second-level sum
 
 // Eight elements from column c on; vec: 16-byte accesses are possible and d is a multiple of 8.
 template <typename T>
@@ -62,8 +65,30 @@ struct EmbSort {
     uint32_t *keys_out, *pos_out;
     long long n, vocab, per_block;    // per_block: a multiple of EMB_SORT_THREADS
     int shift, bits, blocks;
-    uint32_t* hist;                   // [1 << bits][blocks]
+    uint32_t* hist;                   // [blocks][1 << bits]
+    // the gradient's rows, cleared by the blocks behind `blocks`: part `part` of `parts` of them per launch
+    void* out;
+    long long ldo;
+    int d, elt, flat, part, parts;
 };
+
+// flat: the rows follow one another and start on 16 bytes, as one run of vocab * d * elt bytes (a multiple of 16)
+__device__ __forceinline__ void emb_clear(const EmbSort& s) {
+    const long long who = (long long)(blockIdx.x - s.blocks) * EMB_SORT_THREADS + threadIdx.x;
+    const long long step = (long long)(gridDim.x - s.blocks) * EMB_SORT_THREADS;
+    const long long all = s.flat ? s.vocab * s.d * s.elt / 16 : s.vocab * s.d;
+    const long long first = all * s.part / s.parts, last = all * (s.part + 1) / s.parts;
+    if (s.flat) {
+        uint4* o = reinterpret_cast<uint4*>(s.out);
+        for (long long i = first + who; i < last; i += step) o[i] = make_uint4(0, 0, 0, 0);
+    } else {
+        for (long long i = first + who; i < last; i += step) {
+            const long long at = i / s.d * s.ldo + i % s.d;
+            if (s.elt == 4) reinterpret_cast<uint32_t*>(s.out)[at] = 0;
+            else            reinterpret_cast<uint16_t*>(s.out)[at] = 0;
+        }
+    }
+}
 
 __device__ __forceinline__ uint32_t emb_key(const EmbSort& s, long long i) {
     if (s.tokens == nullptr) return s.keys_in[i];
@@ -74,6 +99,7 @@ __device__ __forceinline__ uint32_t emb_key(const EmbSort& s, long long i) {
 // How often each digit occurs in the block's share.
 __global__ void __launch_bounds__(EMB_SORT_THREADS) emb_hist_kernel(const __grid_constant__ EmbSort s) {
     __shared__ uint32_t h[1 << EMB_MAX_BITS];
+    if ((int)blockIdx.x >= s.blocks) { emb_clear(s); return; }
     const int bins = 1 << s.bits;
     for (int b = threadIdx.x; b < bins; b += EMB_SORT_THREADS) h[b] = 0;
     __syncthreads();
@@ -81,7 +107,7 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) emb_hist_kernel(const __grid
     for (long long i = first + threadIdx.x; i < last; i += EMB_SORT_THREADS)
         atomicAdd(&h[(emb_key(s, i) >> s.shift) & (bins - 1)], 1u);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += EMB_SORT_THREADS) s.hist[(long long)b * s.blocks + blockIdx.x] = h[b];
+    for (int b = threadIdx.x; b < bins; b += EMB_SORT_THREADS) s.hist[((long long)blockIdx.x << s.bits) + b] = h[b];
 }
 
 // Exclusive prefix sum over the block's 1024 threads.
@@ -152,12 +178,13 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) emb_scatter_kernel(const __g
     extern __shared__ __align__(16) uint8_t emb_smem[];
     __shared__ uint32_t offs[1 << EMB_MAX_BITS];
     __shared__ uint32_t warp_sums[32];
+    if ((int)blockIdx.x >= s.blocks) { emb_clear(s); return; }
     uint32_t total = 0, before = 0;
     if ((int)threadIdx.x < (1 << s.bits)) {
-        const uint32_t* h = s.hist + (long long)threadIdx.x * s.blocks;
-#pragma unroll 8
+        const uint32_t* h = s.hist + threadIdx.x;
+#pragma unroll 16
         for (int b = 0; b < s.blocks; ++b) {
-            const uint32_t c = h[b];
+            const uint32_t c = h[(long long)b << s.bits];
             total += c;
             before += b < (int)blockIdx.x ? c : 0u;
         }
@@ -175,6 +202,7 @@ emb_sort_small_kernel(EmbSort s, int passes, uint32_t* keys_a, uint32_t* pos_a, 
     extern __shared__ __align__(16) uint8_t emb_smem[];
     __shared__ uint32_t offs[1 << EMB_MAX_BITS];
     __shared__ uint32_t warp_sums[32];
+    if (blockIdx.x > 0) { emb_clear(s); return; }            // s.blocks is 1 here
     const int bins = 1 << s.bits;
     for (int p = 0; p < passes; ++p) {
         s.shift = p * s.bits;
@@ -194,136 +222,175 @@ emb_sort_small_kernel(EmbSort s, int passes, uint32_t* keys_a, uint32_t* pos_a, 
     }
 }
 
-// start[v] = first sorted place whose key is >= v, for v = 0 .. vocab (start[vocab]: how many tokens are in the table).
-__global__ void __launch_bounds__(256)
-emb_start_kernel(const uint32_t* __restrict__ keys, long long n, long long vocab, uint32_t* __restrict__ start) {
-    const long long v = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (v > vocab) return;
-    long long lo = 0, hi = n;
+// A warp works on 256 columns, eight per lane, and keeps several rows' loads in flight: the sums are bound by memory
+// latency unless enough of it overlaps.
+static constexpr int EMB_COLS = 256;
+
+// Eight elements of a row as loaded, widened when they are added.
+template <typename T, bool VEC> struct EmbRaw;
+template <typename T> struct EmbRaw<T, true> {
+    static constexpr int U = sizeof(T) == 4 ? 4 : 8;
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, int, int) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ void add(float (&acc)[8]) const {
+        float v[8];
+        load8(reinterpret_cast<const T*>(w), v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += v[i];
+    }
+};
+template <typename T> struct EmbRaw<T, false> {
+    static constexpr int U = 4;
+    T w[8];
+    __device__ __forceinline__ void load(const T* p, int c, int d) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < d) w[i] = p[i];
+    }
+    __device__ __forceinline__ void add(float (&acc)[8]) const {     // columns past d hold anything and are not stored
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += load1(&w[i]);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void emb_finish(float (&acc)[8], float scale, T* out, long long ldo, long long v, int c, int d, int vec_out) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= scale;
+    store8_any(out + v * ldo, c, d, vec_out, acc);
+}
+
+struct EmbLevels { float *head, *tail, *level2; long long dp; };     // dp: pitch of the sums, a multiple of 8
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(ROW_KERNEL_THREADS, 3)
+emb_chunk_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, long long n, long long vocab,
+                 const T* __restrict__ g, long long ldg, int d, EmbLevels lv, float scale, int vec_out, T* __restrict__ out,
+                 long long ldo, long long chunks, int pieces) {
+    constexpr int U = EmbRaw<T, VEC>::U;
+    const long long unit = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
+    const long long b = unit / pieces;
+    const int lane = threadIdx.x & 31, c = (int)(unit % pieces) * EMB_COLS + lane * 8;
+    if (b >= chunks) return;
+    const long long first = b * EMB_CHUNK;
+    const int m = (int)min((long long)EMB_CHUNK, n - first);
+    const uint32_t none = 0xffffffffu;                               // no key: keys are at most vocab < 2^31
+    const uint32_t key = lane < m ? keys[first + lane] : none;
+    const uint32_t mine = lane < m ? pos[first + lane] : 0u;
+    const uint32_t before = first > 0 ? keys[first - 1] : none;
+    const uint32_t after = first + m < n ? keys[first + m] : none;
+    uint32_t cur = __shfl_sync(0xffffffffu, key, 0);
+    bool from_start = true;                                          // the current run began at the chunk's first place
+    float acc[8] = {};
+    for (int e0 = 0; e0 < m; e0 += U) {
+        EmbRaw<T, VEC> raw[U];
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            const long long row = __shfl_sync(0xffffffffu, mine, (e0 + r) & 31);
+            if (e0 + r < m && c < d) raw[r].load(g + row * ldg + c, c, d);
+        }
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            if (e0 + r >= m) break;
+            const uint32_t k = __shfl_sync(0xffffffffu, key, (e0 + r) & 31);
+            if (k != cur) {                                          // the same for the whole warp
+                if ((long long)cur < vocab) {
+                    if (from_start && before == cur) { if (c < lv.dp) store8(lv.head + b * lv.dp + c, acc); }
+                    else if (c < d) emb_finish(acc, scale, out, ldo, cur, c, d, vec_out);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+                cur = k;
+                from_start = false;
+            }
+            if (c < d) raw[r].add(acc);
+        }
+        if ((long long)cur >= vocab) return;                         // padding sorts last: nothing follows
+    }
+    if (from_start ? (before == cur || after == cur) : after == cur) {
+        if (c < lv.dp) store8((from_start ? lv.head : lv.tail) + b * lv.dp + c, acc);
+    } else if (c < d) {
+        emb_finish(acc, scale, out, ldo, cur, c, d, vec_out);
+    }
+}
+
+// acc += rows [a, b) of fp32 sums
+__device__ __forceinline__ void emb_add_sums(const float* __restrict__ sums, long long dp, long long a, long long b, int c,
+                                             float (&acc)[8]) {
+    constexpr int U = 8;
+    if (c >= dp) return;
+    for (long long r0 = a; r0 < b; r0 += U) {
+        float v[U][8];
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[r][i] = 0.f;
+            if (r0 + r < b) load8(sums + (r0 + r) * dp + c, v[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < U; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += v[r][i];
+    }
+}
+
+__global__ void __launch_bounds__(ROW_KERNEL_THREADS)
+emb_level2_kernel(const uint32_t* __restrict__ keys, long long vocab, EmbLevels lv, long long groups, int pieces) {
+    const long long unit = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
+    const long long b = unit / pieces;
+    const int lane = threadIdx.x & 31, c = (int)(unit % pieces) * EMB_COLS + lane * 8;
+    if (b >= groups) return;
+    const long long size = EMB_CHUNK * EMB_CHUNK;
+    const uint32_t k = keys[b * size];
+    if ((long long)k >= vocab || k != keys[(b + 1) * size - 1]) return;
+    float acc[8] = {};
+    emb_add_sums(lv.head, lv.dp, b * EMB_CHUNK, (b + 1) * EMB_CHUNK, c, acc);
+    if (c < lv.dp) store8(lv.level2 + b * lv.dp + c, acc);
+}
+
+// One warp per chunk and 256 columns: the run that starts in it and goes on behind it.
+template <typename T>
+__global__ void __launch_bounds__(ROW_KERNEL_THREADS)
+emb_join_kernel(const uint32_t* __restrict__ keys, long long n, long long vocab, int d, EmbLevels lv, float scale, int vec_out,
+                T* __restrict__ out, long long ldo, long long chunks, int pieces) {
+    const long long unit = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
+    const long long b = unit / pieces;
+    const int lane = threadIdx.x & 31, c = (int)(unit % pieces) * EMB_COLS + lane * 8;
+    if (b + 1 >= chunks) return;
+    const long long first = b * EMB_CHUNK, next = first + EMB_CHUNK;
+    const uint32_t k = keys[next - 1];
+    if ((long long)k >= vocab || keys[next] != k) return;
+    const bool from_start = keys[first] == k;
+    if (from_start && first > 0 && keys[first - 1] == k) return;     // it started earlier
+    long long lo = next, hi = n;                                     // where the run ends
     while (lo < hi) {
         const long long mid = (lo + hi) >> 1;
-        if (keys[mid] < (uint32_t)v) lo = mid + 1;
+        if (keys[mid] <= k) lo = mid + 1;
         else hi = mid;
     }
-    start[v] = (uint32_t)lo;
-}
-
-static constexpr int EMB_COLS = 4;                   // 256-column pieces a warp keeps in registers
-
-// acc += the gradients at the sorted places [a, b)
-template <typename T>
-__device__ __forceinline__ void emb_add_places(const T* __restrict__ g, long long ldg, const uint32_t* __restrict__ pos,
-                                               long long a, long long b, int c0, int d, int vec, int lane,
-                                               float (&acc)[EMB_COLS][8]) {
-    for (long long at = a; at < b; at += 32) {
-        const int m = (int)min(32ll, b - at);
-        const uint32_t mine = lane < m ? pos[at + lane] : 0u;
-#pragma unroll 2
-        for (int e = 0; e < m; ++e) {
-            const T* row = g + (long long)__shfl_sync(0xffffffffu, mine, e) * ldg;
-#pragma unroll
-            for (int k = 0; k < EMB_COLS; ++k) {
-                const int c = c0 + k * 256 + lane * 8;
-                if (c < d) {
-                    float v[8];
-                    load8_any(row, c, d, vec, v);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[k][i] += v[i];
-                }
-            }
-        }
+    const long long h0 = from_start ? b : b + 1, h1 = (lo + EMB_CHUNK - 1) / EMB_CHUNK;      // heads [h0, h1)
+    // whole groups of 32 full chunks: [g0, g1) lies inside the run
+    const long long g0 = (h0 + EMB_CHUNK - 1) / EMB_CHUNK, g1 = lo / (EMB_CHUNK * EMB_CHUNK);
+    float acc[8] = {};
+    if (!from_start) emb_add_sums(lv.tail, lv.dp, b, b + 1, c, acc);
+    if (lv.level2 != nullptr && g1 > g0) {
+        emb_add_sums(lv.head, lv.dp, h0, g0 * EMB_CHUNK, c, acc);
+        emb_add_sums(lv.level2, lv.dp, g0, g1, c, acc);
+        emb_add_sums(lv.head, lv.dp, g1 * EMB_CHUNK, h1, c, acc);
+    } else {
+        emb_add_sums(lv.head, lv.dp, h0, h1, c, acc);
     }
-}
-// acc += rows [a, b) of fp32 sums with a pitch of dp (a multiple of 8)
-__device__ __forceinline__ void emb_add_sums(const float* __restrict__ sums, long long dp, long long a, long long b, int c0,
-                                             int lane, float (&acc)[EMB_COLS][8]) {
-#pragma unroll 2
-    for (long long r = a; r < b; ++r) {
-#pragma unroll
-        for (int k = 0; k < EMB_COLS; ++k) {
-            const int c = c0 + k * 256 + lane * 8;
-            if (c < dp) {
-                float v[8];
-                load8(sums + r * dp + c, v);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[k][i] += v[i];
-            }
-        }
-    }
-}
-
-// First and second level: chunk b of 32 (1024) sorted places, if all of them belong to one row of the table.
-template <typename T, bool SECOND>
-__global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-emb_chunk_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos, const uint32_t* __restrict__ start,
-                 long long vocab, const T* __restrict__ g, long long ldg, int d, int vec, const float* __restrict__ level1,
-                 float* __restrict__ sums, long long dp, long long chunks) {
-    const long long b = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (b >= chunks) return;
-    const long long size = SECOND ? EMB_CHUNK * EMB_CHUNK : EMB_CHUNK;
-    if ((b + 1) * size > (long long)start[vocab] || keys[b * size] != keys[(b + 1) * size - 1]) return;
-    for (int c0 = 0; c0 < d; c0 += 256 * EMB_COLS) {
-        float acc[EMB_COLS][8] = {};
-        if (SECOND) emb_add_sums(level1, dp, b * EMB_CHUNK, (b + 1) * EMB_CHUNK, c0, lane, acc);
-        else        emb_add_places<T>(g, ldg, pos, b * EMB_CHUNK, (b + 1) * EMB_CHUNK, c0, d, vec, lane, acc);
-#pragma unroll
-        for (int k = 0; k < EMB_COLS; ++k) {
-            const int c = c0 + k * 256 + lane * 8;
-            if (c < dp) store8(sums + b * dp + c, acc[k]);
-        }
-    }
-}
-
-// One warp per row of the table: its run of sorted places, whole chunks from the sums of the levels before; rows that
-// no token names are written as zeros, so the gradient needs no clearing pass.
-template <typename T>
-__global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-emb_rows_kernel(const uint32_t* __restrict__ pos, const uint32_t* __restrict__ start, long long vocab,
-                const T* __restrict__ g, long long ldg, int d, int vec, const float* __restrict__ level1,
-                const float* __restrict__ level2, long long dp, float scale, int vec_out, T* __restrict__ out, long long ldo) {
-    const long long v = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (v >= vocab) return;
-    const long long a = start != nullptr ? start[v] : 0, b = start != nullptr ? start[v + 1] : 0;
-    // whole chunks [f1, l1) and among them whole second-level ones [f2, l2)
-    long long f1 = (a + EMB_CHUNK - 1) / EMB_CHUNK, l1 = b / EMB_CHUNK;
-    const bool use1 = level1 != nullptr && l1 > f1;
-    long long f2 = (f1 + EMB_CHUNK - 1) / EMB_CHUNK, l2 = l1 / EMB_CHUNK;
-    const bool use2 = use1 && level2 != nullptr && l2 > f2;
-    T* row = out + v * ldo;
-    for (int c0 = 0; c0 < d; c0 += 256 * EMB_COLS) {
-        float acc[EMB_COLS][8] = {};
-        if (!use1) {
-            emb_add_places<T>(g, ldg, pos, a, b, c0, d, vec, lane, acc);
-        } else {
-            emb_add_places<T>(g, ldg, pos, a, f1 * EMB_CHUNK, c0, d, vec, lane, acc);
-            if (use2) {
-                emb_add_sums(level1, dp, f1, f2 * EMB_CHUNK, c0, lane, acc);
-                emb_add_sums(level2, dp, f2, l2, c0, lane, acc);
-                emb_add_sums(level1, dp, l2 * EMB_CHUNK, l1, c0, lane, acc);
-            } else {
-                emb_add_sums(level1, dp, f1, l1, c0, lane, acc);
-            }
-            emb_add_places<T>(g, ldg, pos, l1 * EMB_CHUNK, b, c0, d, vec, lane, acc);
-        }
-#pragma unroll
-        for (int k = 0; k < EMB_COLS; ++k) {
-            const int c = c0 + k * 256 + lane * 8;
-            if (c < d) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc[k][i] *= scale;
-                store8_any(row, c, d, vec_out, acc[k]);
-            }
-        }
-    }
+    if (c < d) emb_finish(acc, scale, out, ldo, k, c, d, vec_out);
 }
 
 struct EmbPlan {
     int bits, passes, blocks;
-    long long per_block, chunks1, chunks2, dp;
-    size_t list_bytes, hist_bytes, start_bytes, level1_bytes, level2_bytes;
-    size_t total() const { return 4 * list_bytes + hist_bytes + start_bytes + level1_bytes + level2_bytes; }
+    long long per_block, chunks, groups, dp;
+    size_t list_bytes, hist_bytes, chunk_bytes, group_bytes;
+    size_t total() const { return 4 * list_bytes + hist_bytes + 2 * chunk_bytes + group_bytes; }
 };
 static EmbPlan plan_embed_grad(long long n, long long vocab, long long d) {
     EmbPlan p;
@@ -336,14 +403,13 @@ static EmbPlan plan_embed_grad(long long n, long long vocab, long long d) {
     p.per_block = (per < 1 ? 1 : per) * EMB_SORT_THREADS;
     p.blocks = (int)((n + p.per_block - 1) / p.per_block);
     p.dp = (d + 7) / 8 * 8;
-    // the levels only pay when a run can be longer than a warp adds in the time of another launch
-    p.chunks1 = n >= 512 ? n / EMB_CHUNK : 0;
-    p.chunks2 = n >= 8192 ? n / (EMB_CHUNK * EMB_CHUNK) : 0;
+    p.chunks = (n + EMB_CHUNK - 1) / EMB_CHUNK;
+    // a warp adds 64 heads in about the time that another launch takes
+    p.groups = n >= 2 * EMB_CHUNK * EMB_CHUNK ? n / (EMB_CHUNK * EMB_CHUNK) : 0;
     p.list_bytes = round_up((size_t)n * 4, 256);
     p.hist_bytes = round_up((size_t)(p.blocks < 1 ? 1 : p.blocks) * 4 << p.bits, 256);
-    p.start_bytes = round_up((size_t)(vocab + 1) * 4, 256);
-    p.level1_bytes = round_up((size_t)p.chunks1 * p.dp * 4, 256);
-    p.level2_bytes = round_up((size_t)p.chunks2 * p.dp * 4, 256);
+    p.chunk_bytes = round_up((size_t)p.chunks * p.dp * 4, 256);
+    p.group_bytes = round_up((size_t)p.groups * p.dp * 4, 256);
     return p;
 }
 
@@ -353,42 +419,48 @@ static int embed_grad_t(const long long* tokens, long long n, const T* g, long l
     constexpr int elt = (int)sizeof(T), wpb = ROW_KERNEL_THREADS / 32;
     const int vec = d % 8 == 0 && aligned16(g) && (ldg * elt) % 16 == 0;
     const int vec_out = d % 8 == 0 && aligned16(out) && (ldo * elt) % 16 == 0;
+    const int pieces = (d + EMB_COLS - 1) / EMB_COLS;
+    if ((pl.chunks * pieces + wpb - 1) / wpb > 0x7fffffffLL) return fail(MECLIP_EINVAL, "embed_grad: too much for one launch");
     uint32_t* keys[2] = {reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + pl.list_bytes)};
     uint32_t* pos[2] = {reinterpret_cast<uint32_t*>(ws + 2 * pl.list_bytes), reinterpret_cast<uint32_t*>(ws + 3 * pl.list_bytes)};
-    uint32_t* hist = reinterpret_cast<uint32_t*>(ws + 4 * pl.list_bytes);
-    uint32_t* start = reinterpret_cast<uint32_t*>(ws + 4 * pl.list_bytes + pl.hist_bytes);
-    float* level1 = reinterpret_cast<float*>(ws + 4 * pl.list_bytes + pl.hist_bytes + pl.start_bytes);
-    float* level2 = reinterpret_cast<float*>(ws + 4 * pl.list_bytes + pl.hist_bytes + pl.start_bytes + pl.level1_bytes);
-    const unsigned row_grid = (unsigned)((vocab + wpb - 1) / wpb);
-    if (n == 0) {
-        ScopedTiming timing(s, TAG_ROW, (double)vocab * d * elt);
-        emb_rows_kernel<T><<<row_grid, ROW_KERNEL_THREADS, 0, s>>>(nullptr, nullptr, vocab, g, ldg, d, 0, nullptr, nullptr,
-                                                                  pl.dp, scale, vec_out, out, ldo);
-        MECLIP_CUDA(cudaGetLastError());
-        return MECLIP_OK;
-    }
+    uint8_t* rest = ws + 4 * pl.list_bytes;
+    EmbLevels lv;
+    lv.head = reinterpret_cast<float*>(rest + pl.hist_bytes);
+    lv.tail = reinterpret_cast<float*>(rest + pl.hist_bytes + pl.chunk_bytes);
+    lv.level2 = pl.groups > 0 ? reinterpret_cast<float*>(rest + pl.hist_bytes + 2 * pl.chunk_bytes) : nullptr;
+    lv.dp = pl.dp;
     EmbSort st{};
     st.tokens = tokens; st.n = n; st.vocab = vocab; st.per_block = pl.per_block; st.bits = pl.bits; st.blocks = pl.blocks;
-    st.hist = hist;
+    st.hist = reinterpret_cast<uint32_t*>(rest);
+    st.out = out; st.ldo = ldo; st.d = d; st.elt = elt;
+    st.flat = ldo == d && aligned16(out) && ((size_t)vocab * d * elt) % 16 == 0;
     const int smem = (EMB_SORT_THREADS / 32) * 2 << pl.bits;
+    const int clear_blocks = sm_count();       // beside the sort's blocks: two blocks of 1024 threads fit an SM
     if (n <= EMB_ONE_BLOCK) {
+        st.blocks = 1;
+        st.parts = 1;
         MECLIP_CUDA(cudaFuncSetAttribute(emb_sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        ScopedTiming timing(s, TAG_ROW, 16.0 * (double)n * pl.passes);
-        emb_sort_small_kernel<<<1, EMB_SORT_THREADS, smem, s>>>(st, pl.passes, keys[0], pos[0], keys[1], pos[1]);
+        ScopedTiming timing(s, TAG_ROW, 16.0 * (double)n * pl.passes + (double)vocab * d * elt);
+        emb_sort_small_kernel<<<1 + 2 * clear_blocks, EMB_SORT_THREADS, smem, s>>>(st, pl.passes, keys[0], pos[0], keys[1], pos[1]);
         MECLIP_CUDA(cudaGetLastError());
+        if (n == 0) return MECLIP_OK;
     } else {
         MECLIP_CUDA(cudaFuncSetAttribute(emb_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        st.parts = 2 * pl.passes;
+        const double clear_bytes = (double)vocab * d * elt / st.parts;
         for (int p = 0; p < pl.passes; ++p) {
             st.shift = p * pl.bits;
             st.keys_out = keys[p & 1];
             st.pos_out = pos[p & 1];
+            st.part = 2 * p;
             {
-                ScopedTiming timing(s, TAG_ROW, (p == 0 ? 8.0 : 4.0) * (double)n);
-                emb_hist_kernel<<<pl.blocks, EMB_SORT_THREADS, 0, s>>>(st);
+                ScopedTiming timing(s, TAG_ROW, (p == 0 ? 8.0 : 4.0) * (double)n + clear_bytes);
+                emb_hist_kernel<<<pl.blocks + clear_blocks, EMB_SORT_THREADS, 0, s>>>(st);
             }
+            st.part = 2 * p + 1;
             {
-                ScopedTiming timing(s, TAG_ROW, 16.0 * (double)n);
-                emb_scatter_kernel<<<pl.blocks, EMB_SORT_THREADS, smem, s>>>(st);
+                ScopedTiming timing(s, TAG_ROW, 16.0 * (double)n + clear_bytes);
+                emb_scatter_kernel<<<pl.blocks + clear_blocks, EMB_SORT_THREADS, smem, s>>>(st);
             }
             MECLIP_CUDA(cudaGetLastError());
             st.tokens = nullptr;
@@ -398,24 +470,21 @@ static int embed_grad_t(const long long* tokens, long long n, const T* g, long l
     }
     const uint32_t* ks = keys[(pl.passes - 1) & 1];
     const uint32_t* ps = pos[(pl.passes - 1) & 1];
+    const unsigned grid = (unsigned)((pl.chunks * pieces + wpb - 1) / wpb);
     {
-        ScopedTiming timing(s, TAG_ROW, 4.0 * (double)vocab);
-        emb_start_kernel<<<(unsigned)((vocab + 256) / 256), 256, 0, s>>>(ks, n, vocab, start);
+        ScopedTiming timing(s, TAG_ROW, (double)n * d * elt);
+        if (vec) emb_chunk_kernel<T, true><<<grid, ROW_KERNEL_THREADS, 0, s>>>(ks, ps, n, vocab, g, ldg, d, lv, scale, vec_out, out, ldo, pl.chunks, pieces);
+        else     emb_chunk_kernel<T, false><<<grid, ROW_KERNEL_THREADS, 0, s>>>(ks, ps, n, vocab, g, ldg, d, lv, scale, vec_out, out, ldo, pl.chunks, pieces);
+        MECLIP_CUDA(cudaGetLastError());
     }
-    if (pl.chunks1 > 0) {
+    if (pl.chunks < 2) return MECLIP_OK;
+    if (pl.groups > 0) {
         ScopedTiming timing(s, TAG_ROW, 0.0);
-        emb_chunk_kernel<T, false><<<(unsigned)((pl.chunks1 + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
-            ks, ps, start, vocab, g, ldg, d, vec, nullptr, level1, pl.dp, pl.chunks1);
+        emb_level2_kernel<<<(unsigned)((pl.groups * pieces + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(ks, vocab, lv, pl.groups, pieces);
+        MECLIP_CUDA(cudaGetLastError());
     }
-    if (pl.chunks2 > 0) {
-        ScopedTiming timing(s, TAG_ROW, 0.0);
-        emb_chunk_kernel<T, true><<<(unsigned)((pl.chunks2 + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
-            ks, ps, start, vocab, g, ldg, d, vec, level1, level2, pl.dp, pl.chunks2);
-    }
-    MECLIP_CUDA(cudaGetLastError());
-    ScopedTiming timing(s, TAG_ROW, ((double)vocab + (double)n) * d * elt);
-    emb_rows_kernel<T><<<row_grid, ROW_KERNEL_THREADS, 0, s>>>(ps, start, vocab, g, ldg, d, vec, pl.chunks1 > 0 ? level1 : nullptr,
-                                                              pl.chunks2 > 0 ? level2 : nullptr, pl.dp, scale, vec_out, out, ldo);
+    ScopedTiming timing(s, TAG_ROW, 0.0);
+    emb_join_kernel<T><<<grid, ROW_KERNEL_THREADS, 0, s>>>(ks, n, vocab, d, lv, scale, vec_out, out, ldo, pl.chunks, pieces);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }

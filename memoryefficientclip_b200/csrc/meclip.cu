@@ -615,9 +615,13 @@ static int sm_count() {
 // call yet (PyTorch's autograd thread on its first backward).
 static int check_device() {
     static int supported[64] = {0};   // 0 unknown, 1 ok, -1 unsupported
+    static thread_local int bound = -1;
     int dev = 0;
     MECLIP_CUDA(cudaGetDevice(&dev));
-    MECLIP_CUDA(cudaSetDevice(dev));
+    if (dev != bound) {
+        MECLIP_CUDA(cudaSetDevice(dev));
+        bound = dev;
+    }
     if (dev < 0 || dev >= 64) return fail(MECLIP_EUNSUPPORTED, "device index %d out of range", dev);
     if (supported[dev] == 0) {
         int major = 0;
@@ -710,11 +714,25 @@ struct Operand {
     bool f16 = false;
 };
 
+// Lets a kernel use all of an SM's shared memory: once per kernel and device (`done`: one bit per device).
+template <class Kernel>
+static int allow_all_smem(Kernel kern, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    MECLIP_CUDA(cudaGetDevice(&dev));
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
+    if ((done.load(std::memory_order_relaxed) & bit) != 0) return MECLIP_OK;
+    MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return MECLIP_OK;
+}
+
 template <int EPI, bool A_MN, bool B_MN>
 static int launch_gemm_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const GemmParams& p,
                          size_t smem_bytes, cudaStream_t stream) {
     auto kern = umma_gemm_kernel<EPI, A_MN, B_MN>;
-    MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    static std::atomic<unsigned long long> smem_allowed{0};
+    const int rc = allow_all_smem(kern, smem_allowed);
+    if (rc) return rc;
     const int tiles = p.num_m_tiles * p.num_n_tiles;
     const int units = (tiles + p.strip_len - 1) / p.strip_len;
     const int grid = units < sm_count() ? units : sm_count();
@@ -729,7 +747,9 @@ static int launch_pair_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
                          size_t smem_bytes, cudaStream_t stream, const CUtensorMap* td_opt = nullptr, double flops = -1.0) {
     auto kern = umma_gemm_pair_kernel<EPI, A_MODE, TF32>;
     const CUtensorMap& td = td_opt != nullptr ? *td_opt : tb;
-    MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    static std::atomic<unsigned long long> smem_allowed{0};
+    const int rc = allow_all_smem(kern, smem_allowed);
+    if (rc) return rc;
     // how many CTA pairs the device can hold at once (an SM without a free neighbour cannot host one)
     static int max_clusters[64] = {0};
     int dev = 0;
@@ -783,7 +803,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     if (m < 1 || n < 1 || k < 1) return fail(MECLIP_EINVAL, "gemm extents must be >= 1 (m=%lld n=%lld k=%lld)", m, n, k);
     if (m > 0x7fffffffLL || n > 0x7fffffffLL || k > 0x7fffffffLL) return fail(MECLIP_EINVAL, "gemm extent exceeds 2^31");
     const bool wide = bn > MAX_BN;      // two MMAs per K step, CTA-pair kernel, plain contraction only
-    if (bn < 32 || bn > 2 * MAX_BN || bn % 32 != 0 || ((b.mn_major || epi_is_coef(epi) || epi == EPI_STATS || wide) && bn % 64 != 0) ||
+    if (bn < 32 || bn > 2 * MAX_BN || bn % 32 != 0 || ((b.mn_major || epi_is_coef(epi) || wide) && bn % 64 != 0) ||
         (wide && (epi != EPI_OUT || b.mn_major || g_trace_buf != nullptr || pair_mode() == 0)))
         return fail(MECLIP_EINVAL, "tile width %d not supported", bn);
     const bool f32 = a.f32;
@@ -1625,7 +1645,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 t_tag = TAG_COEF;
                 if (vg != nullptr) {
                     p.sigmoid = 0;
-                    p.fmul = 1.4426950408889634f / temperature;
+                    p.fmul = vg->tile_fmul;
                     p.row_lse = vg->row_lse + r0;
                     p.row_a = vg->row_a + r0;
                     p.row_b = vg->row_b != nullptr ? vg->row_b + r0 : nullptr;
@@ -1633,7 +1653,8 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                         a = Operand{vg->x_f16 + r0 * vg->ldx_f16, vg->ldx_f16, false, 0, false, true};
                         b = Operand{vg->y_f16 + c0 * vg->ldy_f16, vg->ldy_f16, false, 0, false, true};
                     }
-                    rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
+                    // 256-column tiles beyond one row tile: only those run on CTA pairs
+                    rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                     if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, cols, gpanel[gb], plan.row_block, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);

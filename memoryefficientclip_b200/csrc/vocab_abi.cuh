@@ -7,17 +7,18 @@ namespace meclip {
 // workspace however many rows there are, and 16384 rows fill the GPU many times over.
 static constexpr long long VOCAB_ROW_BLOCK = 16384;
 
-// Column-tile width of the statistics pass: the fewest waves x width over the SMs, wider on ties.  The narrower tiles
-// only win when few rows leave SMs without a tile (see pick_contraction_bn for what a narrow tile costs per column).
+// Column-tile width of the statistics pass.  Up to 128 rows there is one row tile, the pass is bound by reading the table,
+// and what counts is that every SM gets the same share of it: the fewest waves x width, in steps of 32 columns (V = 32768:
+// 147 tiles of 224 columns instead of 128 of 256).  With more rows 256: a narrower tile costs more per column than a
+// fuller last wave brings, and only 256 columns run on CTA pairs.
 static int pick_stats_bn(long long rows, long long vocab) {
-    const int cand[4] = {256, 192, 128, 64};
-    const double cost_per_col[4] = {1.0, 1.07, 1.2, 1.5};
+    if (rows > BM) return vocab >= 256 ? 256 : (int)((vocab + 63) / 64 * 64);
     int best = 256;
-    double best_t = 0.0;
-    for (int i = 0; i < 4; ++i) {
-        const long long tiles = ((rows + BM - 1) / BM) * ((vocab + cand[i] - 1) / cand[i]);
-        const double t = (double)((tiles + sm_count() - 1) / sm_count()) * cand[i] * cost_per_col[i];
-        if (i == 0 || t < best_t) { best_t = t; best = cand[i]; }
+    long long best_t = -1;
+    for (int bn = 256; bn >= 64; bn -= 32) {
+        const long long tiles = (vocab + bn - 1) / bn;
+        const long long t = (tiles + sm_count() - 1) / sm_count() * (bn + 8);      // + 8: a tile's own overhead
+        if (best_t < 0 || t < best_t) { best_t = t; best = bn; }
     }
     return best;
 }
@@ -40,20 +41,20 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
     return v;
 }
 
-template <int G, bool DISTILL>
+template <int G, bool DISTILL, bool TOP>
 static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     const int per_block = VOCAB_THREADS / G;
-    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap, G / 32);
+    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap);
     const unsigned grid = (unsigned)((p.rows + per_block - 1) / per_block);
     const double bytes = (double)p.rows * (16.0 * p.slots + (p.top_k > 0 ? 8.0 * p.chunks : 0.0) +
                                            2.0 * p.d * (1 + p.k + p.top_k));
     ScopedTiming timing(s, TAG_ROW, bytes);
     if (f16) {
-        auto kern = vocab_rows_kernel<G, __half, DISTILL>;
+        auto kern = vocab_rows_kernel<G, __half, DISTILL, TOP>;
         if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
     } else {
-        auto kern = vocab_rows_kernel<G, __nv_bfloat16, DISTILL>;
+        auto kern = vocab_rows_kernel<G, __nv_bfloat16, DISTILL, TOP>;
         if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
     }
@@ -76,7 +77,7 @@ static int check_vocab(const char* what, const void* x, const void* table, int d
 
 // Statistics pass and row kernel over blocks of rows.  `r` holds the per-row arguments of the whole problem.
 template <bool DISTILL>
-static int vocab_forward(VocabRows r, int dtype, void* workspace, size_t workspace_bytes, int* status, cudaStream_t s) {
+static int vocab_forward(VocabRows r, float temperature, int dtype, void* workspace, size_t workspace_bytes, int* status, cudaStream_t s) {
     int rc = check_device();
     if (rc) return rc;
     const long long rows = r.rows;
@@ -111,7 +112,7 @@ static int vocab_forward(VocabRows r, int dtype, void* workspace, size_t workspa
         }
         GemmParams p;
         std::memset(&p, 0, sizeof(p));
-        p.fmul = r.fmul;
+        p.fmul = vocab_tile_fmul(temperature, r.d);
         p.stats = const_cast<float4*>(r.stats);
         p.stats_ld = r.stats_ld;
         p.chunk_max = const_cast<float*>(r.chunk_max);
@@ -124,8 +125,9 @@ static int vocab_forward(VocabRows r, int dtype, void* workspace, size_t workspa
         rc = launch_gemm(EPI_STATS, a, t, b.rows, r.vocab, r.d, plan.bn, p, s);
         if (rc) return rc;
         // a few rows: a block each; many: a warp each
-        if (b.rows <= 2 * sm_count()) rc = launch_vocab_rows_t<256, DISTILL>(b, f16, s);
-        else                          rc = launch_vocab_rows_t<32, DISTILL>(b, f16, s);
+        const bool few = b.rows <= 2 * sm_count();
+        if (!DISTILL && r.top_k > 0) rc = few ? launch_vocab_rows_t<256, false, true>(b, f16, s) : launch_vocab_rows_t<32, false, true>(b, f16, s);
+        else                         rc = few ? launch_vocab_rows_t<256, DISTILL, false>(b, f16, s) : launch_vocab_rows_t<32, DISTILL, false>(b, f16, s);
         if (rc) return rc;
     }
     return MECLIP_OK;
@@ -195,7 +197,7 @@ int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t 
     r.tokens = reinterpret_cast<const long long*>(tokens); r.k = (int)per_row;
     r.row_lse = row_lse; r.entropy = entropy; r.token_s2 = token_scores; r.log_probs = log_probs;
     r.top_k = top_k; r.top_log_probs = top_log_probs; r.top_tokens = reinterpret_cast<long long*>(top_tokens);
-    return vocab_forward<false>(r, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
+    return vocab_forward<false>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
 }
 
 int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16,
@@ -227,7 +229,7 @@ int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, cons
     }
     VocabGrad vg{row_lse, row_a, row_b, reinterpret_cast<const long long*>(tokens), token_scores, (int)per_row,
                  grad_log_probs, nullptr, 1.f / temperature, (const __nv_bfloat16*)x_f16, ldx_f16,
-                 (const __nv_bfloat16*)table_f16, ldt_f16};
+                 (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
     return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
                       lddt, ws, plan, status, s);
 }
@@ -255,7 +257,7 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
     r.row_lse = row_lse; r.token_s2 = token_scores;
     r.teacher_logits = teacher_logits; r.teacher_dtype = teacher_dtype; r.inv_teacher_t = 1.f / teacher_temperature;
     r.teacher_probs = teacher_probs; r.row_loss = row_loss; r.row_has = row_has;
-    rc = vocab_forward<true>(r, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
+    rc = vocab_forward<true>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
     if (rc || loss == nullptr) return rc;
     ScopedTiming timing((cudaStream_t)stream, TAG_ROW, 8.0 * (double)rows);
     distill_reduce_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_loss, row_has, rows, mean, loss, inv_count);
@@ -287,7 +289,7 @@ int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* 
         MECLIP_CUDA(cudaGetLastError());
     }
     VocabGrad vg{row_lse, row_a, nullptr, reinterpret_cast<const long long*>(teacher_tokens), token_scores, (int)per_row,
-                 teacher_probs, row_a, -1.f, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16};
+                 teacher_probs, row_a, -1.f, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
     return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
                       lddt, ws, plan, status, s);
 }

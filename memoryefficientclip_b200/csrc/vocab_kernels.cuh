@@ -14,7 +14,6 @@ namespace meclip {
 static constexpr int VOCAB_THREADS = 256;
 static constexpr int VOCAB_MAX_ENTRIES = 256;      // given tokens or teacher entries of one row
 static constexpr int VOCAB_MAX_TOP = 32;           // top alternatives: one per lane
-static constexpr int VOCAB_EXTRA = 32;             // chunks beyond the K best that rounding may have kept apart
 
 // Entries (given tokens, teacher entries) of a backward, and the row factors of the dense part.
 struct VocabGrad {
@@ -31,7 +30,19 @@ struct VocabGrad {
     long long ldx_f16;
     const __nv_bfloat16* y_f16;
     long long ldy_f16;
+    float tile_fmul;
 };
+
+// The tensor cores cut what does not fit into an fp32 accumulator instead of rounding it, once every 16 products, so a
+// score comes out too small in magnitude, on average by a part of the partial sums it ran through.  For a score that
+// grows steadily that is 0.09 ulp-of-itself per step (half of the 2^-24 .. 2^-25 that a cut at one guard bit costs, over
+// a triangle); for the scores that carry a softmax 0.11 to 0.13 was measured (D = 64 .. 1152).  The tile passes scale by
+// that much more, which leaves their log-sum-exp unbiased: its error at D = 1024, scores up to 20, fell from 1e-5 to
+// what VOCAB_KAPPA leaves.
+static constexpr double VOCAB_KAPPA = 0.12;
+static float vocab_tile_fmul(float temperature, long long d) {
+    return (float)(1.4426950408889634 / (double)temperature * (1.0 + VOCAB_KAPPA * (double)((d + 15) / 16) * 0x1p-23));
+}
 
 struct VocabRows {
     const float4* stats; int slots; long long stats_ld;
@@ -55,44 +66,46 @@ struct VocabRows {
 __device__ __forceinline__ void half8(const __nv_bfloat16* p, float (&v)[8]) { load8(p, v); }
 __device__ __forceinline__ void half8(const __half* p, float (&v)[8]) { load8(p, v); }
 
-// Dot products of x with four rows of the table by one warp, in fp32: the products are exact (8 or 11 bits each),
-// a lane adds d / 32 of them.  Operand rows are padded to 16 bytes and 8 elements.
-template <typename T>
-__device__ __forceinline__ void warp_dot4(const T* __restrict__ x, const T* const (&y)[4], int d, int lane, float (&out)[4]) {
-    float acc[4][2] = {};
-    for (int c = lane * 8; c < d; c += 256) {
-        float xv[8], yv[4][8];
-        half8(x + c, xv);
+// Dot products of x with four rows of the table by one warp.  The products are exact in fp32 (8 or 11 bits each); a
+// lane adds d / 32 of them, in fp32 for a score and in fp64 to tell two close alternatives apart.  Two column steps are
+// loaded before the first is used: the rows come from anywhere in the table, so what counts is loads in flight.  Operand
+// rows are padded to 16 bytes and 8 elements.
+template <typename T, typename A>
+__device__ __forceinline__ void dot_step(const uint4& xr, const uint4 (&yr)[4], A (&acc)[4][2]) {
+    float xv[8];
+    half8(reinterpret_cast<const T*>(&xr), xv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) half8(y[r] + c, yv[r]);
+    for (int r = 0; r < 4; ++r) {
+        float yv[8];
+        half8(reinterpret_cast<const T*>(&yr[r]), yv);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[r][i & 1] = fmaf(xv[i], yv[r][i], acc[r][i & 1]);
+        for (int i = 0; i < 8; ++i) {
+            if (sizeof(A) == 4) acc[r][i & 1] = fmaf(xv[i], yv[i], acc[r][i & 1]);
+            else                acc[r][i & 1] += (A)(xv[i] * yv[i]);
+        }
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) out[r] = warp_sum(acc[r][0] + acc[r][1]);
 }
-
-// The same in fp64: which of two close alternatives comes first has to be right, and products are exact in fp32.
-template <typename T>
-__device__ __forceinline__ void warp_dot4(const T* __restrict__ x, const T* const (&y)[4], int d, int lane, double (&out)[4]) {
-    double acc[4] = {};
-    for (int c = lane * 8; c < d; c += 256) {
-        float xv[8], yv[4][8];
-        half8(x + c, xv);
+template <typename T, typename A>
+__device__ __forceinline__ void warp_dot4(const T* __restrict__ x, const T* const (&y)[4], int d, int lane, A (&out)[4]) {
+    A acc[4][2] = {};
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int c = lane * 8; c < d; c += 512) {
+        const bool more = c + 256 < d;
+        const uint4 xa = *reinterpret_cast<const uint4*>(x + c), xb = more ? *reinterpret_cast<const uint4*>(x + c + 256) : zero;
+        uint4 ya[4], yb[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) half8(y[r] + c, yv[r]);
+        for (int r = 0; r < 4; ++r) ya[r] = __ldg(reinterpret_cast<const uint4*>(y[r] + c));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[r] += (double)(xv[i] * yv[r][i]);
+        for (int r = 0; r < 4; ++r) yb[r] = more ? __ldg(reinterpret_cast<const uint4*>(y[r] + c + 256)) : zero;
+        dot_step<T, A>(xa, ya, acc);
+        dot_step<T, A>(xb, yb, acc);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
+        A v = acc[r][0] + acc[r][1];
 #pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) acc[r] += __shfl_xor_sync(0xffffffffu, acc[r], o);
-        out[r] = acc[r];
+        for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        out[r] = v;
     }
 }
 
@@ -116,10 +129,10 @@ template <int G> __device__ __forceinline__ void group_sync() {
 }
 
 // Shared memory of one row, in bytes (a multiple of 16).
-__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int list_cap, int warps) {
+__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int list_cap) {
     return 64 * 8 +                                                       // reductions across warps
            (k * 4 + 15) / 16 * 16 +                                       // scores of the entries
-           (top_k > 0 ? (VOCAB_MAX_TOP + VOCAB_EXTRA) * 4 + list_cap * 4 + warps * VOCAB_MAX_TOP * 16 : 0);
+           (top_k > 0 ? 160 * 12 + 64 * 8 + 16 + list_cap * 4 : 0);       // see RowTopShared
 }
 
 // Sum / maximum over the G threads of a row, the same on all of them.
@@ -140,255 +153,471 @@ __device__ __forceinline__ float group_reduce(float v, float* red, int gt) {
     return v;
 }
 
-// The top alternatives of one row.  The K largest elements lie in the K chunks that come first by (maximum, index),
-// and the tile pass knows each chunk's best column and its second best value up to rounding.  So: take chunks in that
-// order until the K-th is found, go on while rounding could still matter, score in fp64 the best column of each taken
-// chunk - all 32 columns where the second best might be among the K too - and sort.  By warp 0 up to the list of
-// columns, by all warps of the row from there.
+// The top alternatives.  The K largest elements of a row lie in the K chunks that come first by (maximum, index), and the
+// tile pass knows each chunk's best column and, from below, the distance of its second best.  Per row:
+//  (a) every lane keeps the two largest maxima of its share of the chunks; the K-th largest of those 64 is a bound that
+//      K chunks reach, and few others do;
+//  (b) the chunks that reach it, less what rounding may hide, are collected: K and a few;
+//  (c) their K-th largest value decides which of them stay, and where the second best may be among the K too (one row
+//      in fifty at K = 8 of 32768) all 32 columns are looked at.
+// From here on the warps of a block share the work of its rows, since a row that looks at 40 columns would otherwise keep
+// one warp busy long after the others are done:
+//  (d) the columns are scored from the operands in fp32, those that come closer to another than that is exact in fp64;
+//  (e) every column counts who comes before it.
+// Crowds (many equal scores: a row of zeros, repeated table rows) do not fit (b) and are taken chunk by chunk instead.
+static constexpr int VOCAB_LIST = 64;              // chunks collected in (b)
+static constexpr int VOCAB_RANK = 160;             // columns ranked in (e), five per lane: K chunks of which four as a whole
+
+struct RowTopShared {
+    double* z;                                     // [VOCAB_RANK] scores
+    int* chunk;                                    // [VOCAB_LIST] collected, then the chunks taken
+    float* value;                                  // [VOCAB_LIST]
+    int* again;                                    // [VOCAB_RANK] which columns to score again
+    int* count;                                    // [4]: chunks collected, columns, columns again
+    int* list;                                     // [list_cap] columns to score
+};
+
+// Serial form of (a) to (c) for crowds, by one warp: takes the first chunks one after the other.  Returns how many.
+__device__ __forceinline__ int row_top_crowd(const VocabRows& p, const float* cmax, float slack, int lane, int* sel, float& theta) {
+    auto rescan = [&](float tv, int tc, float& bv, int& bc) {
+        bv = -INFINITY; bc = 0x7fffffff;
+#pragma unroll 8
+        for (int c = lane; c < p.chunks; c += 32) {
+            const float v = cmax[c];
+            if (comes_first(tv, tc, v, c) && comes_first(v, c, bv, bc)) { bv = v; bc = c; }
+        }
+    };
+    float bv; int bc;
+    rescan(INFINITY, -1, bv, bc);
+    int taken = 0;
+    theta = -INFINITY;
+    while (taken < VOCAB_LIST) {
+        float v = bv; int c = bc;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            const float ov = __shfl_xor_sync(0xffffffffu, v, o);
+            const int oc = __shfl_xor_sync(0xffffffffu, c, o);
+            if (comes_first(ov, oc, v, c)) { v = ov; c = oc; }
+        }
+        if (c == 0x7fffffff) break;                                      // no chunk left
+        if (taken >= p.top_k && !(v >= theta - slack)) break;
+        if (lane == 0) sel[taken] = c;
+        if (bc == c) rescan(v, c, bv, bc);
+        if (++taken == p.top_k) theta = v;
+    }
+    __syncwarp();
+    return taken;
+}
+
+__device__ __forceinline__ RowTopShared row_top_shared(uint8_t* smem) {
+    RowTopShared sh;
+    sh.z = reinterpret_cast<double*>(smem);
+    sh.chunk = reinterpret_cast<int*>(sh.z + VOCAB_RANK);
+    sh.value = reinterpret_cast<float*>(sh.chunk + VOCAB_LIST);
+    sh.again = reinterpret_cast<int*>(sh.value + VOCAB_LIST);
+    sh.count = sh.again + VOCAB_RANK;
+    sh.list = sh.count + 4;
+    return sh;
+}
+
+// 32 values, one per lane, sorted in descending order.
+__device__ __forceinline__ float warp_sort_desc(float v, int lane) {
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            const float o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool keep_max = ((lane & j) == 0) == ((lane & k) == 0);
+            v = keep_max ? fmaxf(v, o) : fminf(v, o);
+        }
+    return v;
+}
+
+__device__ __forceinline__ void row_top_write(const VocabRows& p, long long row, int at, double z, long long j, float m, float log2l) {
+    p.top_tokens[row * p.top_k + at] = j;
+    p.top_log_probs[row * p.top_k + at] = (float)((z * (double)p.fmul - (double)m - (double)log2l) * 0.6931471805599453);
+}
+
+// (a) to (c): leaves the columns in sh.list, their number in sh.count[1] (0 after a crowd, which is finished here) and
+// 2 |x| |y| in red[3].
 template <int G, typename T>
-__device__ __forceinline__ void row_top(const VocabRows& p, long long row, int gt, uint8_t* smem, float m, float log2l) {
+__device__ __forceinline__ void row_top_select(const VocabRows& p, long long row, int gt, const RowTopShared& sh, float m,
+                                               float log2l, float* red) {
     constexpr int W = G / 32;
     const int lane = gt & 31, w = gt >> 5;
-    int* sel = reinterpret_cast<int*>(smem);                                 // taken chunks
-    int* list = sel + VOCAB_MAX_TOP + VOCAB_EXTRA;                           // columns to score
-    double* lz_s = reinterpret_cast<double*>(list + p.list_cap);
-    long long* lj_s = reinterpret_cast<long long*>(lz_s + W * VOCAB_MAX_TOP);
-    __shared__ int count_s[VOCAB_THREADS / G];
-    int* count_p = &count_s[threadIdx.x / G];
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
     const T* y = reinterpret_cast<const T*>(p.y);
     const float* cmax = p.chunk_max + row * p.chunk_ld;
     const uint32_t* csec = p.chunk_second + row * p.chunk_ld;
     const int K = p.top_k;
-    if (w == 0) {
-        // each lane owns every 32nd chunk and keeps its first one that has not been taken
-        auto rescan = [&](float tv, int tc, float& bv, int& bc) {
-            bv = -INFINITY; bc = 0x7fffffff;
+
+    // (a)
+    float b1 = -INFINITY, b2 = -INFINITY; int bc = 0x7fffffff;
 #pragma unroll 8
-            for (int c = lane; c < p.chunks; c += 32) {
-                const float v = cmax[c];
-                if (comes_first(tv, tc, v, c) && comes_first(v, c, bv, bc)) { bv = v; bc = c; }
-            }
-        };
-        float bv; int bc;
-        rescan(INFINITY, -1, bv, bc);
-        int taken = 0;
-        float theta = -INFINITY, eps = 0.f;
-        while (taken < K + VOCAB_EXTRA) {
-            float v = bv; int c = bc;
-#pragma unroll
-            for (int o = 16; o >= 1; o >>= 1) {
-                const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-                const int oc = __shfl_xor_sync(0xffffffffu, c, o);
-                if (comes_first(ov, oc, v, c)) { v = ov; c = oc; }
-            }
-            if (c == 0x7fffffff) break;                                      // no chunk left
-            if (taken >= K && !(v >= theta - 2.f * eps)) break;
-            if (lane == 0) sel[taken] = c;
-            if (bc == c) rescan(v, c, bv, bc);
-            if (++taken == K) {
-                theta = v;
-                // how far the tile pass may be off: d / 16 accumulation steps that each drop up to an ulp of a partial
-                // sum, which stays below |x| |y|; the best alternative's |y| stands for those of its rivals, doubled
-                __syncwarp();
-                const long long c1 = (long long)sel[0] * 32 + (csec[sel[0]] & 31u);
-                const T* const rows4[4] = {y + c1 * p.ldy, x, x, x};
-                float yy = 0.f, xx = 0.f;
-                for (int i = lane * 8; i < p.d; i += 256) {
-                    float a[8], b[8];
-                    half8(rows4[0] + i, a);
-                    half8(rows4[1] + i, b);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) { yy = fmaf(a[j], a[j], yy); xx = fmaf(b[j], b[j], xx); }
-                }
-                yy = warp_sum(yy); xx = warp_sum(xx);
-                eps = 2.f * 1.1920929e-7f * ((float)p.d * 0.0625f + 4.f) * p.fmul * sqrtf(yy) * sqrtf(xx) +
-                      4.f * 1.1920929e-7f * fabsf(theta);
-            }
-        }
-        if (taken < K) theta = -INFINITY;
-        __syncwarp();
-        int n = 0;
-        for (int i = 0; i < taken; ++i) {
-            const int c = sel[i];
-            const uint32_t sec = csec[c];
-            const bool whole = cmax[c] - __uint_as_float(sec & ~31u) >= theta - 2.f * eps;   // false for "no second" (NaN)
-            if (n + (whole ? 32 : 1) > p.list_cap) break;
-            if (whole) {
-                const int left = (int)min(32ll, p.vocab - (long long)c * 32);
-                if (lane < left) list[n + lane] = c * 32 + lane;
-                n += left;
-            } else {
-                if (lane == 0) list[n] = c * 32 + (int)(sec & 31u);
-                ++n;
-            }
-        }
-        if (lane == 0) *count_p = n;
-    }
-    group_sync<G>();
-    const int n = *count_p;
-    double lz = -INFINITY;
-    long long lj = 0x7fffffffffffffffll;
-    for (int i = w * 4; i < n; i += W * 4) {
-        const T* r4[4];
-        long long j4[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) { j4[r] = list[min(i + r, n - 1)]; r4[r] = y + j4[r] * p.ldy; }
-        double z[4];
-        const T* const rr[4] = {r4[0], r4[1], r4[2], r4[3]};
-        warp_dot4<T>(x, rr, p.d, lane, z);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (i + r < n) list_insert(lz, lj, z[r], j4[r], lane);
+    for (int c = gt; c < p.chunks; c += G) {
+        const float v = cmax[c];
+        b2 = fmaxf(b2, fminf(b1, v));
+        if (v > b1) { b1 = v; bc = c; }
     }
     if (W > 1) {
-        lz_s[w * VOCAB_MAX_TOP + lane] = lz;
-        lj_s[w * VOCAB_MAX_TOP + lane] = lj;
-        group_sync<G>();
-        if (w == 0)
-            for (int i = 1; i < W; ++i)
-                for (int e = 0; e < K; ++e) {
-                    const long long j = lj_s[i * VOCAB_MAX_TOP + e];
-                    if (j == 0x7fffffffffffffffll) break;
-                    list_insert(lz, lj, lz_s[i * VOCAB_MAX_TOP + e], j, lane);
+        int* red_c = reinterpret_cast<int*>(sh.z);          // 128 words each, free until (b) and (d)
+        float* red_2 = reinterpret_cast<float*>(sh.chunk);  // (chunk and value)
+#pragma unroll
+        for (int k = W / 2; k >= 1; k >>= 1) {              // the upper half of the warps hands its maxima to the lower
+            __syncthreads();
+            if (w >= k && w < 2 * k) {
+                red[(w - k) * 32 + lane] = b1; red_2[(w - k) * 32 + lane] = b2; red_c[(w - k) * 32 + lane] = bc;
+            }
+            __syncthreads();
+            if (w < k) {
+                const float o1 = red[w * 32 + lane], o2 = red_2[w * 32 + lane];
+                b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+                if (o1 > b1) { b1 = o1; bc = red_c[w * 32 + lane]; }
+            }
+        }
+        __syncthreads();
+    }
+    float floor_v = -INFINITY, slack = 0.f, size = 0.f;
+    if (w == 0) {
+        // The K-th largest of two sorted lists: i from the first and K - i from the second, for the best split.
+        const float s1 = warp_sort_desc(b1, lane), s2 = warp_sort_desc(b2, lane);
+        const float other = __shfl_sync(0xffffffffu, s2, max(K - lane - 2, 0));
+        float bound = lane >= K ? -INFINITY : lane == K - 1 ? s1 : fminf(s1, other);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+        const float best = __shfl_sync(0xffffffffu, s1, 0);
+        const unsigned who = __ballot_sync(0xffffffffu, b1 == best && bc != 0x7fffffff);
+        if (who != 0) {
+            // How far the tile pass may be off: d / 16 accumulation steps that each drop up to an ulp of a partial sum,
+            // which stays below |x| |y|; the best alternative's |y| stands for those of its rivals, doubled.
+            const int c0 = __shfl_sync(0xffffffffu, bc, __ffs(who) - 1);
+            const T* y0 = y + ((long long)c0 * 32 + (csec[c0] & 31u)) * p.ldy;
+            float yy = 0.f, xx = 0.f;
+            for (int i = lane * 8; i < p.d; i += 256) {
+                float a[8], b[8];
+                half8(y0 + i, a);
+                half8(x + i, b);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { yy = fmaf(a[j], a[j], yy); xx = fmaf(b[j], b[j], xx); }
+            }
+            size = 2.f * sqrtf(warp_sum(yy)) * sqrtf(warp_sum(xx));
+            slack = 2.f * 1.1920929e-7f * (((float)p.d * 0.0625f + 4.f) * p.fmul * size +
+                                           2.f * fabsf(best) + 2.f * fabsf(bound == -INFINITY ? 0.f : bound));
+        }
+        floor_v = bound - slack;
+        if (lane == 0) { sh.count[0] = 0; red[0] = floor_v; red[1] = slack; red[3] = size; }
+    }
+    group_sync<G>();
+    floor_v = red[0];
+    slack = red[1];
+    // (b)
+#pragma unroll 8
+    for (int c = gt; c < p.chunks; c += G) {
+        const float v = cmax[c];
+        if (v >= floor_v) {
+            const int at = atomicAdd(sh.count, 1);
+            if (at < VOCAB_LIST) { sh.chunk[at] = c; sh.value[at] = v; }
+        }
+    }
+    group_sync<G>();
+    // (c)
+    if (w == 0) {
+        int taken = sh.count[0];
+        float theta = -INFINITY;
+        if (taken <= VOCAB_LIST) {
+            for (int i = lane; i < taken; i += 32) {
+                const float v = sh.value[i];
+                const int c = sh.chunk[i];
+                int before = 0;
+                for (int j = 0; j < taken; ++j) before += comes_first(sh.value[j], sh.chunk[j], v, c) ? 1 : 0;
+                if (before == K - 1) red[2] = v;
+            }
+            __syncwarp();
+            if (taken >= K) theta = red[2];
+        }
+        int n = 0;
+        bool crowd = taken > VOCAB_LIST;
+        if (!crowd) {
+#pragma unroll
+            for (int h = 0; h < VOCAB_LIST; h += 32) {
+                const int i = h + lane;
+                int c = 0, size = 0, best = 0;
+                if (i < taken && sh.value[i] >= theta - slack) {
+                    c = sh.chunk[i];
+                    const uint32_t sec = csec[c];
+                    best = (int)(sec & 31u);
+                    const bool whole = sh.value[i] - __uint_as_float(sec & ~31u) >= theta - slack;   // false for "no second" (NaN)
+                    size = whole ? (int)min(32ll, p.vocab - (long long)c * 32) : 1;
                 }
+                int upto = size;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += t;
+                }
+                const int all = __shfl_sync(0xffffffffu, upto, 31);
+                if (n + all > min(p.list_cap, VOCAB_RANK)) { crowd = true; break; }
+                const int at = n + upto - size;
+                if (size == 1) sh.list[at] = c * 32 + best;
+                for (unsigned big = __ballot_sync(0xffffffffu, size > 1); big != 0; big &= big - 1) {
+                    const int src = __ffs(big) - 1;
+                    const int bc_ = __shfl_sync(0xffffffffu, c, src), ba = __shfl_sync(0xffffffffu, at, src),
+                              bs = __shfl_sync(0xffffffffu, size, src);
+                    if (lane < bs) sh.list[ba + lane] = bc_ * 32 + lane;
+                }
+                n += all;
+            }
+        }
+        if (crowd) {
+            __syncwarp();
+            taken = row_top_crowd(p, cmax, slack, lane, sh.chunk, theta);
+            n = 0;
+            for (int i = 0; i < taken; ++i) {
+                const int c = sh.chunk[i];
+                const float v = cmax[c];
+                const uint32_t sec = csec[c];
+                const bool whole = v - __uint_as_float(sec & ~31u) >= theta - slack;
+                if (!(v >= theta - slack)) continue;
+                if (n + (whole ? 32 : 1) > p.list_cap) break;
+                if (whole) {
+                    const int left = (int)min(32ll, p.vocab - (long long)c * 32);
+                    if (lane < left) sh.list[n + lane] = c * 32 + lane;
+                    n += left;
+                } else {
+                    if (lane == 0) sh.list[n] = c * 32 + (int)(sec & 31u);
+                    ++n;
+                }
+            }
+        }
+        if (n > VOCAB_RANK) {
+            // sorted insertion, in fp64 from the start
+            double lz = -INFINITY;
+            long long lj = 0x7fffffffffffffffll;
+            for (int i = 0; i < n; i += 4) {
+                long long j4[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) j4[r] = sh.list[min(i + r, n - 1)];
+                const T* const r4[4] = {y + j4[0] * p.ldy, y + j4[1] * p.ldy, y + j4[2] * p.ldy, y + j4[3] * p.ldy};
+                double z[4];
+                warp_dot4<T, double>(x, r4, p.d, lane, z);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (i + r < n) list_insert(lz, lj, z[r], j4[r], lane);
+            }
+            if (lane < K) row_top_write(p, row, lane, lz, lj, m, log2l);
+            n = -1;
+        }
+        if (lane == 0) sh.count[1] = n;
     }
-    if (w == 0 && lane < K) {
-        const bool any = lj != 0x7fffffffffffffffll;       // false only where a row's scores are not numbers
-        p.top_tokens[row * K + lane] = any ? lj : -1;
-        p.top_log_probs[row * K + lane] =
-            any ? (float)((lz * (double)p.fmul - (double)m - (double)log2l) * 0.6931471805599453) : NAN;
+}
+
+// (d) for all rows of a block: warp `bw` of the block takes every eighth group of four columns, of all columns in fp32 or
+// of those marked in sh.again in fp64.
+template <int G, typename T, typename A>
+__device__ __forceinline__ void rows_top_score(const VocabRows& p, uint8_t* top_base, int stride, int bw, int lane) {
+    constexpr int R = VOCAB_THREADS / G, WARPS = VOCAB_THREADS / 32;
+    constexpr bool AGAIN = sizeof(A) == 8;
+    int turn = 0;
+#pragma unroll 1
+    for (int r = 0; r < R; ++r) {
+        const RowTopShared sh = row_top_shared(top_base + (size_t)r * stride);
+        const int n = AGAIN ? sh.count[2] : sh.count[1];
+        const T* x = reinterpret_cast<const T*>(p.x) + ((long long)blockIdx.x * R + r) * p.ldx;
+        const T* y = reinterpret_cast<const T*>(p.y);
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4, ++turn) {
+            if (turn % WARPS != bw) continue;
+            int at[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) at[q] = AGAIN ? sh.again[min(i + q, n - 1)] : min(i + q, n - 1);
+            const T* const r4[4] = {y + (long long)sh.list[at[0]] * p.ldy, y + (long long)sh.list[at[1]] * p.ldy,
+                                    y + (long long)sh.list[at[2]] * p.ldy, y + (long long)sh.list[at[3]] * p.ldy};
+            A z[4];
+            warp_dot4<T, A>(x, r4, p.d, lane, z);
+            if (lane < 4) sh.z[lane == 0 ? at[0] : lane == 1 ? at[1] : lane == 2 ? at[2] : at[3]] =
+                (double)(lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3]);
+        }
     }
+}
+
+// (e) of column i among the n of its row: how many come before it, and whether another one is closer than `unclear`.
+__device__ __forceinline__ int row_top_rank(const RowTopShared& sh, int n, int i, double unclear, bool& near) {
+    const double z = sh.z[i];
+    const int j = sh.list[i];
+    int before = 0;
+    near = false;
+    for (int o = 0; o < n; ++o) {
+        const double zo = sh.z[o];
+        before += comes_first(zo, sh.list[o], z, j) ? 1 : 0;
+        near |= o != i && fabs(zo - z) <= unclear;
+    }
+    return before;
 }
 
 // One row per G threads.  Bound by memory latency: a row reads its 2 V / 256 partial sums, V / 32 chunk maxima (with
 // alternatives) and one table row per entry; many rows in flight per SM hide that (G = 32), and a few rows are spread
 // over a block each (G = 256).
-template <int G, typename T, bool DISTILL>
-__global__ void __launch_bounds__(VOCAB_THREADS)
+template <int G, typename T, bool DISTILL, bool TOP>
+__global__ void __launch_bounds__(VOCAB_THREADS, 4)
 vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     extern __shared__ __align__(16) uint8_t smem_all[];
     constexpr int W = G / 32;
     const int gt = (int)threadIdx.x % G, lane = gt & 31, w = gt >> 5;
     const long long row = (long long)blockIdx.x * (VOCAB_THREADS / G) + threadIdx.x / G;
-    if (row >= p.rows) return;                    // whole warps (G = 32) or whole blocks (G = 256)
-    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap, W);
+    const bool active = row < p.rows;             // the same for the row's threads
+    if (!TOP && !active) return;                  // (a block of G = 256 has one row, warps of G = 32 do not meet)
+    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap);
     float* red = reinterpret_cast<float*>(smem);
     float* s2 = reinterpret_cast<float*>(smem + 64 * 8);
     uint8_t* top_smem = smem + 64 * 8 + (p.k * 4 + 15) / 16 * 16;
 
     // (1) the row's statistics
-    float m = STATS_EMPTY, l = 0.f, t = 0.f;
-    const float4* st = p.stats + row * p.stats_ld;
-    for (int i = gt; i < p.slots; i += G) {
-        const float4 v = st[i];
-        stats_join(m, l, t, v.x, v.y, v.z);
-    }
+    float m = STATS_EMPTY, l = 0.f, t = 0.f, log2l = 0.f;
+    if (active) {
+        const float4* st = p.stats + row * p.stats_ld;
+        for (int i = gt; i < p.slots; i += G) {
+            const float4 v = st[i];
+            stats_join(m, l, t, v.x, v.y, v.z);
+        }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o),
-                    t2 = __shfl_xor_sync(0xffffffffu, t, o);
-        stats_join(m, l, t, m2, l2, t2);
-    }
-    if (W > 1) {
-        if (lane == 0) { red[w * 4] = m; red[w * 4 + 1] = l; red[w * 4 + 2] = t; }
-        __syncthreads();
-        m = red[0]; l = red[1]; t = red[2];
-        for (int i = 1; i < W; ++i) stats_join(m, l, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2]);
-        __syncthreads();
-    }
-    const float log2l = log2f(l);
-    if (gt == 0) {
-        if (p.row_lse != nullptr) p.row_lse[row] = m + log2l;
-        if (p.entropy != nullptr) p.entropy[row] = 0.6931471805599453f * (log2l - t / l);
-    }
-
-    // (2) the scores of the row's entries
-    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
-    const T* y = reinterpret_cast<const T*>(p.y);
-    const long long* tok = p.tokens + row * p.k;
-    for (int e = w * 4; e < p.k; e += W * 4) {
-        const T* r4[4];
-        bool any = false;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const long long j = e + r < p.k ? tok[e + r] : -1;
-            const bool in = j >= 0 && j < p.vocab;
-            any |= in;
-            r4[r] = y + (in ? j : 0) * p.ldy;
+        for (int o = 16; o >= 1; o >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o),
+                        t2 = __shfl_xor_sync(0xffffffffu, t, o);
+            stats_join(m, l, t, m2, l2, t2);
         }
-        float z[4] = {0.f, 0.f, 0.f, 0.f};
-        const T* const rr[4] = {r4[0], r4[1], r4[2], r4[3]};
-        if (any) warp_dot4<T>(x, rr, p.d, lane, z);
-        if (lane < 4 && e + lane < p.k) {
-            const float zz = lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3];
-            s2[e + lane] = zz * p.fmul;
-        }
-    }
-    group_sync<G>();
-
-    // (3) what is made of them
-    if (!DISTILL) {
-        for (int e = gt; e < p.k; e += G) {
-            const long long j = tok[e];
-            // a token below 0 is padding: 0; one behind the table is a mistake that shows
-            const float lp = (float)(((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453);
-            p.log_probs[row * p.k + e] = j < 0 ? 0.f : j >= p.vocab ? NAN : lp;
-            if (p.token_s2 != nullptr) p.token_s2[row * p.k + e] = s2[e];
-        }
-    } else {
-        // q = softmax of the teacher's logits over the entries that are there; KL = sum q (log q - log p)
-        auto logit = [&](int e) -> float {
-            const long long at = row * p.k + e;
-            const float v = p.teacher_dtype == 1 ? reinterpret_cast<const float*>(p.teacher_logits)[at]
-                            : p.teacher_dtype == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.teacher_logits)[at])
-                                                   : __half2float(reinterpret_cast<const __half*>(p.teacher_logits)[at]);
-            return v * p.inv_teacher_t;
-        };
-        auto there = [&](int e) -> bool { return tok[e] >= 0 && !(logit(e) == -INFINITY); };
-        float um = -INFINITY, seen = 0.f;
-        for (int e = gt; e < p.k; e += G)
-            if (there(e)) { um = fmaxf(um, logit(e)); seen = 1.f; }
-        um = group_reduce<G, true>(um, red, gt);
-        seen = group_reduce<G, true>(seen, red, gt);
-        float sum = 0.f;
-        for (int e = gt; e < p.k; e += G)
-            if (there(e)) sum += expf(logit(e) - um);
-        sum = group_reduce<G, false>(sum, red, gt);
-        const float inv = 1.f / sum, log_sum = logf(sum);
-        double kl = 0.0;
-        for (int e = gt; e < p.k; e += G) {
-            const long long at = row * p.k + e;
-            float q = 0.f;
-            if (there(e)) {
-                const float u = logit(e) - um;
-                q = expf(u) * inv;
-                const double lp = ((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453;
-                if (tok[e] >= p.vocab) q = NAN;
-                if (q != 0.f) kl += (double)q * ((double)u - (double)log_sum - lp);
-            }
-            p.teacher_probs[at] = q;
-            p.token_s2[at] = s2[e];
-        }
-        // the terms are few and of one row: fp64 costs nothing and keeps the difference of two logarithms exact
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
         if (W > 1) {
-            double* red64 = reinterpret_cast<double*>(red);
+            if (lane == 0) { red[w * 4] = m; red[w * 4 + 1] = l; red[w * 4 + 2] = t; }
             __syncthreads();
-            if (lane == 0) red64[w] = kl;
+            m = red[0]; l = red[1]; t = red[2];
+            for (int i = 1; i < W; ++i) stats_join(m, l, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2]);
             __syncthreads();
-            kl = red64[0];
-            for (int i = 1; i < W; ++i) kl += red64[i];
         }
+        log2l = log2f(l);
         if (gt == 0) {
-            p.row_loss[row] = seen > 0.f ? (float)kl : 0.f;
-            p.row_has[row] = seen;
+            if (p.row_lse != nullptr) p.row_lse[row] = m + log2l;
+            if (p.entropy != nullptr) p.entropy[row] = 0.6931471805599453f * (log2l - t / l);
+        }
+
+        // (2) the scores of the row's entries
+        const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+        const T* y = reinterpret_cast<const T*>(p.y);
+        const long long* tok = p.tokens + row * p.k;
+        for (int e = w * 4; e < p.k; e += W * 4) {
+            const T* r4[4];
+            bool any = false;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const long long j = e + r < p.k ? tok[e + r] : -1;
+                const bool in = j >= 0 && j < p.vocab;
+                any |= in;
+                r4[r] = y + (in ? j : 0) * p.ldy;
+            }
+            float z[4] = {0.f, 0.f, 0.f, 0.f};
+            const T* const rr[4] = {r4[0], r4[1], r4[2], r4[3]};
+            if (any) warp_dot4<T, float>(x, rr, p.d, lane, z);
+            if (lane < 4 && e + lane < p.k) {
+                const float zz = lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3];
+                s2[e + lane] = zz * p.fmul;
+            }
+        }
+        group_sync<G>();
+
+        // (3) what is made of them
+        if (!DISTILL) {
+            for (int e = gt; e < p.k; e += G) {
+                const long long j = tok[e];
+                // a token below 0 is padding: 0; one behind the table is a mistake that shows
+                const float lp = (float)(((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453);
+                p.log_probs[row * p.k + e] = j < 0 ? 0.f : j >= p.vocab ? NAN : lp;
+                if (p.token_s2 != nullptr) p.token_s2[row * p.k + e] = s2[e];
+            }
+        } else {
+            // q = softmax of the teacher's logits over the entries that are there; KL = sum q (log q - log p)
+            auto logit = [&](int e) -> float {
+                const long long at = row * p.k + e;
+                const float v = p.teacher_dtype == 1 ? reinterpret_cast<const float*>(p.teacher_logits)[at]
+                                : p.teacher_dtype == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.teacher_logits)[at])
+                                                       : __half2float(reinterpret_cast<const __half*>(p.teacher_logits)[at]);
+                return v * p.inv_teacher_t;
+            };
+            auto there = [&](int e) -> bool { return tok[e] >= 0 && !(logit(e) == -INFINITY); };
+            float um = -INFINITY, seen = 0.f;
+            for (int e = gt; e < p.k; e += G)
+                if (there(e)) { um = fmaxf(um, logit(e)); seen = 1.f; }
+            um = group_reduce<G, true>(um, red, gt);
+            seen = group_reduce<G, true>(seen, red, gt);
+            float sum = 0.f;
+            for (int e = gt; e < p.k; e += G)
+                if (there(e)) sum += expf(logit(e) - um);
+            sum = group_reduce<G, false>(sum, red, gt);
+            const float inv = 1.f / sum, log_sum = logf(sum);
+            double kl = 0.0;
+            for (int e = gt; e < p.k; e += G) {
+                const long long at = row * p.k + e;
+                float q = 0.f;
+                if (there(e)) {
+                    const float u = logit(e) - um;
+                    q = expf(u) * inv;
+                    const double lp = ((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453;
+                    if (tok[e] >= p.vocab) q = NAN;
+                    if (q != 0.f) kl += (double)q * ((double)u - (double)log_sum - lp);
+                }
+                p.teacher_probs[at] = q;
+                p.token_s2[at] = s2[e];
+            }
+            // the terms are few and of one row: fp64 costs nothing and keeps the difference of two logarithms exact
+#pragma unroll
+            for (int o = 16; o >= 1; o >>= 1) kl += __shfl_xor_sync(0xffffffffu, kl, o);
+            if (W > 1) {
+                double* red64 = reinterpret_cast<double*>(red);
+                __syncthreads();
+                if (lane == 0) red64[w] = kl;
+                __syncthreads();
+                kl = red64[0];
+                for (int i = 1; i < W; ++i) kl += red64[i];
+            }
+            if (gt == 0) {
+                p.row_loss[row] = seen > 0.f ? (float)kl : 0.f;
+                p.row_has[row] = seen;
+            }
         }
     }
-    if (!DISTILL && p.top_k > 0) {
+    if (TOP) {
+        const RowTopShared sh = row_top_shared(top_smem);
+        const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap), bw = threadIdx.x >> 5;
+        uint8_t* top_base = smem_all + (top_smem - smem);
         group_sync<G>();
-        row_top<G, T>(p, row, gt, top_smem, m, log2l);
+        if (active) row_top_select<G, T>(p, row, gt, sh, m, log2l, red);
+        else if (gt == 0) sh.count[1] = 0;
+        __syncthreads();
+        rows_top_score<G, T, float>(p, top_base, stride, bw, lane);
+        __syncthreads();
+        // In fp32 an order counts only when it is clear: d / 64 products in a row and a tree of 6, each off by half an ulp
+        // (2^-24) of at most |x| |y|, on both sides.
+        const int n = sh.count[1];
+        if (w == 0) {
+            const double unclear = active ? (double)(1.1920929e-7f * ((float)p.d * 0.015625f + 6.f) * red[3]) : 0.0;
+            int again = 0;
+            for (int i = lane; i - lane < n; i += 32) {
+                bool near = false;
+                if (i < n) row_top_rank(sh, n, i, unclear, near);
+                const unsigned who = __ballot_sync(0xffffffffu, near);
+                if (near) sh.again[again + __popc(who & ((1u << lane) - 1u))] = i;
+                again += __popc(who);
+            }
+            if (lane == 0) sh.count[2] = again;
+        }
+        __syncthreads();
+        rows_top_score<G, T, double>(p, top_base, stride, bw, lane);
+        __syncthreads();
+        if (w != 0 || !active || n < 0) return;
+        for (int i = lane; i < n; i += 32) {
+            bool ignored;
+            const int place = row_top_rank(sh, n, i, 0.0, ignored);
+            if (place < p.top_k) row_top_write(p, row, place, sh.z[i], sh.list[i], m, log2l);
+        }
+        // only where a row's scores are not numbers are there fewer than K
+        if (lane < p.top_k && lane >= n) { p.top_tokens[row * p.top_k + lane] = -1; p.top_log_probs[row * p.top_k + lane] = NAN; }
     }
 }
 

@@ -33,15 +33,13 @@ def embed_tokens(tokens, table, scale=1.0):
     tokens: any shape, int64 or int32; a negative token is padding: its row is zero and it gets no gradient.  A token
     behind the table gives a row of NaN.  table: [V, D] float32, bfloat16 or float16, any D, pitch and alignment.
     """
-    assert tokens.is_cuda and table.is_cuda, "tokens and table must be CUDA tensors"
     ops._check_matrix(table, "table")
     assert tokens.device == table.device, "tokens and table must be on one device"
     assert tokens.dtype in (torch.int64, torch.int32), f"tokens: dtype {tokens.dtype} not supported (int64 or int32)"
     assert not isinstance(scale, torch.Tensor) and math.isfinite(scale), "scale must be a finite Python number"
-    flat = tokens.reshape(-1).to(torch.int64)
+    tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
+    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     table = table if table.stride(1) == 1 else table.contiguous()
-    if torch.is_grad_enabled() and table.requires_grad:
-        out = _EmbedFn.apply(flat, table, float(scale))
-    else:
-        out = ops.embed(flat, table, float(scale))
-    return out.view(*tokens.shape, table.shape[1])
+    if table.requires_grad and torch.is_grad_enabled():
+        return _EmbedFn.apply(tokens, table, float(scale))
+    return ops.embed(tokens, table, float(scale))

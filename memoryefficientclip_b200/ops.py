@@ -719,48 +719,51 @@ def ring_grad(call: RingCall, kind, temperature, row_sum, col_sum_all, grad_out,
 
 
 # ---- softmax over a vocabulary ------------------------------------------------------------------------------
+def _is_operand(x: torch.Tensor) -> bool:
+    """Whether the tile kernels can read a 16-bit matrix as it is: 16-byte aligned rows of a multiple of 8 columns."""
+    return x.shape[1] % 8 == 0 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
+
+
 def vocab_operands(x: torch.Tensor, table: torch.Tensor):
     """(x, table) as the vocabulary passes read them: both fp16 if both inputs are, else both bf16 (fp32 inputs are
     rounded, as everywhere in this package); rows of padded(d) columns, 16-byte aligned."""
-    if x.dtype == torch.float16 and table.dtype == torch.float16:
-        return _as_f16_operand(x), _as_f16_operand(table)
-    return as_operand(x), as_operand(table)
+    if x.dtype == table.dtype == torch.float16:
+        return tuple(t if _is_operand(t) else _padded_f16(t) for t in (x, table))
+    return tuple(t if t.dtype == torch.bfloat16 and _is_operand(t) else normalize_fwd(t, normalize=False)[0]
+                 for t in (x, table))
 
 
-def _as_f16_operand(x: torch.Tensor) -> torch.Tensor:
-    _check_matrix(x, "operand")
-    if x.shape[1] % 8 == 0 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
+def _padded_f16(x: torch.Tensor) -> torch.Tensor:
     out = torch.zeros(x.shape[0], padded(x.shape[1]), dtype=torch.float16, device=x.device)
     out[:, :x.shape[1]] = x
     return out
 
 
-def _vocab_workspace(rows, vocab, top_k, device):
-    n = _lib.load().meclip_vocab_workspace_bytes(rows, vocab, top_k)
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def token_log_probs(x, table, tokens, temperature, top_k=0, want_entropy=True, save=False, status=None):
-    """(log_probs, entropy, top_log_probs, top_tokens, row_lse, token_scores) of operands from vocab_operands; tokens
-    int64 [rows, per_row].  What is not asked for is None (meclip_token_log_probs)."""
+def token_log_probs(x, table, tokens, temperature, top_k=0, save=False, status=None):
+    """(log_probs, entropy, top_log_probs, top_tokens, saved) of operands from vocab_operands; tokens int64, contiguous,
+    [rows] or [rows, k], and log_probs like them.  saved: what token_log_probs_grad needs besides, None unless asked for
+    (meclip_token_log_probs)."""
     rows, d = x.shape
-    vocab, per_row, dev = table.shape[0], tokens.shape[1], x.device
-
-    def new(*shape, dtype=torch.float32):
-        return torch.empty(*shape, dtype=dtype, device=dev)
-
-    lp = new(rows, per_row)
-    entropy = new(rows) if want_entropy else None
-    top_lp, top = (new(rows, top_k), new(rows, top_k, dtype=torch.int64)) if top_k else (None, None)
-    lse, scores = (new(rows), new(rows, per_row)) if save else (None, None)
+    vocab, dev = table.shape[0], x.device
+    per_row = tokens.numel() // rows
+    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_lp = top = saved = lse = scores = None
+    if top_k:
+        top_lp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+        top = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    if save:                    # one buffer: [rows] log-sum-exps, [rows, per_row] scores
+        saved = torch.empty(rows * (1 + per_row), dtype=torch.float32, device=dev)
+        lse = saved.data_ptr()
+        scores = lse + 4 * rows
+    lib = _lib.load()
     with _on_device(dev):
-        ws = _vocab_workspace(rows, vocab, top_k, dev)
-        _lib.check(_lib.load().meclip_token_log_probs(
-            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0),
-            float(temperature), tokens.data_ptr(), per_row, lp.data_ptr(), _ptr(entropy), top_k, _ptr(top_lp), _ptr(top),
-            _ptr(lse), _ptr(scores), ws.data_ptr(), ws.numel(), _ptr(status), _stream(x)))
-    return lp, entropy, top_lp, top, lse, scores
+        ws = torch.empty(lib.meclip_vocab_workspace_bytes(rows, vocab, top_k), dtype=torch.uint8, device=dev)
+        _lib.check(lib.meclip_token_log_probs(
+            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0), temperature,
+            tokens.data_ptr(), per_row, lp.data_ptr(), entropy.data_ptr(), top_k, _ptr(top_lp), _ptr(top), lse, scores,
+            ws.data_ptr(), ws.numel(), _ptr(status), _stream(x)))
+    return lp, entropy, top_lp, top, saved
 
 
 class _VocabGrads:
@@ -770,84 +773,98 @@ class _VocabGrads:
         rows, d = x.shape
         vocab, dev = table.shape[0], x.device
         f16 = x.dtype == torch.float16
-        self.x16, self.t16 = (x, table) if f16 else (None, None)
         # the contractions run on bf16 operands: a coefficient can be far below fp16's smallest number
         self.x, self.t = (normalize_fwd(x, False)[0], normalize_fwd(table, False)[0]) if f16 else (x, table)
-        self.dx = torch.empty(rows, d, dtype=dx_dtype, device=dev) if need_dx else None
-        self.dt = torch.empty(vocab, d, dtype=dtable_dtype, device=dev) if need_dtable else None
+        self.dx = torch.empty((rows, d), dtype=dx_dtype, device=dev) if need_dx else None
+        self.dt = torch.empty((vocab, d), dtype=dtable_dtype, device=dev) if need_dtable else None
         n = _lib.load().meclip_vocab_grad_workspace_bytes(rows, vocab, d)
         self.ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        self.head = (self.x.data_ptr(), self.t.data_ptr(), _ptr(self.x16), _ptr(self.t16), rows, vocab, d,
-                     self.x.stride(0), self.t.stride(0), x.stride(0) if f16 else 0, table.stride(0) if f16 else 0)
-        self.tail = (_ptr(self.dx), _MODE[dx_dtype], d, _ptr(self.dt), _MODE[dtable_dtype], d, self.ws.data_ptr(),
-                     self.ws.numel())
+        f16_args = (x.data_ptr(), table.data_ptr()) if f16 else (None, None)
+        self.head = (self.x.data_ptr(), self.t.data_ptr(), *f16_args, rows, vocab, d, self.x.stride(0), self.t.stride(0),
+                     x.stride(0) if f16 else 0, table.stride(0) if f16 else 0)
+        self.tail = (_ptr(self.dx), _MODE[dx_dtype], d, _ptr(self.dt), _MODE[dtable_dtype], d, self.ws.data_ptr(), n)
 
 
-def token_log_probs_grad(x, table, tokens, temperature, row_lse, entropy, token_scores, grad_log_probs, grad_entropy,
-                         dx_dtype, dtable_dtype, need_dx=True, need_dtable=True, status=None):
+def token_log_probs_grad(x, table, tokens, temperature, saved, entropy, grad_log_probs, grad_entropy, dx_dtype,
+                         dtable_dtype, need_dx=True, need_dtable=True, status=None):
     """(dx, dtable) for the operands of token_log_probs (meclip_token_log_probs_grad); dtypes fp32 or bf16."""
+    rows = x.shape[0]
+    lse = saved.data_ptr()
     with _on_device(x.device):
         g = _VocabGrads(x, table, need_dx, need_dtable, dx_dtype, dtable_dtype)
         _lib.check(_lib.load().meclip_token_log_probs_grad(
-            *g.head, float(temperature), tokens.data_ptr(), tokens.shape[1], row_lse.data_ptr(), _ptr(entropy),
-            _ptr(token_scores), _ptr(grad_log_probs), _ptr(grad_entropy), *g.tail, _ptr(status), _stream(x)))
+            *g.head, temperature, tokens.data_ptr(), tokens.numel() // rows, lse, entropy.data_ptr(), lse + 4 * rows,
+            _ptr(grad_log_probs), _ptr(grad_entropy), *g.tail, _ptr(status), _stream(x)))
     return g.dx, g.dt
 
 
 def distill_forward(x, table, teacher_tokens, teacher_logits, temperature, teacher_temperature, reduction, status=None):
     """(result, saved): the loss of operands from vocab_operands, [rows] with reduction "none" and 0-dim otherwise, and
-    the tensors its gradient needs (meclip_distill)."""
+    one buffer with what its gradient needs (meclip_distill); teacher_tokens int64 and teacher_logits [rows, k] or [rows],
+    contiguous."""
     rows, d = x.shape
-    vocab, per_row, dev = table.shape[0], teacher_tokens.shape[1], x.device
-    row_loss, row_has, lse = torch.empty(3, rows, dtype=torch.float32, device=dev).unbind(0)
-    scores, probs = torch.empty(2, rows, per_row, dtype=torch.float32, device=dev).unbind(0)
+    vocab, dev = table.shape[0], x.device
+    per_row = teacher_tokens.numel() // rows
     reduce = reduction != "none"
-    loss = torch.empty((), dtype=torch.float32, device=dev) if reduce else None
-    inv_count = torch.empty(1, dtype=torch.float32, device=dev) if reduce else None
+    result = torch.empty(() if reduce else (rows,), dtype=torch.float32, device=dev)
+    # [rows] log-sum-exps, [rows, k] scores, [rows, k] probabilities, [rows] whether there is a teacher, 1 / rows that
+    # have one; the rows' losses when only their sum is wanted
+    saved = torch.empty(rows * (3 + 2 * per_row) + 1, dtype=torch.float32, device=dev)
+    lse, scores, probs, has, inv = _distill_saved(saved, rows, per_row)
+    lib = _lib.load()
     with _on_device(dev):
-        ws = _vocab_workspace(rows, vocab, 0, dev)
-        _lib.check(_lib.load().meclip_distill(
-            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0),
-            float(temperature), teacher_tokens.data_ptr(), teacher_logits.data_ptr(), _DT[teacher_logits.dtype], per_row,
-            float(teacher_temperature), int(reduction == "mean"), row_loss.data_ptr(), row_has.data_ptr(), _ptr(loss),
-            _ptr(inv_count), lse.data_ptr(), scores.data_ptr(), probs.data_ptr(), ws.data_ptr(), ws.numel(), _ptr(status),
-            _stream(x)))
-    return (loss if reduce else row_loss), (lse, scores, probs, row_has, inv_count)
+        ws = torch.empty(lib.meclip_vocab_workspace_bytes(rows, vocab, 0), dtype=torch.uint8, device=dev)
+        _lib.check(lib.meclip_distill(
+            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0), temperature,
+            teacher_tokens.data_ptr(), teacher_logits.data_ptr(), _DT[teacher_logits.dtype], per_row, teacher_temperature,
+            int(reduction == "mean"), inv + 4 if reduce else result.data_ptr(), has, result.data_ptr() if reduce else None,
+            inv if reduce else None, lse, scores, probs, ws.data_ptr(), ws.numel(), _ptr(status), _stream(x)))
+    return result, saved
+
+
+def _distill_saved(saved, rows, per_row):
+    lse = saved.data_ptr()
+    scores = lse + 4 * rows
+    probs = scores + 4 * rows * per_row
+    has = probs + 4 * rows * per_row
+    return lse, scores, probs, has, has + 4 * rows
 
 
 def distill_backward(x, table, teacher_tokens, temperature, saved, grad_out, dx_dtype, dtable_dtype, need_dx=True,
                      need_dtable=True, status=None):
     """(dx, dtable) for the operands of distill_forward (meclip_distill_grad); grad_out fp32, one value or [rows]."""
-    lse, scores, probs, row_has, inv_count = saved
+    rows = x.shape[0]
+    per_row = teacher_tokens.numel() // rows
+    lse, scores, probs, has, inv = _distill_saved(saved, rows, per_row)
+    per_grad = grad_out.dim() == 1
     with _on_device(x.device):
         g = _VocabGrads(x, table, need_dx, need_dtable, dx_dtype, dtable_dtype)
         _lib.check(_lib.load().meclip_distill_grad(
-            *g.head, float(temperature), teacher_tokens.data_ptr(), teacher_tokens.shape[1], lse.data_ptr(),
-            scores.data_ptr(), probs.data_ptr(), row_has.data_ptr(), grad_out.data_ptr(), int(inv_count is None),
-            _ptr(inv_count), *g.tail, _ptr(status), _stream(x)))
+            *g.head, temperature, teacher_tokens.data_ptr(), per_row, lse, scores, probs, has, grad_out.data_ptr(),
+            int(per_grad), None if per_grad else inv, *g.tail, _ptr(status), _stream(x)))
     return g.dx, g.dt
 
 
 def embed(tokens: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
-    """scale * table[tokens] for int64 tokens [n] (meclip_embed)."""
-    n, (vocab, d) = tokens.shape[0], table.shape
-    tokens = tokens.contiguous()
-    out = torch.empty(n, d, dtype=table.dtype, device=table.device)
+    """scale * table[tokens] for contiguous int64 tokens of any shape (meclip_embed)."""
+    vocab, d = table.shape
+    out = torch.empty((*tokens.shape, d), dtype=table.dtype, device=table.device)
     with _on_device(table.device):
-        _lib.check(_lib.load().meclip_embed(tokens.data_ptr(), n, table.data_ptr(), _DT[table.dtype], vocab, d,
+        _lib.check(_lib.load().meclip_embed(tokens.data_ptr(), tokens.numel(), table.data_ptr(), _DT[table.dtype], vocab, d,
                                             max(table.stride(0), d), scale, out.data_ptr(), d, _stream(table)))
     return out
 
 
 def embed_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
-    """[vocab, d] gradient of the table from grad [n, d] (meclip_embed_grad)."""
-    n, d = grad.shape
-    tokens, grad = tokens.contiguous(), grad if grad.stride(1) == 1 and grad.stride(0) >= d else grad.contiguous()
-    dt = torch.empty(vocab, d, dtype=grad.dtype, device=grad.device)
+    """[vocab, d] gradient of the table from contiguous int64 tokens and grad [*tokens.shape, d] (meclip_embed_grad)."""
+    n, d = tokens.numel(), grad.shape[-1]
+    if not grad.is_contiguous() and not (grad.dim() == 2 and grad.stride(1) == 1 and grad.stride(0) >= d):
+        grad = grad.contiguous()
+    ldg = grad.stride(0) if grad.dim() == 2 and n > 1 else d
+    dt = torch.empty((vocab, d), dtype=grad.dtype, device=grad.device)
+    lib = _lib.load()
     with _on_device(grad.device):
-        lib = _lib.load()
         ws = torch.empty(lib.meclip_embed_grad_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=grad.device)
-        _lib.check(lib.meclip_embed_grad(tokens.data_ptr(), n, grad.data_ptr(), _DT[grad.dtype], vocab, d,
-                                         max(grad.stride(0), d), scale, dt.data_ptr(), d, ws.data_ptr(), ws.numel(),
-                                         _stream(grad)))
+        _lib.check(lib.meclip_embed_grad(tokens.data_ptr(), n, grad.data_ptr(), _DT[grad.dtype], vocab, d, ldg, scale,
+                                         dt.data_ptr(), d, ws.data_ptr(), ws.numel(), _stream(grad)))
     return dt

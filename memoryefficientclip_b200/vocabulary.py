@@ -38,24 +38,24 @@ class TokenLogProbs(NamedTuple):
 
 
 def _check_inputs(features, table, temperature):
-    assert features.is_cuda and table.is_cuda, "features and table must be CUDA tensors"
     ops._check_matrix(features, "features")
     ops._check_matrix(table, "table")
     assert features.device == table.device, "features and table must be on one device"
     assert features.shape[1] == table.shape[1], \
         f"features have {features.shape[1]} columns, the table has {table.shape[1]}"
     assert not isinstance(temperature, torch.Tensor), "the temperature of a vocabulary softmax is a Python number"
-    assert 0.0 < float(temperature) < math.inf, "temperature must be positive"
+    assert 0.0 < temperature < math.inf, "temperature must be positive"
 
 
 def _check_tokens(tokens, features, name):
-    assert tokens.is_cuda and tokens.device == features.device, f"{name} must be on the features' device"
+    """The tokens as contiguous int64."""
+    assert tokens.device == features.device, f"{name} must be on the features' device"
     assert tokens.dtype in (torch.int64, torch.int32), f"{name}: dtype {tokens.dtype} not supported (int64 or int32)"
     assert tokens.dim() in (1, 2) and tokens.shape[0] == features.shape[0], \
         f"{name} must be [{features.shape[0]}] or [{features.shape[0]}, k]"
-    tokens = tokens.unsqueeze(1) if tokens.dim() == 1 else tokens
-    assert 1 <= tokens.shape[1] <= MAX_ENTRIES, f"{name}: 1 to {MAX_ENTRIES} entries per row"
-    return tokens.to(torch.int64).contiguous()
+    assert tokens.dim() == 1 or 1 <= tokens.shape[1] <= MAX_ENTRIES, f"{name}: 1 to {MAX_ENTRIES} entries per row"
+    tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
+    return tokens if tokens.is_contiguous() else tokens.contiguous()
 
 
 def _grad_dtype(dtype, d):
@@ -63,15 +63,20 @@ def _grad_dtype(dtype, d):
     return (dtype, False) if ops.direct_grad_dtype(dtype, d) else (torch.float32, True)
 
 
+def _f32(g):
+    """An incoming gradient as contiguous fp32."""
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
 class _TokenLogProbsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, features, table, tokens, temperature, top_k):
         status = ops.status_word(features.device)
-        ops.poll_status(features.device)
         x, y = ops.vocab_operands(features, table)
-        lp, entropy, top_lp, top, lse, scores = ops.token_log_probs(x, y, tokens, temperature, top_k, save=True,
-                                                                    status=status)
-        ctx.save_for_backward(x, y, tokens, lse, entropy, scores)
+        lp, entropy, top_lp, top, saved = ops.token_log_probs(x, y, tokens, temperature, top_k, True, status)
+        ctx.save_for_backward(x, y, tokens, entropy, saved)
         ctx.vocab = (temperature, features.dtype, table.dtype, features.shape[1])
         ctx.set_materialize_grads(False)
         if top_k:
@@ -80,17 +85,15 @@ class _TokenLogProbsFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_log_probs, grad_entropy, _top_lp, _top):
-        x, y, tokens, lse, entropy, scores = ctx.saved_tensors
+        x, y, tokens, entropy, saved = ctx.saved_tensors
         temperature, x_dtype, y_dtype, d = ctx.vocab
         need = ctx.needs_input_grad
         if (grad_log_probs is None and grad_entropy is None) or not (need[0] or need[1]):
             return None, None, None, None, None
         dx_t, post_x = _grad_dtype(x_dtype, d)
         dy_t, post_y = _grad_dtype(y_dtype, d)
-        g_lp = None if grad_log_probs is None else grad_log_probs.to(torch.float32).contiguous()
-        g_h = None if grad_entropy is None else grad_entropy.to(torch.float32).contiguous()
-        dx, dy = ops.token_log_probs_grad(x, y, tokens, temperature, lse, entropy, scores, g_lp, g_h, dx_t, dy_t,
-                                          need[0], need[1], status=ops.status_word(x.device))
+        dx, dy = ops.token_log_probs_grad(x, y, tokens, temperature, saved, entropy, _f32(grad_log_probs),
+                                          _f32(grad_entropy), dx_t, dy_t, need[0], need[1], ops.status_word(x.device))
         if dx is not None and post_x:
             dx = ops.normalize_bwd(dx, None, None, x_dtype, d)
         if dy is not None and post_y:
@@ -107,18 +110,17 @@ def token_log_probs(features, table, tokens, temperature=1.0, top_k=0) -> TokenL
     top_k: 0 to 32 alternatives per row, best first; of equal scores the lower token comes first.  They carry no gradient.
     """
     _check_inputs(features, table, temperature)
-    rows = _check_tokens(tokens, features, "tokens")
+    tokens = _check_tokens(tokens, features, "tokens")
     assert isinstance(top_k, int) and 0 <= top_k <= min(MAX_TOP, table.shape[0]), \
         f"top_k must be between 0 and {min(MAX_TOP, table.shape[0])}"
-    if torch.is_grad_enabled() and (features.requires_grad or table.requires_grad):
-        lp, entropy, top_lp, top = _TokenLogProbsFn.apply(features, table, rows, float(temperature), top_k)
-    else:
-        status = ops.status_word(features.device)
-        ops.poll_status(features.device)
-        x, y = ops.vocab_operands(features, table)
-        lp, entropy, top_lp, top, _lse, _scores = ops.token_log_probs(x, y, rows, temperature, top_k, status=status)
-        ops.post_status(features.device)
-    return TokenLogProbs(lp.view(tokens.shape), entropy, top_lp, top)
+    device = features.device
+    ops.poll_status(device)
+    if (features.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+        return TokenLogProbs(*_TokenLogProbsFn.apply(features, table, tokens, float(temperature), top_k))
+    x, y = ops.vocab_operands(features, table)
+    out = ops.token_log_probs(x, y, tokens, float(temperature), top_k, False, ops.status_word(device))
+    ops.post_status(device)
+    return TokenLogProbs(*out[:4])
 
 
 class MemoryEfficientDistillLossFn(torch.autograd.Function):
@@ -132,35 +134,37 @@ class MemoryEfficientDistillLossFn(torch.autograd.Function):
         assert teacher_tokens.shape == teacher_logits.shape, "teacher_tokens and teacher_logits must have one shape"
         assert teacher_logits.device == features.device, "teacher_logits must be on the features' device"
         assert teacher_logits.dtype in ops._DT, f"teacher_logits: dtype {teacher_logits.dtype} not supported"
-        assert 0.0 < float(teacher_temperature) < math.inf, "teacher_temperature must be positive"
+        assert not isinstance(teacher_temperature, torch.Tensor) and 0.0 < teacher_temperature < math.inf, \
+            "teacher_temperature must be a positive Python number"
         assert reduction in ("mean", "sum", "none"), f"unknown reduction {reduction!r}"
         status = ops.status_word(features.device)
         ops.poll_status(features.device)
+        inv_x = inv_y = None
         if normalize:
             x, inv_x = ops.normalize_fwd(features, True)
             y, inv_y = ops.normalize_fwd(table, True)
         else:
-            (x, y), inv_x, inv_y = ops.vocab_operands(features, table), None, None
-        result, saved = ops.distill_forward(x, y, tokens, teacher_logits.detach().contiguous(), temperature,
-                                            teacher_temperature, reduction, status=status)
+            x, y = ops.vocab_operands(features, table)
+        result, saved = ops.distill_forward(x, y, tokens, teacher_logits.contiguous(), float(temperature),
+                                            float(teacher_temperature), reduction, status)
         if not any(ctx.needs_input_grad[:2]):
             ops.post_status(features.device)
-        ctx.save_for_backward(x, y, tokens, inv_x, inv_y, *saved)
+        ctx.save_for_backward(x, y, tokens, saved, inv_x, inv_y)
         ctx.vocab = (float(temperature), features.dtype, table.dtype, features.shape[1])
         return result
 
     @staticmethod
     def backward(ctx, grad_output):
-        x, y, tokens, inv_x, inv_y, *saved = ctx.saved_tensors
+        x, y, tokens, saved, inv_x, inv_y = ctx.saved_tensors
         temperature, x_dtype, y_dtype, d = ctx.vocab
         need = ctx.needs_input_grad
-        dx_t, post_x = _grad_dtype(x_dtype, d)
-        dy_t, post_y = _grad_dtype(y_dtype, d)
-        if inv_x is not None:       # the Jacobian of the normalisation follows: fp32 until it rounds once
+        if inv_x is None:
+            dx_t, post_x = _grad_dtype(x_dtype, d)
+            dy_t, post_y = _grad_dtype(y_dtype, d)
+        else:                       # the Jacobian of the normalisation follows: fp32 until it rounds once
             dx_t, post_x, dy_t, post_y = torch.float32, True, torch.float32, True
-        go = grad_output.detach().to(device=x.device, dtype=torch.float32).contiguous()
-        dx, dy = ops.distill_backward(x, y, tokens, temperature, saved, go, dx_t, dy_t, need[0], need[1],
-                                      status=ops.status_word(x.device))
+        dx, dy = ops.distill_backward(x, y, tokens, temperature, saved, _f32(grad_output), dx_t, dy_t, need[0], need[1],
+                                      ops.status_word(x.device))
         if dx is not None and post_x:
             dx = ops.normalize_bwd(dx, x if inv_x is not None else None, inv_x, x_dtype, d)
         if dy is not None and post_y:

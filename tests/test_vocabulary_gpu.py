@@ -331,9 +331,9 @@ def test_entry_points_stay_inside_their_outputs():
     guard = torch.full((n + 8, d), 7.0, dtype=torch.bfloat16, device="cuda")
     guard[:n] = x.cuda()
     with torch.no_grad():
-        a = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda()[:, None], 1.0, 2)
+        a = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda(), 1.0, 2)
         guard[n:] = float("nan")
-        b = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda()[:, None], 1.0, 2)
+        b = ops.token_log_probs(guard[:n], table.cuda(), tokens.cuda(), 1.0, 2)
     for p, q in zip(a[:4], b[:4]):
         assert torch.equal(p, q)
     ops.check_status()
