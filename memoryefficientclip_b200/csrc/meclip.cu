@@ -733,7 +733,7 @@ static int launch_gemm_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
     static std::atomic<unsigned long long> smem_allowed{0};
     const int rc = allow_all_smem(kern, smem_allowed);
     if (rc) return rc;
-    const int tiles = p.num_m_tiles * p.num_n_tiles;
+    const int tiles = p.num_m_tiles * p.num_n_tiles * p.splits;
     const int units = (tiles + p.strip_len - 1) / p.strip_len;
     const int grid = units < sm_count() ? units : sm_count();
     ScopedTiming timing(stream, t_tag, 2.0 * p.m * p.n * p.k);
@@ -769,7 +769,7 @@ static int launch_pair_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
         max_clusters[dev] = n;
     }
     const int cap = (dev >= 0 && dev < 64) ? max_clusters[dev] : sm_count() / 2;
-    const int tiles = p.dual ? p.tiles0 + p.num_m_tiles2 * p.num_n_tiles : p.num_m_tiles * p.num_n_tiles;
+    const int tiles = p.dual ? p.tiles0 + p.num_m_tiles2 * p.num_n_tiles * p.splits2 : p.num_m_tiles * p.num_n_tiles * p.splits;
     const int units = (tiles + p.strip_len - 1) / p.strip_len;
     const int clusters = units < cap ? units : cap;
     ScopedTiming timing(stream, t_tag, flops >= 0.0 ? flops : 2.0 * p.m * p.n * p.k);
@@ -854,6 +854,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     p.num_m_tiles = (int)((m + BM - 1) / BM);
     p.num_n_tiles = (int)((n + bn - 1) / bn);
     p.k_steps = (int)((k + bk - 1) / bk);
+    if (epi != EPI_OUT || p.splits < 1) { p.splits = 1; p.k_part = p.k_steps; }
     p.trace = g_trace_buf;
     p.trace_capacity = g_trace_capacity;
     p.wait_limit_ns = wait_limit_ns();
@@ -883,7 +884,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
             p.idesc_last = umma_idesc_bf16(BM, last, a.mn_major ? 1 : 0, b.mn_major ? 1 : 0);
         }
     }
-    if ((long long)p.num_m_tiles * p.num_n_tiles > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
+    if ((long long)p.num_m_tiles * p.num_n_tiles * p.splits > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
     // shared memory: [<= 1023 B alignment slack][stages][tail]; as many stages as fit, at least 2
     p.stage_bytes = A_STAGE_BYTES + bn * BK * 2;
     int stages = (SMEM_LIMIT - 1024 - tail_bytes(epi)) / p.stage_bytes;
@@ -986,8 +987,11 @@ static int launch_contractions_dual(const void* panel, long long panel_rows_allo
     p.k_steps2 = (int)((cols + BK - 1) / BK);
     p.out2 = px.out; p.ld_out2 = px.ld_out; p.out_bf16_2 = px.out_bf16; p.acc_in2 = px.acc_in; p.ld_acc2 = px.ld_acc;
     p.dual = 1;
-    p.tiles0 = p.num_m_tiles * p.num_n_tiles;
-    if ((long long)p.tiles0 + (long long)p.num_m_tiles2 * p.num_n_tiles > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
+    if (p.splits < 1) { p.splits = 1; p.k_part = p.k_steps; }
+    p.splits2 = px.splits; p.k_part2 = px.k_part; p.split_stride2 = px.split_stride;
+    if (p.splits2 < 1) { p.splits2 = 1; p.k_part2 = p.k_steps2; }
+    p.tiles0 = p.num_m_tiles * p.num_n_tiles * p.splits;
+    if ((long long)p.num_m_tiles * p.num_n_tiles * p.splits + (long long)p.num_m_tiles2 * p.num_n_tiles * p.splits2 > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
     p.trace = nullptr; p.trace_capacity = 0;
     p.wait_limit_ns = wait_limit_ns();
     p.group_m = 2;
@@ -1153,6 +1157,7 @@ operand_f32_kernel(const float* __restrict__ x, long long ldx, long long rows, i
 
 }  // namespace meclip
 
+#include "split_k.cuh"
 #include "vocab_kernels.cuh"
 
 using namespace meclip;
@@ -1689,8 +1694,12 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 if (!use_dual) {
                     Operand a{gpanel[gb], plan.ldg / 64, true, plan.row_block}, b{X + r0 * ldx, ldx, true};
                     if (transposed_copies) b = Operand{xt + r0, plan.ld_xt, false};   // [d][K = rows] K-major
+                    const int bn = pick_contraction_bn(nc, d, overlap, transposed_copies);
+                    SplitK sk;
+                    if (vg != nullptr) sk = split_alone(p, nc, d, nr, bn, vg->split_buf, vg->split_bytes);
                     t_tag = TAG_DY;
-                    rc = launch_gemm(EPI_OUT, a, b, nc, d, nr, pick_contraction_bn(nc, d, overlap, transposed_copies), p, sy);
+                    rc = launch_gemm(EPI_OUT, a, b, nc, d, nr, bn, p, sy);
+                    if (rc == MECLIP_OK) rc = launch_split_sum(sk, sy);
                     if (rc) return rc;
                     if (overlap) MECLIP_CUDA(cudaEventRecord(side->dy[gb], sy));
                 }
@@ -1713,9 +1722,13 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     else { p.out = dx_scratch; p.ld_out = dn; p.out_bf16 = 0; }
                 }
                 if (use_dual) {
+                    SplitK sky, skx;
+                    if (vg != nullptr) split_dual(py, p, nr, nc, d, vg->split_buf, vg->split_bytes, sky, skx);
                     t_tag = TAG_DX;         // one launch: its time and FLOPs are booked under the dX tag
                     rc = launch_contractions_dual(gpanel[gb], plan.row_block, plan.ldg / 64, xt + r0, plan.ld_xt, yt + c0,
                                                   plan.ld_yt, nr, nc, d, py, p, sx);
+                    if (rc == MECLIP_OK) rc = launch_split_sum(sky, sx);
+                    if (rc == MECLIP_OK) rc = launch_split_sum(skx, sx);
                     if (rc) return rc;
                     if (overlap) {
                         MECLIP_CUDA(cudaEventRecord(side->dx[gb], sx));
@@ -1724,8 +1737,12 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 } else {
                     Operand a{gpanel[gb], plan.ldg / 64, false, plan.row_block}, b{Y + c0 * ldy, ldy, true};
                     if (transposed_copies) b = Operand{yt + c0, plan.ld_yt, false};   // [d][K = cols] K-major
+                    const int bn = pick_contraction_bn(nr, dn, overlap, transposed_copies);
+                    SplitK sk;
+                    if (vg != nullptr) sk = split_alone(p, nr, dn, nc, bn, vg->split_buf2, vg->split_bytes);
                     t_tag = TAG_DX;
-                    rc = launch_gemm(EPI_OUT, a, b, nr, dn, nc, pick_contraction_bn(nr, dn, overlap, transposed_copies), p, sx);
+                    rc = launch_gemm(EPI_OUT, a, b, nr, dn, nc, bn, p, sx);
+                    if (rc == MECLIP_OK) rc = launch_split_sum(sk, sx);
                     if (rc) return rc;
                     if (overlap) MECLIP_CUDA(cudaEventRecord(side->dx[gb], sx));
                 }

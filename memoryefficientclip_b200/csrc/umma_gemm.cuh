@@ -133,6 +133,12 @@ struct GemmParams {
     // Records of 3 words start at trace[2]; role r owns records [r*cap/3, (r+1)*cap/3); unused ones stay zero.
     unsigned long long* trace;
     unsigned int trace_capacity;
+    // Contractions (EPI_OUT) whose K is cut into parts that are tiles of their own: part q covers the K steps
+    // [q * k_part, (q + 1) * k_part) and writes its fp32 partial at out + q * split_stride elements; the host adds the
+    // parts afterwards.  splits >= 1; the second problem of a dual launch has its own.  For outputs of few tiles and
+    // a long K, which would otherwise keep a few SMs busy long after the others are done.
+    int splits, k_part, splits2, k_part2;
+    long long split_stride, split_stride2;
     // EPI_STATS: every (row, warp group of a column tile) stores {maximum of S fmul, sum 2^(S fmul - maximum), sum of
     // the same times its exponent, 0} in stats[row * stats_ld + 2 * column tile + group].  With top alternatives wanted
     // (chunk_max set) every (row, 32-column chunk) also stores the chunk's maximum of S fmul and, as one word, the
@@ -225,9 +231,34 @@ __device__ __forceinline__ int tile_problem(const GemmParams& p, int& tile) {
     if (p.dual && tile >= p.tiles0) { tile -= p.tiles0; return 1; }
     return 0;
 }
-__device__ __forceinline__ OutDesc out_desc(const GemmParams& p, int problem) {
-    if (problem == 0) return OutDesc{p.m, p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc};
-    return OutDesc{p.m2, p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2};
+__device__ __forceinline__ OutDesc out_desc(const GemmParams& p, int problem, int part = 0) {
+    if (problem == 0) return OutDesc{p.m, part > 0 ? reinterpret_cast<float*>(p.out) + part * p.split_stride : p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc};
+    return OutDesc{p.m2, part > 0 ? reinterpret_cast<float*>(p.out2) + part * p.split_stride2 : p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2};
+}
+// Tiles of a problem, parts of K included.
+template <int EPI>
+__device__ __forceinline__ int problem_tiles(const GemmParams& p, int problem) {
+    const int splits = EPI != EPI_OUT ? 1 : problem == 0 ? p.splits : p.splits2;
+    return (problem == 0 ? p.num_m_tiles : p.num_m_tiles2) * p.num_n_tiles * splits;
+}
+// Part of K of a tile id that is relative to its problem; the id is made relative to the part.
+template <int EPI>
+__device__ __forceinline__ int tile_part(const GemmParams& p, int& tile, int problem) {
+    if (EPI != EPI_OUT) return 0;
+    if ((problem == 0 ? p.splits : p.splits2) == 1) return 0;
+    const int per_part = (problem == 0 ? p.num_m_tiles : p.num_m_tiles2) * p.num_n_tiles;
+    const int part = tile / per_part;
+    tile -= part * per_part;
+    return part;
+}
+// K steps of a part: first one and how many.
+template <int EPI>
+__device__ __forceinline__ int part_steps(const GemmParams& p, int problem, int part, int& first) {
+    const int all = problem == 0 ? p.k_steps : p.k_steps2;
+    if (EPI != EPI_OUT) { first = 0; return all; }
+    const int size = problem == 0 ? p.k_part : p.k_part2;
+    first = part * size;
+    return min(size, all - first);
 }
 
 __device__ __forceinline__ void tile_coords(const GemmParams& p, int tile, int& mt, int& nt, int problem = 0) {
@@ -275,7 +306,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int num_tiles = p.num_m_tiles * p.num_n_tiles;
+    const int num_tiles = problem_tiles<EPI>(p, 0);
     const int num_stages = p.num_stages;
     volatile int* abort_flag = &tail->abort_flag;
     const unsigned long long wl = p.wait_limit_ns;      // bound of every wait below (host-set, 2 s by default)
@@ -337,11 +368,13 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 // nothing but the atomic, so nothing waits for its round trip before the strip ends.
                 if (left == strip && p.tile_counter != nullptr)
                     asm volatile("atom.global.add.u32 %0, [%1], 1;" : "=r"(next_unit) : "l"(p.tile_counter) : "memory");
-                int mt, nt;
-                tile_coords(p, tile, mt, nt);
+                int mt, nt, t_rel = tile, ks0;
+                const int part = tile_part<EPI>(p, t_rel, 0);
+                tile_coords(p, t_rel, mt, nt);
+                const int k_steps = part_steps<EPI>(p, 0, part, ks0);
                 const int m0 = mt * BM, n0 = nt * p.bn;
                 trace_event(p, 0, ntrace, TR_LOAD_BEGIN, tile);
-                for (int ks = 0; ks < p.k_steps; ++ks) {
+                for (int ks = ks0; ks < ks0 + k_steps; ++ks) {
                     if (!mbar_wait(smem_u32(&tail->empty_bar[stage]), phase ^ 1u, abort_flag, true, wl)) { ok = false; break; }
                     const uint32_t full = smem_u32(&tail->full_bar[stage]);
                     mbar_expect_tx(full, stage_tx);
@@ -403,11 +436,13 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                 if (!mbar_wait(smem_u32(&tail->tmem_empty_bar[acc]), acc_phase ^ 1u, abort_flag, true, wl)) break;
                 tc_fence_after();
                 trace_event(p, 1, ntrace, TR_MMA_BEGIN, tile);
-                int mt_, nt_;
-                tile_coords(p, tile, mt_, nt_);
+                int mt_, nt_, t_rel = tile, ks0;
+                const int part = tile_part<EPI>(p, t_rel, 0);
+                tile_coords(p, t_rel, mt_, nt_);
+                const int k_steps = part_steps<EPI>(p, 0, part, ks0);
                 const uint32_t idesc = (nt_ == p.num_n_tiles - 1) ? p.idesc_last : p.idesc;
                 const uint32_t tmem_d = tmem_base + (uint32_t)acc * MAX_BN;
-                for (int ks = 0; ks < p.k_steps; ++ks) {
+                for (int ks = 0; ks < k_steps; ++ks) {
                     if (!mbar_wait(smem_u32(&tail->full_bar[stage]), phase, abort_flag, true, wl)) { ok = false; break; }
                     tc_fence_after();
                     if (ks == 0) trace_event(p, 1, ntrace, TR_MMA_FIRST_DATA, tile);
@@ -450,8 +485,9 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             if (++slot == SCHED_DEPTH) { slot = 0; sphase ^= 1u; }
             ok = named_bar_and(2, EPI_THREADS, ok);
             if (!ok || tile < 0) break;
-            int mt, nt;
-            tile_coords(p, tile, mt, nt);
+            int mt, nt, t_rel = tile;
+            const int part = tile_part<EPI>(p, t_rel, 0);
+            tile_coords(p, t_rel, mt, nt);
             ok = mbar_wait(smem_u32(&tail->tmem_full_bar[acc]), acc_phase, abort_flag, false, wl);
             ok = named_bar_and(2, EPI_THREADS, ok);
             if (!ok) break;
@@ -459,7 +495,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * MAX_BN;
             const uint32_t free_bar = smem_u32(&tail->tmem_empty_bar[acc]);
             if (threadIdx.x == 64) trace_event(p, 2, ntrace, TR_EPI_BEGIN, tile);
-            epilogue_tile<EPI>(p, out_desc(p, 0), &tmap_c, tail, st, taddr, mt * BM, nt * p.bn,
+            epilogue_tile<EPI>(p, out_desc(p, 0, part), &tmap_c, tail, st, taddr, mt * BM, nt * p.bn,
                                (nt == p.num_n_tiles - 1) ? p.bn_last : p.bn, warp, lane,
                                [free_bar, &p, &ntrace, tile]() {
                                    mbar_arrive(free_bar);

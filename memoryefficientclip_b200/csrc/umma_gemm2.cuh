@@ -48,7 +48,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();          // 0 = leader of the pair
-    const int num_tiles = DUAL ? p.tiles0 + p.num_m_tiles2 * p.num_n_tiles : p.num_m_tiles * p.num_n_tiles;
+    const int num_tiles = DUAL ? p.tiles0 + problem_tiles<EPI>(p, 1) : problem_tiles<EPI>(p, 0);
     const int num_clusters = (int)(gridDim.x >> 1);
     const int cluster_id = blockIdx.x >> 1;
     const int num_stages = p.num_stages;
@@ -120,15 +120,17 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 if (tile < 0) break;
                 int mt, nt, t_rel = tile;
                 const int prob = DUAL ? tile_problem(p, t_rel) : 0;
+                const int part = tile_part<EPI>(p, t_rel, prob);
                 tile_coords(p, t_rel, mt, nt, prob);
                 const bool a_mn = DUAL ? prob == 0 : A_MODE == 1;
                 const CUtensorMap* ta = (DUAL && prob == 1) ? &tmap_c : &tmap_a;
                 const CUtensorMap* tb = (DUAL && prob == 1) ? &tmap_d : &tmap_b;
-                const int k_steps = (DUAL && prob == 1) ? p.k_steps2 : p.k_steps;
+                int ks0;
+                const int k_steps = part_steps<EPI>(p, prob, part, ks0);
                 const int tile_bn = (nt == p.num_n_tiles - 1) ? p.bn_last : p.bn;
                 const int m0 = mt * PAIR_BM + (int)rank * BM;              // this CTA's rows
                 const int n0 = nt * p.bn + (int)rank * (tile_bn >> 1);      // this CTA's share of the B rows
-                for (int ks = 0; ks < k_steps; ++ks) {
+                for (int ks = ks0; ks < ks0 + k_steps; ++ks) {
                     if (!mbar_wait(smem_u32(&tail->empty_bar[stage]), phase ^ 1u, abort_flag, true, wl)) { ok = false; break; }
                     const uint32_t full_local = smem_u32(&tail->full_bar[stage]);
                     const uint32_t full = mapa_u32(full_local, 0);    // the leader's barrier counts both CTAs' bytes
@@ -183,9 +185,11 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
                 tc_fence_after();
                 int mt_, nt_, t_rel = tile;
                 const int prob = DUAL ? tile_problem(p, t_rel) : 0;
+                const int part = tile_part<EPI>(p, t_rel, prob);
                 tile_coords(p, t_rel, mt_, nt_, prob);
                 const bool a_mn = DUAL ? prob == 0 : A_MODE == 1;
-                const int k_steps = (DUAL && prob == 1) ? p.k_steps2 : p.k_steps;
+                int ks0;
+                const int k_steps = part_steps<EPI>(p, prob, part, ks0);
                 const bool last_nt = nt_ == p.num_n_tiles - 1;
                 const uint32_t idesc = (DUAL && prob == 1) ? (last_nt ? p.idesc_last_p2 : p.idesc_p2)
                                                            : (last_nt ? p.idesc_last : p.idesc);
@@ -253,6 +257,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             if (!ok || tile < 0) break;
             int mt, nt, t_rel = tile;
             const int prob = DUAL ? tile_problem(p, t_rel) : 0;
+            const int part = tile_part<EPI>(p, t_rel, prob);
             tile_coords(p, t_rel, mt, nt, prob);
             ok = mbar_wait(smem_u32(&tail->tmem_full_bar[acc]), acc_phase, abort_flag, false, wl);
             ok = named_bar_and(2, EPI_THREADS, ok);
@@ -260,7 +265,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)acc * MAX_BN;
             const uint32_t free_bar = mapa_u32(smem_u32(&tail->tmem_empty_bar[acc]), 0);   // the leader's barrier
-            epilogue_tile<EPI>(p, out_desc(p, prob), &tmap_c, tail, st, taddr, mt * PAIR_BM + (int)rank * BM, nt * p.bn,
+            epilogue_tile<EPI>(p, out_desc(p, prob, part), &tmap_c, tail, st, taddr, mt * PAIR_BM + (int)rank * BM, nt * p.bn,
                                (nt == p.num_n_tiles - 1) ? p.bn_last : p.bn, warp, lane,
                                [free_bar, lane]() {
                                    __syncwarp();

@@ -133,23 +133,36 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     return MECLIP_OK;
 }
 
-struct VocabGradPlan { size_t rows_bytes, grad_bytes; bool transposed; };
+struct VocabGradPlan {
+    size_t rows_bytes, split_bytes, grad_bytes;
+    int split_bufs;
+    bool transposed;
+    size_t total() const { return 2 * rows_bytes + split_bufs * split_bytes + grad_bytes; }
+};
 static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long d) {
     VocabGradPlan g;
     g.rows_bytes = round_up((size_t)rows * 4, 256);
     // transposed copies of the operands and side streams pay for themselves when the contractions are long
     g.transposed = rows >= 1024 && transposes_allowed();
-    g.grad_bytes = plan_grad(rows, vocab, d, g.transposed).total();
+    const GradPlan plan = plan_grad(rows, vocab, d, g.transposed);
+    g.grad_bytes = plan.total();
+    const bool dual = g.transposed && d >= 256 && dual_allowed() && pair_mode() != 0 && !wide_allowed();
+    g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual);
+    g.split_bufs = g.transposed && !dual ? 2 : 1;          // the two contractions on two streams
     return g;
 }
 
 static int vocab_grad(VocabGrad vg, const void* x_bf16, const void* t_bf16, int64_t rows, int64_t vocab, int64_t d,
                       int64_t ldx, int64_t ldt, float temperature, void* dx, int dx_mode, int64_t lddx, void* dt,
                       int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
+    uint8_t* split = ws + 2 * plan.rows_bytes;
+    vg.split_buf = reinterpret_cast<float*>(split);
+    vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
+    vg.split_bytes = plan.split_bytes;
     return grad_impl(MECLIP_SIGLIP, x_bf16, t_bf16, rows, vocab, d, ldx, ldt, temperature, 0, 0, nullptr, nullptr, nullptr,
-                     1.f, dx, dx_mode, lddx, dt, dt_mode, lddt, ws + 2 * plan.rows_bytes, plan.grad_bytes, status, s,
-                     plan.transposed && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false, DeviceScalars(),
-                     true, nullptr, 0, nullptr, 0, &vg);
+                     1.f, dx, dx_mode, lddx, dt, dt_mode, lddt, split + plan.split_bufs * plan.split_bytes, plan.grad_bytes,
+                     status, s, plan.transposed && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false,
+                     DeviceScalars(), true, nullptr, 0, nullptr, 0, &vg);
 }
 
 static int check_vocab_grad(const char* what, const void* x16, const void* t16, int64_t ldx16, int64_t ldt16, int64_t d,
@@ -158,8 +171,7 @@ static int check_vocab_grad(const char* what, const void* x16, const void* t16, 
         (x16 != nullptr && (ldx16 < d || ldt16 < d || ldx16 % 8 != 0 || ldt16 % 8 != 0 || !aligned16(x16) || !aligned16(t16))))
         return fail(MECLIP_EINVAL, "%s: fp16 operands come as a pair, 16-byte aligned with pitches multiples of 8", what);
     if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(MECLIP_EINVAL, "%s: workspace must be 256-byte aligned", what);
-    if (ws_bytes < 2 * plan.rows_bytes + plan.grad_bytes)
-        return fail(MECLIP_ENOSPC, "%s: workspace %zu < %zu bytes", what, ws_bytes, 2 * plan.rows_bytes + plan.grad_bytes);
+    if (ws_bytes < plan.total()) return fail(MECLIP_ENOSPC, "%s: workspace %zu < %zu bytes", what, ws_bytes, plan.total());
     return MECLIP_OK;
 }
 
@@ -174,8 +186,7 @@ size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
 
 size_t meclip_vocab_grad_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
     if (rows < 1 || vocab < 1 || d < 1) return 0;
-    const VocabGradPlan g = plan_vocab_grad(rows, vocab, d);
-    return 2 * g.rows_bytes + g.grad_bytes;
+    return plan_vocab_grad(rows, vocab, d).total();
 }
 
 int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,

@@ -31,6 +31,8 @@ struct VocabGrad {
     const __nv_bfloat16* y_f16;
     long long ldy_f16;
     float tile_fmul;
+    float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
+    size_t split_bytes;               // of each
 };
 
 // The tensor cores cut what does not fit into an fp32 accumulator instead of rounding it, once every 16 products, so a
