@@ -337,12 +337,28 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         // row factor: g / r_i for the softmax losses, plain g when there are no row sums (sigmoid loss)
         const float inv_r = (VOCAB || !rvalid) ? 0.f : (p.r != nullptr ? p.coef * st.gscale / __ldg(p.r + grow) : p.coef * st.gscale);
         float v_lse = 1e30f, v_a = 0.f, v_b = 0.f;          // a row past the edge: 2^-huge = 0
+        int v_col[VOCAB_TILE_ENTRIES];                      // tile columns of the row's entries, -1: none here
+        float v_val[VOCAB_TILE_ENTRIES];
+#pragma unroll
+        for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e) { v_col[e] = -1; v_val[e] = 0.f; }
+        bool v_here = false;
         if (VOCAB) {
             if (rvalid) {
-                v_lse = __ldg(p.row_lse + grow);
-                v_a = __ldg(p.row_a + grow);
-                if (p.row_b != nullptr) v_b = __ldg(p.row_b + grow);
+                v_lse = __ldg(p.vc.row_lse + grow);
+                vocab_row_factors(p.vc, grow, v_a, v_b);
+                if (p.vc.entries_in_tile) {
+#pragma unroll
+                    for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e)
+                        if (e < p.vc.k) {
+                            const long long col = p.vc.tokens[(long long)grow * p.vc.k + e] - p.vc_col0 - n0;
+                            if (col >= 0 && col < p.bn && n0 + col < p.n && vocab_entry(p.vc, grow, e, v_a, v_b, v_val[e])) v_col[e] = (int)col;
+                        }
+                }
             }
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e) any |= v_col[e] >= 0;
+            v_here = __any_sync(0xffffffffu, any);
         } else {
             named_bar_sync(1, EPI_THREADS);
         }
@@ -382,6 +398,14 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
                     } else {
 #pragma unroll
                         for (int c = 0; c < 32; ++c) gv[c] -= (c == jdc) ? dsub : 0.f;
+                    }
+                }
+                if (VOCAB && v_here) {
+#pragma unroll
+                    for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e) {
+                        const int jc = (v_col[e] >> 5) == ch ? (v_col[e] & 31) : -1;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) gv[c] = (c == jc) ? v_val[e] : gv[c];
                     }
                 }
                 if (!full_tile) {     // columns past the panel edge share a stored chunk with valid ones: zero them

@@ -57,7 +57,7 @@ enum { TAG_SUMS = 0, TAG_COEF = 1, TAG_DX = 2, TAG_DY = 3, TAG_ROW = 4, TAG_NORM
        TAG_TRANSPOSE = 7, TAG_ACCUM = 8, TAG_COUNT = 9 };
 struct ProfileRecord { int tag; cudaEvent_t start, stop; double flops; };
 static std::mutex g_prof_mutex;
-static bool g_prof_on = false;
+static std::atomic<bool> g_prof_on{false};
 static std::vector<ProfileRecord> g_prof;
 static thread_local int t_tag = TAG_ROW;
 
@@ -65,8 +65,7 @@ struct ScopedTiming {   // brackets one launch with events on its stream while p
     cudaStream_t s; bool on; ProfileRecord rec;
     ScopedTiming(cudaStream_t stream, int tag, double flops) : s(stream), on(false) {
         g_launches.fetch_add(1, std::memory_order_relaxed);
-        std::lock_guard<std::mutex> lock(g_prof_mutex);
-        if (!g_prof_on) return;
+        if (!g_prof_on.load(std::memory_order_relaxed)) return;
         rec.tag = tag; rec.flops = flops;
         if (cudaEventCreate(&rec.start) != cudaSuccess) return;
         if (cudaEventCreate(&rec.stop) != cudaSuccess) { cudaEventDestroy(rec.start); return; }
@@ -1583,8 +1582,10 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     const bool use_dual = want_dx && want_dy && transposed_copies && dual_allowed() && pair_mode() != 0 && !wide_allowed() &&
                           dn == d && d >= 256 && g_trace_buf == nullptr;
     if (use_dual) sy = sx;      // one side stream carries the transposes and the contractions
-    // the tile counters are the only part of the workspace that has to start at zero
-    MECLIP_CUDA(cudaMemsetAsync(counters, 0, plan.counter_bytes, s0));
+    // the tile counters are the only part of the workspace that has to start at zero; a vocabulary's gradient on one stream
+    // deals its tiles in turn instead (nothing shares the GPU with it, and a launch less is a few microseconds)
+    const bool use_counters = vg == nullptr || overlap;
+    if (use_counters) MECLIP_CUDA(cudaMemsetAsync(counters, 0, plan.counter_bytes, s0));
     if (transposed_copies) {
         // Y^T is only read by the dX contractions and X^T by the dY contractions, so with side streams
         // the transposes run there, under the first coefficient pass
@@ -1651,16 +1652,16 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 if (vg != nullptr) {
                     p.sigmoid = 0;
                     p.fmul = vg->tile_fmul;
-                    p.row_lse = vg->row_lse + r0;
-                    p.row_a = vg->row_a + r0;
-                    p.row_b = vg->row_b != nullptr ? vg->row_b + r0 : nullptr;
+                    p.vc = vocab_rows_from(vg->coef, r0);
+                    p.vc_col0 = c0;
+                    if (!use_counters) p.tile_counter = nullptr;
                     if (vg->x_f16 != nullptr) {
                         a = Operand{vg->x_f16 + r0 * vg->ldx_f16, vg->ldx_f16, false, 0, false, true};
                         b = Operand{vg->y_f16 + c0 * vg->ldy_f16, vg->ldy_f16, false, 0, false, true};
                     }
                     // 256-column tiles beyond one row tile: only those run on CTA pairs
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
-                    if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, cols, gpanel[gb], plan.row_block, s0);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                 }
@@ -1678,7 +1679,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
             if (want_dy) {
                 GemmParams& p = py;
                 p.status = status;
-                p.tile_counter = counters + 3 * t + 2;
+                p.tile_counter = use_counters ? counters + 3 * t + 2 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dy) + (size_t)c0 * lddy * dy_elt;
                 float* scratch = dy_scratch + (size_t)c0 * d;
                 if (dy_mode == MECLIP_ACCUM_F32) {
@@ -1709,7 +1710,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 GemmParams p;
                 std::memset(&p, 0, sizeof(p));
                 p.status = status;
-                p.tile_counter = counters + 3 * t + 1;
+                p.tile_counter = use_counters ? counters + 3 * t + 1 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dx) + (size_t)r0 * lddx * dx_elt;
                 if (dx_mode == MECLIP_ACCUM_F32) {
                     p.acc_in = reinterpret_cast<const float*>(user); p.ld_acc = lddx;

@@ -119,6 +119,10 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
         p.chunk_second = const_cast<uint32_t*>(r.chunk_second);
         p.chunk_ld = r.chunk_ld;
         p.status = status;
+        if (DISTILL && r.loss != nullptr) {
+            b.blocks_done = reinterpret_cast<unsigned int*>(ws) + 3;
+            if (r0 + plan.row_block < rows) b.loss = nullptr;      // only behind the last block of rows
+        }
         const bool f16 = dtype == MECLIP_F16;
         Operand a{b.x, r.ldx, false, 0, false, f16}, t{r.y, r.ldy, false, 0, false, f16};
         t_tag = TAG_SUMS;
@@ -137,7 +141,7 @@ struct VocabGradPlan {
     size_t rows_bytes, split_bytes, grad_bytes;
     int split_bufs;
     bool transposed;
-    size_t total() const { return 2 * rows_bytes + split_bufs * split_bytes + grad_bytes; }
+    size_t total() const { return rows_bytes + split_bufs * split_bytes + grad_bytes; }
 };
 static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long d) {
     VocabGradPlan g;
@@ -155,7 +159,7 @@ static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long 
 static int vocab_grad(VocabGrad vg, const void* x_bf16, const void* t_bf16, int64_t rows, int64_t vocab, int64_t d,
                       int64_t ldx, int64_t ldt, float temperature, void* dx, int dx_mode, int64_t lddx, void* dt,
                       int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
-    uint8_t* split = ws + 2 * plan.rows_bytes;
+    uint8_t* split = ws + plan.rows_bytes;
     vg.split_buf = reinterpret_cast<float*>(split);
     vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
     vg.split_bytes = plan.split_bytes;
@@ -226,23 +230,22 @@ int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, cons
     const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
     rc = check_vocab_grad("token_log_probs_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
     if (rc) return rc;
-    cudaStream_t s = (cudaStream_t)stream;
-    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-    float* row_a = reinterpret_cast<float*>(ws);
-    float* row_b = grad_entropy != nullptr ? reinterpret_cast<float*>(ws + plan.rows_bytes) : nullptr;
-    const int wpb = ROW_KERNEL_THREADS / 32;
-    {
-        ScopedTiming timing(s, TAG_ROW, (double)rows * (12.0 * per_row + 16.0));
-        token_grad_rows_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
-            grad_log_probs, grad_entropy, entropy, reinterpret_cast<const long long*>(tokens), (int)per_row, rows, vocab,
-            1.f / temperature, row_a, row_b);
+    VocabCoef c{};
+    c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(tokens); c.k = (int)per_row;
+    c.vocab = vocab; c.inv_t = 1.f / temperature;
+    c.grad_log_probs = grad_log_probs; c.grad_entropy = grad_entropy; c.entropy = entropy;
+    c.entries_in_tile = per_row > 0 && per_row <= VOCAB_TILE_ENTRIES && grad_log_probs != nullptr;
+    if (per_row > VOCAB_TILE_ENTRIES && grad_log_probs != nullptr) {
+        float* row_g = reinterpret_cast<float*>(workspace);
+        const int wpb = ROW_KERNEL_THREADS / 32;
+        ScopedTiming timing((cudaStream_t)stream, TAG_ROW, (double)rows * 12.0 * per_row);
+        token_grad_sum_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, (cudaStream_t)stream>>>(c, rows, row_g);
         MECLIP_CUDA(cudaGetLastError());
+        c.row_g = row_g;
     }
-    VocabGrad vg{row_lse, row_a, row_b, reinterpret_cast<const long long*>(tokens), token_scores, (int)per_row,
-                 grad_log_probs, nullptr, 1.f / temperature, (const __nv_bfloat16*)x_f16, ldx_f16,
-                 (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
+    VocabGrad vg{c, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
     return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
-                      lddt, ws, plan, status, s);
+                      lddt, reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }
 
 int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
@@ -268,12 +271,8 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
     r.row_lse = row_lse; r.token_s2 = token_scores;
     r.teacher_logits = teacher_logits; r.teacher_dtype = teacher_dtype; r.inv_teacher_t = 1.f / teacher_temperature;
     r.teacher_probs = teacher_probs; r.row_loss = row_loss; r.row_has = row_has;
-    rc = vocab_forward<true>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
-    if (rc || loss == nullptr) return rc;
-    ScopedTiming timing((cudaStream_t)stream, TAG_ROW, 8.0 * (double)rows);
-    distill_reduce_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(row_loss, row_has, rows, mean, loss, inv_count);
-    MECLIP_CUDA(cudaGetLastError());
-    return MECLIP_OK;
+    r.all_loss = row_loss; r.all_has = row_has; r.all_rows = rows; r.mean = mean; r.loss = loss; r.inv_count = inv_count;
+    return vocab_forward<true>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
 }
 
 int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16, int64_t rows,
@@ -290,19 +289,14 @@ int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* 
     const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
     rc = check_vocab_grad("distill_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
     if (rc) return rc;
-    cudaStream_t s = (cudaStream_t)stream;
-    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-    float* row_a = reinterpret_cast<float*>(ws);
-    {
-        ScopedTiming timing(s, TAG_ROW, (double)rows * 12.0);
-        distill_grad_rows_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, s>>>(grad_out, grad_per_row, inv_count, row_has, rows,
-                                                                               1.f / temperature, row_a);
-        MECLIP_CUDA(cudaGetLastError());
-    }
-    VocabGrad vg{row_lse, row_a, nullptr, reinterpret_cast<const long long*>(teacher_tokens), token_scores, (int)per_row,
-                 teacher_probs, row_a, -1.f, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
+    VocabCoef c{};
+    c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(teacher_tokens);
+    c.k = (int)per_row; c.distill = 1; c.vocab = vocab; c.inv_t = 1.f / temperature;
+    c.grad_out = grad_out; c.grad_per_row = grad_per_row; c.factor = inv_count; c.row_has = row_has; c.probs = teacher_probs;
+    c.entries_in_tile = per_row <= VOCAB_TILE_ENTRIES;
+    VocabGrad vg{c, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
     return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
-                      lddt, ws, plan, status, s);
+                      lddt, reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }
 
 }  // extern "C"

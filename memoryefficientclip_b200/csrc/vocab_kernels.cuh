@@ -15,17 +15,9 @@ static constexpr int VOCAB_THREADS = 256;
 static constexpr int VOCAB_MAX_ENTRIES = 256;      // given tokens or teacher entries of one row
 static constexpr int VOCAB_MAX_TOP = 32;           // top alternatives: one per lane
 
-// Entries (given tokens, teacher entries) of a backward, and the row factors of the dense part.
+// A backward: the coefficients, with their rows counted from the first one of the problem, and where the scores come from.
 struct VocabGrad {
-    const float* row_lse;
-    const float* row_a;
-    const float* row_b;               // null: no log2 p term
-    const long long* tokens;          // [rows, k]
-    const float* token_s2;            // [rows, k], saved by the forward
-    int k;
-    const float* entry;               // [rows, k] and
-    const float* entry_scale;         // [rows] or null: the entry's own term is entry * entry_scale * entry_mul
-    float entry_mul;
+    VocabCoef coef;
     const __nv_bfloat16* x_f16;       // fp16 operands for the scores (typed as 16-bit words), null: the bf16 ones
     long long ldx_f16;
     const __nv_bfloat16* y_f16;
@@ -34,6 +26,20 @@ struct VocabGrad {
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
     size_t split_bytes;               // of each
 };
+// The coefficients of the rows from r0 on.
+static VocabCoef vocab_rows_from(VocabCoef v, long long r0) {
+    v.row_lse += r0;
+    if (v.tokens != nullptr) v.tokens += r0 * v.k;
+    if (v.token_s2 != nullptr) v.token_s2 += r0 * v.k;
+    if (v.grad_log_probs != nullptr) v.grad_log_probs += r0 * v.k;
+    if (v.grad_entropy != nullptr) v.grad_entropy += r0;
+    if (v.entropy != nullptr) v.entropy += r0;
+    if (v.grad_per_row && v.grad_out != nullptr) v.grad_out += r0;
+    if (v.row_has != nullptr) v.row_has += r0;
+    if (v.row_g != nullptr) v.row_g += r0;
+    if (v.probs != nullptr) v.probs += r0 * v.k;
+    return v;
+}
 
 // The tensor cores cut what does not fit into an fp32 accumulator instead of rounding it, once every 16 products, so a
 // score comes out too small in magnitude, on average by a part of the partial sums it ran through.  For a score that
@@ -63,6 +69,12 @@ struct VocabRows {
     float* teacher_probs;             // [rows, k]
     float* row_loss;                  // [rows]
     float* row_has;                   // [rows], 1 where the teacher says anything
+    // sum over the rows by the last block, for the last block of rows of the problem: loss null otherwise
+    unsigned int* blocks_done;        // the unused fourth word of stats[0], which the tile pass has stored as zero
+    const float *all_loss, *all_has;  // of all rows, all_rows of them
+    long long all_rows;
+    int mean;
+    float *loss, *inv_count;
 };
 
 __device__ __forceinline__ void half8(const __nv_bfloat16* p, float (&v)[8]) { load8(p, v); }
@@ -456,6 +468,37 @@ __device__ __forceinline__ int row_top_rank(const RowTopShared& sh, int n, int i
     return before;
 }
 
+// loss = sum of the rows' losses, divided by the number of rows that have one when `mean`; inv_count gets the factor.
+// By the block that is done last, in a fixed order over the rows.  No row at all: loss 0, factor 0.
+__device__ __forceinline__ void distill_reduce(const VocabRows& p) {
+    __shared__ double part[VOCAB_THREADS], cnt[VOCAB_THREADS];
+    __shared__ bool last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(p.blocks_done, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    double a = 0.0, c = 0.0;
+#pragma unroll 8
+    for (long long i = threadIdx.x; i < p.all_rows; i += VOCAB_THREADS) {
+        a += (double)__ldcg(p.all_loss + i);           // other blocks wrote these: not from this SM's L1
+        c += (double)__ldcg(p.all_has + i);
+    }
+    part[threadIdx.x] = a;
+    cnt[threadIdx.x] = c;
+    __syncthreads();
+    for (int s = VOCAB_THREADS / 2; s >= 1; s >>= 1) {
+        if ((int)threadIdx.x < s) { part[threadIdx.x] += part[threadIdx.x + s]; cnt[threadIdx.x] += cnt[threadIdx.x + s]; }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const double f = p.mean ? (cnt[0] > 0.0 ? 1.0 / cnt[0] : 0.0) : 1.0;
+        *p.loss = (float)(part[0] * f);
+        *p.inv_count = (float)f;
+    }
+}
+
 // One row per G threads.  Bound by memory latency: a row reads its 2 V / 256 partial sums, V / 32 chunk maxima (with
 // alternatives) and one table row per entry; many rows in flight per SM hide that (G = 32), and a few rows are spread
 // over a block each (G = 256).
@@ -467,7 +510,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     const int gt = (int)threadIdx.x % G, lane = gt & 31, w = gt >> 5;
     const long long row = (long long)blockIdx.x * (VOCAB_THREADS / G) + threadIdx.x / G;
     const bool active = row < p.rows;             // the same for the row's threads
-    if (!TOP && !active) return;                  // (a block of G = 256 has one row, warps of G = 32 do not meet)
+    if (!TOP && !DISTILL && !active) return;      // (a block of G = 256 has one row, warps of G = 32 do not meet)
     uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap);
     float* red = reinterpret_cast<float*>(smem);
     float* s2 = reinterpret_cast<float*>(smem + 64 * 8);
@@ -584,6 +627,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             }
         }
     }
+    if (DISTILL && p.loss != nullptr) distill_reduce(p);
     if (TOP) {
         const RowTopShared sh = row_top_shared(top_smem);
         const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap), bw = threadIdx.x >> 5;
@@ -623,104 +667,47 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     }
 }
 
-// loss = sum of the rows' losses, divided by the number of rows that have one when `mean`; inv_count gets the factor.
-// One block, fixed order.  No row at all: loss 0, factor 0.
-__global__ void __launch_bounds__(1024)
-distill_reduce_kernel(const float* __restrict__ row_loss, const float* __restrict__ row_has, long long n, int mean,
-                      float* __restrict__ loss, float* __restrict__ inv_count) {
-    __shared__ double part[1024];
-    __shared__ double cnt[1024];
-    double a = 0.0, c = 0.0;
-#pragma unroll 4
-    for (long long i = threadIdx.x; i < n; i += 1024) {
-        a += (double)row_loss[i];
-        c += (double)row_has[i];
-    }
-    part[threadIdx.x] = a;
-    cnt[threadIdx.x] = c;
-    __syncthreads();
-    for (int s = 512; s >= 1; s >>= 1) {
-        if ((int)threadIdx.x < s) { part[threadIdx.x] += part[threadIdx.x + s]; cnt[threadIdx.x] += cnt[threadIdx.x + s]; }
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-        const double f = mean ? (cnt[0] > 0.0 ? 1.0 / cnt[0] : 0.0) : 1.0;
-        *loss = (float)(part[0] * f);
-        *inv_count = (float)f;
-    }
-}
-
-// Row factors of the backward, dz_ij = p_ij (a + b log2 p_ij) + entries, divided by T (in `inv_t`).
-//   token scoring: a = -(sum_k g_k + h H), b = -h ln 2, g_k over the tokens inside the table
+// Sums of the gradients of a row's log probabilities, over the tokens inside the table.
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-token_grad_rows_kernel(const float* __restrict__ grad_log_probs, const float* __restrict__ grad_entropy,
-                       const float* __restrict__ entropy, const long long* __restrict__ tokens, int k, long long rows,
-                       long long vocab, float inv_t, float* __restrict__ row_a, float* __restrict__ row_b) {
+token_grad_sum_kernel(const __grid_constant__ VocabCoef v, long long rows, float* __restrict__ row_g) {
     const long long row = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= rows) return;
     float g = 0.f;
-    if (grad_log_probs != nullptr)
-        for (int e = lane; e < k; e += 32) {
-            const long long j = tokens[row * k + e];
-            if (j >= 0 && j < vocab) g += grad_log_probs[row * k + e];
-        }
-    g = warp_sum(g);
-    if (lane == 0) {
-        const float h = grad_entropy != nullptr ? grad_entropy[row] : 0.f;
-        // h = 0 takes no part, whatever the row's entropy is
-        row_a[row] = -(g + (h != 0.f ? h * entropy[row] : 0.f)) * inv_t;
-        if (row_b != nullptr) row_b[row] = -h * 0.6931471805599453f * inv_t;
+    for (int e = lane; e < v.k; e += 32) {
+        const long long j = v.tokens[row * v.k + e];
+        if (j >= 0 && j < v.vocab) g += v.grad_log_probs[row * v.k + e];
     }
+    g = warp_sum(g);
+    if (lane == 0) row_g[row] = g;
 }
 
-//   distillation: a = w = grad_out * factor / T for the rows that have a teacher, b = 0
-__global__ void __launch_bounds__(256)
-distill_grad_rows_kernel(const float* __restrict__ grad_out, int per_row, const float* __restrict__ factor,
-                         const float* __restrict__ row_has, long long rows, float inv_t, float* __restrict__ row_a) {
-    const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (row >= rows) return;
-    const float f = factor != nullptr ? __ldg(factor) : 1.f;
-    row_a[row] = row_has[row] > 0.f ? grad_out[per_row ? row : 0] * f * inv_t : 0.f;
-}
-
-// Puts the entries' own terms into a coefficient panel: G_ij = p_ij (a + b log2 p_ij) + sum of the row's terms at j,
-// formed in fp32 from the saved scores and rounded to bf16 once, over what the tile pass stored there.  One warp per
-// row; of entries with the same token the first writes and adds the others' terms.
+// Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved scores and rounded to bf16 once, over
+// what the tile pass stored there.  One warp per row.  (Up to VOCAB_TILE_ENTRIES entries per row the tile pass does it.)
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-vocab_entries_kernel(const __grid_constant__ VocabGrad g, long long r0, long long nr, long long c0, long long nc,
+vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long long c0, long long nc,
                      __nv_bfloat16* __restrict__ panel, long long rows_alloc) {
     const long long i = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= nr) return;
-    const long long row = r0 + i;
-    const long long* tok = g.tokens + row * g.k;
-    const float scale = (g.entry_scale != nullptr ? g.entry_scale[row] : 1.f) * g.entry_mul;
-    for (int e = lane; e < g.k; e += 32) {
-        const long long j = tok[e];
+    float a, b;
+    vocab_row_factors(v, i, a, b);
+    for (int e = lane; e < v.k; e += 32) {
+        const long long j = v.tokens[i * v.k + e];
         if (j < c0 || j >= c0 + nc) continue;          // absent, outside the table or in another panel
-        bool first = true;
-        float term = 0.f;
-        for (int o = 0; o < g.k; ++o)
-            if (tok[o] == j) {
-                if (o < e) { first = false; break; }
-                if (g.entry != nullptr) term += g.entry[row * g.k + o];
-            }
-        if (!first) continue;
-        const float u = g.token_s2[row * g.k + e] - g.row_lse[row];
-        const float b = g.row_b != nullptr ? g.row_b[row] : 0.f;
-        const float v = fmaf(exp2f(u), fmaf(b, u, g.row_a[row]), scale != 0.f ? term * scale : 0.f);
+        float value;
+        if (!vocab_entry(v, i, e, a, b, value)) continue;
         const long long col = j - c0;
-        panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = __float2bfloat16_rn(v);
+        panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = __float2bfloat16_rn(value);
     }
 }
 
-static int launch_vocab_entries(const VocabGrad& g, long long r0, long long nr, long long c0, long long nc, long long,
-                                __nv_bfloat16* panel, long long rows_alloc, cudaStream_t s) {
-    if (g.k == 0 || g.entry == nullptr) return MECLIP_OK;
+static int launch_vocab_entries(const VocabCoef& v, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
+                                long long rows_alloc, cudaStream_t s) {
+    if (v.k == 0 || v.entries_in_tile || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
     const int wpb = ROW_KERNEL_THREADS / 32;
-    ScopedTiming timing(s, TAG_ROW, (double)nr * g.k * 18.0);
-    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(g, r0, nr, c0, nc, panel, rows_alloc);
+    ScopedTiming timing(s, TAG_ROW, (double)nr * v.k * 18.0);
+    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }
