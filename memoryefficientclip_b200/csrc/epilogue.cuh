@@ -376,6 +376,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
                 st.stores_in_flight = 0;
             }
             __syncwarp();
+            uint32_t lo[VOCAB ? 32 : 1];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int ch = u * 2 + half;
@@ -426,14 +427,39 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
                     pk.w = pack_bf16x2(gv[pc * 8 + 6], gv[pc * 8 + 7]);
                     const int piece = half * 4 + pc;
                     *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) = pk;
+                    if (VOCAB && p.lo_chunk > 0) {       // what the rounding left, for the second panel
+                        const uint32_t hi[4] = {pk.x, pk.y, pk.z, pk.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float a = gv[pc * 8 + 2 * i] - __uint_as_float(hi[i] << 16);
+                            const float b = gv[pc * 8 + 2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u);
+                            lo[half * 16 + pc * 4 + i] = pack_bf16x2(a, b);
+                        }
+                    }
                 }
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
+            // with a second panel behind the first, chunks past the last column must not be stored into it
+            const bool store = !VOCAB || p.lo_chunk == 0 || (n0 >> 6) + u < (p.n + 63) >> 6;
+            if (lane == 0 && store) {
                 tma_store_3d(tmap_c, smem_u32(buf), 0, m0 + q * 32, (n0 >> 6) + u);
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 st.stores_in_flight = 1;
+            }
+            if (VOCAB && p.lo_chunk > 0 && store) {
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                __syncwarp();
+#pragma unroll
+                for (int piece = 0; piece < 8; ++piece)
+                    *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) =
+                        make_uint4(lo[piece * 4], lo[piece * 4 + 1], lo[piece * 4 + 2], lo[piece * 4 + 3]);
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_3d(tmap_c, smem_u32(buf), 0, m0 + q * 32, (n0 >> 6) + u + p.lo_chunk);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
             }
         }
         tc_fence_before();

@@ -827,8 +827,8 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     int rc;
     if (a.blocked_rows_alloc > 0) {
         // panel of G [rows x cols]: as A = G (K-major) rows = m, cols = k; as A = G^T (MN-major) rows = k, cols = m
-        if (a.mn_major) rc = make_tmap_blocked(&ta, a.ptr, k, (m + 63) / 64, a.blocked_rows_alloc, BK, a.ld);
-        else            rc = make_tmap_blocked(&ta, a.ptr, m, (k + 63) / 64, a.blocked_rows_alloc, BM, a.ld);
+        if (a.mn_major) rc = make_tmap_blocked(&ta, a.ptr, k, p.lo_chunk + (m + 63) / 64, a.blocked_rows_alloc, BK, a.ld);
+        else            rc = make_tmap_blocked(&ta, a.ptr, m, p.lo_chunk + (k + 63) / 64, a.blocked_rows_alloc, BM, a.ld);
         p.a_blocked = 1;
     } else if (a.mn_major) rc = make_tmap(&ta, a.ptr, m, k, a.ld, 64, BK);
     else                   rc = make_tmap(&ta, a.ptr, k, m, a.ld, bk, BM, f32);
@@ -844,7 +844,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     if (rc) return rc;
     if (epi_is_coef(epi)) {
         if (panel == nullptr || !aligned16(panel) || panel_rows_alloc < m) return fail(MECLIP_EINVAL, "coefficient panel misaligned");
-        rc = make_tmap_blocked(&tc, panel, m, (n + 63) / 64, panel_rows_alloc, 32, panel_chunks_alloc);   // one warp's 32 rows x 64 columns per store
+        rc = make_tmap_blocked(&tc, panel, m, p.lo_chunk + (n + 63) / 64, panel_rows_alloc, 32, panel_chunks_alloc);   // one warp's 32 rows x 64 columns per store
         if (rc) return rc;
     } else {
         tc = ta;
@@ -853,6 +853,11 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     p.num_m_tiles = (int)((m + BM - 1) / BM);
     p.num_n_tiles = (int)((n + bn - 1) / bn);
     p.k_steps = (int)((k + bk - 1) / bk);
+    if (p.lo_chunk > 0 && epi == EPI_OUT) {
+        if (pair || a.blocked_rows_alloc == 0) return fail(MECLIP_EINVAL, "a second panel needs the single-CTA kernel");
+        p.k_half = p.k_steps;
+        p.k_steps *= 2;
+    }
     if (epi != EPI_OUT || p.splits < 1) { p.splits = 1; p.k_part = p.k_steps; }
     p.trace = g_trace_buf;
     p.trace_capacity = g_trace_capacity;
@@ -1050,7 +1055,7 @@ static long long env_ll(const char* name) {
 // honour_overrides == false: the built-in constants, whatever the test hook or the environment say
 // (meclip_grad_static promises a plan that fits its fixed scratch).
 static GradPlan plan_grad(long long rows, long long cols, long long d, bool transposed_copies = true,
-                          bool honour_overrides = true) {
+                          bool honour_overrides = true, int panels = 1) {
     GradPlan g;
     static const long long env_row_block = env_ll("MECLIP_ROW_BLOCK") / 128 * 128;
     static const long long env_panel_bytes = env_ll("MECLIP_PANEL_MIB") << 20;
@@ -1072,7 +1077,7 @@ static GradPlan plan_grad(long long rows, long long cols, long long d, bool tran
     g.n_panels = (cols + w - 1) / w;
     g.n_blocks = g.n_row_blocks * g.n_panels;
     g.g_buffers = g.n_blocks > 1 ? 2 : 1;
-    g.g_bytes = round_up((size_t)g.row_block * g.ldg * 2, 256);
+    g.g_bytes = round_up((size_t)panels * g.row_block * g.ldg * 2, 256);
     g.dx_bytes = g.n_panels > 1 ? round_up((size_t)g.row_block * d * 4, 256) : 0;
     g.dy_bytes = g.n_row_blocks > 1 ? round_up((size_t)cols * d * 4, 256) : 0;
     g.counter_bytes = round_up((size_t)g.n_blocks * 3 * sizeof(unsigned int), 256);   // one tile counter per launch
@@ -1548,7 +1553,10 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     if (!siglip && ds.t == nullptr && !(temperature > 0.f)) return fail(MECLIP_EINVAL, "grad: temperature must be positive");
     int rc = check_device();
     if (rc) return rc;
-    const GradPlan plan = plan_grad(rows, cols, dn, transposed_copies, honour_overrides);
+    const bool two_panels = vg != nullptr && vg->two_panels;
+    if (two_panels && transposed_copies) return fail(MECLIP_EINVAL, "grad: two panels without transposed operands only");
+    const GradPlan plan = plan_grad(rows, cols, dn, transposed_copies, honour_overrides, two_panels ? 2 : 1);
+    const int lo_chunk = two_panels ? (int)(plan.ldg / 64) : 0;
     if (workspace_bytes < plan.total())
         return fail(MECLIP_ENOSPC, "grad: workspace %zu < %zu bytes", workspace_bytes, plan.total());
     const bool clip = (kind == MECLIP_CLIP);
@@ -1654,6 +1662,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     p.fmul = vg->tile_fmul;
                     p.vc = vocab_rows_from(vg->coef, r0);
                     p.vc_col0 = c0;
+                    p.lo_chunk = lo_chunk;
                     if (!use_counters) p.tile_counter = nullptr;
                     if (vg->x_f16 != nullptr) {
                         a = Operand{vg->x_f16 + r0 * vg->ldx_f16, vg->ldx_f16, false, 0, false, true};
@@ -1661,7 +1670,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     }
                     // 256-column tiles beyond one row tile: only those run on CTA pairs
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
-                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, s0);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                 }
@@ -1679,6 +1688,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
             if (want_dy) {
                 GemmParams& p = py;
                 p.status = status;
+                p.lo_chunk = lo_chunk;
                 p.tile_counter = use_counters ? counters + 3 * t + 2 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dy) + (size_t)c0 * lddy * dy_elt;
                 float* scratch = dy_scratch + (size_t)c0 * d;
@@ -1710,6 +1720,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 GemmParams p;
                 std::memset(&p, 0, sizeof(p));
                 p.status = status;
+                p.lo_chunk = lo_chunk;
                 p.tile_counter = use_counters ? counters + 3 * t + 1 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dx) + (size_t)r0 * lddx * dx_elt;
                 if (dx_mode == MECLIP_ACCUM_F32) {

@@ -79,7 +79,7 @@ static long long split_parts_alone(long long m, long long n, long long k_steps, 
     return parts > SPLIT_MAX ? SPLIT_MAX : parts;
 }
 static SplitK split_alone(GemmParams& p, long long m, long long n, long long k, int bn, float* buf, size_t bytes) {
-    const long long k_steps = (k + BK - 1) / BK;
+    const long long k_steps = (k + BK - 1) / BK * (p.lo_chunk > 0 ? 2 : 1);
     return split_into(p, m, n, k_steps, split_parts_alone(m, n, k_steps, bn), buf, bytes);
 }
 
@@ -102,7 +102,7 @@ static void split_dual(GemmParams& py, GemmParams& px, long long rows, long long
 }
 
 // Bytes that the parts of one rows x cols block want at most.
-static size_t split_bytes(long long rows, long long cols, long long d, bool dual) {
+static size_t split_bytes(long long rows, long long cols, long long d, bool dual, bool two_panels) {
     if (dual) {
         long long py, px;
         split_parts_dual(rows, cols, d, py, px);
@@ -113,7 +113,7 @@ static size_t split_bytes(long long rows, long long cols, long long d, bool dual
     size_t most = 0;
     for (int which = 0; which < 2; ++which) {
         const long long m = which ? rows : cols, k = which ? cols : rows;
-        const long long parts = split_parts_alone(m, d, (k + BK - 1) / BK, 256);
+        const long long parts = split_parts_alone(m, d, (k + BK - 1) / BK * (two_panels ? 2 : 1), 256);
         // narrower tiles mean more of them and fewer parts, so this is the most
         if (parts > 1) { const size_t b = (size_t)parts * m * d * 4; if (b > most) most = b; }
     }

@@ -205,6 +205,9 @@ struct GemmParams {
     // EPI_VCOEF: u = S fmul - row_lse[i] = log2 p_ij, G_ij = 2^u (a_i + b_i u) + the row's own terms; see VocabCoef
     VocabCoef vc;
     long long vc_col0;        // first column of the panel in the table
+    // A second panel with what the bf16 rounding of the first one left, lo_chunk 64-column chunks behind it (0: none).
+    // EPI_VCOEF writes it; a contraction (single-CTA kernel) then walks K twice, from step k_half on over the second panel.
+    int lo_chunk, k_half;
 };
 
 enum { TR_LOAD_BEGIN = 1, TR_LOAD_END = 2, TR_MMA_BEGIN = 10, TR_MMA_FIRST_DATA = 11, TR_MMA_END = 12,
@@ -432,14 +435,16 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
                     mbar_expect_tx(full, stage_tx);
                     const uint32_t sa = smem_base + (uint32_t)stage * (uint32_t)p.stage_bytes;
                     const uint32_t sb = sa + A_STAGE_BYTES;
-                    const int k0 = ks * BK;
+                    int kk = ks, behind = 0;
+                    if (EPI == EPI_OUT && p.lo_chunk > 0 && ks >= p.k_half) { kk = ks - p.k_half; behind = p.lo_chunk; }
+                    const int k0 = kk * BK;
                     if (p.a_blocked) {
                         // coefficient panel stored as [64-column chunk][row][64]: every box is one contiguous run
                         if (A_MN) {   // A = G^T: M runs along the panel's columns, K along its rows
-                            tma_load_3d(sa, &tmap_a, full, 0, k0, m0 >> 6);
-                            tma_load_3d(sa + BK * 128, &tmap_a, full, 0, k0, (m0 >> 6) + 1);
+                            tma_load_3d(sa, &tmap_a, full, 0, k0, (m0 >> 6) + behind);
+                            tma_load_3d(sa + BK * 128, &tmap_a, full, 0, k0, (m0 >> 6) + behind + 1);
                         } else {      // A = G: M along rows, K along columns
-                            tma_load_3d(sa, &tmap_a, full, 0, m0, ks);
+                            tma_load_3d(sa, &tmap_a, full, 0, m0, kk + behind);
                         }
                     } else if (A_MN) {   // global [K rows][M contiguous]: 64-wide column chunks of BK rows
                         tma_load_2d(sa, &tmap_a, full, m0, k0);

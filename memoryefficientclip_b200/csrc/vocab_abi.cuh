@@ -140,7 +140,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
 struct VocabGradPlan {
     size_t rows_bytes, split_bytes, grad_bytes;
     int split_bufs;
-    bool transposed;
+    bool transposed, two_panels;
     size_t total() const { return rows_bytes + split_bufs * split_bytes + grad_bytes; }
 };
 static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long d) {
@@ -148,10 +148,14 @@ static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long 
     g.rows_bytes = round_up((size_t)rows * 4, 256);
     // transposed copies of the operands and side streams pay for themselves when the contractions are long
     g.transposed = rows >= 1024 && transposes_allowed();
-    const GradPlan plan = plan_grad(rows, vocab, d, g.transposed);
+    // Few rows: the rounding of a coefficient to bf16 (2^-9 on average) does not average out over them - where a row's
+    // gradient is carried by one coefficient, its whole gradient is off by that much.  A second panel with the remainders
+    // removes it; the contractions then walk K twice, a few microseconds for one row tile (128 x 4099 x 512: 17 -> 22 us).
+    g.two_panels = !g.transposed && rows <= BM;
+    const GradPlan plan = plan_grad(rows, vocab, d, g.transposed, true, g.two_panels ? 2 : 1);
     g.grad_bytes = plan.total();
     const bool dual = g.transposed && d >= 256 && dual_allowed() && pair_mode() != 0 && !wide_allowed();
-    g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual);
+    g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual, g.two_panels);
     g.split_bufs = g.transposed && !dual ? 2 : 1;          // the two contractions on two streams
     return g;
 }
@@ -163,6 +167,7 @@ static int vocab_grad(VocabGrad vg, const void* x_bf16, const void* t_bf16, int6
     vg.split_buf = reinterpret_cast<float*>(split);
     vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
     vg.split_bytes = plan.split_bytes;
+    vg.two_panels = plan.two_panels;
     return grad_impl(MECLIP_SIGLIP, x_bf16, t_bf16, rows, vocab, d, ldx, ldt, temperature, 0, 0, nullptr, nullptr, nullptr,
                      1.f, dx, dx_mode, lddx, dt, dt_mode, lddt, split + plan.split_bufs * plan.split_bytes, plan.grad_bytes,
                      status, s, plan.transposed && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false,

@@ -23,6 +23,7 @@ struct VocabGrad {
     const __nv_bfloat16* y_f16;
     long long ldy_f16;
     float tile_fmul;
+    int two_panels;
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
     size_t split_bytes;               // of each
 };
@@ -686,7 +687,7 @@ token_grad_sum_kernel(const __grid_constant__ VocabCoef v, long long rows, float
 // what the tile pass stored there.  One warp per row.  (Up to VOCAB_TILE_ENTRIES entries per row the tile pass does it.)
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
 vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long long c0, long long nc,
-                     __nv_bfloat16* __restrict__ panel, long long rows_alloc) {
+                     __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk) {
     const long long i = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= nr) return;
@@ -698,16 +699,19 @@ vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long lon
         float value;
         if (!vocab_entry(v, i, e, a, b, value)) continue;
         const long long col = j - c0;
-        panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = __float2bfloat16_rn(value);
+        const __nv_bfloat16 hi = __float2bfloat16_rn(value);
+        panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = hi;
+        if (lo_chunk > 0)
+            panel[(((col >> 6) + lo_chunk) * rows_alloc + i) * 64 + (col & 63)] = __float2bfloat16_rn(value - __bfloat162float(hi));
     }
 }
 
 static int launch_vocab_entries(const VocabCoef& v, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
-                                long long rows_alloc, cudaStream_t s) {
+                                long long rows_alloc, int lo_chunk, cudaStream_t s) {
     if (v.k == 0 || v.entries_in_tile || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
     const int wpb = ROW_KERNEL_THREADS / 32;
     ScopedTiming timing(s, TAG_ROW, (double)nr * v.k * 18.0);
-    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc);
+    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc, lo_chunk);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }
