@@ -498,20 +498,21 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
  *                           (both NULL: only row_loss is wanted); no row at all: loss 0.
  *   meclip_distill_grad     dz_ij = w_i (p_ij - q_ij), w_i = grad_out (one scalar, or [rows] with grad_per_row) times
  *                           inv_count (NULL: 1).  The teacher gets no gradient.
- * The gradients read bf16 operands; x_f16 / table_f16 (NULL otherwise) are the fp16 operands of a forward that ran on
- * those, and the scores are formed from them again.  Coefficients are rounded to bf16 once, as in meclip_grad; output
- * modes, blocking and side streams are those of meclip_grad, without atomics.  Either output may be NULL.
+ * The gradients take the forward's operands.  Coefficients are rounded once: to fp16 scaled by a power of two (a bound on
+ * all of them is brought to 2^14, so a coefficient keeps 11 bits down to 2^-28 of the largest), or, for up to 256 rows of
+ * bf16 operands, to two bf16 panels (16 bits).  Output modes, blocking and side streams are those of meclip_grad, without
+ * atomics on sums; a contraction with few output tiles and a long K is cut along K and its parts added in order.  Either
+ * output may be NULL.
  */
 size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
-size_t meclip_vocab_grad_workspace_bytes(int64_t rows, int64_t vocab, int64_t d);
+size_t meclip_vocab_grad_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t d);
 int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
                            int64_t ldx, int64_t ldt, float temperature, const int64_t* tokens, int64_t per_row,
                            float* log_probs, float* entropy, int top_k, float* top_log_probs, int64_t* top_tokens,
                            float* row_lse, float* token_scores, void* workspace, size_t workspace_bytes, int* status,
                            void* stream);
-int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16,
-                                int64_t rows, int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16,
-                                int64_t ldt_f16, float temperature, const int64_t* tokens, int64_t per_row,
+int meclip_token_log_probs_grad(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
+                                int64_t ldx, int64_t ldt, float temperature, const int64_t* tokens, int64_t per_row,
                                 const float* row_lse, const float* entropy, const float* token_scores,
                                 const float* grad_log_probs, const float* grad_entropy, void* dx, int dx_mode, int64_t lddx,
                                 void* dtable, int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes,
@@ -521,9 +522,8 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
                    int teacher_dtype, int64_t per_row, float teacher_temperature, int mean, float* row_loss, float* row_has,
                    float* loss, float* inv_count, float* row_lse, float* token_scores, float* teacher_probs,
                    void* workspace, size_t workspace_bytes, int* status, void* stream);
-int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16, int64_t rows,
-                        int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16, int64_t ldt_f16,
-                        float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
+int meclip_distill_grad(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
+                        int64_t ldt, float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
                         const float* token_scores, const float* teacher_probs, const float* row_has, const float* grad_out,
                         int grad_per_row, const float* inv_count, void* dx, int dx_mode, int64_t lddx, void* dtable,
                         int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes, int* status, void* stream);

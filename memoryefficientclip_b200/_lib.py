@@ -106,21 +106,20 @@ SIGNATURES = {
     "meclip_step_backward": (c_int, [c_int, c_void_p, c_size_t, c_int64, c_int64, c_int, c_float, c_void_p, c_float,
                                      c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "meclip_vocab_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
-    "meclip_vocab_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "meclip_vocab_grad_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "meclip_token_log_probs": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
                                        c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "meclip_token_log_probs_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
-                                            c_int64, c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p,
-                                            c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int,
-                                            c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_token_log_probs_grad": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+                                            c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                            c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p,
+                                            c_void_p]),
     "meclip_distill": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
                                c_void_p, c_int, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "meclip_distill_grad": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
-                                    c_int64, c_int64, c_float, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
-                                    c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_void_p, c_int, c_int64,
-                                    c_void_p, c_size_t, c_void_p, c_void_p]),
+    "meclip_distill_grad": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
+                                    c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                    c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p, c_void_p]),
     "meclip_embed": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_int64, c_float, c_void_p, c_int64,
                              c_void_p]),
     "meclip_embed_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),

@@ -345,15 +345,21 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         if (VOCAB) {
             if (rvalid) {
                 v_lse = __ldg(p.vc.row_lse + grow);
+                const float g_scale = pow2(pow2_exponent(p.panel_max, PANEL_TARGET));
                 vocab_row_factors(p.vc, grow, v_a, v_b);
                 if (p.vc.entries_in_tile) {
 #pragma unroll
                     for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e)
                         if (e < p.vc.k) {
                             const long long col = p.vc.tokens[(long long)grow * p.vc.k + e] - p.vc_col0 - n0;
-                            if (col >= 0 && col < p.bn && n0 + col < p.n && vocab_entry(p.vc, grow, e, v_a, v_b, v_val[e])) v_col[e] = (int)col;
+                            if (col >= 0 && col < p.bn && n0 + col < p.n && vocab_entry(p.vc, grow, e, v_a, v_b, v_val[e])) {
+                                v_col[e] = (int)col;
+                                v_val[e] *= g_scale;
+                            }
                         }
                 }
+                v_a *= g_scale;
+                v_b *= g_scale;
             }
             bool any = false;
 #pragma unroll
@@ -421,10 +427,17 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
 #pragma unroll
                 for (int pc = 0; pc < 4; ++pc) {         // 16-byte piece index within the 128-byte row
                     uint4 pk;
-                    pk.x = pack_bf16x2(gv[pc * 8 + 0], gv[pc * 8 + 1]);
-                    pk.y = pack_bf16x2(gv[pc * 8 + 2], gv[pc * 8 + 3]);
-                    pk.z = pack_bf16x2(gv[pc * 8 + 4], gv[pc * 8 + 5]);
-                    pk.w = pack_bf16x2(gv[pc * 8 + 6], gv[pc * 8 + 7]);
+                    if (VOCAB && p.panel_f16) {
+                        pk.x = pack_f16x2(gv[pc * 8 + 0], gv[pc * 8 + 1]);
+                        pk.y = pack_f16x2(gv[pc * 8 + 2], gv[pc * 8 + 3]);
+                        pk.z = pack_f16x2(gv[pc * 8 + 4], gv[pc * 8 + 5]);
+                        pk.w = pack_f16x2(gv[pc * 8 + 6], gv[pc * 8 + 7]);
+                    } else {
+                        pk.x = pack_bf16x2(gv[pc * 8 + 0], gv[pc * 8 + 1]);
+                        pk.y = pack_bf16x2(gv[pc * 8 + 2], gv[pc * 8 + 3]);
+                        pk.z = pack_bf16x2(gv[pc * 8 + 4], gv[pc * 8 + 5]);
+                        pk.w = pack_bf16x2(gv[pc * 8 + 6], gv[pc * 8 + 7]);
+                    }
                     const int piece = half * 4 + pc;
                     *reinterpret_cast<uint4*>(buf + lane * 128 + ((piece ^ (lane & 7)) << 4)) = pk;
                     if (VOCAB && p.lo_chunk > 0) {       // what the rounding left, for the second panel
@@ -502,6 +515,12 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         // first 128 B rows of CTA 0 and of CTA 1, the second MMA's columns (from TMEM column 256) the remaining rows
         // of each, so accumulator chunk ch maps to tile columns through the four pieces below.  For tiles of up
         // to 256 columns the map is the identity.
+        const bool scaled = od.scale.panel != nullptr || od.scale.operand != nullptr;
+        float unscale_g = 1.f, unscale_b = 1.f;
+        if (scaled) {
+            unscale_g = pow2(-pow2_exponent(od.scale.panel, PANEL_TARGET));
+            unscale_b = pow2(-pow2_exponent(od.scale.operand, OPERAND_TARGET));
+        }
         const int n1 = tile_bn < MAX_BN ? tile_bn : MAX_BN, n2 = tile_bn - n1, h1 = n1 >> 1, half = tile_bn >> 1;
         for (int ch = u_begin; ch < u_end; ++ch) {
             const int c = ch * 32;
@@ -518,6 +537,10 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             uint32_t v[32];
             tmem_ld32(taddr + tcol, v);
             tmem_ld_wait();
+            if (scaled) {             // two factors: their product could leave fp32's range
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * unscale_g * unscale_b);
+            }
             if (rvalid) {
                 const int col0 = n0 + gcol;
                 if (od.acc_in != nullptr) {

@@ -806,7 +806,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         (wide && (epi != EPI_OUT || b.mn_major || g_trace_buf != nullptr || pair_mode() == 0)))
         return fail(MECLIP_EINVAL, "tile width %d not supported", bn);
     const bool f32 = a.f32;
-    if (a.f16 != b.f16 || (a.f16 && (f32 || (epi != EPI_STATS && epi != EPI_VCOEF))))
+    if (a.f16 != b.f16 || (a.f16 && (f32 || epi == EPI_SUMS || epi == EPI_COEF)))
         return fail(MECLIP_EINVAL, "fp16 operands: vocabulary passes only, A and B together");
     // bits 7 and 10 of the instruction descriptor say bf16; cleared they say fp16
     const uint32_t idesc_keep = a.f16 ? ~((1u << 7) | (1u << 10)) : ~0u;
@@ -885,7 +885,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         if (b.mn_major || rest > MAX_BN) last = (int)((rest + 63) / 64 * 64);
         if (last < bn) {
             p.bn_last = last;
-            p.idesc_last = umma_idesc_bf16(BM, last, a.mn_major ? 1 : 0, b.mn_major ? 1 : 0);
+            p.idesc_last = umma_idesc_bf16(BM, last, a.mn_major ? 1 : 0, b.mn_major ? 1 : 0) & idesc_keep;
         }
     }
     if ((long long)p.num_m_tiles * p.num_n_tiles * p.splits > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
@@ -968,7 +968,7 @@ static bool dual_allowed() {
 static int launch_contractions_dual(const void* panel, long long panel_rows_alloc, long long panel_chunks_alloc,
                                     const void* xt, long long ld_xt, const void* yt, long long ld_yt, long long rows,
                                     long long cols, long long n, const GemmParams& py, const GemmParams& px,
-                                    cudaStream_t stream) {
+                                    cudaStream_t stream, bool f16 = false) {
     if (rows < 1 || cols < 1 || n < 1 || rows > 0x7fffffffLL || cols > 0x7fffffffLL) return fail(MECLIP_EINVAL, "dual contraction: bad extents");
     const int bn = 256;
     CUtensorMap tay, tby, tax, tbx;
@@ -989,7 +989,7 @@ static int launch_contractions_dual(const void* panel, long long panel_rows_allo
     p.m2 = (int)rows;
     p.num_m_tiles2 = (int)((rows + PAIR_BM - 1) / PAIR_BM);
     p.k_steps2 = (int)((cols + BK - 1) / BK);
-    p.out2 = px.out; p.ld_out2 = px.ld_out; p.out_bf16_2 = px.out_bf16; p.acc_in2 = px.acc_in; p.ld_acc2 = px.ld_acc;
+    p.out2 = px.out; p.ld_out2 = px.ld_out; p.out_bf16_2 = px.out_bf16; p.acc_in2 = px.acc_in; p.ld_acc2 = px.ld_acc; p.scale2 = px.scale;
     p.dual = 1;
     if (p.splits < 1) { p.splits = 1; p.k_part = p.k_steps; }
     p.splits2 = px.splits; p.k_part2 = px.k_part; p.split_stride2 = px.split_stride;
@@ -1004,10 +1004,11 @@ static int launch_contractions_dual(const void* panel, long long panel_rows_allo
     p.strip_len = 1;
     const long long rest = n - (long long)(p.num_n_tiles - 1) * bn;
     p.bn_last = (int)((rest + 31) / 32 * 32);
-    p.idesc = umma_idesc_bf16(PAIR_BM, bn, 1, 0);
-    p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last, 1, 0);
-    p.idesc_p2 = umma_idesc_bf16(PAIR_BM, bn, 0, 0);
-    p.idesc_last_p2 = umma_idesc_bf16(PAIR_BM, p.bn_last, 0, 0);
+    const uint32_t idesc_keep = f16 ? ~((1u << 7) | (1u << 10)) : ~0u;       // as in launch_gemm
+    p.idesc = umma_idesc_bf16(PAIR_BM, bn, 1, 0) & idesc_keep;
+    p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last, 1, 0) & idesc_keep;
+    p.idesc_p2 = umma_idesc_bf16(PAIR_BM, bn, 0, 0) & idesc_keep;
+    p.idesc_last_p2 = umma_idesc_bf16(PAIR_BM, p.bn_last, 0, 0) & idesc_keep;
     p.wide = 0; p.idesc2 = 0; p.idesc2_last = 0; p.narrow_last = 0;
     static const bool env_static = []() { const char* v = std::getenv("MECLIP_STATIC_SCHED"); return v && v[0] == '1'; }();
     if (env_static) p.tile_counter = nullptr;
@@ -1594,6 +1595,17 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     // deals its tiles in turn instead (nothing shares the GPU with it, and a launch less is a few microseconds)
     const bool use_counters = vg == nullptr || overlap;
     if (use_counters) MECLIP_CUDA(cudaMemsetAsync(counters, 0, plan.counter_bytes, s0));
+    // A vocabulary's panel is fp16 wherever the contractions can read fp16 operands: those of an fp16 problem as they are,
+    // or scaled transposed copies.  An fp16 coefficient is off by 2^-12 on average of a step, a bf16 one by 2^-9.
+    const bool panel_f16 = vg != nullptr && (vg->f16 || transposed_copies);
+    const bool scale_operands = panel_f16 && !vg->f16;
+    const float* panel_max = panel_f16 ? vg->maxima + 2 : nullptr;
+    if (panel_f16) {
+        MECLIP_CUDA(cudaMemsetAsync(vg->maxima, 0, 3 * sizeof(float), s0));
+        ScopedTiming timing(s0, TAG_ROW, (double)rows * 16.0);
+        vocab_bound_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, s0>>>(vg->coef, rows, vg->maxima + 2);
+        MECLIP_CUDA(cudaGetLastError());
+    }
     if (transposed_copies) {
         // Y^T is only read by the dX contractions and X^T by the dY contractions, so with side streams
         // the transposes run there, under the first coefficient pass
@@ -1602,15 +1614,30 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
             if (want_dx) MECLIP_CUDA(cudaStreamWaitEvent(sx, side->fork, 0));
             if (want_dy) MECLIP_CUDA(cudaStreamWaitEvent(sy, side->fork, 0));
         }
+        if (scale_operands) {      // one launch for both when they run on one stream
+            const int both = want_dx && want_dy && sx == sy;
+            const uint16_t *xw = reinterpret_cast<const uint16_t*>(X), *yw = reinterpret_cast<const uint16_t*>(Y);
+            const unsigned blocks = (unsigned)(4 * sm_count());
+            if (want_dx) {
+                ScopedTiming timing(sx, TAG_TRANSPOSE, 2.0 * (double)(cols + (both ? rows : 0)) * (double)d);
+                operand_max_kernel<<<dim3(blocks, both ? 2 : 1), 256, 0, sx>>>(yw, ldy, cols, xw, ldx, rows, (int)d, vg->maxima + 1, vg->maxima);
+            }
+            if (want_dy && !both) {
+                ScopedTiming timing(sy, TAG_TRANSPOSE, 2.0 * (double)rows * (double)d);
+                operand_max_kernel<<<dim3(blocks, 1), 256, 0, sy>>>(xw, ldx, rows, xw, ldx, rows, (int)d, vg->maxima, vg->maxima);
+            }
+        }
         if (want_dx) {
             ScopedTiming timing(sx, TAG_TRANSPOSE, 4.0 * (double)cols * (double)dn);
             dim3 grid((unsigned)((cols + 63) / 64), (unsigned)((dn + 63) / 64));
-            transpose_bf16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, yt, plan.ld_yt);
+            if (scale_operands) transpose_scaled_f16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, vg->maxima + 1, reinterpret_cast<__half*>(yt), plan.ld_yt);
+            else                transpose_bf16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, yt, plan.ld_yt);
         }
         if (want_dy) {
             ScopedTiming timing(sy, TAG_TRANSPOSE, 4.0 * (double)rows * (double)d);
             dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((d + 63) / 64));
-            transpose_bf16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, xt, plan.ld_xt);
+            if (scale_operands) transpose_scaled_f16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, vg->maxima, reinterpret_cast<__half*>(xt), plan.ld_xt);
+            else                transpose_bf16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, xt, plan.ld_xt);
         }
         MECLIP_CUDA(cudaGetLastError());
     }
@@ -1664,13 +1691,12 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     p.vc_col0 = c0;
                     p.lo_chunk = lo_chunk;
                     if (!use_counters) p.tile_counter = nullptr;
-                    if (vg->x_f16 != nullptr) {
-                        a = Operand{vg->x_f16 + r0 * vg->ldx_f16, vg->ldx_f16, false, 0, false, true};
-                        b = Operand{vg->y_f16 + c0 * vg->ldy_f16, vg->ldy_f16, false, 0, false, true};
-                    }
+                    p.panel_f16 = panel_f16;
+                    p.panel_max = panel_max;
+                    a.f16 = b.f16 = vg->f16;
                     // 256-column tiles beyond one row tile: only those run on CTA pairs
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
-                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, s0);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_max, panel_f16, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                 }
@@ -1689,6 +1715,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 GemmParams& p = py;
                 p.status = status;
                 p.lo_chunk = lo_chunk;
+                p.scale = OutScale{panel_max, scale_operands ? vg->maxima : nullptr};
                 p.tile_counter = use_counters ? counters + 3 * t + 2 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dy) + (size_t)c0 * lddy * dy_elt;
                 float* scratch = dy_scratch + (size_t)c0 * d;
@@ -1705,6 +1732,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 if (!use_dual) {
                     Operand a{gpanel[gb], plan.ldg / 64, true, plan.row_block}, b{X + r0 * ldx, ldx, true};
                     if (transposed_copies) b = Operand{xt + r0, plan.ld_xt, false};   // [d][K = rows] K-major
+                    a.f16 = b.f16 = panel_f16;
                     const int bn = pick_contraction_bn(nc, d, overlap, transposed_copies);
                     SplitK sk;
                     if (vg != nullptr) sk = split_alone(p, nc, d, nr, bn, vg->split_buf, vg->split_bytes);
@@ -1721,6 +1749,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 std::memset(&p, 0, sizeof(p));
                 p.status = status;
                 p.lo_chunk = lo_chunk;
+                p.scale = OutScale{panel_max, scale_operands ? vg->maxima + 1 : nullptr};
                 p.tile_counter = use_counters ? counters + 3 * t + 1 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dx) + (size_t)r0 * lddx * dx_elt;
                 if (dx_mode == MECLIP_ACCUM_F32) {
@@ -1738,7 +1767,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     if (vg != nullptr) split_dual(py, p, nr, nc, d, vg->split_buf, vg->split_bytes, sky, skx);
                     t_tag = TAG_DX;         // one launch: its time and FLOPs are booked under the dX tag
                     rc = launch_contractions_dual(gpanel[gb], plan.row_block, plan.ldg / 64, xt + r0, plan.ld_xt, yt + c0,
-                                                  plan.ld_yt, nr, nc, d, py, p, sx);
+                                                  plan.ld_yt, nr, nc, d, py, p, sx, panel_f16);
                     if (rc == MECLIP_OK) rc = launch_split_sum(sky, sx);
                     if (rc == MECLIP_OK) rc = launch_split_sum(skx, sx);
                     if (rc) return rc;
@@ -1749,6 +1778,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 } else {
                     Operand a{gpanel[gb], plan.ldg / 64, false, plan.row_block}, b{Y + c0 * ldy, ldy, true};
                     if (transposed_copies) b = Operand{yt + c0, plan.ld_yt, false};   // [d][K = cols] K-major
+                    a.f16 = b.f16 = panel_f16;
                     const int bn = pick_contraction_bn(nr, dn, overlap, transposed_copies);
                     SplitK sk;
                     if (vg != nullptr) sk = split_alone(p, nr, dn, nc, bn, vg->split_buf2, vg->split_bytes);

@@ -23,6 +23,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "sm100_ptx.cuh"
@@ -54,6 +55,18 @@ static constexpr int STORE_BUF_BYTES = 32 * 128;   // one warp's 32 rows x 64 bf
 
 enum { EPI_SUMS = 0, EPI_COEF = 1, EPI_OUT = 2, EPI_STATS = 3, EPI_VCOEF = 4 };
 __host__ __device__ constexpr bool epi_is_coef(int epi) { return epi == EPI_COEF || epi == EPI_VCOEF; }
+
+// Scaled fp16 operands: a matrix is multiplied by the power of two that brings its largest magnitude to 2^target, so that
+// fp16's 11 bits reach 2^-28 (panel) or 2^-23 (features) of it.  `max` points to that magnitude on the device; null: scale 1.
+static constexpr int PANEL_TARGET = 14, OPERAND_TARGET = 9;
+struct OutScale { const float *panel, *operand; };
+__device__ __forceinline__ int pow2_exponent(const float* max, int target) {
+    if (max == nullptr) return 0;
+    const int e = (int)((__float_as_uint(__ldg(max)) >> 23) & 255u);
+    if (e == 0 || e == 255) return 0;                       // nothing to scale, or not a number anyway
+    return ::min(100, ::max(-100, target - (e - 127)));     // stays a normal fp32 number, and so does its inverse
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // Coefficients of a softmax over a vocabulary, dz_ij / T = p_ij (a_i + b_i log2 p_ij) + sum of the terms of the row's
 // entries at j; what a_i, b_i and the terms are follows from the loss.
@@ -208,6 +221,11 @@ struct GemmParams {
     // A second panel with what the bf16 rounding of the first one left, lo_chunk 64-column chunks behind it (0: none).
     // EPI_VCOEF writes it; a contraction (single-CTA kernel) then walks K twice, from step k_half on over the second panel.
     int lo_chunk, k_half;
+    // fp16 panels: EPI_VCOEF multiplies by the power of two that brings *panel_max (a bound on |G|) to 2^PANEL_TARGET
+    int panel_f16;
+    const float* panel_max;
+    // Contractions of scaled fp16 operands: the result is divided by the scales of the panel and of B (see OutScale)
+    OutScale scale, scale2;
 };
 
 enum { TR_LOAD_BEGIN = 1, TR_LOAD_END = 2, TR_MMA_BEGIN = 10, TR_MMA_FIRST_DATA = 11, TR_MMA_END = 12,
@@ -279,6 +297,7 @@ struct OutDesc {
     int out_bf16;
     const float* acc_in;
     long long ld_acc;
+    OutScale scale;
 };
 
 // Problem of a tile id in a dual launch (0 or 1); the id is made relative to its problem.
@@ -287,8 +306,8 @@ __device__ __forceinline__ int tile_problem(const GemmParams& p, int& tile) {
     return 0;
 }
 __device__ __forceinline__ OutDesc out_desc(const GemmParams& p, int problem, int part = 0) {
-    if (problem == 0) return OutDesc{p.m, part > 0 ? reinterpret_cast<float*>(p.out) + part * p.split_stride : p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc};
-    return OutDesc{p.m2, part > 0 ? reinterpret_cast<float*>(p.out2) + part * p.split_stride2 : p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2};
+    if (problem == 0) return OutDesc{p.m, part > 0 ? reinterpret_cast<float*>(p.out) + part * p.split_stride : p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc, p.scale};
+    return OutDesc{p.m2, part > 0 ? reinterpret_cast<float*>(p.out2) + part * p.split_stride2 : p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2, p.scale2};
 }
 // Tiles of a problem, parts of K included.
 template <int EPI>
@@ -335,6 +354,10 @@ __device__ __forceinline__ void tile_coords(const GemmParams& p, int tile, int& 
     nt = local / rows_in_group;
 }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
 __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
     __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<uint32_t*>(&h);

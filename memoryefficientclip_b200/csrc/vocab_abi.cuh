@@ -137,51 +137,58 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     return MECLIP_OK;
 }
 
+// Up to this many rows the contractions read bf16 operands as they are, and two panels keep the coefficients' bits; beyond
+// it scaled fp16 copies of the operands (a pass over the table and its transposition) cost less than walking K twice.
+static constexpr long long VOCAB_TWO_PANEL_ROWS = 256;
+// From here on side streams pay for their events, for an fp16 problem transposed copies of the operands too.
+static constexpr long long VOCAB_OVERLAP_ROWS = 1024;
+
 struct VocabGradPlan {
     size_t rows_bytes, split_bytes, grad_bytes;
     int split_bufs;
-    bool transposed, two_panels;
-    size_t total() const { return rows_bytes + split_bufs * split_bytes + grad_bytes; }
+    bool transposed, two_panels, overlap;
+    size_t total() const { return rows_bytes + 256 + split_bufs * split_bytes + grad_bytes; }
 };
-static VocabGradPlan plan_vocab_grad(long long rows, long long vocab, long long d) {
+static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab, long long d) {
     VocabGradPlan g;
+    const bool f16 = dtype == MECLIP_F16;
     g.rows_bytes = round_up((size_t)rows * 4, 256);
-    // transposed copies of the operands and side streams pay for themselves when the contractions are long
-    g.transposed = rows >= 1024 && transposes_allowed();
-    // Few rows: the rounding of a coefficient to bf16 (2^-9 on average) does not average out over them - where a row's
-    // gradient is carried by one coefficient, its whole gradient is off by that much.  A second panel with the remainders
-    // removes it; the contractions then walk K twice, a few microseconds for one row tile (128 x 4099 x 512: 17 -> 22 us).
-    g.two_panels = !g.transposed && rows <= BM;
+    g.overlap = rows >= VOCAB_OVERLAP_ROWS;
+    g.transposed = transposes_allowed() && (f16 ? g.overlap : rows > VOCAB_TWO_PANEL_ROWS);
+    // The rounding of a coefficient to bf16 (2^-9 on average) does not average out where a row's gradient is carried by one
+    // coefficient: its whole gradient is off by that much, as much as the output's own rounding.
+    g.two_panels = !f16 && !g.transposed;
     const GradPlan plan = plan_grad(rows, vocab, d, g.transposed, true, g.two_panels ? 2 : 1);
     g.grad_bytes = plan.total();
     const bool dual = g.transposed && d >= 256 && dual_allowed() && pair_mode() != 0 && !wide_allowed();
     g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual, g.two_panels);
-    g.split_bufs = g.transposed && !dual ? 2 : 1;          // the two contractions on two streams
+    g.split_bufs = g.overlap && g.transposed && !dual ? 2 : 1;          // the two contractions on two streams
     return g;
 }
 
-static int vocab_grad(VocabGrad vg, const void* x_bf16, const void* t_bf16, int64_t rows, int64_t vocab, int64_t d,
-                      int64_t ldx, int64_t ldt, float temperature, void* dx, int dx_mode, int64_t lddx, void* dt,
-                      int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
-    uint8_t* split = ws + plan.rows_bytes;
-    vg.split_buf = reinterpret_cast<float*>(split);
-    vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
-    vg.split_bytes = plan.split_bytes;
-    vg.two_panels = plan.two_panels;
-    return grad_impl(MECLIP_SIGLIP, x_bf16, t_bf16, rows, vocab, d, ldx, ldt, temperature, 0, 0, nullptr, nullptr, nullptr,
-                     1.f, dx, dx_mode, lddx, dt, dt_mode, lddt, split + plan.split_bufs * plan.split_bytes, plan.grad_bytes,
-                     status, s, plan.transposed && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false,
-                     DeviceScalars(), true, nullptr, 0, nullptr, 0, &vg);
-}
-
-static int check_vocab_grad(const char* what, const void* x16, const void* t16, int64_t ldx16, int64_t ldt16, int64_t d,
-                            const void* ws, size_t ws_bytes, const VocabGradPlan& plan) {
-    if ((x16 == nullptr) != (t16 == nullptr) ||
-        (x16 != nullptr && (ldx16 < d || ldt16 < d || ldx16 % 8 != 0 || ldt16 % 8 != 0 || !aligned16(x16) || !aligned16(t16))))
-        return fail(MECLIP_EINVAL, "%s: fp16 operands come as a pair, 16-byte aligned with pitches multiples of 8", what);
+static int check_vocab_grad(const char* what, const void* ws, size_t ws_bytes, const VocabGradPlan& plan) {
     if (ws == nullptr || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return fail(MECLIP_EINVAL, "%s: workspace must be 256-byte aligned", what);
     if (ws_bytes < plan.total()) return fail(MECLIP_ENOSPC, "%s: workspace %zu < %zu bytes", what, ws_bytes, plan.total());
     return MECLIP_OK;
+}
+
+static int vocab_grad(const VocabCoef& coef, int dtype, const void* x, const void* t, int64_t rows, int64_t vocab, int64_t d,
+                      int64_t ldx, int64_t ldt, float temperature, void* dx, int dx_mode, int64_t lddx, void* dt,
+                      int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
+    VocabGrad vg;
+    vg.coef = coef;
+    vg.f16 = dtype == MECLIP_F16;
+    vg.tile_fmul = vocab_tile_fmul(temperature, d);
+    vg.two_panels = plan.two_panels;
+    vg.maxima = reinterpret_cast<float*>(ws + plan.rows_bytes);
+    uint8_t* split = ws + plan.rows_bytes + 256;
+    vg.split_buf = reinterpret_cast<float*>(split);
+    vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
+    vg.split_bytes = plan.split_bytes;
+    return grad_impl(MECLIP_SIGLIP, x, t, rows, vocab, d, ldx, ldt, temperature, 0, 0, nullptr, nullptr, nullptr, 1.f, dx,
+                     dx_mode, lddx, dt, dt_mode, lddt, split + plan.split_bufs * plan.split_bytes, plan.grad_bytes, status, s,
+                     plan.overlap && overlap_allowed(), plan.transposed, nullptr, 0.f, 0.f, 0, false, DeviceScalars(), true,
+                     nullptr, 0, nullptr, 0, &vg);
 }
 
 }  // namespace meclip
@@ -193,9 +200,9 @@ size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k) {
     return plan_vocab(rows, vocab, top_k).total;
 }
 
-size_t meclip_vocab_grad_workspace_bytes(int64_t rows, int64_t vocab, int64_t d) {
+size_t meclip_vocab_grad_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t d) {
     if (rows < 1 || vocab < 1 || d < 1) return 0;
-    return plan_vocab_grad(rows, vocab, d).total();
+    return plan_vocab_grad(dtype, rows, vocab, d).total();
 }
 
 int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
@@ -220,20 +227,19 @@ int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t 
     return vocab_forward<false>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
 }
 
-int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16,
-                                int64_t rows, int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16,
-                                int64_t ldt_f16, float temperature, const int64_t* tokens, int64_t per_row,
+int meclip_token_log_probs_grad(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d,
+                                int64_t ldx, int64_t ldt, float temperature, const int64_t* tokens, int64_t per_row,
                                 const float* row_lse, const float* entropy, const float* token_scores,
                                 const float* grad_log_probs, const float* grad_entropy, void* dx, int dx_mode, int64_t lddx,
                                 void* dtable, int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes,
                                 int* status, void* stream) {
     NvtxRange range("meclip_token_log_probs_grad");
-    int rc = check_vocab("token_log_probs_grad", x_bf16, table_bf16, MECLIP_BF16, rows, vocab, d, ldx, ldt, temperature, tokens, per_row);
+    int rc = check_vocab("token_log_probs_grad", x, table, dtype, rows, vocab, d, ldx, ldt, temperature, tokens, per_row);
     if (rc) return rc;
     if (row_lse == nullptr || (per_row > 0 && token_scores == nullptr) || (grad_entropy != nullptr && entropy == nullptr))
         return fail(MECLIP_EINVAL, "token_log_probs_grad: null pointer");
-    const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
-    rc = check_vocab_grad("token_log_probs_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
+    const VocabGradPlan plan = plan_vocab_grad(dtype, rows, vocab, d);
+    rc = check_vocab_grad("token_log_probs_grad", workspace, workspace_bytes, plan);
     if (rc) return rc;
     VocabCoef c{};
     c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(tokens); c.k = (int)per_row;
@@ -241,6 +247,8 @@ int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, cons
     c.grad_log_probs = grad_log_probs; c.grad_entropy = grad_entropy; c.entropy = entropy;
     c.entries_in_tile = per_row > 0 && per_row <= VOCAB_TILE_ENTRIES && grad_log_probs != nullptr;
     if (per_row > VOCAB_TILE_ENTRIES && grad_log_probs != nullptr) {
+        rc = check_device();
+        if (rc) return rc;
         float* row_g = reinterpret_cast<float*>(workspace);
         const int wpb = ROW_KERNEL_THREADS / 32;
         ScopedTiming timing((cudaStream_t)stream, TAG_ROW, (double)rows * 12.0 * per_row);
@@ -248,9 +256,8 @@ int meclip_token_log_probs_grad(const void* x_bf16, const void* table_bf16, cons
         MECLIP_CUDA(cudaGetLastError());
         c.row_g = row_g;
     }
-    VocabGrad vg{c, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
-    return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
-                      lddt, reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
+    return vocab_grad(c, dtype, x, table, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode, lddt,
+                      reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }
 
 int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
@@ -280,28 +287,26 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
     return vocab_forward<true>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
 }
 
-int meclip_distill_grad(const void* x_bf16, const void* table_bf16, const void* x_f16, const void* table_f16, int64_t rows,
-                        int64_t vocab, int64_t d, int64_t ldx, int64_t ldt, int64_t ldx_f16, int64_t ldt_f16,
-                        float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
+int meclip_distill_grad(const void* x, const void* table, int dtype, int64_t rows, int64_t vocab, int64_t d, int64_t ldx,
+                        int64_t ldt, float temperature, const int64_t* teacher_tokens, int64_t per_row, const float* row_lse,
                         const float* token_scores, const float* teacher_probs, const float* row_has, const float* grad_out,
                         int grad_per_row, const float* inv_count, void* dx, int dx_mode, int64_t lddx, void* dtable,
                         int dtable_mode, int64_t lddt, void* workspace, size_t workspace_bytes, int* status, void* stream) {
     NvtxRange range("meclip_distill_grad");
-    int rc = check_vocab("distill_grad", x_bf16, table_bf16, MECLIP_BF16, rows, vocab, d, ldx, ldt, temperature, teacher_tokens, per_row);
+    int rc = check_vocab("distill_grad", x, table, dtype, rows, vocab, d, ldx, ldt, temperature, teacher_tokens, per_row);
     if (rc) return rc;
     if (per_row < 1 || row_lse == nullptr || token_scores == nullptr || teacher_probs == nullptr || row_has == nullptr || grad_out == nullptr)
         return fail(MECLIP_EINVAL, "distill_grad: null pointer");
-    const VocabGradPlan plan = plan_vocab_grad(rows, vocab, d);
-    rc = check_vocab_grad("distill_grad", x_f16, table_f16, ldx_f16, ldt_f16, d, workspace, workspace_bytes, plan);
+    const VocabGradPlan plan = plan_vocab_grad(dtype, rows, vocab, d);
+    rc = check_vocab_grad("distill_grad", workspace, workspace_bytes, plan);
     if (rc) return rc;
     VocabCoef c{};
     c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(teacher_tokens);
     c.k = (int)per_row; c.distill = 1; c.vocab = vocab; c.inv_t = 1.f / temperature;
     c.grad_out = grad_out; c.grad_per_row = grad_per_row; c.factor = inv_count; c.row_has = row_has; c.probs = teacher_probs;
     c.entries_in_tile = per_row <= VOCAB_TILE_ENTRIES;
-    VocabGrad vg{c, (const __nv_bfloat16*)x_f16, ldx_f16, (const __nv_bfloat16*)table_f16, ldt_f16, vocab_tile_fmul(temperature, d)};
-    return vocab_grad(vg, x_bf16, table_bf16, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode,
-                      lddt, reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
+    return vocab_grad(c, dtype, x, table, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode, lddt,
+                      reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -15,15 +15,14 @@ static constexpr int VOCAB_THREADS = 256;
 static constexpr int VOCAB_MAX_ENTRIES = 256;      // given tokens or teacher entries of one row
 static constexpr int VOCAB_MAX_TOP = 32;           // top alternatives: one per lane
 
-// A backward: the coefficients, with their rows counted from the first one of the problem, and where the scores come from.
+// A backward: the coefficients, with their rows counted from the first one of the problem, the type of the operands, and
+// which form the panel takes.
 struct VocabGrad {
     VocabCoef coef;
-    const __nv_bfloat16* x_f16;       // fp16 operands for the scores (typed as 16-bit words), null: the bf16 ones
-    long long ldx_f16;
-    const __nv_bfloat16* y_f16;
-    long long ldy_f16;
+    int f16;                          // operands are fp16, and so is the panel
     float tile_fmul;
-    int two_panels;
+    int two_panels;                   // bf16 panel and a second one with its remainders
+    float* maxima;                    // [3]: largest magnitudes of x and table, bound on the coefficients; cleared by grad_impl
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
     size_t split_bytes;               // of each
 };
@@ -683,22 +682,104 @@ token_grad_sum_kernel(const __grid_constant__ VocabCoef v, long long rows, float
     if (lane == 0) row_g[row] = g;
 }
 
-// Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved scores and rounded to bf16 once, over
+// A bound on the coefficients' magnitude, |a| + 0.5308 |b| + sum |terms| over all rows (p |log2 p| <= log2(e) / e), as the
+// maximum of non-negative floats' bits: the order of the atomics does not matter.
+__global__ void __launch_bounds__(256)
+vocab_bound_kernel(const __grid_constant__ VocabCoef v, long long rows, float* __restrict__ bound) {
+    const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
+    float m = 0.f;
+    if (row < rows) {
+        float a, b;
+        vocab_row_factors(v, row, a, b);
+        m = fabsf(a) + 0.5308f * fabsf(b);
+        if (v.distill) m += fabsf(a);                            // sum q <= 1
+        else if (v.grad_log_probs != nullptr)
+            for (int e = 0; e < v.k; ++e) {
+                const long long j = v.tokens[row * v.k + e];
+                if (j >= 0 && j < v.vocab) m += fabsf(v.grad_log_probs[row * v.k + e]) * v.inv_t;
+            }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) atomicMax(reinterpret_cast<unsigned int*>(bound), __float_as_uint(m));
+}
+
+// Largest magnitude of a bf16 matrix (blockIdx.y = 0) and of a second one (1).  Bound by HBM; the integer maximum of bits
+// without the sign is the maximum of the magnitudes.
+__global__ void __launch_bounds__(256)
+operand_max_kernel(const uint16_t* __restrict__ m0, long long ld0, long long rows0, const uint16_t* __restrict__ m1, long long ld1,
+                   long long rows1, int d, float* __restrict__ max0, float* __restrict__ max1) {
+    const uint16_t* m = blockIdx.y == 0 ? m0 : m1;
+    const long long ld = blockIdx.y == 0 ? ld0 : ld1, rows = blockIdx.y == 0 ? rows0 : rows1;
+    const int per_row = d / 8;
+    const long long all = rows * per_row, step = (long long)gridDim.x * 256;
+    unsigned int best = 0;
+#pragma unroll 4
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(m + i / per_row * ld + i % per_row * 8));
+        best = __vmaxu2(best, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+    }
+    unsigned int top = max(best & 0xffffu, best >> 16) << 16;    // as fp32 bits
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned int*>(blockIdx.y == 0 ? max0 : max1), top);
+}
+
+// out[c][r] = in[r][c] scaled, as fp16: transpose_bf16_kernel (same tiles, same shared-memory layout) with a conversion.
+// bf16's 8 bits fit fp16's 11; what is below 2^-23 of the largest magnitude loses bits.
+__global__ void __launch_bounds__(256)
+transpose_scaled_f16_kernel(const __nv_bfloat16* __restrict__ in, long long ld_in, long long rows, int cols,
+                            const float* __restrict__ largest, __half* __restrict__ out, long long ld_out) {
+    __shared__ __align__(16) uint32_t tile[64][32];
+    const long long r0 = (long long)blockIdx.x * 64;
+    const int c0 = blockIdx.y * 64;
+    const int t = threadIdx.x;
+    const float scale = pow2(pow2_exponent(largest, OPERAND_TARGET));
+    {
+        const int k = t & 7, rp = t >> 3;
+        const long long r = r0 + 2 * rp;
+        const int c = c0 + 8 * k;
+        float a[8] = {}, b[8] = {};
+        if (c < cols) {
+            if (r < rows) load8(in + r * ld_in + c, a);
+            if (r + 1 < rows) load8(in + (r + 1) * ld_in + c, b);
+        }
+        const int pw = rp ^ (k << 2);
+#pragma unroll
+        for (int m = 0; m < 8; ++m) tile[8 * k + m][pw] = pack_f16x2(a[m] * scale, b[m] * scale);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int oc = (t >> 3) + h * 32, g = t & 7;
+        if (c0 + oc < cols && r0 + 8 * g < rows) {
+            const uint4 v = *reinterpret_cast<const uint4*>(&tile[oc][4 * (g ^ ((oc >> 3) & 7))]);
+            *reinterpret_cast<uint4*>(out + (long long)(c0 + oc) * ld_out + r0 + 8 * g) = v;
+        }
+    }
+}
+
+// Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved scores and rounded once, over
 // what the tile pass stored there.  One warp per row.  (Up to VOCAB_TILE_ENTRIES entries per row the tile pass does it.)
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
 vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long long c0, long long nc,
-                     __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk) {
+                     __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk, const float* __restrict__ panel_max, int f16) {
     const long long i = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= nr) return;
     float a, b;
     vocab_row_factors(v, i, a, b);
+    const float g_scale = pow2(pow2_exponent(panel_max, PANEL_TARGET));
     for (int e = lane; e < v.k; e += 32) {
         const long long j = v.tokens[i * v.k + e];
         if (j < c0 || j >= c0 + nc) continue;          // absent, outside the table or in another panel
         float value;
         if (!vocab_entry(v, i, e, a, b, value)) continue;
         const long long col = j - c0;
+        if (f16) {
+            reinterpret_cast<__half*>(panel)[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = __float2half_rn(value * g_scale);
+            continue;
+        }
         const __nv_bfloat16 hi = __float2bfloat16_rn(value);
         panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = hi;
         if (lo_chunk > 0)
@@ -707,11 +788,12 @@ vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long lon
 }
 
 static int launch_vocab_entries(const VocabCoef& v, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
-                                long long rows_alloc, int lo_chunk, cudaStream_t s) {
+                                long long rows_alloc, int lo_chunk, const float* panel_max, int f16, cudaStream_t s) {
     if (v.k == 0 || v.entries_in_tile || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
     const int wpb = ROW_KERNEL_THREADS / 32;
     ScopedTiming timing(s, TAG_ROW, (double)nr * v.k * 18.0);
-    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc, lo_chunk);
+    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc, lo_chunk,
+                                                                                                   panel_max, f16);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }

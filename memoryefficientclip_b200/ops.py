@@ -767,21 +767,16 @@ def token_log_probs(x, table, tokens, temperature, top_k=0, save=False, status=N
 
 
 class _VocabGrads:
-    """What both gradients share: bf16 operands beside fp16 ones, the outputs, the workspace."""
+    """What both gradients share: the outputs, the workspace, and the arguments that name them and the operands."""
 
     def __init__(self, x, table, need_dx, need_dtable, dx_dtype, dtable_dtype):
         rows, d = x.shape
-        vocab, dev = table.shape[0], x.device
-        f16 = x.dtype == torch.float16
-        # the contractions run on bf16 operands: a coefficient can be far below fp16's smallest number
-        self.x, self.t = (normalize_fwd(x, False)[0], normalize_fwd(table, False)[0]) if f16 else (x, table)
+        vocab, dev, code = table.shape[0], x.device, _DT[x.dtype]
         self.dx = torch.empty((rows, d), dtype=dx_dtype, device=dev) if need_dx else None
         self.dt = torch.empty((vocab, d), dtype=dtable_dtype, device=dev) if need_dtable else None
-        n = _lib.load().meclip_vocab_grad_workspace_bytes(rows, vocab, d)
+        n = _lib.load().meclip_vocab_grad_workspace_bytes(code, rows, vocab, d)
         self.ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        f16_args = (x.data_ptr(), table.data_ptr()) if f16 else (None, None)
-        self.head = (self.x.data_ptr(), self.t.data_ptr(), *f16_args, rows, vocab, d, self.x.stride(0), self.t.stride(0),
-                     x.stride(0) if f16 else 0, table.stride(0) if f16 else 0)
+        self.head = (x.data_ptr(), table.data_ptr(), code, rows, vocab, d, x.stride(0), table.stride(0))
         self.tail = (_ptr(self.dx), _MODE[dx_dtype], d, _ptr(self.dt), _MODE[dtable_dtype], d, self.ws.data_ptr(), n)
 
 

@@ -46,16 +46,16 @@ def test_entry_points_refuse(lib):
                 dict(inv=None), dict(probs=None)):
         assert teach(**bad) == _lib.EINVAL, bad
 
-    def grad(rows=4, lse=p, scores=p, h=p, ent=p, x16=None, t16=None, ld16=0, ws=p, nws=big):
-        return lib.meclip_token_log_probs_grad(p, p, x16, t16, rows, 9, 8, 8, 8, ld16, ld16, 1.0, p, 1, lse, ent, scores, p, h,
-                                               p, _lib.STORE_BF16, 8, p, _lib.STORE_BF16, 8, ws, nws, None, None)
+    def grad(rows=4, dtype=_lib.BF16, lse=p, scores=p, h=p, ent=p, ws=p, nws=big):
+        return lib.meclip_token_log_probs_grad(p, p, dtype, rows, 9, 8, 8, 8, 1.0, p, 1, lse, ent, scores, p, h, p,
+                                               _lib.STORE_BF16, 8, p, _lib.STORE_BF16, 8, ws, nws, None, None)
 
-    for bad in (dict(rows=0), dict(lse=None), dict(scores=None), dict(ent=None), dict(x16=p), dict(x16=p, t16=p, ld16=4),
-                dict(ws=None), dict(ws=ctypes.c_void_p(0x1010))):
+    for bad in (dict(rows=0), dict(dtype=_lib.F32), dict(lse=None), dict(scores=None), dict(ent=None), dict(ws=None),
+                dict(ws=ctypes.c_void_p(0x1010))):
         assert grad(**bad) == _lib.EINVAL, bad
     assert grad(nws=16) == _lib.ENOSPC
-    assert lib.meclip_distill_grad(p, p, None, None, 4, 9, 8, 8, 8, 0, 0, 1.0, p, 2, p, p, p, p, None, 0, p, p, 0, 8, p, 0, 8,
-                                   p, big, None, None) == _lib.EINVAL                  # no grad_out
+    assert lib.meclip_distill_grad(p, p, _lib.BF16, 4, 9, 8, 8, 8, 1.0, p, 2, p, p, p, p, None, 0, p, p, 0, 8, p, 0, 8, p, big,
+                                   None, None) == _lib.EINVAL                  # no grad_out
 
 
 def test_workspace_sizes(lib):
@@ -63,8 +63,8 @@ def test_workspace_sizes(lib):
     plain, top = lib.meclip_vocab_workspace_bytes(4096, 32768, 0), lib.meclip_vocab_workspace_bytes(4096, 32768, 8)
     assert plain == 4096 * 32768 // 128 * 16 and top == plain + 4096 * 1024 * 8
     assert lib.meclip_vocab_workspace_bytes(1 << 20, 32768, 0) == lib.meclip_vocab_workspace_bytes(16384, 32768, 0)
-    assert lib.meclip_vocab_workspace_bytes(0, 8, 0) == 0 and lib.meclip_vocab_grad_workspace_bytes(4, 0, 8) == 0
-    assert lib.meclip_vocab_grad_workspace_bytes(128, 4096, 512) >= 128 * 4096 * 2
+    assert lib.meclip_vocab_workspace_bytes(0, 8, 0) == 0 and lib.meclip_vocab_grad_workspace_bytes(0, 4, 0, 8) == 0
+    assert lib.meclip_vocab_grad_workspace_bytes(0, 128, 4096, 512) >= 2 * 128 * 4096 * 2
 
 
 def test_module_defaults_follow_the_package():
