@@ -485,8 +485,8 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
  *   meclip_token_log_probs  log_probs [rows, per_row] = z - lse (0 for an absent token); entropy [rows] =
  *                           lse - sum_j p z (may be NULL); the top_k (<= 32, <= vocab) best tokens of each row and
  *                           their log probabilities, larger first and the lower token first among equals (decided on
- *                           fp64 dot products).  row_lse [rows] (base 2) and token_scores [rows, per_row] are saved for
- *                           the gradient; NULL when there will be none.
+ *                           fp64 dot products).  row_lse [rows] and token_scores [rows, per_row] (log probabilities), both
+ *                           base 2, are saved for the gradient; NULL when there will be none.
  *   meclip_token_log_probs_grad  dx = dz Y / T, dtable = dz^T X / T for
  *                           dz_ij = sum_k g_ik ([j = token_ik] - p_ij) - h_i p_ij (log p_ij + entropy_i),
  *                           g = grad_log_probs, h = grad_entropy (either may be NULL: zero).

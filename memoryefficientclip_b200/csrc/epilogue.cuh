@@ -80,15 +80,17 @@ __device__ __forceinline__ void coef_chunk(const uint32_t (&v)[32], float fmul, 
     }
 }
 
-// One 32-column chunk of the vocabulary statistics of a row.  Everything is relative to the chunk's own maximum:
-// u_c = S_c fmul - cm <= 0 (up to the rounding of cm), l = sum 2^u, t = sum 2^u u; nv of the 32 columns exist.
-// With CAND also the column of the best and a lower bound of the second best's distance: the two smallest of the
-// integers |u| bits (low five cleared) | column.  Non-negative floats order like their bits and the low bits break
-// ties towards the lower column, so that is one logic operation and three integer minima / maxima per element.
+// One 32-column chunk of the vocabulary statistics of a row, relative to the chunk's own maximum: u_c = S_c fmul - cm <= 0
+// (up to the rounding of cm), r = sum 2^u - 1, t = sum 2^u u; nv of the 32 columns exist.  The maximum's own 1 is left out
+// of the sum: where one column holds nearly all the probability its log probability is -log(1 + r), and r would drown in
+// the rounding of 1 + r.  With CAND also the column of the best and a lower bound of the second best's distance: the two
+// smallest of the integers |u| bits (low five cleared) | column.  Non-negative floats order like their bits and the low
+// bits break ties towards the lower column, so that is one logic operation and three integer minima / maxima per element.
 template <bool CAND>
-__device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul, int nv, float& cm, float& l, float& t,
+__device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul, int nv, float& cm, float& r, float& t,
                                             uint32_t& second) {
     float l0 = 0.f, l1 = 0.f, t0 = 0.f, t1 = 0.f;
+    int tops = 0;                                   // columns that share the maximum
     uint32_t n1 = 0x7fffffffu, n2 = 0x7fffffffu;
     if (nv >= 32) {
         float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]), m2 = __uint_as_float(v[2]), m3 = __uint_as_float(v[3]);
@@ -99,11 +101,15 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
             m2 = fmaxf(m2, __uint_as_float(v[c + 2]));
             m3 = fmaxf(m3, __uint_as_float(v[c + 3]));
         }
-        cm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * fmul;
+        const float sm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        cm = sm * fmul;
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
-            const float ua = fmaf(__uint_as_float(v[c]), fmul, -cm), ub = fmaf(__uint_as_float(v[c + 1]), fmul, -cm);
-            const float ea = ex2_approx(ua), eb = ex2_approx(ub);
+            const float sa = __uint_as_float(v[c]), sb = __uint_as_float(v[c + 1]);
+            const float ua = fmaf(sa, fmul, -cm), ub = fmaf(sb, fmul, -cm);
+            float ea = ex2_approx(ua), eb = ex2_approx(ub);
+            if (sa == sm) { ea = 0.f; ++tops; }
+            if (sb == sm) { eb = 0.f; ++tops; }
             l0 += ea; l1 += eb;
             t0 = fmaf(ea, ua, t0); t1 = fmaf(eb, ub, t1);
             if (CAND) {
@@ -114,16 +120,18 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
             }
         }
     } else {
-        float m = __uint_as_float(v[0]);           // nv >= 1: column 0 exists
+        float sm = __uint_as_float(v[0]);           // nv >= 1: column 0 exists
 #pragma unroll
         for (int c = 1; c < 32; ++c)
-            if (c < nv) m = fmaxf(m, __uint_as_float(v[c]));
-        cm = m * fmul;
+            if (c < nv) sm = fmaxf(sm, __uint_as_float(v[c]));
+        cm = sm * fmul;
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
             if (c < nv) {
-                const float u = fmaf(__uint_as_float(v[c]), fmul, -cm);
-                const float e = ex2_approx(u);
+                const float s = __uint_as_float(v[c]);
+                const float u = fmaf(s, fmul, -cm);
+                float e = ex2_approx(u);
+                if (s == sm) { e = 0.f; ++tops; }
                 l0 += e;
                 t0 = fmaf(e, u, t0);
                 if (CAND) {
@@ -133,19 +141,20 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
             }
         }
     }
-    l = l0 + l1;
+    r = (l0 + l1) + (float)(tops - 1);
     t = t0 + t1;
     second = (n2 & ~31u) | (n1 & 31u);
 }
 
-// Joins {maximum m2, sum l2, moment t2} to {m, l, t}: the sums are rescaled to the larger maximum and the exponents
-// inside the moment shift with it.  An empty side has a finite m of -1e30 and l = t = 0, so no infinities meet.
-__device__ __forceinline__ void stats_join(float& m, float& l, float& t, float m2, float l2, float t2) {
+// Joins {maximum m2, sum less one r2, moment t2} to {m, r, t}: the sums are rescaled to the larger maximum and the exponents
+// inside the moment shift with it.  An empty side has a finite m of -1e30, r = -1 and t = 0, so no infinities meet.
+__device__ __forceinline__ void stats_join(float& m, float& r, float& t, float m2, float r2, float t2) {
     const float mn = fmaxf(m, m2);
     const float a = m - mn, b = m2 - mn;
     const float fa = ex2_approx(a), fb = ex2_approx(b);
+    const float l = 1.f + r, l2 = 1.f + r2;
     t = fa * fmaf(a, l, t) + fb * fmaf(b, l2, t2);
-    l = fa * l + fb * l2;
+    r = m >= m2 ? fmaf(fb, l2, r) : fmaf(fa, l, r2);
     m = mn;
 }
 static constexpr float STATS_EMPTY = -1e30f;
@@ -486,7 +495,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             if (lane == 0) { atomicAdd(p.sg_acc, sg); atomicAdd(p.sg_acc + 1, sg1); }
         }
     } else if (EPI == EPI_STATS) {
-        float m = STATS_EMPTY, l = 0.f, t = 0.f;
+        float m = STATS_EMPTY, r = -1.f, t = 0.f;
         const bool cand = p.chunk_max != nullptr;
         for (int ch = u_begin; ch < u_end; ++ch) {
             uint32_t v[32];
@@ -495,11 +504,11 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             const int col0 = n0 + ch * 32;
             const int nv = p.n - col0;
             if (nv > 0) {                      // the same for the whole warp
-                float cm, cl, ct;
+                float cm, cr, ct;
                 uint32_t second;
-                if (cand) stats_chunk<true>(v, st.fmul, nv, cm, cl, ct, second);
-                else      stats_chunk<false>(v, st.fmul, nv, cm, cl, ct, second);
-                stats_join(m, l, t, cm, cl, ct);
+                if (cand) stats_chunk<true>(v, st.fmul, nv, cm, cr, ct, second);
+                else      stats_chunk<false>(v, st.fmul, nv, cm, cr, ct, second);
+                stats_join(m, r, t, cm, cr, ct);
                 if (cand && rvalid) {
                     const long long at = (long long)grow * p.chunk_ld + (col0 >> 5);
                     p.chunk_max[at] = cm;
@@ -509,7 +518,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         }
         tc_fence_before();
         release();
-        if (rvalid) p.stats[(long long)grow * p.stats_ld + 2 * (n0 / p.bn) + wg] = make_float4(m, l, t, 0.f);
+        if (rvalid) p.stats[(long long)grow * p.stats_ld + 2 * (n0 / p.bn) + wg] = make_float4(m, r, t, 0.f);
     } else {   // EPI_OUT
         // Wide tiles (two MMAs per K step, see GemmParams::wide): the first MMA's 256 accumulator columns hold the
         // first 128 B rows of CTA 0 and of CTA 1, the second MMA's columns (from TMEM column 256) the remaining rows

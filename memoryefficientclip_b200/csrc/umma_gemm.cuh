@@ -72,7 +72,7 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 // entries at j; what a_i, b_i and the terms are follows from the loss.
 struct VocabCoef {
     const float* row_lse;             // base 2
-    const float* token_s2;            // [rows, k] scores of the entries, base 2, saved by the forward
+    const float* token_lp2;           // [rows, k] base-2 log probabilities of the entries, saved by the forward
     const long long* tokens;          // [rows, k]
     int k;
     int distill;
@@ -105,7 +105,7 @@ __device__ __forceinline__ void vocab_row_factors(const VocabCoef& v, long long 
     a = -(g + (h != 0.f ? h * v.entropy[row] : 0.f)) * v.inv_t;      // h = 0 takes no part, whatever the entropy is
     b = -h * 0.6931471805599453f * v.inv_t;
 }
-// Coefficient at entry e of a row: the dense part from the saved score, and the terms of all entries that name the same
+// Coefficient at entry e of a row: the dense part from the saved log probability, and the terms of all entries that name the same
 // token.  Entries but the first of a token return false.
 __device__ __forceinline__ bool vocab_entry(const VocabCoef& v, long long row, int e, float a, float b, float& value) {
     const long long* tok = v.tokens + row * v.k;
@@ -116,7 +116,7 @@ __device__ __forceinline__ bool vocab_entry(const VocabCoef& v, long long row, i
             if (o < e) return false;
             if (term != nullptr) sum += term[row * v.k + o];
         }
-    const float u = v.token_s2[row * v.k + e] - v.row_lse[row];
+    const float u = v.token_lp2[row * v.k + e];
     const float scale = v.distill ? -a : v.inv_t;
     value = fmaf(exp2f(u), fmaf(b, u, a), scale != 0.f ? sum * scale : 0.f);     // (no teacher: whatever q is)
     return true;
@@ -206,7 +206,7 @@ struct GemmParams {
     // a long K, which would otherwise keep a few SMs busy long after the others are done.
     int splits, k_part, splits2, k_part2;
     long long split_stride, split_stride2;
-    // EPI_STATS: every (row, warp group of a column tile) stores {maximum of S fmul, sum 2^(S fmul - maximum), sum of
+    // EPI_STATS: every (row, warp group of a column tile) stores {maximum of S fmul, sum 2^(S fmul - maximum) - 1, sum of
     // the same times its exponent, 0} in stats[row * stats_ld + 2 * column tile + group].  With top alternatives wanted
     // (chunk_max set) every (row, 32-column chunk) also stores the chunk's maximum of S fmul and, as one word, the
     // distance of its second best (fp32 bits, low five cleared, so never too large) | the column of its best.

@@ -101,7 +101,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
         if (r.tokens != nullptr) b.tokens = r.tokens + r0 * r.k;
         if (r.row_lse != nullptr) b.row_lse = r.row_lse + r0;
         if (r.entropy != nullptr) b.entropy = r.entropy + r0;
-        if (r.token_s2 != nullptr) b.token_s2 = r.token_s2 + r0 * r.k;
+        if (r.token_lp2 != nullptr) b.token_lp2 = r.token_lp2 + r0 * r.k;
         if (r.log_probs != nullptr) b.log_probs = r.log_probs + r0 * r.k;
         if (r.top_k > 0) { b.top_log_probs = r.top_log_probs + r0 * r.top_k; b.top_tokens = r.top_tokens + r0 * r.top_k; }
         if (DISTILL) {
@@ -222,7 +222,7 @@ int meclip_token_log_probs(const void* x, const void* table, int dtype, int64_t 
     r.x = x; r.y = table; r.ldx = ldx; r.ldy = ldt; r.d = (int)d; r.rows = rows; r.vocab = vocab;
     r.fmul = 1.4426950408889634f / temperature;
     r.tokens = reinterpret_cast<const long long*>(tokens); r.k = (int)per_row;
-    r.row_lse = row_lse; r.entropy = entropy; r.token_s2 = token_scores; r.log_probs = log_probs;
+    r.row_lse = row_lse; r.entropy = entropy; r.token_lp2 = token_scores; r.log_probs = log_probs;
     r.top_k = top_k; r.top_log_probs = top_log_probs; r.top_tokens = reinterpret_cast<long long*>(top_tokens);
     return vocab_forward<false>(r, temperature, dtype, workspace, workspace_bytes, status, (cudaStream_t)stream);
 }
@@ -242,7 +242,7 @@ int meclip_token_log_probs_grad(const void* x, const void* table, int dtype, int
     rc = check_vocab_grad("token_log_probs_grad", workspace, workspace_bytes, plan);
     if (rc) return rc;
     VocabCoef c{};
-    c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(tokens); c.k = (int)per_row;
+    c.row_lse = row_lse; c.token_lp2 = token_scores; c.tokens = reinterpret_cast<const long long*>(tokens); c.k = (int)per_row;
     c.vocab = vocab; c.inv_t = 1.f / temperature;
     c.grad_log_probs = grad_log_probs; c.grad_entropy = grad_entropy; c.entropy = entropy;
     c.entries_in_tile = per_row > 0 && per_row <= VOCAB_TILE_ENTRIES && grad_log_probs != nullptr;
@@ -280,7 +280,7 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
     r.x = x; r.y = table; r.ldx = ldx; r.ldy = ldt; r.d = (int)d; r.rows = rows; r.vocab = vocab;
     r.fmul = 1.4426950408889634f / temperature;
     r.tokens = reinterpret_cast<const long long*>(teacher_tokens); r.k = (int)per_row;
-    r.row_lse = row_lse; r.token_s2 = token_scores;
+    r.row_lse = row_lse; r.token_lp2 = token_scores;
     r.teacher_logits = teacher_logits; r.teacher_dtype = teacher_dtype; r.inv_teacher_t = 1.f / teacher_temperature;
     r.teacher_probs = teacher_probs; r.row_loss = row_loss; r.row_has = row_has;
     r.all_loss = row_loss; r.all_has = row_has; r.all_rows = rows; r.mean = mean; r.loss = loss; r.inv_count = inv_count;
@@ -301,7 +301,7 @@ int meclip_distill_grad(const void* x, const void* table, int dtype, int64_t row
     rc = check_vocab_grad("distill_grad", workspace, workspace_bytes, plan);
     if (rc) return rc;
     VocabCoef c{};
-    c.row_lse = row_lse; c.token_s2 = token_scores; c.tokens = reinterpret_cast<const long long*>(teacher_tokens);
+    c.row_lse = row_lse; c.token_lp2 = token_scores; c.tokens = reinterpret_cast<const long long*>(teacher_tokens);
     c.k = (int)per_row; c.distill = 1; c.vocab = vocab; c.inv_t = 1.f / temperature;
     c.grad_out = grad_out; c.grad_per_row = grad_per_row; c.factor = inv_count; c.row_has = row_has; c.probs = teacher_probs;
     c.entries_in_tile = per_row <= VOCAB_TILE_ENTRIES;

@@ -5,7 +5,7 @@
 // The tile pass leaves, per row and half column tile, {maximum, sum, first moment} in base-2 units, and per 32 columns
 // the maximum; nothing of size rows x V is stored.  vocab_rows_kernel joins those, and forms from the operands
 // themselves the few scores that are wanted one by one: those of given tokens, of a teacher's entries, of the best.
-// Base 2: s2 = <x, y> log2(e)/T, lse2 = log2 sum_j 2^s2_j, so log p = (s2 - lse2) ln 2.
+// Base 2: s2 = <x, y> log2(e)/T, lse2 = log2 sum_j 2^s2_j = m + log2(1 + r), log2 p = s2 - lse2.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -30,7 +30,7 @@ struct VocabGrad {
 static VocabCoef vocab_rows_from(VocabCoef v, long long r0) {
     v.row_lse += r0;
     if (v.tokens != nullptr) v.tokens += r0 * v.k;
-    if (v.token_s2 != nullptr) v.token_s2 += r0 * v.k;
+    if (v.token_lp2 != nullptr) v.token_lp2 += r0 * v.k;
     if (v.grad_log_probs != nullptr) v.grad_log_probs += r0 * v.k;
     if (v.grad_entropy != nullptr) v.grad_entropy += r0;
     if (v.entropy != nullptr) v.entropy += r0;
@@ -61,7 +61,7 @@ struct VocabRows {
     const long long* tokens; int k;
     float* row_lse;                   // base 2, may be null
     float* entropy;                   // nats, may be null
-    float* token_s2;                  // may be null
+    float* token_lp2;                 // may be null
     float* log_probs;                 // [rows, k], token scoring
     int top_k; float* top_log_probs; long long* top_tokens; int list_cap;
     // distillation
@@ -76,6 +76,16 @@ struct VocabRows {
     int mean;
     float *loss, *inv_count;
 };
+
+// log2 p of a score s2 that was formed from the operands, in a row with maximum m and sum 1 + r of the tile pass.  The
+// maximum itself takes the tile pass's score: its log probability is then -log2(1 + r), exact however small r is, and what
+// the tile pass is off by cancels.  Another column can be mistaken for the maximum only where the tile pass cannot tell
+// them apart (an ulp for every 64 columns of d).
+__device__ __forceinline__ double vocab_lp2(const VocabRows& p, double s2, float m, float r, float log2l) {
+    const float off = fabsf((float)(s2 - (double)m));
+    const bool is_max = off <= 1.2e-7f * ((float)p.d * 0.015625f + 1.f) * (fabsf(m) + 8.f) || (r < 0.25f && off < 0.5f);
+    return (is_max ? 0.0 : s2 - (double)m) - (double)log2l;
+}
 
 __device__ __forceinline__ void half8(const __nv_bfloat16* p, float (&v)[8]) { load8(p, v); }
 __device__ __forceinline__ void half8(const __half* p, float (&v)[8]) { load8(p, v); }
@@ -247,16 +257,16 @@ __device__ __forceinline__ float warp_sort_desc(float v, int lane) {
     return v;
 }
 
-__device__ __forceinline__ void row_top_write(const VocabRows& p, long long row, int at, double z, long long j, float m, float log2l) {
+__device__ __forceinline__ void row_top_write(const VocabRows& p, long long row, int at, double z, long long j, float m, float r, float log2l) {
     p.top_tokens[row * p.top_k + at] = j;
-    p.top_log_probs[row * p.top_k + at] = (float)((z * (double)p.fmul - (double)m - (double)log2l) * 0.6931471805599453);
+    p.top_log_probs[row * p.top_k + at] = (float)(vocab_lp2(p, z * (double)p.fmul, m, r, log2l) * 0.6931471805599453);
 }
 
 // (a) to (c): leaves the columns in sh.list, their number in sh.count[1] (0 after a crowd, which is finished here) and
 // 2 |x| |y| in red[3].
 template <int G, typename T>
 __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row, int gt, const RowTopShared& sh, float m,
-                                               float log2l, float* red) {
+                                               float r, float log2l, float* red) {
     constexpr int W = G / 32;
     const int lane = gt & 31, w = gt >> 5;
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
@@ -418,7 +428,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                 for (int r = 0; r < 4; ++r)
                     if (i + r < n) list_insert(lz, lj, z[r], j4[r], lane);
             }
-            if (lane < K) row_top_write(p, row, lane, lz, lj, m, log2l);
+            if (lane < K) row_top_write(p, row, lane, lz, lj, m, r, log2l);
             n = -1;
         }
         if (lane == 0) sh.count[1] = n;
@@ -517,30 +527,30 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     uint8_t* top_smem = smem + 64 * 8 + (p.k * 4 + 15) / 16 * 16;
 
     // (1) the row's statistics
-    float m = STATS_EMPTY, l = 0.f, t = 0.f, log2l = 0.f;
+    float m = STATS_EMPTY, r = -1.f, t = 0.f, log2l = 0.f;
     if (active) {
         const float4* st = p.stats + row * p.stats_ld;
         for (int i = gt; i < p.slots; i += G) {
             const float4 v = st[i];
-            stats_join(m, l, t, v.x, v.y, v.z);
+            stats_join(m, r, t, v.x, v.y, v.z);
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o),
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), r2 = __shfl_xor_sync(0xffffffffu, r, o),
                         t2 = __shfl_xor_sync(0xffffffffu, t, o);
-            stats_join(m, l, t, m2, l2, t2);
+            stats_join(m, r, t, m2, r2, t2);
         }
         if (W > 1) {
-            if (lane == 0) { red[w * 4] = m; red[w * 4 + 1] = l; red[w * 4 + 2] = t; }
+            if (lane == 0) { red[w * 4] = m; red[w * 4 + 1] = r; red[w * 4 + 2] = t; }
             __syncthreads();
-            m = red[0]; l = red[1]; t = red[2];
-            for (int i = 1; i < W; ++i) stats_join(m, l, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2]);
+            m = red[0]; r = red[1]; t = red[2];
+            for (int i = 1; i < W; ++i) stats_join(m, r, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2]);
             __syncthreads();
         }
-        log2l = log2f(l);
+        log2l = log1pf(r) * 1.4426950408889634f;
         if (gt == 0) {
             if (p.row_lse != nullptr) p.row_lse[row] = m + log2l;
-            if (p.entropy != nullptr) p.entropy[row] = 0.6931471805599453f * (log2l - t / l);
+            if (p.entropy != nullptr) p.entropy[row] = 0.6931471805599453f * (log2l - t / (1.f + r));
         }
 
         // (2) the scores of the row's entries
@@ -572,9 +582,9 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             for (int e = gt; e < p.k; e += G) {
                 const long long j = tok[e];
                 // a token below 0 is padding: 0; one behind the table is a mistake that shows
-                const float lp = (float)(((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453);
-                p.log_probs[row * p.k + e] = j < 0 ? 0.f : j >= p.vocab ? NAN : lp;
-                if (p.token_s2 != nullptr) p.token_s2[row * p.k + e] = s2[e];
+                const double lp2 = vocab_lp2(p, (double)s2[e], m, r, log2l);
+                p.log_probs[row * p.k + e] = j < 0 ? 0.f : j >= p.vocab ? NAN : (float)(lp2 * 0.6931471805599453);
+                if (p.token_lp2 != nullptr) p.token_lp2[row * p.k + e] = (float)lp2;
             }
         } else {
             // q = softmax of the teacher's logits over the entries that are there; KL = sum q (log q - log p)
@@ -600,15 +610,16 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             for (int e = gt; e < p.k; e += G) {
                 const long long at = row * p.k + e;
                 float q = 0.f;
+                // of every entry that names a row, also an impossible one: the backward stores a coefficient at each
+                const double lp2 = vocab_lp2(p, (double)s2[e], m, r, log2l);
                 if (there(e)) {
                     const float u = logit(e) - um;
                     q = expf(u) * inv;
-                    const double lp = ((double)s2[e] - (double)m - (double)log2l) * 0.6931471805599453;
                     if (tok[e] >= p.vocab) q = NAN;
-                    if (q != 0.f) kl += (double)q * ((double)u - (double)log_sum - lp);
+                    if (q != 0.f) kl += (double)q * ((double)u - (double)log_sum - lp2 * 0.6931471805599453);
                 }
                 p.teacher_probs[at] = q;
-                p.token_s2[at] = s2[e];
+                p.token_lp2[at] = (float)lp2;
             }
             // the terms are few and of one row: fp64 costs nothing and keeps the difference of two logarithms exact
 #pragma unroll
@@ -633,7 +644,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
         const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap), bw = threadIdx.x >> 5;
         uint8_t* top_base = smem_all + (top_smem - smem);
         group_sync<G>();
-        if (active) row_top_select<G, T>(p, row, gt, sh, m, log2l, red);
+        if (active) row_top_select<G, T>(p, row, gt, sh, m, r, log2l, red);
         else if (gt == 0) sh.count[1] = 0;
         __syncthreads();
         rows_top_score<G, T, float>(p, top_base, stride, bw, lane);
@@ -660,7 +671,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
         for (int i = lane; i < n; i += 32) {
             bool ignored;
             const int place = row_top_rank(sh, n, i, 0.0, ignored);
-            if (place < p.top_k) row_top_write(p, row, place, sh.z[i], sh.list[i], m, log2l);
+            if (place < p.top_k) row_top_write(p, row, place, sh.z[i], sh.list[i], m, r, log2l);
         }
         // only where a row's scores are not numbers are there fewer than K
         if (lane < p.top_k && lane >= n) { p.top_tokens[row * p.top_k + lane] = -1; p.top_log_probs[row * p.top_k + lane] = NAN; }

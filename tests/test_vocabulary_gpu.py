@@ -95,6 +95,23 @@ def test_all_scores_low_and_far_apart():
     assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
 
 
+@pytest.mark.parametrize("d,bump", [(64, 24.0), (512, 16.0), (512, 40.0), (1024, 24.0)])
+def test_rows_that_one_token_holds(d, bump):
+    """log p = -log(1 + R), R = sum_j exp(z_j - z_t): down to 1e-11 it is as exact as the scores, which make every term of
+    R off by at most the errors of its two scores."""
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, _ = _pair(200, 3000, d, torch.bfloat16, 9, bump)
+    z, err = oracle.scores(x, table, 1.0)
+    rest = torch.exp(z - z.gather(1, tokens[:, None])).scatter(1, tokens[:, None], 0.0).sum(1)
+    want = -torch.log1p(rest)
+    best = z.argmax(1) == tokens
+    assert best.sum() > 100
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=2)
+    bound = (2.2 * err + 16 * oracle.ULP) * want.abs()
+    _inside(got.log_probs[best.cuda()], want[best], bound[best], "log_probs")
+    _inside(got.top_log_probs[best.cuda(), 0], want[best], bound[best], "top_log_probs")
+
+
 def test_padding_and_tokens_behind_the_table():
     from memoryefficientclip_b200 import token_log_probs
     x, table, tokens, _ = _pair(70, 300, 64, torch.bfloat16, 1)
