@@ -530,6 +530,56 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             unscale_g = pow2(-pow2_exponent(od.scale.panel, PANEL_TARGET));
             unscale_b = pow2(-pow2_exponent(od.scale.operand, OPERAND_TARGET));
         }
+        if (p.tile_out) {
+            // 32 rows x 128 bytes per warp and store: 64 bf16 or 32 fp32 columns (two or one accumulator chunks).  The map's
+            // third dimension is the part of K; rows and columns outside the output are clipped.
+            const int per_unit = od.out_bf16 ? 2 : 1;
+            const int chunks = tile_bn >> 5, tu = (chunks + per_unit - 1) / per_unit, tu_split = (tu + 1) >> 1;
+            uint8_t* buf = tail->scratch + (size_t)(warp - 2) * STORE_BUF_BYTES;
+            for (int u = wg == 0 ? 0 : tu_split; u < (wg == 0 ? tu_split : tu); ++u) {
+                if (lane == 0 && st.stores_in_flight > 0) {
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    st.stores_in_flight = 0;
+                }
+                __syncwarp();
+                for (int h = 0; h < per_unit; ++h) {
+                    uint32_t v[32];
+                    tmem_ld32(taddr + (u * per_unit + h) * 32, v);
+                    tmem_ld_wait();
+                    if (scaled) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * unscale_g * unscale_b);
+                    }
+                    if (od.out_bf16) {
+#pragma unroll
+                        for (int pc = 0; pc < 4; ++pc) {
+                            uint4 pk;
+                            pk.x = pack_bf16x2(__uint_as_float(v[pc * 8 + 0]), __uint_as_float(v[pc * 8 + 1]));
+                            pk.y = pack_bf16x2(__uint_as_float(v[pc * 8 + 2]), __uint_as_float(v[pc * 8 + 3]));
+                            pk.z = pack_bf16x2(__uint_as_float(v[pc * 8 + 4]), __uint_as_float(v[pc * 8 + 5]));
+                            pk.w = pack_bf16x2(__uint_as_float(v[pc * 8 + 6]), __uint_as_float(v[pc * 8 + 7]));
+                            *reinterpret_cast<uint4*>(buf + lane * 128 + (((h * 4 + pc) ^ (lane & 7)) << 4)) = pk;
+                        }
+                    } else {
+#pragma unroll
+                        for (int pc = 0; pc < 8; ++pc)
+                            *reinterpret_cast<uint4*>(buf + lane * 128 + ((pc ^ (lane & 7)) << 4)) =
+                                make_uint4(v[pc * 4], v[pc * 4 + 1], v[pc * 4 + 2], v[pc * 4 + 3]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                const int col = n0 + u * per_unit * 32;
+                if (lane == 0 && col < p.n && m0 + q * 32 < od.m) {
+                    tma_store_3d(&p.out_map[od.problem], smem_u32(buf), col, m0 + q * 32, od.part);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    st.stores_in_flight = 1;
+                }
+            }
+            tc_fence_before();
+            release();
+            return;
+        }
         const int n1 = tile_bn < MAX_BN ? tile_bn : MAX_BN, n2 = tile_bn - n1, h1 = n1 >> 1, half = tile_bn >> 1;
         for (int ch = u_begin; ch < u_end; ++ch) {
             const int c = ch * 32;
@@ -603,7 +653,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
 // (Pending column sums are flushed by the kernels, which know whether the tile loop ended cleanly.)
 template <int EPI>
 __device__ __forceinline__ void epilogue_drain(const EpiState& st, int lane) {
-    if (epi_is_coef(EPI) && lane == 0 && st.stores_in_flight > 0) {
+    if ((epi_is_coef(EPI) || EPI == EPI_OUT) && lane == 0 && st.stores_in_flight > 0) {
         asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 }

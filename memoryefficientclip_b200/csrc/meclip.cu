@@ -597,6 +597,24 @@ static int make_tmap_blocked(CUtensorMap* tm, const void* base, long long rows, 
     return MECLIP_OK;
 }
 
+// Output of a contraction for TMA stores: [parts][rows][cols] bf16 or fp32, boxes of 32 rows x 128 bytes, swizzled.
+static int make_tmap_out(CUtensorMap* tm, void* base, long long cols, long long rows, long long ld, long long parts,
+                         long long part_stride, bool bf16) {
+    EncodeTiledFn enc = get_encode_fn();
+    if (enc == nullptr) return fail(MECLIP_EUNSUPPORTED, "cuTensorMapEncodeTiled not available from this driver");
+    const int elt = bf16 ? 2 : 4;
+    cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)parts};
+    cuuint64_t strides[2] = {(cuuint64_t)ld * elt, (cuuint64_t)(parts > 1 ? part_stride : ld * rows) * elt};
+    cuuint32_t box[3] = {(cuuint32_t)(128 / elt), 32, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(MECLIP_ECUDA, "cuTensorMapEncodeTiled (output) failed (%d) cols=%lld rows=%lld ld=%lld parts=%lld", (int)r, cols, rows, ld, parts);
+    return MECLIP_OK;
+}
+
 static int sm_count() {
     static int cached[64] = {0};
     int dev = 0;
@@ -889,9 +907,15 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         }
     }
     if ((long long)p.num_m_tiles * p.num_n_tiles * p.splits > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
+    if (epi != EPI_OUT || wide || p.acc_in != nullptr) p.tile_out = 0;
+    if (p.tile_out) {
+        rc = make_tmap_out(&p.out_map[0], p.out, n, m, p.ld_out, p.splits, p.split_stride, p.out_bf16 != 0);
+        if (rc) return rc;
+    }
+    const int tail_size = tail_bytes(epi, p.tile_out != 0);
     // shared memory: [<= 1023 B alignment slack][stages][tail]; as many stages as fit, at least 2
     p.stage_bytes = A_STAGE_BYTES + bn * BK * 2;
-    int stages = (SMEM_LIMIT - 1024 - tail_bytes(epi)) / p.stage_bytes;
+    int stages = (SMEM_LIMIT - 1024 - tail_size) / p.stage_bytes;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     static const int env_max_stages = []() { const char* v = std::getenv("MECLIP_MAX_STAGES"); return v ? std::atoi(v) : 0; }();
     static const bool env_static = []() { const char* v = std::getenv("MECLIP_STATIC_SCHED"); return v && v[0] == '1'; }();
@@ -918,11 +942,11 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last < MAX_BN ? p.bn_last : MAX_BN, amn, 0) & idesc_keep;
         p.idesc2_last = p.bn_last > MAX_BN ? umma_idesc_bf16(PAIR_BM, p.bn_last - MAX_BN, amn, 0) : 0u;
         p.stage_bytes = A_STAGE_BYTES + (bn / 2) * BK * 2;
-        stages = (SMEM_LIMIT - 1024 - tail_bytes(epi)) / p.stage_bytes;
+        stages = (SMEM_LIMIT - 1024 - tail_size) / p.stage_bytes;
         if (stages > MAX_STAGES) stages = MAX_STAGES;
         if (env_max_stages >= 2 && stages > env_max_stages) stages = env_max_stages;
         p.num_stages = stages;
-        const size_t pair_smem = 1024 + (size_t)stages * p.stage_bytes + tail_bytes(epi);
+        const size_t pair_smem = 1024 + (size_t)stages * p.stage_bytes + tail_size;
         if (f32) {
             p.idesc = p.idesc_last = umma_idesc_tf32(PAIR_BM, bn);
             if (epi == EPI_SUMS) return launch_pair_t<EPI_SUMS, 0, true>(ta, tb, tc, p, pair_smem, stream);
@@ -937,7 +961,7 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         return fail(MECLIP_EINVAL, "unknown epilogue %d", epi);
     }
     p.num_stages = stages;
-    const size_t smem_bytes = 1024 + (size_t)stages * p.stage_bytes + tail_bytes(epi);
+    const size_t smem_bytes = 1024 + (size_t)stages * p.stage_bytes + tail_size;
 #define MECLIP_DISPATCH(E)                                                                                        \
     if (epi == E) {                                                                                               \
         if (!a.mn_major && !b.mn_major) return launch_gemm_t<E, false, false>(ta, tb, tc, p, smem_bytes, stream); \
@@ -1012,13 +1036,20 @@ static int launch_contractions_dual(const void* panel, long long panel_rows_allo
     p.wide = 0; p.idesc2 = 0; p.idesc2_last = 0; p.narrow_last = 0;
     static const bool env_static = []() { const char* v = std::getenv("MECLIP_STATIC_SCHED"); return v && v[0] == '1'; }();
     if (env_static) p.tile_counter = nullptr;
+    if (py.acc_in != nullptr || px.acc_in != nullptr) p.tile_out = 0;
+    if (p.tile_out) {
+        rc = make_tmap_out(&p.out_map[0], p.out, n, cols, p.ld_out, p.splits, p.split_stride, p.out_bf16 != 0);
+        if (rc == MECLIP_OK) rc = make_tmap_out(&p.out_map[1], p.out2, n, rows, p.ld_out2, p.splits2, p.split_stride2, p.out_bf16_2 != 0);
+        if (rc) return rc;
+    }
+    const int tail_size = tail_bytes(EPI_OUT, p.tile_out != 0);
     p.stage_bytes = A_STAGE_BYTES + (bn / 2) * BK * 2;
-    int stages = (SMEM_LIMIT - 1024 - tail_bytes(EPI_OUT)) / p.stage_bytes;
+    int stages = (SMEM_LIMIT - 1024 - tail_size) / p.stage_bytes;
     if (stages > MAX_STAGES) stages = MAX_STAGES;
     static const int env_max_stages = []() { const char* v = std::getenv("MECLIP_MAX_STAGES"); return v ? std::atoi(v) : 0; }();
     if (env_max_stages >= 2 && stages > env_max_stages) stages = env_max_stages;
     p.num_stages = stages;
-    const size_t smem = 1024 + (size_t)stages * p.stage_bytes + tail_bytes(EPI_OUT);
+    const size_t smem = 1024 + (size_t)stages * p.stage_bytes + tail_size;
     return launch_pair_t<EPI_OUT, 2>(tay, tby, tax, p, smem, stream, &tbx, 4.0 * (double)rows * (double)cols * (double)n);
 }
 
@@ -1056,7 +1087,7 @@ static long long env_ll(const char* name) {
 // honour_overrides == false: the built-in constants, whatever the test hook or the environment say
 // (meclip_grad_static promises a plan that fits its fixed scratch).
 static GradPlan plan_grad(long long rows, long long cols, long long d, bool transposed_copies = true,
-                          bool honour_overrides = true, int panels = 1) {
+                          bool honour_overrides = true, int panels = 1, long long widest = 32768) {
     GradPlan g;
     static const long long env_row_block = env_ll("MECLIP_ROW_BLOCK") / 128 * 128;
     static const long long env_panel_bytes = env_ll("MECLIP_PANEL_MIB") << 20;
@@ -1070,7 +1101,7 @@ static GradPlan plan_grad(long long rows, long long cols, long long d, bool tran
     g.row_block = rows < row_block_max ? rows : row_block_max;
     long long w = panel_bytes / (g.row_block * 2) / 256 * 256;
     if (w < 256) w = 256;
-    if (w > 32768) w = 32768;
+    if (w > widest) w = widest;
     if (w > cols) w = cols;
     g.panel_w = w;
     g.ldg = (long long)round_up((size_t)w, 64);
@@ -1556,7 +1587,8 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     if (rc) return rc;
     const bool two_panels = vg != nullptr && vg->two_panels;
     if (two_panels && transposed_copies) return fail(MECLIP_EINVAL, "grad: two panels without transposed operands only");
-    const GradPlan plan = plan_grad(rows, cols, dn, transposed_copies, honour_overrides, two_panels ? 2 : 1);
+    const GradPlan plan = plan_grad(rows, cols, dn, transposed_copies, honour_overrides, two_panels ? 2 : 1,
+                                    vg != nullptr ? vg->widest : 32768);
     const int lo_chunk = two_panels ? (int)(plan.ldg / 64) : 0;
     if (workspace_bytes < plan.total())
         return fail(MECLIP_ENOSPC, "grad: workspace %zu < %zu bytes", workspace_bytes, plan.total());
@@ -1716,6 +1748,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 p.status = status;
                 p.lo_chunk = lo_chunk;
                 p.scale = OutScale{panel_max, scale_operands ? vg->maxima : nullptr};
+                p.tile_out = vg != nullptr;
                 p.tile_counter = use_counters ? counters + 3 * t + 2 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dy) + (size_t)c0 * lddy * dy_elt;
                 float* scratch = dy_scratch + (size_t)c0 * d;
@@ -1733,7 +1766,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     Operand a{gpanel[gb], plan.ldg / 64, true, plan.row_block}, b{X + r0 * ldx, ldx, true};
                     if (transposed_copies) b = Operand{xt + r0, plan.ld_xt, false};   // [d][K = rows] K-major
                     a.f16 = b.f16 = panel_f16;
-                    const int bn = pick_contraction_bn(nc, d, overlap, transposed_copies);
+                    const int bn = vg != nullptr ? split_tile_width(nc, d, nr, overlap, transposed_copies) : pick_contraction_bn(nc, d, overlap, transposed_copies);
                     SplitK sk;
                     if (vg != nullptr) sk = split_alone(p, nc, d, nr, bn, vg->split_buf, vg->split_bytes);
                     t_tag = TAG_DY;
@@ -1750,6 +1783,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 p.status = status;
                 p.lo_chunk = lo_chunk;
                 p.scale = OutScale{panel_max, scale_operands ? vg->maxima + 1 : nullptr};
+                p.tile_out = vg != nullptr;
                 p.tile_counter = use_counters ? counters + 3 * t + 1 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dx) + (size_t)r0 * lddx * dx_elt;
                 if (dx_mode == MECLIP_ACCUM_F32) {
@@ -1779,7 +1813,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     Operand a{gpanel[gb], plan.ldg / 64, false, plan.row_block}, b{Y + c0 * ldy, ldy, true};
                     if (transposed_copies) b = Operand{yt + c0, plan.ld_yt, false};   // [d][K = cols] K-major
                     a.f16 = b.f16 = panel_f16;
-                    const int bn = pick_contraction_bn(nr, dn, overlap, transposed_copies);
+                    const int bn = vg != nullptr ? split_tile_width(nr, dn, nc, overlap, transposed_copies) : pick_contraction_bn(nr, dn, overlap, transposed_copies);
                     SplitK sk;
                     if (vg != nullptr) sk = split_alone(p, nr, dn, nc, bn, vg->split_buf2, vg->split_bytes);
                     t_tag = TAG_DX;

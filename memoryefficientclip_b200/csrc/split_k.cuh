@@ -71,6 +71,12 @@ static SplitK split_into(GemmParams& p, long long m, long long n, long long k_st
     return s;
 }
 
+// Tile width of a contraction that may be cut: 256 columns where K is long, since parts fill the SMs then and every column
+// tile reads the panel again (64 x 32768 x 1152: 18 tiles of 64 columns 49 us, 5 of 256 25 us); else as for others.
+static int split_tile_width(long long m, long long n, long long k, bool shares_gpu, bool b_k_major) {
+    return n >= 256 && k >= 64 * BK ? 256 : pick_contraction_bn(m, n, shares_gpu, b_k_major);
+}
+
 // A contraction that has the GPU to itself: as many parts as SMs have no tile.
 static long long split_parts_alone(long long m, long long n, long long k_steps, int bn) {
     const long long tiles = ((m + BM - 1) / BM) * ((n + bn - 1) / bn);

@@ -206,6 +206,10 @@ struct GemmParams {
     // a long K, which would otherwise keep a few SMs busy long after the others are done.
     int splits, k_part, splits2, k_part2;
     long long split_stride, split_stride2;
+    // Contractions whose output leaves through shared memory and TMA stores (tile_out; needs the scratch tiles): one map
+    // per problem.  A lane's own 16-byte stores touch 32 rows at a time and cost more than a tile of a short K computes.
+    int tile_out;
+    alignas(64) CUtensorMap out_map[2];
     // EPI_STATS: every (row, warp group of a column tile) stores {maximum of S fmul, sum 2^(S fmul - maximum) - 1, sum of
     // the same times its exponent, 0} in stats[row * stats_ld + 2 * column tile + group].  With top alternatives wanted
     // (chunk_max set) every (row, 32-column chunk) also stores the chunk's maximum of S fmul and, as one word, the
@@ -262,9 +266,9 @@ struct SharedTail {
     int abort_flag;
 };
 
-__host__ __device__ constexpr int tail_bytes(int epi) {
+__host__ __device__ constexpr int tail_bytes(int epi, bool tile_out = false) {
     // the scratch union is the first member; kernels that do not need all of it start the tail later
-    return (int)sizeof(SharedTail) - (epi_is_coef(epi) ? 0 : epi == EPI_SUMS ? 4 * 2 * STORE_BUF_BYTES - 4 * MAX_BN * 4
+    return (int)sizeof(SharedTail) - (epi_is_coef(epi) || tile_out ? 0 : epi == EPI_SUMS ? 4 * 2 * STORE_BUF_BYTES - 4 * MAX_BN * 4
                                                                             : 4 * 2 * STORE_BUF_BYTES);   // OUT, STATS
 }
 
@@ -298,6 +302,7 @@ struct OutDesc {
     const float* acc_in;
     long long ld_acc;
     OutScale scale;
+    int problem, part;
 };
 
 // Problem of a tile id in a dual launch (0 or 1); the id is made relative to its problem.
@@ -306,8 +311,8 @@ __device__ __forceinline__ int tile_problem(const GemmParams& p, int& tile) {
     return 0;
 }
 __device__ __forceinline__ OutDesc out_desc(const GemmParams& p, int problem, int part = 0) {
-    if (problem == 0) return OutDesc{p.m, part > 0 ? reinterpret_cast<float*>(p.out) + part * p.split_stride : p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc, p.scale};
-    return OutDesc{p.m2, part > 0 ? reinterpret_cast<float*>(p.out2) + part * p.split_stride2 : p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2, p.scale2};
+    if (problem == 0) return OutDesc{p.m, part > 0 ? reinterpret_cast<float*>(p.out) + part * p.split_stride : p.out, p.ld_out, p.out_bf16, p.acc_in, p.ld_acc, p.scale, 0, part};
+    return OutDesc{p.m2, part > 0 ? reinterpret_cast<float*>(p.out2) + part * p.split_stride2 : p.out2, p.ld_out2, p.out_bf16_2, p.acc_in2, p.ld_acc2, p.scale2, 1, part};
 }
 // Tiles of a problem, parts of K included.
 template <int EPI>
@@ -379,7 +384,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     // The tail sits behind the stages; its unused leading part of `scratch` overlaps the last stage
     // region on purpose for SUMS / OUT (they never touch those bytes), see tail_bytes().
     const uint32_t stages_bytes = (uint32_t)p.num_stages * (uint32_t)p.stage_bytes;
-    const uint32_t tail_off = ((stages_bytes + 1023u) & ~1023u) + (uint32_t)tail_bytes(EPI) - (uint32_t)sizeof(SharedTail);
+    const uint32_t tail_off = ((stages_bytes + 1023u) & ~1023u) + (uint32_t)tail_bytes(EPI, EPI == EPI_OUT && p.tile_out) - (uint32_t)sizeof(SharedTail);
     SharedTail* tail = reinterpret_cast<SharedTail*>(smem + (int)tail_off);
 
     const int warp = threadIdx.x >> 5;

@@ -42,7 +42,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     uint8_t* smem = smem_raw + pad;
     const uint32_t smem_base = raw_addr + pad;
     const uint32_t stages_bytes = (uint32_t)p.num_stages * (uint32_t)p.stage_bytes;
-    const uint32_t tail_off = ((stages_bytes + 1023u) & ~1023u) + (uint32_t)tail_bytes(EPI) - (uint32_t)sizeof(SharedTail);
+    const uint32_t tail_off = ((stages_bytes + 1023u) & ~1023u) + (uint32_t)tail_bytes(EPI, EPI == EPI_OUT && p.tile_out) - (uint32_t)sizeof(SharedTail);
     SharedTail* tail = reinterpret_cast<SharedTail*>(smem + (int)tail_off);
 
     const int warp = threadIdx.x >> 5;

@@ -145,6 +145,7 @@ static constexpr long long VOCAB_OVERLAP_ROWS = 1024;
 
 struct VocabGradPlan {
     size_t rows_bytes, split_bytes, grad_bytes;
+    long long widest;
     int split_bufs;
     bool transposed, two_panels, overlap;
     size_t total() const { return rows_bytes + 256 + split_bufs * split_bytes + grad_bytes; }
@@ -158,7 +159,8 @@ static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab,
     // The rounding of a coefficient to bf16 (2^-9 on average) does not average out where a row's gradient is carried by one
     // coefficient: its whole gradient is off by that much, as much as the output's own rounding.
     g.two_panels = !f16 && !g.transposed;
-    const GradPlan plan = plan_grad(rows, vocab, d, g.transposed, true, g.two_panels ? 2 : 1);
+    g.widest = vocab;           // the panel's bytes are limit enough; every further panel is three launches
+    const GradPlan plan = plan_grad(rows, vocab, d, g.transposed, true, g.two_panels ? 2 : 1, g.widest);
     g.grad_bytes = plan.total();
     const bool dual = g.transposed && d >= 256 && dual_allowed() && pair_mode() != 0 && !wide_allowed();
     g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual, g.two_panels);
@@ -180,6 +182,7 @@ static int vocab_grad(const VocabCoef& coef, int dtype, const void* x, const voi
     vg.f16 = dtype == MECLIP_F16;
     vg.tile_fmul = vocab_tile_fmul(temperature, d);
     vg.two_panels = plan.two_panels;
+    vg.widest = plan.widest;
     vg.maxima = reinterpret_cast<float*>(ws + plan.rows_bytes);
     uint8_t* split = ws + plan.rows_bytes + 256;
     vg.split_buf = reinterpret_cast<float*>(split);

@@ -21,6 +21,7 @@ struct VocabGrad {
     VocabCoef coef;
     int f16;                          // operands are fp16, and so is the panel
     float tile_fmul;
+    long long widest;                 // columns of a coefficient panel at most
     int two_panels;                   // bf16 panel and a second one with its remainders
     float* maxima;                    // [3]: largest magnitudes of x and table, bound on the coefficients; cleared by grad_impl
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
@@ -722,12 +723,14 @@ operand_max_kernel(const uint16_t* __restrict__ m0, long long ld0, long long row
                    long long rows1, int d, float* __restrict__ max0, float* __restrict__ max1) {
     const uint16_t* m = blockIdx.y == 0 ? m0 : m1;
     const long long ld = blockIdx.y == 0 ? ld0 : ld1, rows = blockIdx.y == 0 ? rows0 : rows1;
-    const int per_row = d / 8;
-    const long long all = rows * per_row, step = (long long)gridDim.x * 256;
+    // rows that follow one another are one long row
+    const long long per_row = ld == d ? rows * d / 8 : d / 8, lines = ld == d ? 1 : rows;
+    const long long all = lines * per_row, step = (long long)gridDim.x * 256;
     unsigned int best = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(m + i / per_row * ld + i % per_row * 8));
+        const long long at = lines == 1 ? i * 8 : i / per_row * ld + i % per_row * 8;
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(m + at));
         best = __vmaxu2(best, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
     }
     unsigned int top = max(best & 0xffffu, best >> 16) << 16;    // as fp32 bits
