@@ -89,29 +89,32 @@ __device__ __forceinline__ void coef_chunk(const uint32_t (&v)[32], float fmul, 
 template <bool CAND>
 __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul, int nv, float& cm, float& r, float& t,
                                             uint32_t& second) {
-    float l0 = 0.f, l1 = 0.f, t0 = 0.f, t1 = 0.f;
+    float lsum, tsum;
     int tops = 0;                                   // columns that share the maximum
     uint32_t n1 = 0x7fffffffu, n2 = 0x7fffffffu;
     if (nv >= 32) {
-        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]), m2 = __uint_as_float(v[2]), m3 = __uint_as_float(v[3]);
+        float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
 #pragma unroll
-        for (int c = 4; c < 32; c += 4) {
-            m0 = fmaxf(m0, __uint_as_float(v[c]));
-            m1 = fmaxf(m1, __uint_as_float(v[c + 1]));
-            m2 = fmaxf(m2, __uint_as_float(v[c + 2]));
-            m3 = fmaxf(m3, __uint_as_float(v[c + 3]));
+        for (int c = 2; c < 30; c += 4) {
+            m0 = max3(m0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+            m1 = max3(m1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
         }
-        const float sm = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+        const float sm = fmaxf(m0, max3(m1, __uint_as_float(v[30]), __uint_as_float(v[31])));
         cm = sm * fmul;
+        // two columns per instruction where there is one for it; `all` keeps the maxima in, to count them
+        const uint64_t mul2 = f32x2(fmul, fmul), sub2 = f32x2(-cm, -cm);
+        uint64_t l = 0, all = 0, t2 = 0;
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
             const float sa = __uint_as_float(v[c]), sb = __uint_as_float(v[c + 1]);
-            const float ua = fmaf(sa, fmul, -cm), ub = fmaf(sb, fmul, -cm);
-            float ea = ex2_approx(ua), eb = ex2_approx(ub);
-            if (sa == sm) { ea = 0.f; ++tops; }
-            if (sb == sm) { eb = 0.f; ++tops; }
-            l0 += ea; l1 += eb;
-            t0 = fmaf(ea, ua, t0); t1 = fmaf(eb, ub, t1);
+            const uint64_t u = fma_f32x2(f32x2(sa, sb), mul2, sub2);
+            float ua, ub;
+            f32x2_split(u, ua, ub);
+            const float ea = ex2_approx(ua), eb = ex2_approx(ub);
+            all = add_f32x2(all, f32x2(ea, eb));
+            const uint64_t e = f32x2(sa == sm ? 0.f : ea, sb == sm ? 0.f : eb);
+            l = add_f32x2(l, e);
+            t2 = fma_f32x2(e, u, t2);
             if (CAND) {
                 const uint32_t ka = (__float_as_uint(ua) & 0x7fffffe0u) | (uint32_t)c;
                 const uint32_t kb = (__float_as_uint(ub) & 0x7fffffe0u) | (uint32_t)(c + 1);
@@ -119,12 +122,20 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
                 n2 = min(n2, max(n1, kb)); n1 = min(n1, kb);
             }
         }
+        float x0, x1, y0, y1, z0, z1;
+        f32x2_split(l, x0, x1);
+        f32x2_split(t2, y0, y1);
+        f32x2_split(all, z0, z1);
+        lsum = x0 + x1;
+        tsum = y0 + y1;
+        tops = __float2int_rn((z0 + z1) - lsum);    // each is 1 up to the rounding of cm
     } else {
         float sm = __uint_as_float(v[0]);           // nv >= 1: column 0 exists
 #pragma unroll
         for (int c = 1; c < 32; ++c)
             if (c < nv) sm = fmaxf(sm, __uint_as_float(v[c]));
         cm = sm * fmul;
+        lsum = tsum = 0.f;
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
             if (c < nv) {
@@ -132,8 +143,8 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
                 const float u = fmaf(s, fmul, -cm);
                 float e = ex2_approx(u);
                 if (s == sm) { e = 0.f; ++tops; }
-                l0 += e;
-                t0 = fmaf(e, u, t0);
+                lsum += e;
+                tsum = fmaf(e, u, tsum);
                 if (CAND) {
                     const uint32_t k = (__float_as_uint(u) & 0x7fffffe0u) | (uint32_t)c;
                     n2 = min(n2, max(n1, k)); n1 = min(n1, k);
@@ -141,8 +152,8 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
             }
         }
     }
-    r = (l0 + l1) + (float)(tops - 1);
-    t = t0 + t1;
+    r = lsum + (float)(tops - 1);
+    t = tsum;
     second = (n2 & ~31u) | (n1 & 31u);
 }
 
@@ -162,10 +173,13 @@ static constexpr float STATS_EMPTY = -1e30f;
 // Coefficients of a chunk over a vocabulary: 2^u (a + b u), u = log2 of the row's softmax.
 __device__ __forceinline__ void vocab_chunk(const uint32_t (&v)[32], float fmul, float lse, float a, float b,
                                             float (&gv)[32]) {
+    const uint64_t mul2 = f32x2(fmul, fmul), sub2 = f32x2(-lse, -lse), a2 = f32x2(a, a), b2 = f32x2(b, b);
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-        const float u = fmaf(__uint_as_float(v[c]), fmul, -lse);
-        gv[c] = ex2_approx(u) * fmaf(b, u, a);
+    for (int c = 0; c < 32; c += 2) {
+        const uint64_t u = fma_f32x2(f32x2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), mul2, sub2);
+        float ua, ub;
+        f32x2_split(u, ua, ub);
+        f32x2_split(mul_f32x2(f32x2(ex2_approx(ua), ex2_approx(ub)), fma_f32x2(b2, u, a2)), gv[c], gv[c + 1]);
     }
 }
 
@@ -353,22 +367,23 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         bool v_here = false;
         if (VOCAB) {
             if (rvalid) {
-                v_lse = __ldg(p.vc.row_lse + grow);
                 const float g_scale = pow2(pow2_exponent(p.panel_max, PANEL_TARGET));
-                vocab_row_factors(p.vc, grow, v_a, v_b);
-                if (p.vc.entries_in_tile) {
+                const float4 f = __ldg(p.row_factors + grow);
+                v_lse = f.x;
+                v_a = f.y * g_scale;
+                v_b = f.z * g_scale;
+                if (p.row_entries != nullptr) {
+                    const float4 en = __ldg(p.row_entries + grow);
+                    const float cols[2] = {en.x, en.z}, vals[2] = {en.y, en.w};
 #pragma unroll
-                    for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e)
-                        if (e < p.vc.k) {
-                            const long long col = p.vc.tokens[(long long)grow * p.vc.k + e] - p.vc_col0 - n0;
-                            if (col >= 0 && col < p.bn && n0 + col < p.n && vocab_entry(p.vc, grow, e, v_a, v_b, v_val[e])) {
-                                v_col[e] = (int)col;
-                                v_val[e] *= g_scale;
-                            }
+                    for (int e = 0; e < VOCAB_TILE_ENTRIES; ++e) {
+                        const long long col = (long long)__float_as_int(cols[e]) - p.panel_col0 - n0;
+                        if (__float_as_int(cols[e]) >= 0 && col >= 0 && col < p.bn && n0 + col < p.n) {
+                            v_col[e] = (int)col;
+                            v_val[e] = vals[e] * g_scale;
                         }
+                    }
                 }
-                v_a *= g_scale;
-                v_b *= g_scale;
             }
             bool any = false;
 #pragma unroll

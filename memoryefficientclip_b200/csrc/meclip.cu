@@ -1632,10 +1632,12 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     const bool panel_f16 = vg != nullptr && (vg->f16 || transposed_copies);
     const bool scale_operands = panel_f16 && !vg->f16;
     const float* panel_max = panel_f16 ? vg->maxima + 2 : nullptr;
-    if (panel_f16) {
-        MECLIP_CUDA(cudaMemsetAsync(vg->maxima, 0, 3 * sizeof(float), s0));
-        ScopedTiming timing(s0, TAG_ROW, (double)rows * 16.0);
-        vocab_bound_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, s0>>>(vg->coef, rows, vg->maxima + 2);
+    if (vg != nullptr) {
+        if (panel_f16) MECLIP_CUDA(cudaMemsetAsync(vg->maxima, 0, 3 * sizeof(float), s0));
+        const int wpb = ROW_KERNEL_THREADS / 32;
+        ScopedTiming timing(s0, TAG_ROW, (double)rows * (48.0 + 12.0 * vg->coef.k));
+        vocab_prepare_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s0>>>(
+            vg->coef, rows, vg->row_factors, vg->row_entries, panel_f16 ? vg->maxima + 2 : nullptr);
         MECLIP_CUDA(cudaGetLastError());
     }
     if (transposed_copies) {
@@ -1719,8 +1721,9 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 if (vg != nullptr) {
                     p.sigmoid = 0;
                     p.fmul = vg->tile_fmul;
-                    p.vc = vocab_rows_from(vg->coef, r0);
-                    p.vc_col0 = c0;
+                    p.row_factors = vg->row_factors + r0;
+                    p.row_entries = vg->row_entries != nullptr ? vg->row_entries + r0 : nullptr;
+                    p.panel_col0 = c0;
                     p.lo_chunk = lo_chunk;
                     if (!use_counters) p.tile_counter = nullptr;
                     p.panel_f16 = panel_f16;
@@ -1728,7 +1731,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     a.f16 = b.f16 = vg->f16;
                     // 256-column tiles beyond one row tile: only those run on CTA pairs
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
-                    if (rc == MECLIP_OK) rc = launch_vocab_entries(p.vc, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_max, panel_f16, s0);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_max, panel_f16, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                 }

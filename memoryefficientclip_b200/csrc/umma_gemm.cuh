@@ -68,59 +68,7 @@ __device__ __forceinline__ int pow2_exponent(const float* max, int target) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// Coefficients of a softmax over a vocabulary, dz_ij / T = p_ij (a_i + b_i log2 p_ij) + sum of the terms of the row's
-// entries at j; what a_i, b_i and the terms are follows from the loss.
-struct VocabCoef {
-    const float* row_lse;             // base 2
-    const float* token_lp2;           // [rows, k] base-2 log probabilities of the entries, saved by the forward
-    const long long* tokens;          // [rows, k]
-    int k;
-    int distill;
-    long long vocab;
-    float inv_t;
-    // token scoring: a = -(sum of g over the tokens inside the table + h H) / T, b = -h ln 2 / T, terms g / T
-    const float *grad_log_probs, *grad_entropy, *entropy;        // g [rows, k], h, H [rows]; g, h may be null
-    const float* row_g;               // [rows] sums of g, formed beforehand for more than a few entries, else null
-    // distillation: a = w = grad_out * factor / T where there is a teacher, b = 0, terms -w q
-    const float *grad_out, *factor, *row_has, *probs;            // probs = q [rows, k]; factor may be null
-    int grad_per_row;
-    int entries_in_tile;              // the tile pass adds the entries' terms itself (k <= VOCAB_TILE_ENTRIES)
-};
-static constexpr int VOCAB_TILE_ENTRIES = 2;
-
-__device__ __forceinline__ void vocab_row_factors(const VocabCoef& v, long long row, float& a, float& b) {
-    if (v.distill) {
-        a = v.row_has[row] > 0.f ? v.grad_out[v.grad_per_row ? row : 0] * (v.factor != nullptr ? __ldg(v.factor) : 1.f) * v.inv_t : 0.f;
-        b = 0.f;
-        return;
-    }
-    float g = 0.f;
-    if (v.row_g != nullptr) g = v.row_g[row];
-    else if (v.grad_log_probs != nullptr)
-        for (int e = 0; e < v.k; ++e) {
-            const long long j = v.tokens[row * v.k + e];
-            if (j >= 0 && j < v.vocab) g += v.grad_log_probs[row * v.k + e];
-        }
-    const float h = v.grad_entropy != nullptr ? v.grad_entropy[row] : 0.f;
-    a = -(g + (h != 0.f ? h * v.entropy[row] : 0.f)) * v.inv_t;      // h = 0 takes no part, whatever the entropy is
-    b = -h * 0.6931471805599453f * v.inv_t;
-}
-// Coefficient at entry e of a row: the dense part from the saved log probability, and the terms of all entries that name the same
-// token.  Entries but the first of a token return false.
-__device__ __forceinline__ bool vocab_entry(const VocabCoef& v, long long row, int e, float a, float b, float& value) {
-    const long long* tok = v.tokens + row * v.k;
-    const float* term = v.distill ? v.probs : v.grad_log_probs;
-    float sum = 0.f;
-    for (int o = 0; o < v.k; ++o)
-        if (tok[o] == tok[e]) {
-            if (o < e) return false;
-            if (term != nullptr) sum += term[row * v.k + o];
-        }
-    const float u = v.token_lp2[row * v.k + e];
-    const float scale = v.distill ? -a : v.inv_t;
-    value = fmaf(exp2f(u), fmaf(b, u, a), scale != 0.f ? sum * scale : 0.f);     // (no teacher: whatever q is)
-    return true;
-}
+static constexpr int VOCAB_TILE_ENTRIES = 2;       // entries of a row that the tile pass adds itself (GemmParams::row_entries)
 
 struct GemmParams {
     int m, n, k;              // valid extents of the problem
@@ -219,9 +167,11 @@ struct GemmParams {
     float* chunk_max;
     uint32_t* chunk_second;
     long long chunk_ld;
-    // EPI_VCOEF: u = S fmul - row_lse[i] = log2 p_ij, G_ij = 2^u (a_i + b_i u) + the row's own terms; see VocabCoef
-    VocabCoef vc;
-    long long vc_col0;        // first column of the panel in the table
+    // EPI_VCOEF: u = S fmul - lse_i = log2 p_ij, G_ij = 2^u (a_i + b_i u); row_factors = {lse, a, b, 0}.  row_entries (null:
+    // another kernel stores them) = up to two {column in the table as int bits or -1, coefficient} that replace the dense ones.
+    const float4* row_factors;
+    const float4* row_entries;
+    long long panel_col0;     // first column of the panel in the table
     // A second panel with what the bf16 rounding of the first one left, lo_chunk 64-column chunks behind it (0: none).
     // EPI_VCOEF writes it; a contraction (single-CTA kernel) then walks K twice, from step k_half on over the second panel.
     int lo_chunk, k_half;

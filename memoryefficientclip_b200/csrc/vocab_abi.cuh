@@ -153,7 +153,7 @@ struct VocabGradPlan {
 static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab, long long d) {
     VocabGradPlan g;
     const bool f16 = dtype == MECLIP_F16;
-    g.rows_bytes = round_up((size_t)rows * 4, 256);
+    g.rows_bytes = round_up((size_t)rows * 2 * sizeof(float4), 256);
     g.overlap = rows >= VOCAB_OVERLAP_ROWS;
     g.transposed = transposes_allowed() && (f16 ? g.overlap : rows > VOCAB_TWO_PANEL_ROWS);
     // The rounding of a coefficient to bf16 (2^-9 on average) does not average out where a row's gradient is carried by one
@@ -179,6 +179,8 @@ static int vocab_grad(const VocabCoef& coef, int dtype, const void* x, const voi
                       int dt_mode, int64_t lddt, uint8_t* ws, const VocabGradPlan& plan, int* status, cudaStream_t s) {
     VocabGrad vg;
     vg.coef = coef;
+    vg.row_factors = reinterpret_cast<float4*>(ws);
+    vg.row_entries = coef.k <= VOCAB_TILE_ENTRIES ? vg.row_factors + rows : nullptr;
     vg.f16 = dtype == MECLIP_F16;
     vg.tile_fmul = vocab_tile_fmul(temperature, d);
     vg.two_panels = plan.two_panels;
@@ -248,17 +250,6 @@ int meclip_token_log_probs_grad(const void* x, const void* table, int dtype, int
     c.row_lse = row_lse; c.token_lp2 = token_scores; c.tokens = reinterpret_cast<const long long*>(tokens); c.k = (int)per_row;
     c.vocab = vocab; c.inv_t = 1.f / temperature;
     c.grad_log_probs = grad_log_probs; c.grad_entropy = grad_entropy; c.entropy = entropy;
-    c.entries_in_tile = per_row > 0 && per_row <= VOCAB_TILE_ENTRIES && grad_log_probs != nullptr;
-    if (per_row > VOCAB_TILE_ENTRIES && grad_log_probs != nullptr) {
-        rc = check_device();
-        if (rc) return rc;
-        float* row_g = reinterpret_cast<float*>(workspace);
-        const int wpb = ROW_KERNEL_THREADS / 32;
-        ScopedTiming timing((cudaStream_t)stream, TAG_ROW, (double)rows * 12.0 * per_row);
-        token_grad_sum_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, (cudaStream_t)stream>>>(c, rows, row_g);
-        MECLIP_CUDA(cudaGetLastError());
-        c.row_g = row_g;
-    }
     return vocab_grad(c, dtype, x, table, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode, lddt,
                       reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }
@@ -307,7 +298,6 @@ int meclip_distill_grad(const void* x, const void* table, int dtype, int64_t row
     c.row_lse = row_lse; c.token_lp2 = token_scores; c.tokens = reinterpret_cast<const long long*>(teacher_tokens);
     c.k = (int)per_row; c.distill = 1; c.vocab = vocab; c.inv_t = 1.f / temperature;
     c.grad_out = grad_out; c.grad_per_row = grad_per_row; c.factor = inv_count; c.row_has = row_has; c.probs = teacher_probs;
-    c.entries_in_tile = per_row <= VOCAB_TILE_ENTRIES;
     return vocab_grad(c, dtype, x, table, rows, vocab, d, ldx, ldt, temperature, dx, dx_mode, lddx, dtable, dtable_mode, lddt,
                       reinterpret_cast<uint8_t*>(workspace), plan, status, (cudaStream_t)stream);
 }

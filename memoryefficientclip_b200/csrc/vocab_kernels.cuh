@@ -15,10 +15,44 @@ static constexpr int VOCAB_THREADS = 256;
 static constexpr int VOCAB_MAX_ENTRIES = 256;      // given tokens or teacher entries of one row
 static constexpr int VOCAB_MAX_TOP = 32;           // top alternatives: one per lane
 
-// A backward: the coefficients, with their rows counted from the first one of the problem, the type of the operands, and
-// which form the panel takes.
+// Coefficients of a softmax over a vocabulary, dz_ij / T = p_ij (a_i + b_i log2 p_ij) + sum of the terms of the row's
+// entries at j; what a_i, b_i and the terms are follows from the loss.
+struct VocabCoef {
+    const float* row_lse;             // base 2
+    const float* token_lp2;           // [rows, k] base-2 log probabilities of the entries, saved by the forward
+    const long long* tokens;          // [rows, k]
+    int k;
+    int distill;
+    long long vocab;
+    float inv_t;
+    // token scoring: a = -(sum of g over the tokens inside the table + h H) / T, b = -h ln 2 / T, terms g / T
+    const float *grad_log_probs, *grad_entropy, *entropy;        // g [rows, k], h, H [rows]; g, h may be null
+    // distillation: a = w = grad_out * factor / T where there is a teacher, b = 0, terms -w q
+    const float *grad_out, *factor, *row_has, *probs;            // probs = q [rows, k]; factor may be null
+    int grad_per_row;
+};
+
+// Coefficient at entry e of a row: the dense part from the saved log probability, and the terms of all entries that name the
+// same token.  Entries but the first of a token return false.
+__device__ __forceinline__ bool vocab_entry(const VocabCoef& v, long long row, int e, float a, float b, float& value) {
+    const long long* tok = v.tokens + row * v.k;
+    const float* term = v.distill ? v.probs : v.grad_log_probs;
+    float sum = 0.f;
+    for (int o = 0; o < v.k; ++o)
+        if (tok[o] == tok[e]) {
+            if (o < e) return false;
+            if (term != nullptr) sum += term[row * v.k + o];
+        }
+    const float u = v.token_lp2[row * v.k + e];
+    const float scale = v.distill ? -a : v.inv_t;
+    value = fmaf(exp2f(u), fmaf(b, u, a), scale != 0.f ? sum * scale : 0.f);     // (no teacher: whatever q is)
+    return true;
+}
+
+// A backward: the coefficients, the type of the operands, and which form the panel takes.
 struct VocabGrad {
     VocabCoef coef;
+    float4 *row_factors, *row_entries;          // see GemmParams; entries null: vocab_entries_kernel stores them
     int f16;                          // operands are fp16, and so is the panel
     float tile_fmul;
     long long widest;                 // columns of a coefficient panel at most
@@ -27,20 +61,6 @@ struct VocabGrad {
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
     size_t split_bytes;               // of each
 };
-// The coefficients of the rows from r0 on.
-static VocabCoef vocab_rows_from(VocabCoef v, long long r0) {
-    v.row_lse += r0;
-    if (v.tokens != nullptr) v.tokens += r0 * v.k;
-    if (v.token_lp2 != nullptr) v.token_lp2 += r0 * v.k;
-    if (v.grad_log_probs != nullptr) v.grad_log_probs += r0 * v.k;
-    if (v.grad_entropy != nullptr) v.grad_entropy += r0;
-    if (v.entropy != nullptr) v.entropy += r0;
-    if (v.grad_per_row && v.grad_out != nullptr) v.grad_out += r0;
-    if (v.row_has != nullptr) v.row_has += r0;
-    if (v.row_g != nullptr) v.row_g += r0;
-    if (v.probs != nullptr) v.probs += r0 * v.k;
-    return v;
-}
 
 // The tensor cores cut what does not fit into an fp32 accumulator instead of rounding it, once every 16 products, so a
 // score comes out too small in magnitude, on average by a part of the partial sums it ran through.  For a score that
@@ -679,41 +699,53 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     }
 }
 
-// Sums of the gradients of a row's log probabilities, over the tokens inside the table.
+// Row factors and, for rows of few entries, their coefficients, so that a tile pass loads two vectors per row; one warp per
+// row.  Also a bound on all coefficients' magnitude, |a| + 0.5308 |b| + sum |terms| (p |log2 p| <= log2(e) / e), as the
+// maximum of non-negative floats' bits: the order of the atomics does not matter.
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-token_grad_sum_kernel(const __grid_constant__ VocabCoef v, long long rows, float* __restrict__ row_g) {
+vocab_prepare_kernel(const __grid_constant__ VocabCoef v, long long rows, float4* __restrict__ factors,
+                     float4* __restrict__ entries, float* __restrict__ bound) {
+    __shared__ float most[ROW_KERNEL_THREADS / 32];
     const long long row = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    float g = 0.f;
-    for (int e = lane; e < v.k; e += 32) {
-        const long long j = v.tokens[row * v.k + e];
-        if (j >= 0 && j < v.vocab) g += v.grad_log_probs[row * v.k + e];
-    }
-    g = warp_sum(g);
-    if (lane == 0) row_g[row] = g;
-}
-
-// A bound on the coefficients' magnitude, |a| + 0.5308 |b| + sum |terms| over all rows (p |log2 p| <= log2(e) / e), as the
-// maximum of non-negative floats' bits: the order of the atomics does not matter.
-__global__ void __launch_bounds__(256)
-vocab_bound_kernel(const __grid_constant__ VocabCoef v, long long rows, float* __restrict__ bound) {
-    const long long row = (long long)blockIdx.x * 256 + threadIdx.x;
     float m = 0.f;
     if (row < rows) {
-        float a, b;
-        vocab_row_factors(v, row, a, b);
-        m = fabsf(a) + 0.5308f * fabsf(b);
-        if (v.distill) m += fabsf(a);                            // sum q <= 1
-        else if (v.grad_log_probs != nullptr)
-            for (int e = 0; e < v.k; ++e) {
-                const long long j = v.tokens[row * v.k + e];
-                if (j >= 0 && j < v.vocab) m += fabsf(v.grad_log_probs[row * v.k + e]) * v.inv_t;
+        float a, b = 0.f;
+        if (v.distill) {
+            a = v.row_has[row] > 0.f ? v.grad_out[v.grad_per_row ? row : 0] * (v.factor != nullptr ? __ldg(v.factor) : 1.f) * v.inv_t : 0.f;
+            m = 2.f * fabsf(a);                                  // sum q <= 1
+        } else {
+            float g = 0.f, size = 0.f;
+            if (v.grad_log_probs != nullptr)
+                for (int e = lane; e < v.k; e += 32) {
+                    const long long j = v.tokens[row * v.k + e];
+                    if (j >= 0 && j < v.vocab) { const float x = v.grad_log_probs[row * v.k + e]; g += x; size += fabsf(x); }
+                }
+            g = warp_sum(g);
+            size = warp_sum(size);
+            const float h = v.grad_entropy != nullptr ? v.grad_entropy[row] : 0.f;
+            a = -(g + (h != 0.f ? h * v.entropy[row] : 0.f)) * v.inv_t;      // h = 0 takes no part, whatever the entropy is
+            b = -h * 0.6931471805599453f * v.inv_t;
+            m = fabsf(a) + 0.5308f * fabsf(b) + size * v.inv_t;
+        }
+        if (lane == 0) factors[row] = make_float4(v.row_lse[row], a, b, 0.f);
+        if (entries != nullptr && lane < VOCAB_TILE_ENTRIES) {
+            float value = 0.f;
+            int col = -1;
+            if (lane < v.k) {
+                const long long j = v.tokens[row * v.k + lane];
+                if (j >= 0 && j < v.vocab && vocab_entry(v, row, lane, a, b, value)) col = (int)j;
             }
+            reinterpret_cast<float2*>(entries + row)[lane] = make_float2(__int_as_float(col), value);
+        }
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) atomicMax(reinterpret_cast<unsigned int*>(bound), __float_as_uint(m));
+    if (bound == nullptr) return;
+    if (lane == 0) most[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < ROW_KERNEL_THREADS / 32; ++i) m = fmaxf(m, most[i]);
+        atomicMax(reinterpret_cast<unsigned int*>(bound), __float_as_uint(m));
+    }
 }
 
 // Largest magnitude of a bf16 matrix (blockIdx.y = 0) and of a second one (1).  Bound by HBM; the integer maximum of bits
@@ -773,41 +805,41 @@ transpose_scaled_f16_kernel(const __nv_bfloat16* __restrict__ in, long long ld_i
     }
 }
 
-// Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved scores and rounded once, over
-// what the tile pass stored there.  One warp per row.  (Up to VOCAB_TILE_ENTRIES entries per row the tile pass does it.)
+// Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved log probabilities and rounded once,
+// over what the tile pass stored there.  One warp per row.
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
-vocab_entries_kernel(const __grid_constant__ VocabCoef v, long long nr, long long c0, long long nc,
-                     __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk, const float* __restrict__ panel_max, int f16) {
+vocab_entries_kernel(const __grid_constant__ VocabCoef v, const float4* __restrict__ factors, long long r0, long long nr,
+                     long long c0, long long nc, __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk,
+                     const float* __restrict__ panel_max, int f16) {
     const long long i = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= nr) return;
-    float a, b;
-    vocab_row_factors(v, i, a, b);
+    const float4 f = factors[r0 + i];
     const float g_scale = pow2(pow2_exponent(panel_max, PANEL_TARGET));
     for (int e = lane; e < v.k; e += 32) {
-        const long long j = v.tokens[i * v.k + e];
+        const long long j = v.tokens[(r0 + i) * v.k + e];
         if (j < c0 || j >= c0 + nc) continue;          // absent, outside the table or in another panel
         float value;
-        if (!vocab_entry(v, i, e, a, b, value)) continue;
-        const long long col = j - c0;
+        if (!vocab_entry(v, r0 + i, e, f.y, f.z, value)) continue;
+        const long long col = j - c0, at = ((col >> 6) * rows_alloc + i) * 64 + (col & 63);
         if (f16) {
-            reinterpret_cast<__half*>(panel)[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = __float2half_rn(value * g_scale);
+            reinterpret_cast<__half*>(panel)[at] = __float2half_rn(value * g_scale);
             continue;
         }
         const __nv_bfloat16 hi = __float2bfloat16_rn(value);
-        panel[((col >> 6) * rows_alloc + i) * 64 + (col & 63)] = hi;
-        if (lo_chunk > 0)
-            panel[(((col >> 6) + lo_chunk) * rows_alloc + i) * 64 + (col & 63)] = __float2bfloat16_rn(value - __bfloat162float(hi));
+        panel[at] = hi;
+        if (lo_chunk > 0) panel[at + (long long)lo_chunk * rows_alloc * 64] = __float2bfloat16_rn(value - __bfloat162float(hi));
     }
 }
 
-static int launch_vocab_entries(const VocabCoef& v, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
+static int launch_vocab_entries(const VocabGrad& g, long long r0, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
                                 long long rows_alloc, int lo_chunk, const float* panel_max, int f16, cudaStream_t s) {
-    if (v.k == 0 || v.entries_in_tile || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
+    const VocabCoef& v = g.coef;
+    if (v.k == 0 || g.row_entries != nullptr || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
     const int wpb = ROW_KERNEL_THREADS / 32;
     ScopedTiming timing(s, TAG_ROW, (double)nr * v.k * 18.0);
-    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(v, nr, c0, nc, panel, rows_alloc, lo_chunk,
-                                                                                                   panel_max, f16);
+    vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
+        v, g.row_factors, r0, nr, c0, nc, panel, rows_alloc, lo_chunk, panel_max, f16);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }
