@@ -34,7 +34,7 @@ def embed_tokens(tokens, table, scale=1.0):
     behind the table gives a row of NaN.  table: [V, D] float32, bfloat16 or float16, any D, pitch and alignment.
     """
     ops._check_matrix(table, "table")
-    assert tokens.device == table.device, "tokens and table must be on one device"
+    assert tokens.get_device() == table.get_device(), "tokens and table must be on one device"
     assert tokens.dtype in (torch.int64, torch.int32), f"tokens: dtype {tokens.dtype} not supported (int64 or int32)"
     assert not isinstance(scale, torch.Tensor) and math.isfinite(scale), "scale must be a finite Python number"
     tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)

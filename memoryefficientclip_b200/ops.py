@@ -728,9 +728,10 @@ def vocab_operands(x: torch.Tensor, table: torch.Tensor):
     """(x, table) as the vocabulary passes read them: both fp16 if both inputs are, else both bf16 (fp32 inputs are
     rounded, as everywhere in this package); rows of padded(d) columns, 16-byte aligned."""
     if x.dtype == table.dtype == torch.float16:
-        return tuple(t if _is_operand(t) else _padded_f16(t) for t in (x, table))
-    return tuple(t if t.dtype == torch.bfloat16 and _is_operand(t) else normalize_fwd(t, normalize=False)[0]
-                 for t in (x, table))
+        return (x if _is_operand(x) else _padded_f16(x)), (table if _is_operand(table) else _padded_f16(table))
+    bf16 = torch.bfloat16
+    return (x if x.dtype == bf16 and _is_operand(x) else normalize_fwd(x, normalize=False)[0],
+            table if table.dtype == bf16 and _is_operand(table) else normalize_fwd(table, normalize=False)[0])
 
 
 def _padded_f16(x: torch.Tensor) -> torch.Tensor:
@@ -743,26 +744,33 @@ def token_log_probs(x, table, tokens, temperature, top_k=0, save=False, status=N
     """(log_probs, entropy, top_log_probs, top_tokens, saved) of operands from vocab_operands; tokens int64, contiguous,
     [rows] or [rows, k], and log_probs like them.  saved: what token_log_probs_grad needs besides, None unless asked for
     (meclip_token_log_probs)."""
+    dev = x.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return token_log_probs(x, table, tokens, temperature, top_k, save, status)
     rows, d = x.shape
-    vocab, dev = table.shape[0], x.device
-    per_row = tokens.numel() // rows
-    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    top_lp = top = saved = lse = scores = None
+    vocab, shape, empty, f32 = table.shape[0], tokens.shape, torch.empty, torch.float32
+    per_row = 1 if len(shape) == 1 else shape[1]
+    lp = empty(shape, dtype=f32, device=dev)
+    entropy = empty(rows, dtype=f32, device=dev)
+    top_lp = top = saved = lse = scores = top_lp_at = top_at = None
     if top_k:
-        top_lp = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-        top = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+        top_lp = empty((rows, top_k), dtype=f32, device=dev)
+        top = empty((rows, top_k), dtype=torch.int64, device=dev)
+        top_lp_at, top_at = top_lp.data_ptr(), top.data_ptr()
     if save:                    # one buffer: [rows] log-sum-exps, [rows, per_row] scores
-        saved = torch.empty(rows * (1 + per_row), dtype=torch.float32, device=dev)
+        saved = empty(rows * (1 + per_row), dtype=f32, device=dev)
         lse = saved.data_ptr()
         scores = lse + 4 * rows
     lib = _lib.load()
-    with _on_device(dev):
-        ws = torch.empty(lib.meclip_vocab_workspace_bytes(rows, vocab, top_k), dtype=torch.uint8, device=dev)
-        _lib.check(lib.meclip_token_log_probs(
-            x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0), temperature,
-            tokens.data_ptr(), per_row, lp.data_ptr(), entropy.data_ptr(), top_k, _ptr(top_lp), _ptr(top), lse, scores,
-            ws.data_ptr(), ws.numel(), _ptr(status), _stream(x)))
+    n = lib.meclip_vocab_workspace_bytes(rows, vocab, top_k)
+    ws = empty(n, dtype=torch.uint8, device=dev)
+    rc = lib.meclip_token_log_probs(
+        x.data_ptr(), table.data_ptr(), _DT[x.dtype], rows, vocab, d, x.stride(0), table.stride(0), temperature,
+        tokens.data_ptr(), per_row, lp.data_ptr(), entropy.data_ptr(), top_k, top_lp_at, top_at, lse, scores,
+        ws.data_ptr(), n, _ptr(status), _stream(x))
+    if rc:
+        _lib.check(rc)
     return lp, entropy, top_lp, top, saved
 
 
@@ -842,24 +850,35 @@ def distill_backward(x, table, teacher_tokens, temperature, saved, grad_out, dx_
 
 def embed(tokens: torch.Tensor, table: torch.Tensor, scale: float) -> torch.Tensor:
     """scale * table[tokens] for contiguous int64 tokens of any shape (meclip_embed)."""
+    dev = table.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return embed(tokens, table, scale)
     vocab, d = table.shape
-    out = torch.empty((*tokens.shape, d), dtype=table.dtype, device=table.device)
-    with _on_device(table.device):
-        _lib.check(_lib.load().meclip_embed(tokens.data_ptr(), tokens.numel(), table.data_ptr(), _DT[table.dtype], vocab, d,
-                                            max(table.stride(0), d), scale, out.data_ptr(), d, _stream(table)))
+    out = torch.empty((*tokens.shape, d), dtype=table.dtype, device=dev)
+    rc = _lib.load().meclip_embed(tokens.data_ptr(), tokens.numel(), table.data_ptr(), _DT[table.dtype], vocab, d,
+                                  max(table.stride(0), d), scale, out.data_ptr(), d, _stream(table))
+    if rc:
+        _lib.check(rc)
     return out
 
 
 def embed_grad(tokens: torch.Tensor, grad: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
     """[vocab, d] gradient of the table from contiguous int64 tokens and grad [*tokens.shape, d] (meclip_embed_grad)."""
+    dev = grad.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return embed_grad(tokens, grad, vocab, scale)
     n, d = tokens.numel(), grad.shape[-1]
     if not grad.is_contiguous() and not (grad.dim() == 2 and grad.stride(1) == 1 and grad.stride(0) >= d):
         grad = grad.contiguous()
     ldg = grad.stride(0) if grad.dim() == 2 and n > 1 else d
-    dt = torch.empty((vocab, d), dtype=grad.dtype, device=grad.device)
+    dt = torch.empty((vocab, d), dtype=grad.dtype, device=dev)
     lib = _lib.load()
-    with _on_device(grad.device):
-        ws = torch.empty(lib.meclip_embed_grad_workspace_bytes(n, vocab, d), dtype=torch.uint8, device=grad.device)
-        _lib.check(lib.meclip_embed_grad(tokens.data_ptr(), n, grad.data_ptr(), _DT[grad.dtype], vocab, d, ldg, scale,
-                                         dt.data_ptr(), d, ws.data_ptr(), ws.numel(), _stream(grad)))
+    size = lib.meclip_embed_grad_workspace_bytes(n, vocab, d)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    rc = lib.meclip_embed_grad(tokens.data_ptr(), n, grad.data_ptr(), _DT[grad.dtype], vocab, d, ldg, scale, dt.data_ptr(), d,
+                               ws.data_ptr(), size, _stream(grad))
+    if rc:
+        _lib.check(rc)
     return dt

@@ -40,7 +40,7 @@ class TokenLogProbs(NamedTuple):
 def _check_inputs(features, table, temperature):
     ops._check_matrix(features, "features")
     ops._check_matrix(table, "table")
-    assert features.device == table.device, "features and table must be on one device"
+    assert features.get_device() == table.get_device(), "features and table must be on one device"
     assert features.shape[1] == table.shape[1], \
         f"features have {features.shape[1]} columns, the table has {table.shape[1]}"
     assert not isinstance(temperature, torch.Tensor), "the temperature of a vocabulary softmax is a Python number"
@@ -49,7 +49,7 @@ def _check_inputs(features, table, temperature):
 
 def _check_tokens(tokens, features, name):
     """The tokens as contiguous int64."""
-    assert tokens.device == features.device, f"{name} must be on the features' device"
+    assert tokens.get_device() == features.get_device(), f"{name} must be on the features' device"
     assert tokens.dtype in (torch.int64, torch.int32), f"{name}: dtype {tokens.dtype} not supported (int64 or int32)"
     assert tokens.dim() in (1, 2) and tokens.shape[0] == features.shape[0], \
         f"{name} must be [{features.shape[0]}] or [{features.shape[0]}, k]"
@@ -118,9 +118,10 @@ def token_log_probs(features, table, tokens, temperature=1.0, top_k=0) -> TokenL
     if (features.requires_grad or table.requires_grad) and torch.is_grad_enabled():
         return TokenLogProbs(*_TokenLogProbsFn.apply(features, table, tokens, float(temperature), top_k))
     x, y = ops.vocab_operands(features, table)
-    out = ops.token_log_probs(x, y, tokens, float(temperature), top_k, False, ops.status_word(device))
+    lp, entropy, top_lp, top, _saved = ops.token_log_probs(x, y, tokens, float(temperature), top_k, False,
+                                                           ops.status_word(device))
     ops.post_status(device)
-    return TokenLogProbs(*out[:4])
+    return TokenLogProbs(lp, entropy, top_lp, top)
 
 
 class MemoryEfficientDistillLossFn(torch.autograd.Function):
