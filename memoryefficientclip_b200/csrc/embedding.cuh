@@ -179,18 +179,26 @@ __global__ void __launch_bounds__(EMB_SORT_THREADS) emb_scatter_kernel(const __g
     __shared__ uint32_t offs[1 << EMB_MAX_BITS];
     __shared__ uint32_t warp_sums[32];
     if ((int)blockIdx.x >= s.blocks) { emb_clear(s); return; }
-    uint32_t total = 0, before = 0;
-    if ((int)threadIdx.x < (1 << s.bits)) {
-        const uint32_t* h = s.hist + threadIdx.x;
+    // a bin's counts, one per block, are read by 1024 >> bits threads: the reads are a chain of L2 latencies otherwise
+    __shared__ uint32_t total[1 << EMB_MAX_BITS], before[1 << EMB_MAX_BITS];
+    total[threadIdx.x] = 0;
+    before[threadIdx.x] = 0;
+    __syncthreads();
+    {
+        const int bin = threadIdx.x & ((1 << s.bits) - 1), part = threadIdx.x >> s.bits, parts = EMB_SORT_THREADS >> s.bits;
+        uint32_t t = 0, u = 0;
 #pragma unroll 16
-        for (int b = 0; b < s.blocks; ++b) {
-            const uint32_t c = h[(long long)b << s.bits];
-            total += c;
-            before += b < (int)blockIdx.x ? c : 0u;
+        for (int b = part; b < s.blocks; b += parts) {
+            const uint32_t c = s.hist[((long long)b << s.bits) + bin];
+            t += c;
+            u += b < (int)blockIdx.x ? c : 0u;
         }
+        if (t != 0) atomicAdd(&total[bin], t);
+        if (u != 0) atomicAdd(&before[bin], u);
     }
-    const uint32_t start = emb_block_scan(total, warp_sums);
-    offs[threadIdx.x] = start + before;
+    __syncthreads();
+    const uint32_t start = emb_block_scan(total[threadIdx.x], warp_sums);
+    offs[threadIdx.x] = start + before[threadIdx.x];
     __syncthreads();
     const long long first = blockIdx.x * s.per_block;
     emb_scatter(s, first, min(s.n, first + s.per_block), offs, reinterpret_cast<uint16_t*>(emb_smem));
@@ -239,7 +247,7 @@ template <typename T> struct EmbRaw<T, true> {
         float v[8];
         load8(reinterpret_cast<const T*>(w), v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += v[i];
+        for (int i = 0; i < 8; i += 2) f32x2_split(add_f32x2(f32x2(acc[i], acc[i + 1]), f32x2(v[i], v[i + 1])), acc[i], acc[i + 1]);
     }
 };
 template <typename T> struct EmbRaw<T, false> {
@@ -282,39 +290,49 @@ emb_chunk_kernel(const uint32_t* __restrict__ keys, const uint32_t* __restrict__
     const uint32_t mine = lane < m ? pos[first + lane] : 0u;
     const uint32_t before = first > 0 ? keys[first - 1] : none;
     const uint32_t after = first + m < n ? keys[first + m] : none;
-    uint32_t cur = __shfl_sync(0xffffffffu, key, 0);
+    // places where another run begins, and how many places hold tokens of the table (padding sorts last)
+    const uint32_t prev = __shfl_up_sync(0xffffffffu, key, 1);
+    const uint32_t begins = __ballot_sync(0xffffffffu, lane > 0 && key != prev);
+    const int valid = __popc(__ballot_sync(0xffffffffu, (long long)key < vocab));
+    if (valid == 0) return;
+    const bool here = c < d;
     bool from_start = true;                                          // the current run began at the chunk's first place
     float acc[8] = {};
-    for (int e0 = 0; e0 < m; e0 += U) {
+    auto hand_in = [&](int e) {                                      // the run that ends before place e
+        const uint32_t cur = __shfl_sync(0xffffffffu, key, e - 1);
+        const bool goes_on = e == m && after == cur, came_in = from_start && before == cur;
+        if (goes_on || came_in) {
+            if (c < lv.dp) store8((from_start ? lv.head : lv.tail) + b * lv.dp + c, acc);
+        } else if (here) {
+            emb_finish(acc, scale, out, ldo, cur, c, d, vec_out);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+        from_start = false;
+    };
+#pragma unroll 1
+    for (int e0 = 0; e0 < valid; e0 += U) {
         EmbRaw<T, VEC> raw[U];
+        const int live = min(U, valid - e0);
 #pragma unroll
         for (int r = 0; r < U; ++r) {
             const long long row = __shfl_sync(0xffffffffu, mine, (e0 + r) & 31);
-            if (e0 + r < m && c < d) raw[r].load(g + row * ldg + c, c, d);
+            if (r < live && here) raw[r].load(g + row * ldg + c, c, d);
         }
+        const uint32_t marks = (begins >> e0) & ((1u << U) - 1u);    // the same for the whole warp
+        if (marks == 0 && live == U) {
 #pragma unroll
-        for (int r = 0; r < U; ++r) {
-            if (e0 + r >= m) break;
-            const uint32_t k = __shfl_sync(0xffffffffu, key, (e0 + r) & 31);
-            if (k != cur) {                                          // the same for the whole warp
-                if ((long long)cur < vocab) {
-                    if (from_start && before == cur) { if (c < lv.dp) store8(lv.head + b * lv.dp + c, acc); }
-                    else if (c < d) emb_finish(acc, scale, out, ldo, cur, c, d, vec_out);
-                }
+            for (int r = 0; r < U; ++r) raw[r].add(acc);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-                cur = k;
-                from_start = false;
+            for (int r = 0; r < U; ++r) {
+                if (r >= live) break;
+                if ((marks >> r) & 1u) hand_in(e0 + r);
+                raw[r].add(acc);
             }
-            if (c < d) raw[r].add(acc);
         }
-        if ((long long)cur >= vocab) return;                         // padding sorts last: nothing follows
     }
-    if (from_start ? (before == cur || after == cur) : after == cur) {
-        if (c < lv.dp) store8((from_start ? lv.head : lv.tail) + b * lv.dp + c, acc);
-    } else if (c < d) {
-        emb_finish(acc, scale, out, ldo, cur, c, d, vec_out);
-    }
+    hand_in(valid);
 }
 
 // acc += rows [a, b) of fp32 sums
@@ -365,11 +383,14 @@ emb_join_kernel(const uint32_t* __restrict__ keys, long long n, long long vocab,
     if ((long long)k >= vocab || keys[next] != k) return;
     const bool from_start = keys[first] == k;
     if (from_start && first > 0 && keys[first - 1] == k) return;     // it started earlier
-    long long lo = next, hi = n;                                     // where the run ends
+    long long lo = next, hi = n;                                     // where the run ends: 32 probes at a time
     while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        if (keys[mid] <= k) lo = mid + 1;
-        else hi = mid;
+        const long long step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const uint32_t in_run = __ballot_sync(0xffffffffu, at < hi && keys[min(at, hi - 1)] <= k);
+        if (in_run == 0) { hi = lo; break; }
+        const long long last = lo + (31 - __clz(in_run)) * step;     // the last probe inside the run
+        hi = min(hi, last + step);
+        lo = last + 1;
     }
     const long long h0 = from_start ? b : b + 1, h1 = (lo + EMB_CHUNK - 1) / EMB_CHUNK;      // heads [h0, h1)
     // whole groups of 32 full chunks: [g0, g1) lies inside the run

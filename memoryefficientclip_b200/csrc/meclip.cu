@@ -841,6 +841,10 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     if (!aligned16(a.ptr) || !aligned16(b.ptr) || (a.blocked_rows_alloc == 0 && a.ld % 8 != 0) || b.ld % 8 != 0)
         return fail(MECLIP_EINVAL, "operands must be 16-byte aligned with pitches that are multiples of 8 elements");
     const int bk = f32 ? BK / 2 : BK;         // elements per K step: 128 bytes per row either way
+    // A few rows against a vocabulary: only they are loaded, in groups of eight (the swizzle's period).  The rest of the A
+    // tile is whatever was there; it ends in accumulator rows that are never read.
+    const bool few = m < BM && (epi == EPI_STATS || epi == EPI_VCOEF);
+    const int a_rows = few ? (int)((m + 7) / 8 * 8) : BM;
     CUtensorMap ta, tb, tc;
     int rc;
     if (a.blocked_rows_alloc > 0) {
@@ -849,8 +853,9 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         else            rc = make_tmap_blocked(&ta, a.ptr, m, p.lo_chunk + (k + 63) / 64, a.blocked_rows_alloc, BM, a.ld);
         p.a_blocked = 1;
     } else if (a.mn_major) rc = make_tmap(&ta, a.ptr, m, k, a.ld, 64, BK);
-    else                   rc = make_tmap(&ta, a.ptr, k, m, a.ld, bk, BM, f32);
+    else                   rc = make_tmap(&ta, a.ptr, k, m, a.ld, bk, a_rows, f32);
     if (rc) return rc;
+    p.a_bytes = a_rows * 128;
     // CTA pairs (256 x bn tiles) whenever B is K-major; the single-CTA kernel keeps MN-major B
     const int pmode = pair_mode();
     const bool pair = !b.mn_major && bn % 64 == 0 && g_trace_buf == nullptr &&      // the in-kernel trace is a single-CTA hook
@@ -884,7 +889,9 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     // groups (a strip shares its columns).  A contraction streams its A operand (the coefficient panel) from HBM:
     // with short groups the column tiles that share panel rows run at the same time and hit L2, which is worth
     // 6 % on the isolated contraction (1086 -> 1152 TFLOP/s sustained, 0.91 -> 0.86 pJ/FLOP) and 2.5 % on the step.
-    p.group_m = epi == EPI_OUT ? 2 : 16;
+    // A vocabulary's passes keep nothing over a strip; twice as tall groups read the table half as often (coefficient pass at
+    // 4096 x 32768 x 768: 169 -> 164 us, statistics at 8192 x 49999 x 1152: 709 -> 702 us).
+    p.group_m = epi == EPI_OUT ? 2 : epi == EPI_STATS || epi == EPI_VCOEF ? 32 : 16;
     static const int env_group_m = []() { const char* v = std::getenv("MECLIP_GROUP_M"); return v ? std::atoi(v) : 0; }();
     if (env_group_m > 0 && epi == EPI_OUT) p.group_m = env_group_m;
     // strips: tile ids inside a group of 16 m-tiles share their columns; the sums pass keeps column

@@ -77,6 +77,7 @@ struct GemmParams {
     int group_m;              // rasterisation: m-tiles per group swept along n
     int num_stages;           // operand ring depth, from the shared memory left over
     int stage_bytes;          // A_STAGE_BYTES + bn * 128
+    int a_bytes;              // of them loaded for A: fewer rows than 128 when the whole problem has fewer (single-CTA kernel)
     uint32_t idesc;
     // The last column tile may be narrower (EPI_OUT only): 1152 columns = 4 tiles of 256 + one of 128, which
     // feeds the tensor cores better than six tiles of 192.  bn_last == bn when there is no such tile.
@@ -375,7 +376,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     if (warp == 0) {
         // ------------------- tile scheduler + TMA producer -------------------------
         if (lane == 0) {
-            const uint32_t stage_tx = (uint32_t)A_STAGE_BYTES + (uint32_t)p.bn * BK * 2;
+            const uint32_t stage_tx = (uint32_t)p.a_bytes + (uint32_t)p.bn * BK * 2;
             int stage = 0, slot = 0;
             uint32_t phase = 0, sphase = 0;
             // Work is handed out in strips of strip_len consecutive tile ids (same columns, next rows):

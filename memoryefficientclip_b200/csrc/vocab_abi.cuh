@@ -49,15 +49,9 @@ static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     const double bytes = (double)p.rows * (16.0 * p.slots + (p.top_k > 0 ? 8.0 * p.chunks : 0.0) +
                                            2.0 * p.d * (1 + p.k + p.top_k));
     ScopedTiming timing(s, TAG_ROW, bytes);
-    if (f16) {
-        auto kern = vocab_rows_kernel<G, __half, DISTILL, TOP>;
-        if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
-    } else {
-        auto kern = vocab_rows_kernel<G, __nv_bfloat16, DISTILL, TOP>;
-        if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
-    }
+    auto kern = f16 ? vocab_rows_kernel<G, __half, DISTILL, TOP> : vocab_rows_kernel<G, __nv_bfloat16, DISTILL, TOP>;
+    if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }

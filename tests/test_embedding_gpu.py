@@ -63,6 +63,14 @@ def test_common_tokens(n):
         _check(tokens, table, grad, 1.0)
 
 
+@pytest.mark.parametrize("n,v,d", [(5000, 1200000, 8), (3000, 1100000, 4), (70000, 1023, 260), (6000, 1024, 257)])
+def test_wide_keys_and_several_column_blocks(n, v, d):
+    """Three sorting passes, keys that fill their bits, rows of more than one warp's columns."""
+    g = torch.Generator().manual_seed(v)
+    tokens = torch.randint(-1, v, (n,), generator=g)
+    _check(tokens, torch.randn(v, d, generator=g), torch.randn(n, d, generator=g), 1.5)
+
+
 def test_shapes_layouts_and_repeats():
     from memoryefficientclip_b200 import embed_tokens
     g = torch.Generator().manual_seed(1)

@@ -354,3 +354,81 @@ def test_entry_points_stay_inside_their_outputs():
     for p, q in zip(a[:4], b[:4]):
         assert torch.equal(p, q)
     ops.check_status()
+
+
+def test_more_rows_than_a_block_of_them():
+    """Rows beyond 16384 go through the passes in blocks: scores, loss over all of them, gradients."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss, token_log_probs
+    n, v, d = 16384 + 77, 90, 24
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 3, 4.0)
+    t, logits = torch.randint(-1, v, (n, 3), generator=g), torch.randn(n, 3, generator=g)
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    got = token_log_probs(xg, yg, tokens.cuda(), top_k=2)
+    want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, 2)
+    _inside(got.log_probs, want["log_probs"][:, 0], want["err_lp"], "log_probs")
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+    loss = MemoryEfficientDistillLoss(1.0, True)(xg, yg, t.cuda(), logits.cuda())
+    kl, has, err = oracle.distill(x, table, t, logits, 1.0)
+    count = has.sum().double()
+    _inside(loss, kl.sum() / count, err.sum() / count + 2 * oracle.ULP * kl.sum() / count, "loss")
+    dx, dy = torch.autograd.grad(loss, [xg, yg])
+    wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, 1.0, torch.ones(n) / count, (torch.bfloat16,) * 2)
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("n", [40, 300, 1100])
+@pytest.mark.parametrize("k", [1, 2, 3])
+def test_few_entries_and_the_same_one_twice(n, k):
+    """One or two entries are added by the tile pass, three by the row kernel; each with repeats and padding."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    v, d = 777, 264
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, n + k)
+    t = torch.stack([tokens] * k, 1)
+    t[n // 2:, -1] = (t[n // 2:, -1] + 1) % v
+    t[::7, 0] = -1
+    t[1] = -1
+    logits = torch.randn(n, k, generator=g)
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    loss = MemoryEfficientDistillLoss(0.9, True, reduction="sum")(xg, yg, t.cuda(), logits.cuda())
+    dx, dy = torch.autograd.grad(loss, [xg, yg])
+    wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, 0.9, torch.ones(n), (torch.bfloat16,) * 2)
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+
+
+def test_two_calls_on_two_streams():
+    """Calls that overlap have workspaces of their own."""
+    from memoryefficientclip_b200 import token_log_probs
+    a = _pair(700, 3000, 256, torch.bfloat16, 41)
+    b = _pair(900, 2000, 512, torch.bfloat16, 42)
+    want = [token_log_probs(x.cuda(), t.cuda(), k.cuda(), top_k=4) for x, t, k, _ in (a, b)]
+    data = [(x.cuda(), t.cuda(), k.cuda()) for x, t, k, _ in (a, b)]
+    streams = [torch.cuda.Stream() for _ in data]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, d in zip(streams, data):
+            with torch.cuda.stream(s):
+                got.append(token_log_probs(*d, top_k=4))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        for p, q in zip(g, want[i % 2]):
+            assert torch.equal(p, q)
+
+
+def test_large_and_small_magnitudes():
+    """Features and tables far from 1: the fp16 operands of the gradient are scaled, nothing over- or underflows."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    n, v, d, k = 400, 600, 264, 4
+    for size_x, size_y, weight in ((1e5, 1e-5, 1.0), (1e-6, 1e6, 1e-6), (1e4, 1e4, 1e8)):
+        x, table, _tokens, g = _pair(n, v, d, torch.bfloat16, 51)
+        x, table = (x.float() * size_x).bfloat16(), (table.float() * size_y).bfloat16()
+        t, logits = _teacher(n, v, k, g)
+        temp = size_x * size_y
+        xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+        loss = MemoryEfficientDistillLoss(temp, True, reduction="sum")(xg, yg, t.cuda(), logits.cuda())
+        dx, dy = torch.autograd.grad(loss, [xg, yg], torch.tensor(weight).cuda())
+        wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, temp, torch.full((n,), weight), (torch.bfloat16,) * 2)
+        _inside(dx, wx, bx, "dx")
+        _inside(dy, wy, by, "dtable")
