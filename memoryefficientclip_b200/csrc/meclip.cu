@@ -803,6 +803,10 @@ static int launch_pair_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
 // 8.94.  Auto: the contractions (K = panel width, thousands) always run as pairs; the sums and coefficient
 // passes (K = D) do from PAIR_MIN_K on.
 static constexpr long long PAIR_MIN_K = 800;
+// The vocabulary's passes have heavier epilogues, which two CTAs with a tile each hide better, up to a longer K (4096 x
+// 32768, under the power cap, statistics and selection: K = 1024 single 307 us, pairs 317; 8192 x 49999 x 1152, a step
+// with its gradients: single 3560 us, pairs 3540).
+static constexpr long long VOCAB_PAIR_MIN_K = 1100;
 static int pair_mode() {
     static const int mode = []() {
         const char* v = std::getenv("MECLIP_PAIR");
@@ -860,7 +864,8 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     const int pmode = pair_mode();
     const bool pair = !b.mn_major && bn % 64 == 0 && g_trace_buf == nullptr &&      // the in-kernel trace is a single-CTA hook
                       (f32 || wide || pmode == 1 || ((pmode == 2 || pmode < 0) && epi == EPI_OUT && bn == 256) ||
-                       (pmode < 0 && epi != EPI_OUT && bn == 256 && k >= PAIR_MIN_K)) &&
+                       (pmode < 0 && epi != EPI_OUT && bn == 256 &&
+                        k >= (epi == EPI_STATS || epi == EPI_VCOEF ? VOCAB_PAIR_MIN_K : PAIR_MIN_K))) &&
                       !(m <= BM && (epi == EPI_STATS || epi == EPI_VCOEF));     // half of every pair would have no rows
     if (b.mn_major) rc = make_tmap(&tb, b.ptr, n, k, b.ld, 64, BK);
     else            rc = make_tmap(&tb, b.ptr, k, n, b.ld, bk, pair ? bn / 2 : bn, f32);

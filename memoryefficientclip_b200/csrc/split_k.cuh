@@ -1,8 +1,11 @@
 // Contractions with few output tiles and a long K, cut into parts of K (GemmParams::splits): rules and the sum of the parts.
 //
 // A gradient of `rows` features against a vocabulary has rows / 256 x d / 256 tiles of K = vocab for dX: 16 tiles of 500
-// K steps at 2047 x 32001 x 512 on 74 CTA pairs.  Cut so that no tile is longer than half of what a pair has to do in
-// all, the launch ends when the work does.  The parts are fp32, written once and read once, and added in order.
+// K steps at 2047 x 32001 x 512 on 74 CTA pairs.  Cut so that no tile is longer than a quarter of what a pair has to do in
+// all, the launch ends when the work does.  The parts are fp32, written once and read once, and added in order.  Both
+// contractions in one launch, whole tiles or parts of at most a half, of a quarter of a pair's share (their sum, 10 to
+// 19 us, included where there are parts): 2047 x 32001 x 512 - / 149 / 139 us, 4096 x 32768 x 768 - / 384 / 340,
+// x 1152 630 / 630 / 566 (half leaves them whole), x 1536 716 / 716 / 655, 4736 x 32768 x 1024 632 / 632 / 561.
 #pragma once
 
 namespace meclip {
@@ -72,7 +75,7 @@ static SplitK split_into(GemmParams& p, long long m, long long n, long long k_st
 }
 
 // Tile width of a contraction that may be cut: 256 columns where K is long, since parts fill the SMs then and every column
-// tile reads the panel again (64 x 32768 x 1152: 18 tiles of 64 columns 49 us, 5 of 256 25 us); else as for others.
+// tile reads the panel again (dX of 64 x 50000 x 1152: 18 tiles of 64 columns 78 us, 5 of 256 42 us); else as for others.
 static int split_tile_width(long long m, long long n, long long k, bool shares_gpu, bool b_k_major) {
     return n >= 256 && k >= 64 * BK ? 256 : pick_contraction_bn(m, n, shares_gpu, b_k_major);
 }
@@ -89,11 +92,11 @@ static SplitK split_alone(GemmParams& p, long long m, long long n, long long k, 
     return split_into(p, m, n, k_steps, split_parts_alone(m, n, k_steps, bn), buf, bytes);
 }
 
-// Both contractions of a block in one launch: parts for tiles that are longer than half of a pair's share of all steps.
+// Both contractions of a block in one launch: parts for tiles that are longer than a quarter of a pair's share of all steps.
 static void split_parts_dual(long long rows, long long cols, long long d, long long& parts_y, long long& parts_x) {
     const long long nt = (d + 255) / 256, my = (cols + PAIR_BM - 1) / PAIR_BM, mx = (rows + PAIR_BM - 1) / PAIR_BM;
     const long long ky = (rows + BK - 1) / BK, kx = (cols + BK - 1) / BK, pairs = sm_count() / 2;
-    long long limit = (nt * (my * ky + mx * kx) + 2 * pairs - 1) / (2 * pairs);
+    long long limit = (nt * (my * ky + mx * kx) + 4 * pairs - 1) / (4 * pairs);
     if (limit < 2 * SPLIT_MIN_STEPS) limit = 2 * SPLIT_MIN_STEPS;
     parts_y = (ky + limit - 1) / limit;
     parts_x = (kx + limit - 1) / limit;
