@@ -1634,7 +1634,8 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     // and the 256-column CTA-pair tiles
     const bool use_dual = want_dx && want_dy && transposed_copies && dual_allowed() && pair_mode() != 0 && !wide_allowed() &&
                           dn == d && d >= 256 && g_trace_buf == nullptr;
-    if (use_dual) sy = sx;      // one side stream carries the transposes and the contractions
+    // one side stream carries the transposes and the contractions, also where there is one buffer for the parts of both
+    if (use_dual || (vg != nullptr && vg->split_buf2 == vg->split_buf)) sy = sx;
     // the tile counters are the only part of the workspace that has to start at zero; a vocabulary's gradient on one stream
     // deals its tiles in turn instead (nothing shares the GPU with it, and a launch less is a few microseconds)
     const bool use_counters = vg == nullptr || overlap;

@@ -158,7 +158,7 @@ static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab,
     g.grad_bytes = plan.total();
     const bool dual = g.transposed && d >= 256 && dual_allowed() && pair_mode() != 0 && !wide_allowed();
     g.split_bytes = split_bytes(plan.row_block, plan.panel_w, d, dual, g.two_panels);
-    g.split_bufs = g.overlap && g.transposed && !dual ? 2 : 1;          // the two contractions on two streams
+    g.split_bufs = g.overlap && !dual ? 2 : 1;          // the two contractions on two streams
     return g;
 }
 

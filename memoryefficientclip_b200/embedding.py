@@ -9,6 +9,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -21,6 +22,7 @@ class _EmbedFn(torch.autograd.Function):
         return ops.embed(tokens, table, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         (tokens,) = ctx.saved_tensors
         shape, scale = ctx.embed
@@ -39,7 +41,7 @@ def embed_tokens(tokens, table, scale=1.0):
     assert not isinstance(scale, torch.Tensor) and math.isfinite(scale), "scale must be a finite Python number"
     tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    table = table if table.stride(1) == 1 else table.contiguous()
+    table = ops.row_major(table)
     if table.requires_grad and torch.is_grad_enabled():
         return _EmbedFn.apply(tokens, table, float(scale))
     return ops.embed(tokens, table, float(scale))

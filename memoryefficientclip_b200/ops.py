@@ -54,6 +54,12 @@ def _check_matrix(t: torch.Tensor, name: str):
     assert t.shape[0] >= 1 and t.shape[1] >= 1, f"{name}: empty input"
 
 
+def row_major(t: torch.Tensor) -> torch.Tensor:
+    """t itself if its rows are runs of adjacent elements that do not overlap (what the kernels address by a pitch), else
+    a contiguous copy: of a transposed matrix, or of one row expanded to many."""
+    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1) else t.contiguous()
+
+
 def padded(d: int) -> int:
     """Columns of a bf16 operand: the tile loads need 16-byte rows."""
     return (d + 7) // 8 * 8
@@ -193,9 +199,9 @@ def normalize_fwd(x: torch.Tensor, normalize: bool = True, extra_cols: int = 0):
     zero up to padded(d); extra_cols (a multiple of 8) are left for the caller to fill.
 
     Any feature count, row pitch and alignment is taken as it is (the kernel reads element-wise when
-    16-byte loads are not possible); only a non-unit column stride costs a copy."""
+    16-byte loads are not possible); only a non-unit column stride or overlapping rows cost a copy."""
     _check_matrix(x, "x")
-    x = x if x.stride(1) == 1 else x.contiguous()
+    x = row_major(x)
     rows, d = x.shape
     dp = padded(d)
     out = torch.empty(rows, dp + extra_cols, dtype=torch.bfloat16, device=x.device)
@@ -721,7 +727,8 @@ def ring_grad(call: RingCall, kind, temperature, row_sum, col_sum_all, grad_out,
 # ---- softmax over a vocabulary ------------------------------------------------------------------------------
 def _is_operand(x: torch.Tensor) -> bool:
     """Whether the tile kernels can read a 16-bit matrix as it is: 16-byte aligned rows of a multiple of 8 columns."""
-    return x.shape[1] % 8 == 0 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0
+    return (x.shape[1] % 8 == 0 and x.stride(1) == 1 and x.stride(0) % 8 == 0 and x.stride(0) >= x.shape[1] and
+            x.data_ptr() % 16 == 0)
 
 
 def vocab_operands(x: torch.Tensor, table: torch.Tensor):

@@ -22,6 +22,7 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -84,6 +85,7 @@ class _TokenLogProbsFn(torch.autograd.Function):
         return lp, entropy, top_lp, top
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_log_probs, grad_entropy, _top_lp, _top):
         x, y, tokens, entropy, saved = ctx.saved_tensors
         temperature, x_dtype, y_dtype, d = ctx.vocab
@@ -155,6 +157,7 @@ class MemoryEfficientDistillLossFn(torch.autograd.Function):
         return result
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_output):
         x, y, tokens, saved, inv_x, inv_y = ctx.saved_tensors
         temperature, x_dtype, y_dtype, d = ctx.vocab

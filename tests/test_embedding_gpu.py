@@ -151,3 +151,26 @@ def test_a_tied_table_as_it_is_used():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], loss) and torch.equal(out[1], dt)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_broadcast_and_overlapping_tables(dtype):
+    """One row expanded to many, rows that overlap, and a single row of whatever pitch."""
+    from memoryefficientclip_b200 import embed_tokens
+    table = torch.randn(300, 64, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    tokens = (torch.arange(90) * 7 % 300).cuda()
+    for t, at in ((table[:1].expand(300, 64), tokens), (table.reshape(-1).as_strided((300, 64), (8, 1)), tokens),
+                  (table[:1].as_strided((1, 64), (0, 1)), tokens.clamp(max=0))):
+        assert torch.equal(embed_tokens(at, t, 0.5), (t.float()[at] * 0.5).to(dtype))
+    one = table[:1].clone().requires_grad_(True)
+    embed_tokens(tokens, one.expand(300, 64)).float().sum().backward()
+    assert torch.equal(one.grad.float(), torch.full((1, 64), 90.0, device="cuda"))
+
+
+def test_second_derivatives_are_refused():
+    from memoryefficientclip_b200 import embed_tokens
+    table = torch.randn(30, 8, device="cuda", requires_grad=True)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    (dt,) = torch.autograd.grad(embed_tokens(torch.arange(9, device="cuda"), table).sum() * w, table, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dt.sum().backward()

@@ -71,3 +71,13 @@ def test_module_defaults_follow_the_package():
     mod = m.MemoryEfficientDistillLoss()
     assert (mod.temperature, mod.normalized_inputs, mod.teacher_temperature, mod.reduction) == (0.07, False, 1.0, "mean")
     assert not list(mod.parameters())
+
+
+def test_rows_that_the_kernels_can_address():
+    """Broadcast and overlapping rows are copied, whatever else stays as it is."""
+    from memoryefficientclip_b200 import ops
+    m = torch.zeros(40, 64, dtype=torch.bfloat16)
+    for view, plain in ((m, True), (m[::2], True), (m[:, :32], True), (m[:1].expand(40, 64), False), (m.T, False),
+                        (m.reshape(-1).as_strided((30, 64), (8, 1)), False), (m[:1].as_strided((1, 64), (0, 1)), True)):
+        assert (ops.row_major(view) is view) == plain
+        assert view.shape[0] == 1 or ops._is_operand(view) == plain

@@ -1,6 +1,9 @@
 """Token log probabilities and distillation over a vocabulary against the 64-bit oracle (oracle/vocabulary.py, which
 derives the bounds from the roundings of the computation)."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -432,3 +435,50 @@ def test_large_and_small_magnitudes():
         wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, temp, torch.full((n,), weight), (torch.bfloat16,) * 2)
         _inside(dx, wx, bx, "dx")
         _inside(dy, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("switch", ["MECLIP_NO_TRANSPOSE=1", "MECLIP_DUAL=0", "MECLIP_PAIR=0", "MECLIP_SERIAL=1"])
+def test_gradients_under_every_switch(switch):
+    """The library's switches are read once per process: the gradient tests again, in a child."""
+    name, value = switch.split("=")
+    out = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", __file__,
+                          "-k", "test_score_gradients or test_distillation_of_two_towers"],
+                         env=dict(os.environ, **{name: value}), capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0, out.stdout[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_broadcast_and_overlapping_rows(dtype):
+    """One row expanded to many, rows that overlap, and a single row of whatever pitch, against contiguous copies."""
+    from memoryefficientclip_b200 import token_log_probs, MemoryEfficientDistillLoss
+    n, v, d = 70, 333, 64
+    x, table, tokens, g = _pair(n, v, d, dtype, 8)
+    x, table, tokens = x.cuda(), table.cuda(), tokens.cuda()
+    flat = table.reshape(-1)
+    cases = [(x[:1].expand(n, d), table, tokens), (x, table[:1].expand(v, d), tokens),
+             (x, flat.as_strided((v, d), (8, 1)), tokens), (x[:1].as_strided((1, d), (0, 1)), table, tokens[:1]),
+             (x, table[:1].as_strided((1, d), (8, 1)), tokens.clamp(max=0))]
+    for a, b, t in cases:
+        for got, want in zip(token_log_probs(a, b, t, top_k=1), token_log_probs(a.contiguous().clone(), b.contiguous().clone(), t, top_k=1)):
+            assert torch.equal(got, want)
+        logits = torch.zeros(t.shape[0], 1, device="cuda")
+        for normalized in (True, False):
+            loss = MemoryEfficientDistillLoss(1.0, normalized)
+            assert torch.equal(loss(a, b, t[:, None], logits), loss(a.contiguous().clone(), b.contiguous().clone(), t[:, None], logits))
+    one = x[:1].clone().requires_grad_(True)            # the gradient of a broadcast input is the sum over its copies
+    token_log_probs(one.expand(n, d), table, tokens).log_probs.sum().backward()
+    many = x[:1].expand(n, d).clone().requires_grad_(True)
+    token_log_probs(many, table, tokens).log_probs.sum().backward()
+    assert torch.equal(one.grad, many.grad.sum(0, keepdim=True))
+
+
+def test_second_derivatives_are_refused():
+    from memoryefficientclip_b200 import token_log_probs, MemoryEfficientDistillLoss
+    x, table, tokens, _g = _pair(20, 50, 64, torch.float32, 8)
+    x, table, tokens = x.cuda().requires_grad_(True), table.cuda(), tokens.cuda()
+    w = torch.ones((), device="cuda", requires_grad=True)
+    for out in (token_log_probs(x, table, tokens).log_probs.sum() * w,
+                MemoryEfficientDistillLoss(1.0)(x, table, tokens[:, None], torch.zeros(20, 1, device="cuda")) * w):
+        (dx,) = torch.autograd.grad(out, x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            dx.sum().backward()
