@@ -482,3 +482,52 @@ def test_second_derivatives_are_refused():
         (dx,) = torch.autograd.grad(out, x, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             dx.sum().backward()
+
+
+@pytest.mark.parametrize("n", [3, 260])
+def test_offsets_past_32_bits(n):
+    """A table of 2^31 elements and more than 2^32 bytes.  All rows but a few are zero, so that the oracle needs only
+    those: V - R scores of exactly 0."""
+    from memoryefficientclip_b200 import embed_tokens, token_log_probs
+    v, d, r = 2_100_000, 1024, 400
+    g = torch.Generator().manual_seed(n)
+    where = torch.cat([torch.tensor([0, v - 1, v - 2, 2 ** 31 // d, 2 ** 31 // d - 1]), torch.randint(0, v, (r,), generator=g)]).unique()
+    rows = (torch.randn(len(where), d, generator=g) / math.sqrt(d)).bfloat16()
+    pick = torch.randint(0, len(where), (n,), generator=g)
+    pick[0] = len(where) - 1
+    x = (2.0 * torch.randn(n, d, generator=g) + 20.0 * rows.float()[pick]).bfloat16()
+    table = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    table[where.cuda()] = rows.cuda()
+    table.requires_grad_(True)
+    xg, tokens = x.cuda().requires_grad_(True), where[pick].cuda()
+    got = token_log_probs(xg, table, tokens, top_k=1)
+    z, err = oracle.scores(x, rows, 1.0)
+    zeros = float(v - len(where))
+    lse = torch.logsumexp(torch.cat([z, torch.full((n, 1), math.log(zeros))], 1), 1)
+    lp = z.gather(1, pick[:, None])[:, 0] - lse
+    _inside(got.log_probs, lp, 2 * err, "log_probs")
+    assert torch.equal(got.top_tokens[:, 0].cpu(), where[z.argmax(1)])
+    dx, dt = torch.autograd.grad(got.log_probs.sum(), [xg, table])
+    p = (z - lse[:, None]).exp()
+    one = torch.zeros_like(p).scatter_(1, pick[:, None], 1.0)
+    wx, wy, bx, by = oracle._gradients(x, rows, 1.0, -p, one, p, (torch.bfloat16,) * 2, 0.0)
+    # the zero rows' part of dX is zero; the panel's scaled fp16 form cuts coefficients below 2^-24 of the largest bound
+    cut = 2.0 ** -24 * 2.0
+    _inside(dx, wx, bx + cut * rows.double().abs().sum(0), "dx")
+    _inside(dt[where.cuda()], wy, by + cut * x.double().abs().sum(0), "dtable")
+    others = torch.randint(0, v, (2000,), generator=g)
+    others = others[~torch.isin(others, where)]
+    w0 = -(torch.exp(-lse)[:, None] * x.double()).sum(0)
+    b0 = (torch.exp(-lse)[:, None] * (2.0 ** -8 + 2 * err[:, None] + 16 * oracle.ULP) * x.double().abs()).sum(0)
+    b0 = b0 + 2.0 ** -8 * (w0.abs() + b0) + cut * x.double().abs().sum(0)
+    worst = ((dt[others.cuda()].double().cpu() - w0).abs() / b0).max().item()
+    assert worst <= 1.0, worst
+    del dx, dt
+    out = embed_tokens(tokens, table, 2.0)
+    assert torch.equal(out.detach().float().cpu(), 2.0 * rows.float()[pick])
+    go = torch.randn(n, d, generator=g).bfloat16()
+    (dt,) = torch.autograd.grad(out, table, go.cuda())
+    want = torch.zeros(len(where), d, dtype=torch.float64).index_add_(0, pick, 2.0 * go.double())
+    size = torch.zeros(len(where), d, dtype=torch.float64).index_add_(0, pick, 2.0 * go.double().abs())
+    assert ((dt[where.cuda()].double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + (n + 2) * 2.0 ** -23 * size).all()
+    assert dt[others.cuda()].abs().max().item() == 0 and int(torch.count_nonzero(dt.abs().amax(1))) == len(pick.unique())
