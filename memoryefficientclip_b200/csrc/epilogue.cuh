@@ -159,9 +159,10 @@ __device__ __forceinline__ void stats_chunk(const uint32_t (&v)[32], float fmul,
 
 // Joins {maximum m2, sum less one r2, moment t2} to {m, r, t}: the sums are rescaled to the larger maximum and the exponents
 // inside the moment shift with it.  An empty side has a finite m of -1e30, r = -1 and t = 0, so no infinities meet.
-__device__ __forceinline__ void stats_join(float& m, float& r, float& t, float m2, float r2, float t2) {
+// `unit`: what the maxima are in, where they are not in base-2 units themselves.
+__device__ __forceinline__ void stats_join(float& m, float& r, float& t, float m2, float r2, float t2, float unit = 1.f) {
     const float mn = fmaxf(m, m2);
-    const float a = m - mn, b = m2 - mn;
+    const float a = (m - mn) * unit, b = (m2 - mn) * unit;
     const float fa = ex2_approx(a), fb = ex2_approx(b);
     const float l = 1.f + r, l2 = 1.f + r2;
     t = fa * fmaf(a, l, t) + fb * fmaf(b, l2, t2);

@@ -24,7 +24,7 @@ static int pick_stats_bn(long long rows, long long vocab) {
 }
 
 struct VocabPlan {
-    long long row_block, slots, chunks, chunk_ld;
+    long long row_block, slots, chunks, chunk_ld, few_blocks;
     int bn;
     size_t stats_bytes, chunk_bytes, total;
 };
@@ -34,6 +34,8 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
     v.bn = pick_stats_bn(v.row_block, vocab);
     v.slots = 2 * ((vocab + v.bn - 1) / v.bn);
     v.chunks = (vocab + 31) / 32;
+    v.few_blocks = v.chunks < VOCAB_FEW_BLOCKS * sm_count() ? v.chunks : VOCAB_FEW_BLOCKS * sm_count();
+    if (rows <= VOCAB_FEW_ROWS && v.slots < v.few_blocks) v.slots = v.few_blocks;
     v.chunk_ld = (long long)round_up((size_t)v.chunks, 4);
     v.stats_bytes = round_up((size_t)v.row_block * v.slots * 16, 256);
     v.chunk_bytes = top_k > 0 ? round_up((size_t)v.row_block * v.chunk_ld * 4, 256) : 0;
@@ -54,6 +56,20 @@ static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
+}
+
+template <typename T, int R>
+static int launch_vocab_few_r(const VocabFew& p, unsigned blocks, cudaStream_t s) {
+    const int smem = VOCAB_FEW_RING + R * p.d_smem * 2;
+    MECLIP_CUDA(cudaFuncSetAttribute(vocab_few_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    vocab_few_kernel<T, R><<<blocks, VOCAB_FEW_THREADS, smem, s>>>(p);
+    MECLIP_CUDA(cudaGetLastError());
+    return MECLIP_OK;
+}
+template <typename T>
+static int launch_vocab_few(const VocabFew& p, unsigned blocks, cudaStream_t s) {
+    ScopedTiming timing(s, TAG_SUMS, 2.0 * (double)p.rows * (double)p.vocab * (double)p.d);
+    return p.rows == 1 ? launch_vocab_few_r<T, 1>(p, blocks, s) : launch_vocab_few_r<T, 2>(p, blocks, s);
 }
 
 // What both forwards ask of their operands.
@@ -83,6 +99,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     r.stats = reinterpret_cast<const float4*>(ws);
     r.slots = (int)plan.slots;
     r.stats_ld = plan.slots;
+    r.unit = 1.f;
     r.chunk_max = r.top_k > 0 ? reinterpret_cast<const float*>(ws + plan.stats_bytes) : nullptr;
     r.chunk_second = r.top_k > 0 ? reinterpret_cast<const uint32_t*>(ws + plan.stats_bytes + plan.chunk_bytes) : nullptr;
     r.chunks = (int)plan.chunks;
@@ -118,9 +135,23 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
             if (r0 + plan.row_block < rows) b.loss = nullptr;      // only behind the last block of rows
         }
         const bool f16 = dtype == MECLIP_F16;
+        const long long d_smem = (r.d + 255LL) / 256 * 256;
+        // (an empty partial sum's -1e30 has to stay finite in base 2)
+        const bool by_lines = rows <= VOCAB_FEW_ROWS && d_smem * 2 * VOCAB_FEW_ROWS <= VOCAB_FEW_X && r.fmul < 1e8f;
+        if (by_lines) {
+            b.slots = (int)plan.few_blocks;
+            b.unit = r.fmul;
+            VocabFew f{};
+            f.x = b.x; f.y = r.y; f.ldx = r.ldx; f.ldy = r.ldy; f.d = r.d; f.d_smem = (int)d_smem; f.rows = (int)rows;
+            f.vocab = r.vocab; f.chunks = plan.chunks; f.fmul = r.fmul;
+            f.stats = p.stats; f.stats_ld = p.stats_ld;
+            f.chunk_max = p.chunk_max; f.chunk_second = p.chunk_second; f.chunk_ld = p.chunk_ld;
+            rc = f16 ? launch_vocab_few<__half>(f, (unsigned)plan.few_blocks, s) : launch_vocab_few<__nv_bfloat16>(f, (unsigned)plan.few_blocks, s);
+            if (rc) return rc;
+        }
         Operand a{b.x, r.ldx, false, 0, false, f16}, t{r.y, r.ldy, false, 0, false, f16};
         t_tag = TAG_SUMS;
-        rc = launch_gemm(EPI_STATS, a, t, b.rows, r.vocab, r.d, plan.bn, p, s);
+        if (!by_lines) rc = launch_gemm(EPI_STATS, a, t, b.rows, r.vocab, r.d, plan.bn, p, s);
         if (rc) return rc;
         // a few rows: a block each; many: a warp each
         const bool few = b.rows <= 2 * sm_count();

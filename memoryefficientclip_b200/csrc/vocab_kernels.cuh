@@ -75,6 +75,7 @@ static float vocab_tile_fmul(float temperature, long long d) {
 
 struct VocabRows {
     const float4* stats; int slots; long long stats_ld;
+    float unit;                       // of the maxima in stats: fmul for plain scores, 1 for base 2
     const float* chunk_max; const uint32_t* chunk_second; int chunks; long long chunk_ld;
     const void* x; const void* y; long long ldx, ldy; int d;
     long long rows, vocab;
@@ -98,14 +99,15 @@ struct VocabRows {
     float *loss, *inv_count;
 };
 
-// log2 p of a score s2 that was formed from the operands, in a row with maximum m and sum 1 + r of the tile pass.  The
-// maximum itself takes the tile pass's score: its log probability is then -log2(1 + r), exact however small r is, and what
-// the tile pass is off by cancels.  Another column can be mistaken for the maximum only where the tile pass cannot tell
-// them apart (an ulp for every 64 columns of d).
-__device__ __forceinline__ double vocab_lp2(const VocabRows& p, double s2, float m, float r, float log2l) {
-    const float off = fabsf((float)(s2 - (double)m));
-    const bool is_max = off <= 1.2e-7f * ((float)p.d * 0.015625f + 1.f) * (fabsf(m) + 8.f) || (r < 0.25f && off < 0.5f);
-    return (is_max ? 0.0 : s2 - (double)m) - (double)log2l;
+// log2 p of a score z that was formed from the operands, in a row with maximum m (in p.unit) and sum 1 + r of the tile pass.
+// The maximum itself takes the pass's score: its log probability is then -log2(1 + r), exact however small r is, and what
+// the pass is off by cancels.  Another column can be mistaken for the maximum only where the pass cannot tell them apart (an
+// ulp for every 64 columns of d).
+__device__ __forceinline__ double vocab_lp2(const VocabRows& p, double z, float m, float r, float log2l) {
+    const double below = p.unit == 1.f ? z * (double)p.fmul - (double)m : (z - (double)m) * (double)p.unit;
+    const float off = fabsf((float)below);
+    const bool is_max = off <= 1.2e-7f * ((float)p.d * 0.015625f + 1.f) * (fabsf(m * p.unit) + 8.f) || (r < 0.25f && off < 0.5f);
+    return (is_max ? 0.0 : below) - (double)log2l;
 }
 
 __device__ __forceinline__ void half8(const __nv_bfloat16* p, float (&v)[8]) { load8(p, v); }
@@ -152,6 +154,161 @@ __device__ __forceinline__ void warp_dot4(const T* __restrict__ x, const T* cons
         for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         out[r] = v;
     }
+}
+
+// The statistics of a few rows (a token at a time is answered like that) without the tensor cores, whose tile would be empty
+// but for these rows: a pass over the table at the memory's rate, with fp32 multiplications and additions that round instead
+// of cutting.  A block takes chunks of 32 columns, a warp eight of them, 256 elements of each at a time.  A lane copies what
+// it will read itself into a ring in shared memory, so nothing but its own copies has to be waited for, and the ring runs on
+// into the next chunk.  Then a warp looks at the chunk for a row: a lane per column.  Leaves what EPI_STATS leaves, with one
+// partial sum per block and its maximum as a plain score, whose difference to another is exact where the difference of
+// scaled ones carries the rounding of both.
+// 1 x 250000 x 1152: 91 us, 6.3 TB/s (the tile pass 93.5, loads through registers instead of the ring 118); 1 x 32768 x 1024
+// 15 us (18), 1 x 4099 x 512 9 us (14), events included.  Two rows take as long as the tile pass takes from large tables, four
+// 10 % longer and eight twice as long: the arithmetic shows then.
+static constexpr int VOCAB_FEW_THREADS = 128;
+static constexpr int VOCAB_FEW_BLOCKS = 3;         // per SM
+static constexpr int VOCAB_FEW_ROWS = 2;
+static constexpr int VOCAB_FEW_STAGES = 4;
+static constexpr int VOCAB_FEW_RING = VOCAB_FEW_STAGES * VOCAB_FEW_THREADS * 8 * 16;      // bytes
+static constexpr int VOCAB_FEW_X = 64 * 1024;      // bytes of features at most
+
+struct VocabFew {
+    const void *x, *y; long long ldx, ldy; int d, d_smem, rows;      // d_smem: d rounded up to 256
+    long long vocab, chunks;
+    float fmul;
+    float4* stats; long long stats_ld;
+    float* chunk_max; uint32_t* chunk_second; long long chunk_ld;
+};
+
+__device__ __forceinline__ void wide8(const __nv_bfloat16*, const uint4& w, uint64_t (&v)[4]) {
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f32x2(__uint_as_float(a[i] << 16), __uint_as_float(a[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void wide8(const __half*, const uint4& w, uint64_t (&v)[4]) {
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+        v[i] = f32x2(f.x, f.y);
+    }
+}
+
+template <typename T, int R>
+__global__ void __launch_bounds__(VOCAB_FEW_THREADS, VOCAB_FEW_BLOCKS)
+vocab_few_kernel(const __grid_constant__ VocabFew p) {
+    constexpr int S = VOCAB_FEW_STAGES;
+    static_assert(R <= VOCAB_FEW_THREADS / 32, "a warp per row");
+    extern __shared__ __align__(16) uint8_t few_smem[];
+    __shared__ float scores[2][R][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint4* ring = reinterpret_cast<uint4*>(few_smem) + threadIdx.x;       // [S][8] of the lane's own, VOCAB_FEW_THREADS apart
+    T* xs = reinterpret_cast<T*>(few_smem + VOCAB_FEW_RING);
+    // what is copied next: 256 elements of eight columns
+    long long next_ch = blockIdx.x;
+    int next_c = lane * 8, next_slot = 0;
+    auto copy = [&]() {
+        if (next_ch < p.chunks) {
+            long long col = min(next_ch * 32 + w * 8, p.vocab - 1);
+            const T* src = reinterpret_cast<const T*>(p.y) + col * p.ldy;
+            const bool in = next_c < p.d;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + (next_slot * 8 + j) * VOCAB_FEW_THREADS);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src + (in ? next_c : 0)), "r"(in ? 16 : 0) : "memory");
+                if (++col < p.vocab) src += p.ldy;                        // columns behind the last repeat it
+            }
+            next_c += 256;
+            if (next_c >= p.d_smem) { next_c = lane * 8; next_ch += gridDim.x; }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        next_slot = next_slot + 1 == S ? 0 : next_slot + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy();
+    for (int i = threadIdx.x * 8; i < R * p.d_smem; i += VOCAB_FEW_THREADS * 8) {
+        const int r = i / p.d_smem, c = i % p.d_smem;
+        *reinterpret_cast<uint4*>(xs + i) = r < p.rows && c < p.d
+            ? *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.x) + r * p.ldx + c) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    float m = STATS_EMPTY, l = -1.f, t = 0.f;          // of the lane's columns in the warp's row: maximum, sum less one, moment
+    int buf = 0, slot = 0;
+    for (long long ch = blockIdx.x; ch < p.chunks; ch += gridDim.x, buf ^= 1) {
+        uint64_t acc[8][R] = {};
+#pragma unroll 1
+        for (int c = lane * 8; c < p.d_smem; c += 256) {
+            asm volatile("cp.async.wait_group %0;" :: "n"(S - 2) : "memory");
+            copy();                    // into the slot that the step before this one has read
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                uint64_t yv[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) wide8(xs, ring[(slot * 8 + h + j) * VOCAB_FEW_THREADS], yv[j]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    uint64_t xv[4];
+                    wide8(xs, *reinterpret_cast<const uint4*>(xs + r * p.d_smem + c), xv);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[h + j][r] = fma_f32x2(xv[i], yv[j][i], acc[h + j][r]);
+                }
+            }
+            slot = slot + 1 == S ? 0 : slot + 1;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            // eight sums over 32 lanes: halves change hands until a lane holds one column, then the rest is added up
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float a, b;
+                f32x2_split(acc[j][r], a, b);
+                v[j] = a + b;
+            }
+#pragma unroll
+            for (int h = 4; h >= 1; h >>= 1)
+#pragma unroll
+                for (int j = 0; j < h; ++j) {
+                    const bool up = (lane & h) != 0;
+                    const float keep = up ? v[j + h] : v[j], give = up ? v[j] : v[j + h];
+                    v[j] = keep + __shfl_xor_sync(0xffffffffu, give, h);
+                }
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], 8);
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], 16);
+            if (lane < 8) scores[buf][r][w * 8 + lane] = v[0];
+        }
+        __syncthreads();               // the other buffer is written next, this one again only behind the next barrier
+        if (w < p.rows) {
+            const float score = scores[buf][w < R ? w : 0][lane];
+            const bool in = ch * 32 + lane < p.vocab;
+            // one column: sum less one is 0 (NaN for a score that is not a number, which the maximum would hide)
+            if (in) stats_join(m, l, t, score, score - score, 0.f, p.fmul);
+            if (p.chunk_max != nullptr) {          // see stats_chunk
+                float cm = in ? score * p.fmul : -INFINITY;
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, o));
+                const uint32_t key = in ? (__float_as_uint(fmaf(score, p.fmul, -cm)) & 0x7fffffe0u) | (uint32_t)lane : 0x7fffffffu;
+                const uint32_t n1 = __reduce_min_sync(0xffffffffu, key);
+                const uint32_t n2 = __reduce_min_sync(0xffffffffu, key == n1 ? 0x7fffffffu : key);
+                if (lane == 0) {
+                    p.chunk_max[w * p.chunk_ld + ch] = cm;
+                    p.chunk_second[w * p.chunk_ld + ch] = (n2 & ~31u) | (n1 & 31u);
+                }
+            }
+        }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (w >= p.rows) return;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o),
+                    t2 = __shfl_xor_sync(0xffffffffu, t, o);
+        stats_join(m, l, t, m2, l2, t2, p.fmul);
+    }
+    if (lane == 0) p.stats[w * p.stats_ld + blockIdx.x] = make_float4(m, l, t, 0.f);
 }
 
 // (value, index) order of alternatives: larger value first, then the lower index.
@@ -280,7 +437,7 @@ __device__ __forceinline__ float warp_sort_desc(float v, int lane) {
 
 __device__ __forceinline__ void row_top_write(const VocabRows& p, long long row, int at, double z, long long j, float m, float r, float log2l) {
     p.top_tokens[row * p.top_k + at] = j;
-    p.top_log_probs[row * p.top_k + at] = (float)(vocab_lp2(p, z * (double)p.fmul, m, r, log2l) * 0.6931471805599453);
+    p.top_log_probs[row * p.top_k + at] = (float)(vocab_lp2(p, z, m, r, log2l) * 0.6931471805599453);
 }
 
 // (a) to (c): leaves the columns in sh.list, their number in sh.count[1] (0 after a crowd, which is finished here) and
@@ -544,7 +701,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     if (!TOP && !DISTILL && !active) return;      // (a block of G = 256 has one row, warps of G = 32 do not meet)
     uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap);
     float* red = reinterpret_cast<float*>(smem);
-    float* s2 = reinterpret_cast<float*>(smem + 64 * 8);
+    float* z_of = reinterpret_cast<float*>(smem + 64 * 8);
     uint8_t* top_smem = smem + 64 * 8 + (p.k * 4 + 15) / 16 * 16;
 
     // (1) the row's statistics
@@ -553,24 +710,24 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
         const float4* st = p.stats + row * p.stats_ld;
         for (int i = gt; i < p.slots; i += G) {
             const float4 v = st[i];
-            stats_join(m, r, t, v.x, v.y, v.z);
+            stats_join(m, r, t, v.x, v.y, v.z, p.unit);
         }
 #pragma unroll
         for (int o = 16; o >= 1; o >>= 1) {
             const float m2 = __shfl_xor_sync(0xffffffffu, m, o), r2 = __shfl_xor_sync(0xffffffffu, r, o),
                         t2 = __shfl_xor_sync(0xffffffffu, t, o);
-            stats_join(m, r, t, m2, r2, t2);
+            stats_join(m, r, t, m2, r2, t2, p.unit);
         }
         if (W > 1) {
             if (lane == 0) { red[w * 4] = m; red[w * 4 + 1] = r; red[w * 4 + 2] = t; }
             __syncthreads();
             m = red[0]; r = red[1]; t = red[2];
-            for (int i = 1; i < W; ++i) stats_join(m, r, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2]);
+            for (int i = 1; i < W; ++i) stats_join(m, r, t, red[i * 4], red[i * 4 + 1], red[i * 4 + 2], p.unit);
             __syncthreads();
         }
         log2l = log1pf(r) * 1.4426950408889634f;
         if (gt == 0) {
-            if (p.row_lse != nullptr) p.row_lse[row] = m + log2l;
+            if (p.row_lse != nullptr) p.row_lse[row] = m * p.unit + log2l;
             if (p.entropy != nullptr) p.entropy[row] = 0.6931471805599453f * (log2l - t / (1.f + r));
         }
 
@@ -593,7 +750,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             if (any) warp_dot4<T, float>(x, rr, p.d, lane, z);
             if (lane < 4 && e + lane < p.k) {
                 const float zz = lane == 0 ? z[0] : lane == 1 ? z[1] : lane == 2 ? z[2] : z[3];
-                s2[e + lane] = zz * p.fmul;
+                z_of[e + lane] = zz;
             }
         }
         group_sync<G>();
@@ -603,7 +760,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             for (int e = gt; e < p.k; e += G) {
                 const long long j = tok[e];
                 // a token below 0 is padding: 0; one behind the table is a mistake that shows
-                const double lp2 = vocab_lp2(p, (double)s2[e], m, r, log2l);
+                const double lp2 = vocab_lp2(p, (double)z_of[e], m, r, log2l);
                 p.log_probs[row * p.k + e] = j < 0 ? 0.f : j >= p.vocab ? NAN : (float)(lp2 * 0.6931471805599453);
                 if (p.token_lp2 != nullptr) p.token_lp2[row * p.k + e] = (float)lp2;
             }
@@ -632,7 +789,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
                 const long long at = row * p.k + e;
                 float q = 0.f;
                 // of every entry that names a row, also an impossible one: the backward stores a coefficient at each
-                const double lp2 = vocab_lp2(p, (double)s2[e], m, r, log2l);
+                const double lp2 = vocab_lp2(p, (double)z_of[e], m, r, log2l);
                 if (there(e)) {
                     const float u = logit(e) - um;
                     q = expf(u) * inv;

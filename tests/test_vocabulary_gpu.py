@@ -531,3 +531,28 @@ def test_offsets_past_32_bits(n):
     size = torch.zeros(len(where), d, dtype=torch.float64).index_add_(0, pick, 2.0 * go.double().abs())
     assert ((dt[where.cuda()].double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + (n + 2) * 2.0 ** -23 * size).all()
     assert dt[others.cuda()].abs().max().item() == 0 and int(torch.count_nonzero(dt.abs().amax(1))) == len(pick.unique())
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 1, 8), (2, 31, 8), (1, 33, 264), (2, 95, 250), (1, 14209, 256), (2, 50001, 768),
+                                   (1, 300, 16384), (2, 300, 16392), (1, 120000, 72)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_one_and_two_rows(n, v, d, dtype):
+    """A token at a time: tables that end inside a chunk, of fewer chunks than blocks and more, widths up to the kernel's
+    limit and behind it; rows around the operands hold what would show."""
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, d, dtype, n + v)
+    xg = torch.full((n + 2, d), float("nan"), dtype=dtype, device="cuda")
+    xg[1:n + 1] = x.cuda()
+    yg = torch.full((v + 33, d), float("nan"), dtype=dtype, device="cuda")
+    yg[:v] = table.cuda()
+    top_k = min(5, v)
+    got = token_log_probs(xg[1:n + 1], yg[:v], tokens.cuda(), top_k=top_k)
+    want = oracle.token_log_probs(*_operands(x, table), tokens[:, None], 1.0, top_k)
+    _inside(got.log_probs, want["log_probs"][:, 0], want["err_lp"], "log_probs")
+    _inside(got.entropy, want["entropy"], want["err_entropy"], "entropy")
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+    _inside(got.top_log_probs, want["top_log_probs"], want["err_lp"][:, None], "top_log_probs")
+    bad = x.clone()
+    bad[0, d // 2] = float("nan")
+    out = token_log_probs(bad.cuda(), table.cuda(), tokens.cuda())
+    assert out.log_probs[0].isnan() and out.entropy[0].isnan() and (n == 1 or torch.isfinite(out.log_probs[1]))
