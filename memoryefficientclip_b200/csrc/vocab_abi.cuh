@@ -46,7 +46,7 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
 template <int G, bool DISTILL, bool TOP>
 static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     const int per_block = VOCAB_THREADS / G;
-    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap);
+    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap);
     const unsigned grid = (unsigned)((p.rows + per_block - 1) / per_block);
     const double bytes = (double)p.rows * (16.0 * p.slots + (p.top_k > 0 ? 8.0 * p.chunks : 0.0) +
                                            2.0 * p.d * (1 + p.k + p.top_k));
@@ -153,8 +153,11 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
         t_tag = TAG_SUMS;
         if (!by_lines) rc = launch_gemm(EPI_STATS, a, t, b.rows, r.vocab, r.d, plan.bn, p, s);
         if (rc) return rc;
-        // a few rows: a block each; many: a warp each
-        const bool few = b.rows <= 2 * sm_count();
+        // A few rows: a block each; many: a warp each.  Where the table has hardly more chunks than alternatives are wanted, most
+        // columns are candidates and a block takes a row too (4096 x 1000, K = 32: 500 us instead of 1240; K = 8: 88 instead of
+        // 62, so not there).
+        const bool few = b.rows <= 2 * sm_count() || plan.chunks <= 2 * r.top_k;
+        b.rank_cap = r.top_k > 0 ? vocab_rank_cap(b.list_cap, b.top_k, few || plan.chunks <= 4 * r.top_k) : 0;
         if (!DISTILL && r.top_k > 0) rc = few ? launch_vocab_rows_t<256, false, true>(b, f16, s) : launch_vocab_rows_t<32, false, true>(b, f16, s);
         else                         rc = few ? launch_vocab_rows_t<256, DISTILL, false>(b, f16, s) : launch_vocab_rows_t<32, DISTILL, false>(b, f16, s);
         if (rc) return rc;

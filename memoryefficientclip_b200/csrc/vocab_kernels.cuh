@@ -85,7 +85,7 @@ struct VocabRows {
     float* entropy;                   // nats, may be null
     float* token_lp2;                 // may be null
     float* log_probs;                 // [rows, k], token scoring
-    int top_k; float* top_log_probs; long long* top_tokens; int list_cap;
+    int top_k; float* top_log_probs; long long* top_tokens; int list_cap, rank_cap;
     // distillation
     const void* teacher_logits; int teacher_dtype; float inv_teacher_t;
     float* teacher_probs;             // [rows, k]
@@ -331,10 +331,10 @@ template <int G> __device__ __forceinline__ void group_sync() {
 }
 
 // Shared memory of one row, in bytes (a multiple of 16).
-__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int list_cap) {
-    return 64 * 8 +                                                       // reductions across warps
-           (k * 4 + 15) / 16 * 16 +                                       // scores of the entries
-           (top_k > 0 ? 160 * 12 + 64 * 8 + 16 + list_cap * 4 : 0);       // see RowTopShared
+__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int list_cap, int rank_cap) {
+    return 64 * 8 +                                                            // reductions across warps
+           (k * 4 + 15) / 16 * 16 +                                            // scores of the entries
+           (top_k > 0 ? rank_cap * 12 + 64 * 8 + 16 + list_cap * 4 : 0);       // see RowTopShared
 }
 
 // Sum / maximum over the G threads of a row, the same on all of them.
@@ -368,13 +368,15 @@ __device__ __forceinline__ float group_reduce(float v, float* red, int gt) {
 //  (e) every column counts who comes before it.
 // Crowds (many equal scores: a row of zeros, repeated table rows) do not fit (b) and are taken chunk by chunk instead.
 static constexpr int VOCAB_LIST = 64;              // chunks collected in (b)
-static constexpr int VOCAB_RANK = 160;             // columns ranked in (e), five per lane: K chunks of which four as a whole
+// Columns scored in (d): all candidates where a block has one row or the table is small; else K chunks of which a few as a
+// whole, and shared memory for more warps (a row in a million has more, from 32768 columns).
+static int vocab_rank_cap(int list_cap, int top_k, bool all) { return all ? list_cap : 128 + 4 * top_k; }
 
 struct RowTopShared {
-    double* z;                                     // [VOCAB_RANK] scores
+    double* z;                                     // [rank_cap] scores
     int* chunk;                                    // [VOCAB_LIST] collected, then the chunks taken
     float* value;                                  // [VOCAB_LIST]
-    int* again;                                    // [VOCAB_RANK] which columns to score again
+    int* again;                                    // [rank_cap] which columns to score again
     int* count;                                    // [4]: chunks collected, columns, columns again
     int* list;                                     // [list_cap] columns to score
 };
@@ -411,13 +413,13 @@ __device__ __forceinline__ int row_top_crowd(const VocabRows& p, const float* cm
     return taken;
 }
 
-__device__ __forceinline__ RowTopShared row_top_shared(uint8_t* smem) {
+__device__ __forceinline__ RowTopShared row_top_shared(uint8_t* smem, int rank_cap) {
     RowTopShared sh;
     sh.z = reinterpret_cast<double*>(smem);
-    sh.chunk = reinterpret_cast<int*>(sh.z + VOCAB_RANK);
+    sh.chunk = reinterpret_cast<int*>(sh.z + rank_cap);
     sh.value = reinterpret_cast<float*>(sh.chunk + VOCAB_LIST);
     sh.again = reinterpret_cast<int*>(sh.value + VOCAB_LIST);
-    sh.count = sh.again + VOCAB_RANK;
+    sh.count = sh.again + rank_cap;
     sh.list = sh.count + 4;
     return sh;
 }
@@ -433,6 +435,18 @@ __device__ __forceinline__ float warp_sort_desc(float v, int lane) {
             v = keep_max ? fmaxf(v, o) : fminf(v, o);
         }
     return v;
+}
+
+// The K-th largest (K <= 32) of 64 values, two per lane, and the largest: both halves are sorted, and i come from the first
+// and K - i from the second for the best split.
+__device__ __forceinline__ float warp_kth(float b1, float b2, int K, int lane, float& best) {
+    const float s1 = warp_sort_desc(b1, lane), s2 = warp_sort_desc(b2, lane);
+    const float other = __shfl_sync(0xffffffffu, s2, max(K - lane - 2, 0));
+    float bound = lane >= K ? -INFINITY : lane == K - 1 ? s1 : fminf(s1, other);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+    best = __shfl_sync(0xffffffffu, s1, 0);
+    return bound;
 }
 
 __device__ __forceinline__ void row_top_write(const VocabRows& p, long long row, int at, double z, long long j, float m, float r, float log2l) {
@@ -481,13 +495,8 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
     }
     float floor_v = -INFINITY, slack = 0.f, size = 0.f;
     if (w == 0) {
-        // The K-th largest of two sorted lists: i from the first and K - i from the second, for the best split.
-        const float s1 = warp_sort_desc(b1, lane), s2 = warp_sort_desc(b2, lane);
-        const float other = __shfl_sync(0xffffffffu, s2, max(K - lane - 2, 0));
-        float bound = lane >= K ? -INFINITY : lane == K - 1 ? s1 : fminf(s1, other);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
-        const float best = __shfl_sync(0xffffffffu, s1, 0);
+        float best;
+        const float bound = warp_kth(b1, b2, K, lane, best);
         const unsigned who = __ballot_sync(0xffffffffu, b1 == best && bc != 0x7fffffff);
         if (who != 0) {
             // How far the tile pass may be off: d / 16 accumulation steps that each drop up to an ulp of a partial sum,
@@ -531,6 +540,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                 const float v = sh.value[i];
                 const int c = sh.chunk[i];
                 int before = 0;
+#pragma unroll 8
                 for (int j = 0; j < taken; ++j) before += comes_first(sh.value[j], sh.chunk[j], v, c) ? 1 : 0;
                 if (before == K - 1) red[2] = v;
             }
@@ -558,7 +568,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                     if (lane >= o) upto += t;
                 }
                 const int all = __shfl_sync(0xffffffffu, upto, 31);
-                if (n + all > min(p.list_cap, VOCAB_RANK)) { crowd = true; break; }
+                if (n + all > min(p.list_cap, p.rank_cap)) { crowd = true; break; }
                 const int at = n + upto - size;
                 if (size == 1) sh.list[at] = c * 32 + best;
                 for (unsigned big = __ballot_sync(0xffffffffu, size > 1); big != 0; big &= big - 1) {
@@ -591,7 +601,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                 }
             }
         }
-        if (n > VOCAB_RANK) {
+        if (n > p.rank_cap) {
             // sorted insertion, in fp64 from the start
             double lz = -INFINITY;
             long long lj = 0x7fffffffffffffffll;
@@ -609,7 +619,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
             if (lane < K) row_top_write(p, row, lane, lz, lj, m, r, log2l);
             n = -1;
         }
-        if (lane == 0) sh.count[1] = n;
+        if (lane == 0) { sh.count[1] = n; sh.count[2] = 0; }
     }
 }
 
@@ -622,7 +632,7 @@ __device__ __forceinline__ void rows_top_score(const VocabRows& p, uint8_t* top_
     int turn = 0;
 #pragma unroll 1
     for (int r = 0; r < R; ++r) {
-        const RowTopShared sh = row_top_shared(top_base + (size_t)r * stride);
+        const RowTopShared sh = row_top_shared(top_base + (size_t)r * stride, p.rank_cap);
         const int n = AGAIN ? sh.count[2] : sh.count[1];
         const T* x = reinterpret_cast<const T*>(p.x) + ((long long)blockIdx.x * R + r) * p.ldx;
         const T* y = reinterpret_cast<const T*>(p.y);
@@ -642,12 +652,40 @@ __device__ __forceinline__ void rows_top_score(const VocabRows& p, uint8_t* top_
     }
 }
 
+// Between (d) and (e), by one warp: of many columns those stay that reach the K-th largest of the lanes' two best, less what is
+// unclear; K and a few.
+__device__ __forceinline__ void row_top_prune(const RowTopShared& sh, int K, double unclear, int lane) {
+    const int n = sh.count[1];
+    if (n <= 64) return;
+    float b1 = -INFINITY, b2 = -INFINITY, best;
+    for (int i = lane; i < n; i += 32) {
+        const float v = (float)sh.z[i];            // fp32 scores: exact
+        b2 = fmaxf(b2, fminf(b1, v));
+        b1 = fmaxf(b1, v);
+    }
+    const double bound = (double)warp_kth(b1, b2, K, lane, best) - unclear;
+    int kept = 0;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int i = i0 + lane;
+        const double z = i < n ? sh.z[i] : 0.0;
+        const int j = i < n ? sh.list[i] : 0;
+        const bool keep = i < n && z >= bound;
+        const unsigned who = __ballot_sync(0xffffffffu, keep);       // (all have read before one writes)
+        const int at = kept + __popc(who & ((1u << lane) - 1u));
+        if (keep) { sh.z[at] = z; sh.list[at] = j; }
+        kept += __popc(who);
+        __syncwarp();
+    }
+    if (lane == 0) sh.count[1] = kept;
+}
+
 // (e) of column i among the n of its row: how many come before it, and whether another one is closer than `unclear`.
 __device__ __forceinline__ int row_top_rank(const RowTopShared& sh, int n, int i, double unclear, bool& near) {
     const double z = sh.z[i];
     const int j = sh.list[i];
     int before = 0;
     near = false;
+#pragma unroll 8
     for (int o = 0; o < n; ++o) {
         const double zo = sh.z[o];
         before += comes_first(zo, sh.list[o], z, j) ? 1 : 0;
@@ -699,7 +737,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     const long long row = (long long)blockIdx.x * (VOCAB_THREADS / G) + threadIdx.x / G;
     const bool active = row < p.rows;             // the same for the row's threads
     if (!TOP && !DISTILL && !active) return;      // (a block of G = 256 has one row, warps of G = 32 do not meet)
-    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap);
+    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap);
     float* red = reinterpret_cast<float*>(smem);
     float* z_of = reinterpret_cast<float*>(smem + 64 * 8);
     uint8_t* top_smem = smem + 64 * 8 + (p.k * 4 + 15) / 16 * 16;
@@ -818,41 +856,42 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     }
     if (DISTILL && p.loss != nullptr) distill_reduce(p);
     if (TOP) {
-        const RowTopShared sh = row_top_shared(top_smem);
-        const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap), bw = threadIdx.x >> 5;
+        const RowTopShared sh = row_top_shared(top_smem, p.rank_cap);
+        const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap), bw = threadIdx.x >> 5;
         uint8_t* top_base = smem_all + (top_smem - smem);
         group_sync<G>();
         if (active) row_top_select<G, T>(p, row, gt, sh, m, r, log2l, red);
-        else if (gt == 0) sh.count[1] = 0;
+        else if (gt == 0) sh.count[1] = sh.count[2] = 0;
         __syncthreads();
         rows_top_score<G, T, float>(p, top_base, stride, bw, lane);
         __syncthreads();
         // In fp32 an order counts only when it is clear: d / 64 products in a row and a tree of 6, each off by half an ulp
         // (2^-24) of at most |x| |y|, on both sides.
+        const double unclear = active ? (double)(1.1920929e-7f * ((float)p.d * 0.015625f + 6.f) * red[3]) : 0.0;
+        if (w == 0) row_top_prune(sh, p.top_k, unclear, lane);
+        group_sync<G>();
         const int n = sh.count[1];
-        if (w == 0) {
-            const double unclear = active ? (double)(1.1920929e-7f * ((float)p.d * 0.015625f + 6.f) * red[3]) : 0.0;
-            int again = 0;
-            for (int i = lane; i - lane < n; i += 32) {
-                bool near = false;
-                if (i < n) row_top_rank(sh, n, i, unclear, near);
-                const unsigned who = __ballot_sync(0xffffffffu, near);
-                if (near) sh.again[again + __popc(who & ((1u << lane) - 1u))] = i;
-                again += __popc(who);
-            }
-            if (lane == 0) sh.count[2] = again;
+        for (int i0 = w * 32; i0 < n; i0 += G) {
+            const int i = i0 + lane;
+            bool near = false;
+            if (i < n) row_top_rank(sh, n, i, unclear, near);
+            const unsigned who = __ballot_sync(0xffffffffu, near);
+            int at = 0;
+            if (lane == 0 && who != 0) at = atomicAdd(sh.count + 2, __popc(who));
+            at = __shfl_sync(0xffffffffu, at, 0);
+            if (near) sh.again[at + __popc(who & ((1u << lane) - 1u))] = i;
         }
         __syncthreads();
         rows_top_score<G, T, double>(p, top_base, stride, bw, lane);
         __syncthreads();
-        if (w != 0 || !active || n < 0) return;
-        for (int i = lane; i < n; i += 32) {
+        if (!active || n < 0) return;
+        for (int i = gt; i < n; i += G) {
             bool ignored;
             const int place = row_top_rank(sh, n, i, 0.0, ignored);
             if (place < p.top_k) row_top_write(p, row, place, sh.z[i], sh.list[i], m, r, log2l);
         }
         // only where a row's scores are not numbers are there fewer than K
-        if (lane < p.top_k && lane >= n) { p.top_tokens[row * p.top_k + lane] = -1; p.top_log_probs[row * p.top_k + lane] = NAN; }
+        if (w == 0 && lane < p.top_k && lane >= n) { p.top_tokens[row * p.top_k + lane] = -1; p.top_log_probs[row * p.top_k + lane] = NAN; }
     }
 }
 

@@ -556,3 +556,16 @@ def test_one_and_two_rows(n, v, d, dtype):
     bad[0, d // 2] = float("nan")
     out = token_log_probs(bad.cuda(), table.cuda(), tokens.cuda())
     assert out.log_probs[0].isnan() and out.entropy[0].isnan() and (n == 1 or torch.isfinite(out.log_probs[1]))
+
+
+@pytest.mark.parametrize("n,v,top_k", [(1, 256, 8), (3, 1000, 32), (1, 1000, 31), (200, 257, 9), (400, 600, 32), (2, 33, 32),
+                                       (1, 2047, 32), (300, 64, 32)])
+def test_alternatives_of_small_tables(n, v, top_k):
+    """So few chunks that most columns are candidates, some of them equal."""
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, 72, torch.bfloat16, v)
+    table[v // 2:v // 2 + 7] = table[3]
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=top_k)
+    want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, top_k)
+    assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
+    _inside(got.top_log_probs, want["top_log_probs"], want["err_lp"][:, None], "top_log_probs")
