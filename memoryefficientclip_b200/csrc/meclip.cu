@@ -731,14 +731,14 @@ struct Operand {
     bool f16 = false;
 };
 
-// Lets a kernel use all of an SM's shared memory: once per kernel and device (`done`: one bit per device).
+// Lets a kernel use all of an SM's shared memory, or `bytes` of it: once per kernel and device (`done`: one bit per device).
 template <class Kernel>
-static int allow_all_smem(Kernel kern, std::atomic<unsigned long long>& done) {
+static int allow_all_smem(Kernel kern, std::atomic<unsigned long long>& done, int bytes = SMEM_LIMIT) {
     int dev = 0;
     MECLIP_CUDA(cudaGetDevice(&dev));
     const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
     if ((done.load(std::memory_order_relaxed) & bit) != 0) return MECLIP_OK;
-    MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
+    MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     done.fetch_or(bit, std::memory_order_relaxed);
     return MECLIP_OK;
 }
@@ -919,7 +919,8 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         }
     }
     if ((long long)p.num_m_tiles * p.num_n_tiles * p.splits > 0x7fffffffLL) return fail(MECLIP_EINVAL, "too many tiles");
-    if (epi != EPI_OUT || wide || p.acc_in != nullptr) p.tile_out = 0;
+    // (a bf16 store is 64 columns wide: one that is half another tile's must not happen)
+    if (epi != EPI_OUT || wide || p.acc_in != nullptr || (p.num_n_tiles > 1 && bn % 64 != 0)) p.tile_out = 0;
     if (p.tile_out) {
         rc = make_tmap_out(&p.out_map[0], p.out, n, m, p.ld_out, p.splits, p.split_stride, p.out_bf16 != 0);
         if (rc) return rc;

@@ -61,7 +61,9 @@ static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
 template <typename T, int R>
 static int launch_vocab_few_r(const VocabFew& p, unsigned blocks, cudaStream_t s) {
     const int smem = VOCAB_FEW_RING + R * p.d_smem * 2;
-    MECLIP_CUDA(cudaFuncSetAttribute(vocab_few_kernel<T, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    static std::atomic<unsigned long long> smem_allowed{0};
+    const int rc = allow_all_smem(vocab_few_kernel<T, R>, smem_allowed, VOCAB_FEW_RING + VOCAB_FEW_X);
+    if (rc) return rc;
     vocab_few_kernel<T, R><<<blocks, VOCAB_FEW_THREADS, smem, s>>>(p);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;

@@ -569,3 +569,90 @@ def test_alternatives_of_small_tables(n, v, top_k):
     want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, top_k)
     assert torch.equal(got.top_tokens.cpu(), want["top_tokens"])
     _inside(got.top_log_probs, want["top_log_probs"], want["err_lp"][:, None], "top_log_probs")
+
+
+def _c_grad(n, v, d, operands, tokens, per_row, saved, entropy, g, h, dx, dt, mode):
+    """meclip_token_log_probs_grad as a C caller makes the call."""
+    from memoryefficientclip_b200 import _lib, ops
+    x, table = operands
+    lib = _lib.load()
+    size = lib.meclip_vocab_grad_workspace_bytes(0, n, v, d)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    lse = saved.data_ptr()
+    _lib.check(lib.meclip_token_log_probs_grad(
+        x.data_ptr(), table.data_ptr(), 0, n, v, d, x.stride(0), table.stride(0), 1.0, ops._ptr(tokens), per_row, lse,
+        ops._ptr(entropy), lse + 4 * n, ops._ptr(g), ops._ptr(h), ops._ptr(dx), mode, d, ops._ptr(dt), mode, d,
+        ws.data_ptr(), size, ops.status_word(x.device).data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 700, 64), (40, 4099, 264), (300, 2051, 264), (1100, 999, 72), (1100, 2051, 512)])
+def test_c_calls_without_tokens_and_with_accumulation(n, v, d):
+    """No token per row (entropy and alternatives only), gradients that are added to what is there, none at all."""
+    from memoryefficientclip_b200 import _lib, ops
+    x, table, tokens, gen = _pair(n, v, d, torch.bfloat16, n)
+    xg, yg, tg = x.cuda(), table.cuda(), tokens.cuda()
+    lib = _lib.load()
+    size = lib.meclip_vocab_workspace_bytes(n, v, 2)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    entropy, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    top_lp, top = torch.empty(n, 2, device="cuda"), torch.empty(n, 2, dtype=torch.int64, device="cuda")
+    _lib.check(lib.meclip_token_log_probs(
+        xg.data_ptr(), yg.data_ptr(), 0, n, v, d, d, d, 1.0, None, 0, None, entropy.data_ptr(), 2, top_lp.data_ptr(),
+        top.data_ptr(), lse.data_ptr(), None, ws.data_ptr(), size, None, torch.cuda.current_stream().cuda_stream))
+    want = oracle.token_log_probs(x, table, tokens[:, None], 1.0, 2)
+    _inside(entropy, want["entropy"], want["err_entropy"], "entropy")
+    assert torch.equal(top.cpu(), want["top_tokens"])
+    h = torch.randn(n, generator=gen)
+    dx, dt = torch.empty(n, d, device="cuda"), torch.empty(v, d, device="cuda")
+    _c_grad(n, v, d, (xg, yg), None, 0, lse, entropy, None, h.cuda(), dx, dt, ops._MODE[torch.float32])
+    wx, wy, bx, by = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.0, torch.zeros(n, 1), h, (torch.float32,) * 2)
+    _inside(dx, wx, bx, "dx")
+    _inside(dt, wy, by, "dtable")
+    _c_grad(n, v, d, (xg, yg), None, 0, lse, entropy, None, None, dx, dt, ops._MODE[torch.float32])
+    assert dx.abs().max().item() == 0 and dt.abs().max().item() == 0
+    # accumulation: the same gradient twice onto a start value
+    lp, ent, _a, _b, saved = ops.token_log_probs(xg, yg, tg, 1.0, 0, True, ops.status_word(xg.device))
+    g = torch.randn(n, 1, generator=gen)
+    ax, at = torch.full((n, d), 0.5, device="cuda"), torch.full((v, d), -0.25, device="cuda")
+    for _ in range(2):
+        _c_grad(n, v, d, (xg, yg), tg, 1, saved, ent, g.cuda(), h.cuda(), ax, at, 2)
+    wx, wy, bx, by = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.0, g, h, (torch.float32,) * 2)
+    _inside(ax, 0.5 + 2 * wx, 2 * bx + oracle.ULP * (1 + 2 * wx.abs()), "dx")
+    _inside(at, -0.25 + 2 * wy, 2 * by + oracle.ULP * (1 + 2 * wy.abs()), "dtable")
+    ops.check_status()
+
+
+def test_two_threads_at_once():
+    """Forward and backward from two threads, each on a stream of its own."""
+    import threading
+    from memoryefficientclip_b200 import embed_tokens, token_log_probs
+    x, table, tokens, _g = _pair(1300, 3001, 264, torch.bfloat16, 2)
+    x, table, tokens = x.cuda(), table.cuda(), tokens.cuda()
+
+    def step():
+        xl, tl = x.clone().requires_grad_(True), table.clone().requires_grad_(True)
+        out = token_log_probs(xl + embed_tokens(tokens, tl, 0.1), tl, tokens, top_k=3)
+        return [out.log_probs.detach(), out.top_tokens, *torch.autograd.grad(out.log_probs.sum() - out.entropy.sum(), [xl, tl])]
+
+    want = step()
+    torch.cuda.synchronize()
+    found, failed = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    found[i] = step()
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:          # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i in range(2):
+        for a, b in zip(found[i], want):
+            assert torch.equal(a, b)
