@@ -493,7 +493,8 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
  *   meclip_distill          KL(q || p) per row for a teacher that is known by its top logits: q = softmax of
  *                           teacher_logits / teacher_temperature (teacher_dtype, [rows, per_row]) over the row's
  *                           entries that are present (token >= 0 and logit > -inf).  A row without one has loss 0,
- *                           row_has 0 and no gradient.  Entries that name the same token add up.
+ *                           row_has 0 and no gradient.  An entry counts by itself where a row names a
+ *                           token twice.
  *                           loss = sum of row_loss, times inv_count = 1 / (rows with an entry) when `mean` is set
  *                           (both NULL: only row_loss is wanted); no row at all: loss 0.
  *   meclip_distill_grad     dz_ij = w_i (p_ij - q_ij), w_i = grad_out (one scalar, or [rows] with grad_per_row) times

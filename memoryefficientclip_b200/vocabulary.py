@@ -185,7 +185,7 @@ class MemoryEfficientDistillLoss(nn.Module):
     table, teacher_tokens, teacher_logits)``: teacher_tokens [N, k] (k up to 256, int64 or int32) name rows of the table,
     teacher_logits [N, k] are their logits (float32, bfloat16 or float16; no gradient).  An entry with a negative token or
     a logit of -inf is absent, whatever else stands in its place; a row without entries adds nothing and gets no gradient;
-    entries of a row that name the same token add up.  reduction: "mean" over the rows that have entries, "sum", or "none"
+    an entry counts by itself where a row names a token twice.  reduction: "mean" over the rows that have entries, "sum", or "none"
     for the [N] losses.  With normalized_inputs=False features and table are L2-normalised inside, as in the contrastive
     losses: the table is then the other tower's output and the teacher's entries its best pairs.
     """
