@@ -6,8 +6,10 @@ Bounds count the roundings of the computation, for operands that are exact:
              of a partial sum that stays below |x_i| |y_j|; scale and exponent add a few ulps of the score itself
   p, log p   the error of the scores, plus that of summing V exponentials (a few ulps: the partial sums are positive)
   entropy    sum_j p_j |log p_j + H| <= 2 ln V times the error of the scores
-  gradients  every coefficient is rounded to bf16 once (half a step, 2^-8 relative), carries the error of its p, and the
-             contraction drops up to 2^-23 of a partial sum every 16 terms; then one rounding to the output's type
+  gradients  every coefficient is rounded once to fp16 that is scaled so that a bound on all of them comes to 2^14 (half
+             a step, 2^-11 relative, or half of fp16's smallest, 2^-25, over the scale: 2^-39 of that bound) or to two
+             bf16 numbers (less); it carries the error of its p, and the contraction drops up to 2^-23 of a partial sum
+             every 16 terms; then one rounding to the output's type
 """
 import torch
 
@@ -50,8 +52,8 @@ def _gradients(x, table, temperature, dense, entries, dense_size, out_dtypes, op
     _z, err = scores(x, table, temperature)
     dz = (dense + entries) / temperature
     size = (dense_size + entries.abs()) / temperature
-    # a coefficient: half a bf16 step of itself, and the score's error on every part of it
-    off = 2.0 ** -8 * dz.abs() + (2 * err[:, None] + 16 * ULP) * size
+    # a coefficient: half an fp16 step of itself or of the smallest number, and the score's error on every part of it
+    off = 2.0 ** -11 * dz.abs() + 2.0 ** -39 * size.sum(1).max() + (2 * err[:, None] + 16 * ULP) * size
     out = []
     for dim, (g, o, sz, other, dtype) in enumerate(((dz, off, size, y, out_dtypes[0]),
                                                     (dz.T, off.T, size.T, x, out_dtypes[1]))):
