@@ -459,18 +459,21 @@ static int embed_grad_t(const long long* tokens, long long n, const T* g, long l
     st.hist = reinterpret_cast<uint32_t*>(rest);
     st.out = out; st.ldo = ldo; st.d = d; st.elt = elt;
     st.flat = ldo == d && aligned16(out) && ((size_t)vocab * d * elt) % 16 == 0;
-    const int smem = (EMB_SORT_THREADS / 32) * 2 << pl.bits;
+    const int smem = (EMB_SORT_THREADS / 32) * 2 << pl.bits, most_smem = (EMB_SORT_THREADS / 32) * 2 << EMB_MAX_BITS;
+    static std::atomic<unsigned long long> smem_small{0}, smem_scatter{0};
     const int clear_blocks = sm_count();       // beside the sort's blocks: two blocks of 1024 threads fit an SM
     if (n <= EMB_ONE_BLOCK) {
         st.blocks = 1;
         st.parts = 1;
-        MECLIP_CUDA(cudaFuncSetAttribute(emb_sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        const int rc = allow_all_smem(emb_sort_small_kernel, smem_small, most_smem);
+        if (rc) return rc;
         ScopedTiming timing(s, TAG_ROW, 16.0 * (double)n * pl.passes + (double)vocab * d * elt);
         emb_sort_small_kernel<<<1 + 2 * clear_blocks, EMB_SORT_THREADS, smem, s>>>(st, pl.passes, keys[0], pos[0], keys[1], pos[1]);
         MECLIP_CUDA(cudaGetLastError());
         if (n == 0) return MECLIP_OK;
     } else {
-        MECLIP_CUDA(cudaFuncSetAttribute(emb_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        const int rc = allow_all_smem(emb_scatter_kernel, smem_scatter, most_smem);
+        if (rc) return rc;
         st.parts = 2 * pl.passes;
         const double clear_bytes = (double)vocab * d * elt / st.parts;
         for (int p = 0; p < pl.passes; ++p) {

@@ -43,6 +43,9 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
     return v;
 }
 
+static constexpr int VOCAB_ROWS_SMEM = 200 * 1024;      // dynamic shared memory of a block of the row kernel at most
+static constexpr int vocab_list_cap(int top_k) { return 32 * top_k + 64; }
+
 template <int G, bool DISTILL, bool TOP>
 static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     const int per_block = VOCAB_THREADS / G;
@@ -52,7 +55,11 @@ static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
                                            2.0 * p.d * (1 + p.k + p.top_k));
     ScopedTiming timing(s, TAG_ROW, bytes);
     auto kern = f16 ? vocab_rows_kernel<G, __half, DISTILL, TOP> : vocab_rows_kernel<G, __nv_bfloat16, DISTILL, TOP>;
-    if (smem > 48 * 1024) MECLIP_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    // (once to the most: a limit that follows the call could shrink between another thread's setting and its launch)
+    static_assert(VOCAB_THREADS / 32 * vocab_row_smem(VOCAB_MAX_ENTRIES, VOCAB_MAX_TOP, vocab_list_cap(VOCAB_MAX_TOP), vocab_list_cap(VOCAB_MAX_TOP)) <= VOCAB_ROWS_SMEM, "shared memory of a block");
+    static std::atomic<unsigned long long> smem_allowed[2] = {{0}, {0}};
+    const int rc = allow_all_smem(kern, smem_allowed[f16 ? 1 : 0], VOCAB_ROWS_SMEM);
+    if (rc) return rc;
     kern<<<grid, VOCAB_THREADS, smem, s>>>(p);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
@@ -106,7 +113,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     r.chunk_second = r.top_k > 0 ? reinterpret_cast<const uint32_t*>(ws + plan.stats_bytes + plan.chunk_bytes) : nullptr;
     r.chunks = (int)plan.chunks;
     r.chunk_ld = plan.chunk_ld;
-    r.list_cap = r.top_k > 0 ? 32 * r.top_k + 64 : 0;
+    r.list_cap = r.top_k > 0 ? vocab_list_cap(r.top_k) : 0;
     for (long long r0 = 0; r0 < rows; r0 += plan.row_block) {
         VocabRows b = r;
         b.rows = rows - r0 < plan.row_block ? rows - r0 : plan.row_block;

@@ -656,3 +656,36 @@ def test_two_threads_at_once():
     for i in range(2):
         for a, b in zip(found[i], want):
             assert torch.equal(a, b)
+
+
+def test_two_threads_with_different_sizes():
+    """Calls that want different amounts of shared memory from the same kernels."""
+    import threading
+    from memoryefficientclip_b200 import embed_tokens, token_log_probs
+    x, table, tokens, _g = _pair(400, 40000, 72, torch.bfloat16, 5)
+    x, table, tokens = x.cuda(), table.cuda(), tokens.cuda()
+    many = torch.stack([tokens] * 256, 1)
+    calls = [lambda: token_log_probs(x, table[:600], tokens, top_k=32), lambda: token_log_probs(x, table, many, top_k=1),
+             lambda: token_log_probs(x[:1], table, many[:1], top_k=32), lambda: token_log_probs(x[:1, :64], table[:, :64], tokens[:1])]
+    tables = [table.clone().requires_grad_(True), table[:100].clone().requires_grad_(True)]
+    calls += [lambda t=t: torch.autograd.grad(embed_tokens(tokens % t.shape[0], t).float().sum(), t) for t in tables]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(which):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    for a, b in zip(calls[which](), want[which]):
+                        # (tokens behind the smaller table are NaN on both sides)
+                        assert a is b or torch.allclose(a, b, rtol=0, atol=0, equal_nan=True)
+        except BaseException as e:      # noqa: BLE001
+            failed.append((which, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(calls))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
