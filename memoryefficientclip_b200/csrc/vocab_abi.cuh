@@ -24,7 +24,8 @@ static int pick_stats_bn(long long rows, long long vocab) {
 }
 
 struct VocabPlan {
-    long long row_block, slots, chunks, chunk_ld, few_blocks;
+    long long row_block, slots, chunks, chunk_ld, few_blocks;      // slots: room for the partial sums of either pass
+    long long tile_slots;                                           // those that the tile pass writes
     int bn;
     size_t stats_bytes, chunk_bytes, total;
 };
@@ -32,7 +33,7 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
     VocabPlan v;
     v.row_block = rows < VOCAB_ROW_BLOCK ? rows : VOCAB_ROW_BLOCK;
     v.bn = pick_stats_bn(v.row_block, vocab);
-    v.slots = 2 * ((vocab + v.bn - 1) / v.bn);
+    v.slots = v.tile_slots = 2 * ((vocab + v.bn - 1) / v.bn);
     v.chunks = (vocab + 31) / 32;
     v.few_blocks = v.chunks < VOCAB_FEW_BLOCKS * sm_count() ? v.chunks : VOCAB_FEW_BLOCKS * sm_count();
     if (rows <= VOCAB_FEW_ROWS && v.slots < v.few_blocks) v.slots = v.few_blocks;
@@ -106,7 +107,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     if (workspace_bytes < plan.total) return fail(MECLIP_ENOSPC, "vocabulary pass: workspace %zu < %zu bytes", workspace_bytes, plan.total);
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     r.stats = reinterpret_cast<const float4*>(ws);
-    r.slots = (int)plan.slots;
+    r.slots = (int)plan.tile_slots;
     r.stats_ld = plan.slots;
     r.unit = 1.f;
     r.chunk_max = r.top_k > 0 ? reinterpret_cast<const float*>(ws + plan.stats_bytes) : nullptr;
