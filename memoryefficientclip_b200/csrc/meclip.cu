@@ -951,9 +951,9 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         const int amn = a.mn_major ? 1 : 0;
         p.wide = wide ? 1 : 0;
         p.idesc = umma_idesc_bf16(PAIR_BM, bn < MAX_BN ? bn : MAX_BN, amn, 0) & idesc_keep;
-        p.idesc2 = wide ? umma_idesc_bf16(PAIR_BM, bn - MAX_BN, amn, 0) : 0u;
+        p.idesc2 = wide ? umma_idesc_bf16(PAIR_BM, bn - MAX_BN, amn, 0) & idesc_keep : 0u;
         p.idesc_last = umma_idesc_bf16(PAIR_BM, p.bn_last < MAX_BN ? p.bn_last : MAX_BN, amn, 0) & idesc_keep;
-        p.idesc2_last = p.bn_last > MAX_BN ? umma_idesc_bf16(PAIR_BM, p.bn_last - MAX_BN, amn, 0) : 0u;
+        p.idesc2_last = p.bn_last > MAX_BN ? umma_idesc_bf16(PAIR_BM, p.bn_last - MAX_BN, amn, 0) & idesc_keep : 0u;
         p.stage_bytes = A_STAGE_BYTES + (bn / 2) * BK * 2;
         stages = (SMEM_LIMIT - 1024 - tail_size) / p.stage_bytes;
         if (stages > MAX_STAGES) stages = MAX_STAGES;

@@ -54,3 +54,31 @@ def test_one_and_two_rows_in_a_used_workspace(n, v, d, temperature):
     _inside(row_loss, kl, err, "row loss")
     _inside(loss, kl.mean(), err.mean() + 2 * oracle.ULP * kl.mean(), "loss")
     assert there.all()
+
+
+@pytest.mark.parametrize("switch", ["MECLIP_WIDE=1", "MECLIP_WIDE=1 MECLIP_SERIAL=1", "MECLIP_WIDE=1 MECLIP_NO_TRANSPOSE=1",
+                                    "MECLIP_PAIR=1", "MECLIP_STATIC_SCHED=1"])
+def test_gradients_under_the_other_switches(switch):
+    """Switches are read once per process: the widths below in a child, with tiles of more than 256 columns among them."""
+    out = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider", __file__,
+                          "-k", "test_gradients_of_wide_features"],
+                         env=dict(os.environ, **dict(s.split("=") for s in switch.split())), capture_output=True, text=True,
+                         timeout=300)
+    assert out.returncode == 0, out.stdout[-2000:]
+
+
+@pytest.mark.parametrize("n,v,d", [(300, 2100, 512), (257, 5000, 1152), (1100, 3000, 520), (60, 4099, 768)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sides", ["both", "features", "table"])
+def test_gradients_of_wide_features(n, v, d, dtype, sides):
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, d, dtype, n + v, bump=6.0)
+    g_lp, g_h = torch.randn(n, generator=g), torch.randn(n, generator=g) * 0.3
+    xg, yg = x.cuda().requires_grad_(sides != "table"), table.cuda().requires_grad_(sides != "features")
+    got = token_log_probs(xg, yg, tokens.cuda(), temperature=1.3)
+    (got.log_probs * g_lp.cuda() + got.entropy * g_h.cuda()).sum().backward()
+    wx, wy, bx, by = oracle.token_log_probs_grad(x, table, tokens[:, None], 1.3, g_lp[:, None], g_h, (dtype, dtype))
+    if sides != "table":
+        _inside(xg.grad, wx, bx, "dx")
+    if sides != "features":
+        _inside(yg.grad, wy, by, "dtable")
