@@ -42,6 +42,6 @@ def embed_tokens(tokens, table, scale=1.0):
     tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     table = ops.row_major(table)
-    if table.requires_grad and torch.is_grad_enabled():
+    if ops.differentiated(table):
         return _EmbedFn.apply(tokens, table, float(scale))
     return ops.embed(tokens, table, float(scale))

@@ -8,6 +8,7 @@ import math
 import os
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 
@@ -58,6 +59,13 @@ def row_major(t: torch.Tensor) -> torch.Tensor:
     """t itself if its rows are runs of adjacent elements that do not overlap (what the kernels address by a pitch), else
     a contiguous copy: of a transposed matrix, or of one row expanded to many."""
     return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1) else t.contiguous()
+
+
+def differentiated(*tensors: torch.Tensor) -> bool:
+    """Whether autograd has to see a call on these: grad mode with an input that requires a gradient, or a forward-mode
+    tangent on one (which an autograd node without a forward derivative refuses instead of dropping it)."""
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or \
+        any(unpack_dual(t).tangent is not None for t in tensors)
 
 
 def padded(d: int) -> int:

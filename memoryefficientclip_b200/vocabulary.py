@@ -117,7 +117,7 @@ def token_log_probs(features, table, tokens, temperature=1.0, top_k=0) -> TokenL
         f"top_k must be between 0 and {min(MAX_TOP, table.shape[0])}"
     device = features.device
     ops.poll_status(device)
-    if (features.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+    if ops.differentiated(features, table):
         return TokenLogProbs(*_TokenLogProbsFn.apply(features, table, tokens, float(temperature), top_k))
     x, y = ops.vocab_operands(features, table)
     lp, entropy, top_lp, top, _saved = ops.token_log_probs(x, y, tokens, float(temperature), top_k, False,

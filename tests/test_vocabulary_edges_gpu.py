@@ -82,3 +82,28 @@ def test_gradients_of_wide_features(n, v, d, dtype, sides):
         _inside(xg.grad, wx, bx, "dx")
     if sides != "features":
         _inside(yg.grad, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_forward_mode_derivatives_are_refused(dtype):
+    """There is none of these operators; a tangent is never dropped, with or without grad mode."""
+    import torch.autograd.forward_ad as fwd
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss, embed_tokens, token_log_probs
+    x, table, tokens, _g = _pair(20, 50, 64, dtype, 8)
+    x, table, tokens = x.cuda(), table.cuda(), tokens.cuda()
+    want = token_log_probs(x, table, tokens, top_k=2), embed_tokens(tokens, table)
+    distill = MemoryEfficientDistillLoss(1.0)
+    logits = torch.zeros(20, 1, device="cuda")
+    with fwd.dual_level():
+        dual_x, dual_t = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(table, torch.ones_like(table))
+        for grad_mode in (True, False):
+            with torch.set_grad_enabled(grad_mode):
+                for call in (lambda: token_log_probs(dual_x, table, tokens), lambda: token_log_probs(x, dual_t, tokens, top_k=1),
+                             lambda: embed_tokens(tokens, dual_t), lambda: distill(dual_x, table, tokens[:, None], logits),
+                             lambda: distill(x, dual_t, tokens[:, None], logits)):
+                    with pytest.raises((RuntimeError, NotImplementedError)):
+                        call()
+                # plain inputs are answered as ever while such a level is open
+                for a, b in zip(token_log_probs(x, table, tokens, top_k=2), want[0]):
+                    assert torch.equal(a, b)
+                assert torch.equal(embed_tokens(tokens, table), want[1])
