@@ -45,19 +45,18 @@ static VocabPlan plan_vocab(long long rows, long long vocab, int top_k) {
 }
 
 static constexpr int VOCAB_ROWS_SMEM = 200 * 1024;      // dynamic shared memory of a block of the row kernel at most
-static constexpr int vocab_list_cap(int top_k) { return 32 * top_k + 64; }
 
 template <int G, bool DISTILL, bool TOP>
 static int launch_vocab_rows_t(const VocabRows& p, int f16, cudaStream_t s) {
     const int per_block = VOCAB_THREADS / G;
-    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap);
+    const size_t smem = (size_t)per_block * vocab_row_smem(p.k, p.top_k, p.rank_cap);
     const unsigned grid = (unsigned)((p.rows + per_block - 1) / per_block);
     const double bytes = (double)p.rows * (16.0 * p.slots + (p.top_k > 0 ? 8.0 * p.chunks : 0.0) +
                                            2.0 * p.d * (1 + p.k + p.top_k));
     ScopedTiming timing(s, TAG_ROW, bytes);
     auto kern = f16 ? vocab_rows_kernel<G, __half, DISTILL, TOP> : vocab_rows_kernel<G, __nv_bfloat16, DISTILL, TOP>;
     // (once to the most: a limit that follows the call could shrink between another thread's setting and its launch)
-    static_assert(VOCAB_THREADS / 32 * vocab_row_smem(VOCAB_MAX_ENTRIES, VOCAB_MAX_TOP, vocab_list_cap(VOCAB_MAX_TOP), vocab_list_cap(VOCAB_MAX_TOP)) <= VOCAB_ROWS_SMEM, "shared memory of a block");
+    static_assert(VOCAB_THREADS / 32 * vocab_row_smem(VOCAB_MAX_ENTRIES, VOCAB_MAX_TOP, vocab_rank_cap(VOCAB_MAX_TOP, true)) <= VOCAB_ROWS_SMEM, "shared memory of a block");
     static std::atomic<unsigned long long> smem_allowed[2] = {{0}, {0}};
     const int rc = allow_all_smem(kern, smem_allowed[f16 ? 1 : 0], VOCAB_ROWS_SMEM);
     if (rc) return rc;
@@ -114,7 +113,6 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
     r.chunk_second = r.top_k > 0 ? reinterpret_cast<const uint32_t*>(ws + plan.stats_bytes + plan.chunk_bytes) : nullptr;
     r.chunks = (int)plan.chunks;
     r.chunk_ld = plan.chunk_ld;
-    r.list_cap = r.top_k > 0 ? vocab_list_cap(r.top_k) : 0;
     for (long long r0 = 0; r0 < rows; r0 += plan.row_block) {
         VocabRows b = r;
         b.rows = rows - r0 < plan.row_block ? rows - r0 : plan.row_block;
@@ -167,7 +165,7 @@ static int vocab_forward(VocabRows r, float temperature, int dtype, void* worksp
         // columns are candidates and a block takes a row too (4096 x 1000, K = 32: 500 us instead of 1240; K = 8: 88 instead of
         // 62, so not there).
         const bool few = b.rows <= 2 * sm_count() || plan.chunks <= 2 * r.top_k;
-        b.rank_cap = r.top_k > 0 ? vocab_rank_cap(b.list_cap, b.top_k, few || plan.chunks <= 4 * r.top_k) : 0;
+        b.rank_cap = r.top_k > 0 ? vocab_rank_cap(b.top_k, few || plan.chunks <= 4 * r.top_k) : 0;
         if (!DISTILL && r.top_k > 0) rc = few ? launch_vocab_rows_t<256, false, true>(b, f16, s) : launch_vocab_rows_t<32, false, true>(b, f16, s);
         else                         rc = few ? launch_vocab_rows_t<256, DISTILL, false>(b, f16, s) : launch_vocab_rows_t<32, DISTILL, false>(b, f16, s);
         if (rc) return rc;

@@ -85,7 +85,7 @@ struct VocabRows {
     float* entropy;                   // nats, may be null
     float* token_lp2;                 // may be null
     float* log_probs;                 // [rows, k], token scoring
-    int top_k; float* top_log_probs; long long* top_tokens; int list_cap, rank_cap;
+    int top_k; float* top_log_probs; long long* top_tokens; int rank_cap;
     // distillation
     const void* teacher_logits; int teacher_dtype; float inv_teacher_t;
     float* teacher_probs;             // [rows, k]
@@ -316,11 +316,11 @@ template <typename V, typename I>
 __device__ __forceinline__ bool comes_first(V a, I ia, V b, I ib) { return a > b || (a == b && ia < ib); }
 
 // A warp's sorted list, one element per lane: inserts (z, j), the last lane's element falls off.
-__device__ __forceinline__ void list_insert(double& lz, long long& lj, double z, long long j, int lane) {
+__device__ __forceinline__ void list_insert(double& lz, int& lj, double z, int j, int lane) {
     const unsigned ahead = __ballot_sync(0xffffffffu, comes_first(lz, lj, z, j));
     const int pos = __popc(ahead);               // the list is sorted: the lanes ahead are the first ones
     const double pz = __shfl_up_sync(0xffffffffu, lz, 1);
-    const long long pj = __shfl_up_sync(0xffffffffu, lj, 1);
+    const int pj = __shfl_up_sync(0xffffffffu, lj, 1);
     if (lane > pos) { lz = pz; lj = pj; }
     if (lane == pos) { lz = z; lj = j; }
 }
@@ -331,10 +331,10 @@ template <int G> __device__ __forceinline__ void group_sync() {
 }
 
 // Shared memory of one row, in bytes (a multiple of 16).
-__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int list_cap, int rank_cap) {
+__host__ __device__ constexpr int vocab_row_smem(int k, int top_k, int rank_cap) {
     return 64 * 8 +                                                            // reductions across warps
            (k * 4 + 15) / 16 * 16 +                                            // scores of the entries
-           (top_k > 0 ? rank_cap * 12 + 64 * 8 + 16 + list_cap * 4 : 0);       // see RowTopShared
+           (top_k > 0 ? rank_cap * 16 + 64 * 8 + 16 : 0);                      // see RowTopShared
 }
 
 // Sum / maximum over the G threads of a row, the same on all of them.
@@ -366,11 +366,12 @@ __device__ __forceinline__ float group_reduce(float v, float* red, int gt) {
 // one warp busy long after the others are done:
 //  (d) the columns are scored from the operands in fp32, those that come closer to another than that is exact in fp64;
 //  (e) every column counts who comes before it.
-// Crowds (many equal scores: a row of zeros, repeated table rows) do not fit (b) and are taken chunk by chunk instead.
+// Crowds (many scores that are equal or nearly so: a row of zeros, repeated table rows) do not fit (b) or (c) and are taken
+// chunk by chunk instead.
 static constexpr int VOCAB_LIST = 64;              // chunks collected in (b)
-// Columns scored in (d): all candidates where a block has one row or the table is small; else K chunks of which a few as a
-// whole, and shared memory for more warps (a row in a million has more, from 32768 columns).
-static int vocab_rank_cap(int list_cap, int top_k, bool all) { return all ? list_cap : 128 + 4 * top_k; }
+// Columns scored in (d), a multiple of 4: K whole chunks and a few where a block has one row or the table is small; else K
+// chunks of which a few as a whole, and shared memory for more warps (a row in a million has more, from 32768 columns).
+__host__ __device__ constexpr int vocab_rank_cap(int top_k, bool all) { return all ? 32 * top_k + 64 : 128 + 4 * top_k; }
 
 struct RowTopShared {
     double* z;                                     // [rank_cap] scores
@@ -378,40 +379,8 @@ struct RowTopShared {
     float* value;                                  // [VOCAB_LIST]
     int* again;                                    // [rank_cap] which columns to score again
     int* count;                                    // [4]: chunks collected, columns, columns again
-    int* list;                                     // [list_cap] columns to score
+    int* list;                                     // [rank_cap] columns to score
 };
-
-// Serial form of (a) to (c) for crowds, by one warp: takes the first chunks one after the other.  Returns how many.
-__device__ __forceinline__ int row_top_crowd(const VocabRows& p, const float* cmax, float slack, int lane, int* sel, float& theta) {
-    auto rescan = [&](float tv, int tc, float& bv, int& bc) {
-        bv = -INFINITY; bc = 0x7fffffff;
-#pragma unroll 8
-        for (int c = lane; c < p.chunks; c += 32) {
-            const float v = cmax[c];
-            if (comes_first(tv, tc, v, c) && comes_first(v, c, bv, bc)) { bv = v; bc = c; }
-        }
-    };
-    float bv; int bc;
-    rescan(INFINITY, -1, bv, bc);
-    int taken = 0;
-    theta = -INFINITY;
-    while (taken < VOCAB_LIST) {
-        float v = bv; int c = bc;
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, v, o);
-            const int oc = __shfl_xor_sync(0xffffffffu, c, o);
-            if (comes_first(ov, oc, v, c)) { v = ov; c = oc; }
-        }
-        if (c == 0x7fffffff) break;                                      // no chunk left
-        if (taken >= p.top_k && !(v >= theta - slack)) break;
-        if (lane == 0) sel[taken] = c;
-        if (bc == c) rescan(v, c, bv, bc);
-        if (++taken == p.top_k) theta = v;
-    }
-    __syncwarp();
-    return taken;
-}
 
 __device__ __forceinline__ RowTopShared row_top_shared(uint8_t* smem, int rank_cap) {
     RowTopShared sh;
@@ -454,11 +423,72 @@ __device__ __forceinline__ void row_top_write(const VocabRows& p, long long row,
     p.top_log_probs[row * p.top_k + at] = (float)(vocab_lp2(p, z, m, r, log2l) * 0.6931471805599453);
 }
 
-// (a) to (c): leaves the columns in sh.list, their number in sh.count[1] (0 after a crowd, which is finished here) and
-// 2 |x| |y| in red[3].
+// A crowd, by the warps of its row: of the chunks that reach red[0] every column that the tile pass cannot rule out is scored in
+// fp64 and inserted into the K best so far, whose last one rules out more as it grows.  However many columns are close to one
+// another, all are looked at; of equal scores the first K are (a row of zeros, where the pass is exact, reads the maxima and
+// scores a chunk a warp).  Bound by the latency of the table's rows, four at a time per warp: K = 8 from a table whose rows are
+// all equal, 1 x 32768 x 1024 3.7 ms, 4096 rows 50 ms (a quarter of the features zero 0.32 ms; no crowd 0.30).
 template <int G, typename T>
-__device__ __forceinline__ void row_top_select(const VocabRows& p, long long row, int gt, const RowTopShared& sh, float m,
-                                               float r, float log2l, float* red) {
+__device__ __forceinline__ void row_top_crowd(const VocabRows& p, long long row, int gt, const RowTopShared& sh, float m, float r,
+                                              float log2l, const float* red) {
+    constexpr int W = G / 32;
+    constexpr int NONE = 0x7fffffff;
+    const int lane = gt & 31, w = gt >> 5, K = p.top_k;
+    const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
+    const T* y = reinterpret_cast<const T*>(p.y);
+    const float* cmax = p.chunk_max + row * p.chunk_ld;
+    const uint32_t* csec = p.chunk_second + row * p.chunk_ld;
+    const float floor_v = red[0], slack = red[1];
+    double lz = -INFINITY, kth = -INFINITY;
+    int lj = NONE;
+    float ruled_out = -INFINITY;                   // a score of the tile pass up to here is not among the K
+    for (int c0 = w * 32; c0 < p.chunks; c0 += W * 32) {
+        const float v = c0 + lane < p.chunks ? cmax[c0 + lane] : -INFINITY;
+        unsigned who = __ballot_sync(0xffffffffu, c0 + lane < p.chunks && v >= floor_v && v > ruled_out);
+        for (; who != 0; who &= who - 1) {
+            const int src = __ffs(who) - 1, c = c0 + src;
+            const float vc = __shfl_sync(0xffffffffu, v, src);
+            if (!(vc > ruled_out)) continue;
+            const uint32_t sec = csec[c];
+            const float second = vc - __uint_as_float(sec & ~31u);           // NaN: there is none
+            const bool whole = second >= floor_v && second > ruled_out;
+            const int first = c * 32 + (whole ? 0 : (int)(sec & 31u));
+            const int n = whole ? (int)min(32ll, p.vocab - first) : 1;
+            for (int i = 0; i < n; i += 4) {
+                const T* r4[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) r4[q] = y + (long long)(first + min(i + q, n - 1)) * p.ldy;
+                const T* const rr[4] = {r4[0], r4[1], r4[2], r4[3]};
+                double z[4];
+                warp_dot4<T, double>(x, rr, p.d, lane, z);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (i + q < n && z[q] > kth) {  // a later column has a higher index: equal is not enough
+                        list_insert(lz, lj, z[q], first + i + q, lane);
+                        kth = __shfl_sync(0xffffffffu, lz, K - 1);
+                    }
+            }
+            ruled_out = (float)(kth * (double)p.fmul) - slack;
+        }
+    }
+    if (W > 1) {                                   // the first warp takes in the others' lists
+        if (lane < K) { sh.z[w * K + lane] = lz; sh.list[w * K + lane] = lj; }
+        __syncthreads();
+        if (w > 0) return;
+        for (int i = K; i < W * K; ++i) {
+            const double z = sh.z[i];
+            const int j = sh.list[i];
+            if (j != NONE) list_insert(lz, lj, z, j, lane);
+        }
+    }
+    if (lane >= K) return;
+    if (lj != NONE) row_top_write(p, row, lane, lz, lj, m, r, log2l);
+    else { p.top_tokens[row * K + lane] = -1; p.top_log_probs[row * K + lane] = NAN; }     // scores that are not numbers
+}
+
+// (a) to (c): leaves the columns in sh.list, their number in sh.count[1] (-1 for a crowd) and 2 |x| |y| in red[3].
+template <int G, typename T>
+__device__ __forceinline__ void row_top_select(const VocabRows& p, long long row, int gt, const RowTopShared& sh, float* red) {
     constexpr int W = G / 32;
     const int lane = gt & 31, w = gt >> 5;
     const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
@@ -533,7 +563,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
     group_sync<G>();
     // (c)
     if (w == 0) {
-        int taken = sh.count[0];
+        const int taken = sh.count[0];
         float theta = -INFINITY;
         if (taken <= VOCAB_LIST) {
             for (int i = lane; i < taken; i += 32) {
@@ -568,7 +598,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                     if (lane >= o) upto += t;
                 }
                 const int all = __shfl_sync(0xffffffffu, upto, 31);
-                if (n + all > min(p.list_cap, p.rank_cap)) { crowd = true; break; }
+                if (n + all > p.rank_cap) { crowd = true; break; }
                 const int at = n + upto - size;
                 if (size == 1) sh.list[at] = c * 32 + best;
                 for (unsigned big = __ballot_sync(0xffffffffu, size > 1); big != 0; big &= big - 1) {
@@ -580,46 +610,7 @@ __device__ __forceinline__ void row_top_select(const VocabRows& p, long long row
                 n += all;
             }
         }
-        if (crowd) {
-            __syncwarp();
-            taken = row_top_crowd(p, cmax, slack, lane, sh.chunk, theta);
-            n = 0;
-            for (int i = 0; i < taken; ++i) {
-                const int c = sh.chunk[i];
-                const float v = cmax[c];
-                const uint32_t sec = csec[c];
-                const bool whole = v - __uint_as_float(sec & ~31u) >= theta - slack;
-                if (!(v >= theta - slack)) continue;
-                if (n + (whole ? 32 : 1) > p.list_cap) break;
-                if (whole) {
-                    const int left = (int)min(32ll, p.vocab - (long long)c * 32);
-                    if (lane < left) sh.list[n + lane] = c * 32 + lane;
-                    n += left;
-                } else {
-                    if (lane == 0) sh.list[n] = c * 32 + (int)(sec & 31u);
-                    ++n;
-                }
-            }
-        }
-        if (n > p.rank_cap) {
-            // sorted insertion, in fp64 from the start
-            double lz = -INFINITY;
-            long long lj = 0x7fffffffffffffffll;
-            for (int i = 0; i < n; i += 4) {
-                long long j4[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) j4[r] = sh.list[min(i + r, n - 1)];
-                const T* const r4[4] = {y + j4[0] * p.ldy, y + j4[1] * p.ldy, y + j4[2] * p.ldy, y + j4[3] * p.ldy};
-                double z[4];
-                warp_dot4<T, double>(x, r4, p.d, lane, z);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (i + r < n) list_insert(lz, lj, z[r], j4[r], lane);
-            }
-            if (lane < K) row_top_write(p, row, lane, lz, lj, m, r, log2l);
-            n = -1;
-        }
-        if (lane == 0) { sh.count[1] = n; sh.count[2] = 0; }
+        if (lane == 0) { sh.count[1] = crowd ? -1 : n; sh.count[2] = 0; }
     }
 }
 
@@ -738,7 +729,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     const long long row = (long long)blockIdx.x * (VOCAB_THREADS / G) + threadIdx.x / G;
     const bool active = row < p.rows;             // the same for the row's threads
     if (!TOP && !DISTILL && !active) return;      // (a block of G = 256 has one row, warps of G = 32 do not meet)
-    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap);
+    uint8_t* smem = smem_all + (size_t)(threadIdx.x / G) * vocab_row_smem(p.k, p.top_k, p.rank_cap);
     float* red = reinterpret_cast<float*>(smem);
     float* z_of = reinterpret_cast<float*>(smem + 64 * 8);
     uint8_t* top_smem = smem + 64 * 8 + (p.k * 4 + 15) / 16 * 16;
@@ -858,10 +849,10 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
     if (DISTILL && p.loss != nullptr) distill_reduce(p);
     if (TOP) {
         const RowTopShared sh = row_top_shared(top_smem, p.rank_cap);
-        const int stride = vocab_row_smem(p.k, p.top_k, p.list_cap, p.rank_cap), bw = threadIdx.x >> 5;
+        const int stride = vocab_row_smem(p.k, p.top_k, p.rank_cap), bw = threadIdx.x >> 5;
         uint8_t* top_base = smem_all + (top_smem - smem);
         group_sync<G>();
-        if (active) row_top_select<G, T>(p, row, gt, sh, m, r, log2l, red);
+        if (active) row_top_select<G, T>(p, row, gt, sh, red);
         else if (gt == 0) sh.count[1] = sh.count[2] = 0;
         __syncthreads();
         rows_top_score<G, T, float>(p, top_base, stride, bw, lane);
@@ -885,7 +876,8 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
         __syncthreads();
         rows_top_score<G, T, double>(p, top_base, stride, bw, lane);
         __syncthreads();
-        if (!active || n < 0) return;
+        if (!active) return;
+        if (n < 0) { row_top_crowd<G, T>(p, row, gt, sh, m, r, log2l, red); return; }
         for (int i = gt; i < n; i += G) {
             bool ignored;
             const int place = row_top_rank(sh, n, i, 0.0, ignored);

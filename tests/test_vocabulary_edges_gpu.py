@@ -107,3 +107,51 @@ def test_forward_mode_derivatives_are_refused(dtype):
                 for a, b in zip(token_log_probs(x, table, tokens, top_k=2), want[0]):
                     assert torch.equal(a, b)
                 assert torch.equal(embed_tokens(tokens, table), want[1])
+
+
+def _near_ties(n, v, members, seed):
+    """Features and a table of whole numbers (every product and sum is exact in 64 bits): the rows of `members` score the same
+    but for steps of 2^-26, far below what an fp32 sum of this size holds, in a random order; all others score far less."""
+    g = torch.Generator().manual_seed(seed)
+    d = 64
+    table = torch.zeros(v, d)
+    x = torch.zeros(n, d)
+    x[:, :40] = torch.randint(4, 12, (n, 40), generator=g).float()
+    place = torch.randperm(len(members), generator=g)
+    table[members, :40] = 8.0
+    table[members, 40], table[members, 41] = (place // 64).float(), (place % 64).float()
+    x[:, 40], x[:, 41] = 2.0 ** -20, 2.0 ** -26
+    return x.bfloat16(), table.bfloat16()
+
+
+@pytest.mark.parametrize("top_k", [1, 2, 8, 32])
+@pytest.mark.parametrize("n", [1, 2, 40, 400])
+@pytest.mark.parametrize("which", ["all", "two of a chunk in few chunks", "two of a chunk in all chunks", "the last chunks"])
+def test_near_ties_in_many_chunks(n, top_k, which):
+    """The order is that of exact scores, however many columns are closer than the tile pass can tell apart."""
+    from memoryefficientclip_b200 import token_log_probs
+    v = 4001
+    every = torch.arange(v)
+    members = {"all": every, "two of a chunk in few chunks": every[(every % 32 < 2) & (every // 32 % 16 == 5)],
+               "two of a chunk in all chunks": every[every % 32 < 2], "the last chunks": every[v - 100:]}[which]
+    x, table = _near_ties(n, v, members, top_k + n)
+    if len(members) < top_k:
+        pytest.skip("fewer of them than alternatives")
+    z = x.double() @ table.double().T
+    want = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top_k]
+    got = token_log_probs(x.cuda(), table.cuda(), want[:, 0].contiguous().cuda(), top_k=top_k)
+    assert torch.equal(got.top_tokens.cpu(), want)
+    lp = torch.log_softmax(z, 1).gather(1, want)
+    _z, err = oracle.scores(x, table, 1.0)
+    _inside(got.top_log_probs, lp, 2 * err[:, None], "top_log_probs")
+
+
+def test_crowds_of_equal_scores_stay_cheap():
+    """Rows of zeros tie everywhere: the first tokens win, and the row does not look at every column to find that out."""
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, _g = _pair(700, 20000, 128, torch.bfloat16, 4)
+    x[::3] = 0
+    got = token_log_probs(x.cuda(), table.cuda(), tokens.cuda(), top_k=9)
+    assert torch.equal(got.top_tokens[::3].cpu(), torch.arange(9).expand(234, 9))
+    _inside(got.top_log_probs[::3], torch.full((234, 9), -math.log(20000), dtype=torch.float64),
+            torch.full((), 8 * oracle.ULP * math.log(20000), dtype=torch.float64), "top_log_probs")
