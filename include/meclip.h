@@ -499,11 +499,14 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
  *                           (both NULL: only row_loss is wanted); no row at all: loss 0.
  *   meclip_distill_grad     dz_ij = w_i (p_ij - q_ij), w_i = grad_out (one scalar, or [rows] with grad_per_row) times
  *                           inv_count (NULL: 1).  The teacher gets no gradient.
- * The gradients take the forward's operands.  Coefficients are rounded once: to fp16 scaled by a power of two (a bound on
- * all of them is brought to 2^14, so a coefficient keeps 11 bits down to 2^-28 of the largest), or, for up to 256 rows of
- * bf16 operands, to two bf16 panels (16 bits).  Output modes, blocking and side streams are those of meclip_grad, without
- * atomics on sums; a contraction with few output tiles and a long K is cut along K and its parts added in order.  Either
- * output may be NULL.
+ * The gradients take the forward's operands.  Coefficients are rounded once: to fp16, each row scaled by a power of two of
+ * its own (a bound on the row's coefficients is brought to 2^14, so one keeps 11 bits down to 2^-28 of that bound), or, for
+ * up to 256 rows of bf16 operands, to two bf16 panels (16 bits).  So a row of dx is as exact as if it were alone, and a row
+ * that is not finite shows in that row only.  dtable adds all rows up: one whose part of it is far below the heaviest row's
+ * counts with an error of 2^-39 of the heaviest part, and one that is not finite shows everywhere.  A bf16 table is read as
+ * scaled fp16 beyond 256 rows: what is below 2^-23 of its largest magnitude loses bits.  Output modes, blocking and side
+ * streams are those of meclip_grad, without atomics on sums; a contraction with few output tiles and a long K is cut along
+ * K and its parts added in order.  Either output may be NULL.
  */
 size_t meclip_vocab_workspace_bytes(int64_t rows, int64_t vocab, int top_k);
 size_t meclip_vocab_grad_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t d);

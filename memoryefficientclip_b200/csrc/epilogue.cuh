@@ -369,8 +369,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         bool v_here = false;
         if (VOCAB) {
             if (rvalid) {
-                const float g_scale = pow2(pow2_exponent(p.panel_max, PANEL_TARGET));
                 const float4 f = __ldg(p.row_factors + grow);
+                const float g_scale = pow2(row_exponent(f.w));
                 v_lse = f.x;
                 v_a = f.y * g_scale;
                 v_b = f.z * g_scale;
@@ -543,11 +543,15 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, const OutDesc
         // first 128 B rows of CTA 0 and of CTA 1, the second MMA's columns (from TMEM column 256) the remaining rows
         // of each, so accumulator chunk ch maps to tile columns through the four pieces below.  For tiles of up
         // to 256 columns the map is the identity.
-        const bool scaled = od.scale.panel != nullptr || od.scale.operand != nullptr;
+        const bool scaled = od.scale.rows != nullptr || od.scale.total != nullptr;
         float unscale_g = 1.f, unscale_b = 1.f;
-        if (scaled) {
-            unscale_g = pow2(-pow2_exponent(od.scale.panel, PANEL_TARGET));
+        if (od.scale.rows != nullptr) {
+            if (rvalid) unscale_g = pow2(-row_exponent(__ldg(&od.scale.rows[grow].w)));
             unscale_b = pow2(-pow2_exponent(od.scale.operand, OPERAND_TARGET));
+        } else if (od.scale.total != nullptr) {      // two factors: one could leave fp32's range (below 2^-252 all is zero)
+            const int e = -total_exponent(od.scale.total);
+            unscale_g = pow2(::max(e >> 1, -126));
+            unscale_b = pow2(::max(e - (e >> 1), -126));
         }
         if (p.tile_out) {
             // 32 rows x 128 bytes per warp and store: 64 bf16 or 32 fp32 columns (two or one accumulator chunks).  The map's

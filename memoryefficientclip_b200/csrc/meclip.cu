@@ -1641,17 +1641,29 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
     // deals its tiles in turn instead (nothing shares the GPU with it, and a launch less is a few microseconds)
     const bool use_counters = vg == nullptr || overlap;
     if (use_counters) MECLIP_CUDA(cudaMemsetAsync(counters, 0, plan.counter_bytes, s0));
-    // A vocabulary's panel is fp16 wherever the contractions can read fp16 operands: those of an fp16 problem as they are,
-    // or scaled transposed copies.  An fp16 coefficient is off by 2^-12 on average of a step, a bf16 one by 2^-9.
+    // A vocabulary's panel is fp16 wherever the contractions can read fp16 operands: an fp16 table as it is, scaled transposed
+    // copies of a bf16 one.  An fp16 coefficient is off by 2^-12 on average of a step, a bf16 one by 2^-9.  The features are
+    // scaled copies either way (see OutScale).
     const bool panel_f16 = vg != nullptr && (vg->f16 || transposed_copies);
-    const bool scale_operands = panel_f16 && !vg->f16;
-    const float* panel_max = panel_f16 ? vg->maxima + 2 : nullptr;
+    const bool scale_table = panel_f16 && !vg->f16 && want_dx;
+    const bool scale_features = panel_f16 && want_dy;
+    const uint16_t *xw = reinterpret_cast<const uint16_t*>(X), *yw = reinterpret_cast<const uint16_t*>(Y);
+    const __half* xh = reinterpret_cast<const __half*>(X);
+    const unsigned max_blocks = (unsigned)(4 * sm_count());
     if (vg != nullptr) {
-        if (panel_f16) MECLIP_CUDA(cudaMemsetAsync(vg->maxima, 0, 3 * sizeof(float), s0));
+        if (panel_f16) MECLIP_CUDA(cudaMemsetAsync(vg->total, 0, 2 * sizeof(float), s0));
         const int wpb = ROW_KERNEL_THREADS / 32;
         ScopedTiming timing(s0, TAG_ROW, (double)rows * (48.0 + 12.0 * vg->coef.k));
         vocab_prepare_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s0>>>(
-            vg->coef, rows, vg->row_factors, vg->row_entries, panel_f16 ? vg->maxima + 2 : nullptr);
+            vg->coef, rows, vg->row_factors, vg->row_entries, panel_f16);
+        if (scale_features && !transposed_copies) {
+            {
+                ScopedTiming timing_max(s0, TAG_ROW, 2.0 * (double)rows * (double)d);
+                operand_max_kernel<<<dim3(max_blocks, 1), 256, 0, s0>>>(yw, ldy, cols, xw, ldx, rows, (int)d, 1, vg->f16, vg->row_factors, vg->table_max, vg->total);
+            }
+            ScopedTiming timing_scale(s0, TAG_ROW, 4.0 * (double)rows * (double)d);
+            scale_features_f16_kernel<<<(unsigned)((rows + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s0>>>(xh, ldx, rows, (int)d, vg->row_factors, vg->total, vg->features);
+        }
         MECLIP_CUDA(cudaGetLastError());
     }
     if (transposed_copies) {
@@ -1662,30 +1674,28 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
             if (want_dx) MECLIP_CUDA(cudaStreamWaitEvent(sx, side->fork, 0));
             if (want_dy) MECLIP_CUDA(cudaStreamWaitEvent(sy, side->fork, 0));
         }
-        if (scale_operands) {      // one launch for both when they run on one stream
-            const int both = want_dx && want_dy && sx == sy;
-            const uint16_t *xw = reinterpret_cast<const uint16_t*>(X), *yw = reinterpret_cast<const uint16_t*>(Y);
-            const unsigned blocks = (unsigned)(4 * sm_count());
-            if (want_dx) {
-                ScopedTiming timing(sx, TAG_TRANSPOSE, 2.0 * (double)(cols + (both ? rows : 0)) * (double)d);
-                operand_max_kernel<<<dim3(blocks, both ? 2 : 1), 256, 0, sx>>>(yw, ldy, cols, xw, ldx, rows, (int)d, vg->maxima + 1, vg->maxima);
-            }
-            if (want_dy && !both) {
-                ScopedTiming timing(sy, TAG_TRANSPOSE, 2.0 * (double)rows * (double)d);
-                operand_max_kernel<<<dim3(blocks, 1), 256, 0, sy>>>(xw, ldx, rows, xw, ldx, rows, (int)d, vg->maxima, vg->maxima);
-            }
+        const bool both = scale_table && scale_features && sx == sy;      // one launch for both when they run on one stream
+        if (scale_table) {
+            ScopedTiming timing(sx, TAG_TRANSPOSE, 2.0 * (double)(cols + (both ? rows : 0)) * (double)d);
+            operand_max_kernel<<<dim3(max_blocks, both ? 2 : 1), 256, 0, sx>>>(yw, ldy, cols, xw, ldx, rows, (int)d, 0, vg->f16, vg->row_factors, vg->table_max, vg->total);
+        }
+        if (scale_features && !both) {
+            ScopedTiming timing(sy, TAG_TRANSPOSE, 2.0 * (double)rows * (double)d);
+            operand_max_kernel<<<dim3(max_blocks, 1), 256, 0, sy>>>(yw, ldy, cols, xw, ldx, rows, (int)d, 1, vg->f16, vg->row_factors, vg->table_max, vg->total);
         }
         if (want_dx) {
             ScopedTiming timing(sx, TAG_TRANSPOSE, 4.0 * (double)cols * (double)dn);
             dim3 grid((unsigned)((cols + 63) / 64), (unsigned)((dn + 63) / 64));
-            if (scale_operands) transpose_scaled_f16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, vg->maxima + 1, reinterpret_cast<__half*>(yt), plan.ld_yt);
-            else                transpose_bf16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, yt, plan.ld_yt);
+            if (scale_table) transpose_scaled_f16_kernel<__nv_bfloat16, false><<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, vg->table_max, nullptr, nullptr, reinterpret_cast<__half*>(yt), plan.ld_yt);
+            else             transpose_bf16_kernel<<<grid, 256, 0, sx>>>(Y, ldy, cols, (int)dn, yt, plan.ld_yt);
         }
         if (want_dy) {
             ScopedTiming timing(sy, TAG_TRANSPOSE, 4.0 * (double)rows * (double)d);
             dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((d + 63) / 64));
-            if (scale_operands) transpose_scaled_f16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, vg->maxima, reinterpret_cast<__half*>(xt), plan.ld_xt);
-            else                transpose_bf16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, xt, plan.ld_xt);
+            __half* xt_half = reinterpret_cast<__half*>(xt);
+            if (scale_features && vg->f16) transpose_scaled_f16_kernel<__half, true><<<grid, 256, 0, sy>>>(xh, ldx, rows, (int)d, nullptr, vg->row_factors, vg->total, xt_half, plan.ld_xt);
+            else if (scale_features) transpose_scaled_f16_kernel<__nv_bfloat16, true><<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, nullptr, vg->row_factors, vg->total, xt_half, plan.ld_xt);
+            else transpose_bf16_kernel<<<grid, 256, 0, sy>>>(X, ldx, rows, (int)d, xt, plan.ld_xt);
         }
         MECLIP_CUDA(cudaGetLastError());
     }
@@ -1741,11 +1751,10 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     p.lo_chunk = lo_chunk;
                     if (!use_counters) p.tile_counter = nullptr;
                     p.panel_f16 = panel_f16;
-                    p.panel_max = panel_max;
                     a.f16 = b.f16 = vg->f16;
                     // 256-column tiles beyond one row tile: only those run on CTA pairs
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
-                    if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_max, panel_f16, s0);
+                    if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_f16, s0);
                 } else {
                     rc = launch_gemm(EPI_COEF, a, b, nr, nc, d, pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                 }
@@ -1764,7 +1773,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 GemmParams& p = py;
                 p.status = status;
                 p.lo_chunk = lo_chunk;
-                p.scale = OutScale{panel_max, scale_operands ? vg->maxima : nullptr};
+                if (panel_f16) p.scale.total = vg->total;
                 p.tile_out = vg != nullptr;
                 p.tile_counter = use_counters ? counters + 3 * t + 2 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dy) + (size_t)c0 * lddy * dy_elt;
@@ -1781,6 +1790,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 }
                 if (!use_dual) {
                     Operand a{gpanel[gb], plan.ldg / 64, true, plan.row_block}, b{X + r0 * ldx, ldx, true};
+                    if (scale_features && !transposed_copies) b = Operand{vg->features + r0 * d, d, true};
                     if (transposed_copies) b = Operand{xt + r0, plan.ld_xt, false};   // [d][K = rows] K-major
                     a.f16 = b.f16 = panel_f16;
                     const int bn = vg != nullptr ? split_tile_width(nc, d, nr, overlap, transposed_copies) : pick_contraction_bn(nc, d, overlap, transposed_copies);
@@ -1799,7 +1809,8 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                 std::memset(&p, 0, sizeof(p));
                 p.status = status;
                 p.lo_chunk = lo_chunk;
-                p.scale = OutScale{panel_max, scale_operands ? vg->maxima + 1 : nullptr};
+                if (panel_f16) p.scale.rows = vg->row_factors + r0;
+                if (scale_table) p.scale.operand = vg->table_max;
                 p.tile_out = vg != nullptr;
                 p.tile_counter = use_counters ? counters + 3 * t + 1 : nullptr;
                 uint8_t* user = reinterpret_cast<uint8_t*>(dx) + (size_t)r0 * lddx * dx_elt;

@@ -56,17 +56,33 @@ static constexpr int STORE_BUF_BYTES = 32 * 128;   // one warp's 32 rows x 64 bf
 enum { EPI_SUMS = 0, EPI_COEF = 1, EPI_OUT = 2, EPI_STATS = 3, EPI_VCOEF = 4 };
 __host__ __device__ constexpr bool epi_is_coef(int epi) { return epi == EPI_COEF || epi == EPI_VCOEF; }
 
-// Scaled fp16 operands: a matrix is multiplied by the power of two that brings its largest magnitude to 2^target, so that
-// fp16's 11 bits reach 2^-28 (panel) or 2^-23 (features) of it.  `max` points to that magnitude on the device; null: scale 1.
-static constexpr int PANEL_TARGET = 14, OPERAND_TARGET = 9;
-struct OutScale { const float *panel, *operand; };
+// Scaled fp16 operands, all by powers of two.
+//   Panel: each row by its own 2^e_i, which brings a bound on its coefficients to 2^14, so that 11 bits reach 2^-28 of that
+//     bound whatever other rows weigh.  e_i stands in row_factors[i].w.
+//   Features as operand of the table's gradient: row i by the rest, 2^(28 - M - e_i), so that all rows of the product carry
+//     2^(28 - M); M = max_i (14 - e_i + exponent of row i's largest feature) is what the heaviest row's part of that gradient
+//     comes to, and brings it to 2^14: a row keeps 11 bits down to 2^-28 of the heaviest one's part.
+//   Table: by what brings its largest magnitude, `operand`, to 2^9 (11 bits down to 2^-23 of it).
+// OutScale: what a contraction's result is divided by: `rows` for a gradient of features, `total` (M) for the table's.
+static constexpr int PANEL_TARGET = 14, FEATURE_TARGET = 14, OPERAND_TARGET = 9;
+struct OutScale { const float4* rows; const unsigned int* total; const float* operand; };
 __device__ __forceinline__ int pow2_exponent(const float* max, int target) {
     if (max == nullptr) return 0;
     const int e = (int)((__float_as_uint(__ldg(max)) >> 23) & 255u);
     if (e == 0 || e == 255) return 0;                       // nothing to scale, or not a number anyway
-    return ::min(100, ::max(-100, target - (e - 127)));     // stays a normal fp32 number, and so does its inverse
+    return ::min(126, ::max(-126, target - (e - 127)));     // stays a normal fp32 number, and so does its inverse
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+static constexpr int ROW_EMPTY = 1 << 20;                   // instead of e_i: a row without coefficients
+__device__ __forceinline__ int row_exponent(float w) {
+    const int e = __float_as_int(w);
+    return e == ROW_EMPTY ? 0 : e;
+}
+static constexpr unsigned int TOTAL_BIAS = 1024;            // M is kept as an unsigned number; 0: no row has a part
+__device__ __forceinline__ int total_exponent(const unsigned int* total) {      // 28 - M
+    const unsigned int m = __ldg(total);
+    return m == 0 ? 0 : PANEL_TARGET + FEATURE_TARGET - (int)(m - TOTAL_BIAS);
+}
 
 static constexpr int VOCAB_TILE_ENTRIES = 2;       // entries of a row that the tile pass adds itself (GemmParams::row_entries)
 
@@ -168,7 +184,7 @@ struct GemmParams {
     float* chunk_max;
     uint32_t* chunk_second;
     long long chunk_ld;
-    // EPI_VCOEF: u = S fmul - lse_i = log2 p_ij, G_ij = 2^u (a_i + b_i u); row_factors = {lse, a, b, 0}.  row_entries (null:
+    // EPI_VCOEF: u = S fmul - lse_i = log2 p_ij, G_ij = 2^u (a_i + b_i u); row_factors = {lse, a, b, e}.  row_entries (null:
     // another kernel stores them) = up to two {column in the table as int bits or -1, coefficient} that replace the dense ones.
     const float4* row_factors;
     const float4* row_entries;
@@ -176,10 +192,8 @@ struct GemmParams {
     // A second panel with what the bf16 rounding of the first one left, lo_chunk 64-column chunks behind it (0: none).
     // EPI_VCOEF writes it; a contraction (single-CTA kernel) then walks K twice, from step k_half on over the second panel.
     int lo_chunk, k_half;
-    // fp16 panels: EPI_VCOEF multiplies by the power of two that brings *panel_max (a bound on |G|) to 2^PANEL_TARGET
-    int panel_f16;
-    const float* panel_max;
-    // Contractions of scaled fp16 operands: the result is divided by the scales of the panel and of B (see OutScale)
+    int panel_f16;            // fp16 panel, its rows multiplied by 2^e; else bf16, e = 0
+    // Contractions of scaled fp16 operands: the result is divided by the scales of both
     OutScale scale, scale2;
 };
 

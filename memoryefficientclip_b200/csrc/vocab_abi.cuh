@@ -181,11 +181,11 @@ static constexpr long long VOCAB_TWO_PANEL_ROWS = 256;
 static constexpr long long VOCAB_OVERLAP_ROWS = 1024;
 
 struct VocabGradPlan {
-    size_t rows_bytes, split_bytes, grad_bytes;
+    size_t rows_bytes, features_bytes, split_bytes, grad_bytes;
     long long widest;
     int split_bufs;
     bool transposed, two_panels, overlap;
-    size_t total() const { return rows_bytes + 256 + split_bufs * split_bytes + grad_bytes; }
+    size_t total() const { return rows_bytes + 256 + features_bytes + split_bufs * split_bytes + grad_bytes; }
 };
 static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab, long long d) {
     VocabGradPlan g;
@@ -193,6 +193,7 @@ static VocabGradPlan plan_vocab_grad(int dtype, long long rows, long long vocab,
     g.rows_bytes = round_up((size_t)rows * 2 * sizeof(float4), 256);
     g.overlap = rows >= VOCAB_OVERLAP_ROWS;
     g.transposed = transposes_allowed() && (f16 ? g.overlap : rows > VOCAB_TWO_PANEL_ROWS);
+    g.features_bytes = f16 && !g.transposed ? round_up((size_t)rows * d * 2, 256) : 0;
     // The rounding of a coefficient to bf16 (2^-9 on average) does not average out where a row's gradient is carried by one
     // coefficient: its whole gradient is off by that much, as much as the output's own rounding.
     g.two_panels = !f16 && !g.transposed;
@@ -222,8 +223,10 @@ static int vocab_grad(const VocabCoef& coef, int dtype, const void* x, const voi
     vg.tile_fmul = vocab_tile_fmul(temperature, d);
     vg.two_panels = plan.two_panels;
     vg.widest = plan.widest;
-    vg.maxima = reinterpret_cast<float*>(ws + plan.rows_bytes);
-    uint8_t* split = ws + plan.rows_bytes + 256;
+    vg.total = reinterpret_cast<unsigned int*>(ws + plan.rows_bytes);
+    vg.table_max = reinterpret_cast<float*>(vg.total + 1);
+    vg.features = reinterpret_cast<__half*>(ws + plan.rows_bytes + 256);
+    uint8_t* split = ws + plan.rows_bytes + 256 + plan.features_bytes;
     vg.split_buf = reinterpret_cast<float*>(split);
     vg.split_buf2 = reinterpret_cast<float*>(split + (plan.split_bufs > 1 ? plan.split_bytes : 0));
     vg.split_bytes = plan.split_bytes;

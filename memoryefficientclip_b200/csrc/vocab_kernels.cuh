@@ -57,7 +57,9 @@ struct VocabGrad {
     float tile_fmul;
     long long widest;                 // columns of a coefficient panel at most
     int two_panels;                   // bf16 panel and a second one with its remainders
-    float* maxima;                    // [3]: largest magnitudes of x and table, bound on the coefficients; cleared by grad_impl
+    unsigned int* total;              // see OutScale; it and table_max behind it are cleared by grad_impl
+    float* table_max;
+    __half* features;                 // [rows, d] scaled features where no transposed copies are made of an fp16 problem
     float *split_buf, *split_buf2;    // parts of contractions that are cut along K: dX's own when both run at a time
     size_t split_bytes;               // of each
 };
@@ -889,99 +891,124 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
 }
 
 // Row factors and, for rows of few entries, their coefficients, so that a tile pass loads two vectors per row; one warp per
-// row.  Also a bound on all coefficients' magnitude, |a| + 0.5308 |b| + sum |terms| (p |log2 p| <= log2(e) / e), as the
-// maximum of non-negative floats' bits: the order of the atomics does not matter.  Bound by latency: 7 us at 2047 rows.
+// row.  With `scale` also the row's exponent (see OutScale), from a bound on its coefficients' magnitude, |a| + 0.5308 |b| +
+// sum |terms| (p |log2 p| <= log2(e) / e).  Bound by latency: 7 us at 2047 rows.
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
 vocab_prepare_kernel(const __grid_constant__ VocabCoef v, long long rows, float4* __restrict__ factors,
-                     float4* __restrict__ entries, float* __restrict__ bound) {
-    __shared__ float most[ROW_KERNEL_THREADS / 32];
+                     float4* __restrict__ entries, int scale) {
     const long long row = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    float m = 0.f;
-    if (row < rows) {
-        float a, b = 0.f;
-        if (v.distill) {
-            a = v.row_has[row] > 0.f ? v.grad_out[v.grad_per_row ? row : 0] * (v.factor != nullptr ? __ldg(v.factor) : 1.f) * v.inv_t : 0.f;
-            m = 2.f * fabsf(a);                                  // sum q <= 1
-        } else {
-            float g = 0.f, size = 0.f;
-            if (v.grad_log_probs != nullptr)
-                for (int e = lane; e < v.k; e += 32) {
-                    const long long j = v.tokens[row * v.k + e];
-                    if (j >= 0 && j < v.vocab) { const float x = v.grad_log_probs[row * v.k + e]; g += x; size += fabsf(x); }
-                }
-            g = warp_sum(g);
-            size = warp_sum(size);
-            const float h = v.grad_entropy != nullptr ? v.grad_entropy[row] : 0.f;
-            a = -(g + (h != 0.f ? h * v.entropy[row] : 0.f)) * v.inv_t;      // h = 0 takes no part, whatever the entropy is
-            b = -h * 0.6931471805599453f * v.inv_t;
-            m = fabsf(a) + 0.5308f * fabsf(b) + size * v.inv_t;
-        }
-        if (lane == 0) factors[row] = make_float4(v.row_lse[row], a, b, 0.f);
-        if (entries != nullptr && lane < VOCAB_TILE_ENTRIES) {
-            float value = 0.f;
-            int col = -1;
-            if (lane < v.k) {
-                const long long j = v.tokens[row * v.k + lane];
-                if (j >= 0 && j < v.vocab && vocab_entry(v, row, lane, a, b, value)) col = (int)j;
+    if (row >= rows) return;
+    float m, a, b = 0.f;
+    if (v.distill) {
+        a = v.row_has[row] > 0.f ? v.grad_out[v.grad_per_row ? row : 0] * (v.factor != nullptr ? __ldg(v.factor) : 1.f) * v.inv_t : 0.f;
+        m = 2.f * fabsf(a);                                  // sum q <= 1
+    } else {
+        float g = 0.f, size = 0.f;
+        if (v.grad_log_probs != nullptr)
+            for (int e = lane; e < v.k; e += 32) {
+                const long long j = v.tokens[row * v.k + e];
+                if (j >= 0 && j < v.vocab) { const float x = v.grad_log_probs[row * v.k + e]; g += x; size += fabsf(x); }
             }
-            reinterpret_cast<float2*>(entries + row)[lane] = make_float2(__int_as_float(col), value);
-        }
+        g = warp_sum(g);
+        size = warp_sum(size);
+        const float h = v.grad_entropy != nullptr ? v.grad_entropy[row] : 0.f;
+        a = -(g + (h != 0.f ? h * v.entropy[row] : 0.f)) * v.inv_t;      // h = 0 takes no part, whatever the entropy is
+        b = -h * 0.6931471805599453f * v.inv_t;
+        m = fabsf(a) + 0.5308f * fabsf(b) + size * v.inv_t;
     }
-    if (bound == nullptr) return;
-    if (lane == 0) most[threadIdx.x >> 5] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < ROW_KERNEL_THREADS / 32; ++i) m = fmaxf(m, most[i]);
-        atomicMax(reinterpret_cast<unsigned int*>(bound), __float_as_uint(m));
+    if (lane == 0) {
+        int e = 0;                               // also where the bound is no number: the row's coefficients are none either
+        if (scale && m == 0.f) e = ROW_EMPTY;
+        else if (scale && m < INFINITY) e = min(126, PANEL_TARGET + 127 - (int)(__float_as_uint(m) >> 23));   // (subnormal: 126)
+        factors[row] = make_float4(v.row_lse[row], a, b, __int_as_float(e));
+    }
+    if (entries != nullptr && lane < VOCAB_TILE_ENTRIES) {
+        float value = 0.f;
+        int col = -1;
+        if (lane < v.k) {
+            const long long j = v.tokens[row * v.k + lane];
+            if (j >= 0 && j < v.vocab && vocab_entry(v, row, lane, a, b, value)) col = (int)j;
+        }
+        reinterpret_cast<float2*>(entries + row)[lane] = make_float2(__int_as_float(col), value);
     }
 }
 
-// Largest magnitude of a bf16 matrix (blockIdx.y = 0) and of a second one (1): the integer maximum of bits without the sign.
-// Bound by HBM; it and the transposition after it read the matrix from L2 the second time (32001 x 512: 15 us each).
+__device__ __forceinline__ unsigned int max_bits8(const uint16_t* p, unsigned int best) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+    return __vmaxu2(best, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+}
+
+// Largest magnitude of a bf16 table, the integer maximum of bits without the sign (blockIdx.y + first = 0), and the heaviest
+// row's part M of the table's gradient (1; see OutScale): maxima, so the order of the atomics does not matter.
+// Bound by HBM; it and the transposition after it read the matrices from L2 the second time (34048 x 512: 15 us each).
 __global__ void __launch_bounds__(256)
-operand_max_kernel(const uint16_t* __restrict__ m0, long long ld0, long long rows0, const uint16_t* __restrict__ m1, long long ld1,
-                   long long rows1, int d, float* __restrict__ max0, float* __restrict__ max1) {
-    const uint16_t* m = blockIdx.y == 0 ? m0 : m1;
-    const long long ld = blockIdx.y == 0 ? ld0 : ld1, rows = blockIdx.y == 0 ? rows0 : rows1;
+operand_max_kernel(const uint16_t* __restrict__ table, long long ldt, long long vocab, const uint16_t* __restrict__ x, long long ldx,
+                   long long rows, int d, int first, int f16, const float4* __restrict__ factors, float* __restrict__ table_max,
+                   unsigned int* __restrict__ total) {
+    const int lane = threadIdx.x & 31;
+    if (blockIdx.y + first == 1) {
+        unsigned int most = 0;
+        for (long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (long long)gridDim.x * 8) {
+            unsigned int best = 0;
+#pragma unroll 4
+            for (int c = lane * 8; c < d; c += 256) best = max_bits8(x + r * ldx + c, best);
+            const unsigned int top = __reduce_max_sync(0xffffffffu, max(best & 0xffffu, best >> 16));
+            const int e = __float_as_int(__ldg(&factors[r].w));
+            const float size = f16 ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16);
+            if (e != ROW_EMPTY && size > 0.f && size < INFINITY)
+                most = max(most, (unsigned int)(PANEL_TARGET - e + max((int)(__float_as_uint(size) >> 23), 1) - 127) + TOTAL_BIAS);
+        }
+        if (lane == 0 && most != 0) atomicMax(total, most);
+        return;
+    }
     // rows that follow one another are one long row
-    const long long per_row = ld == d ? rows * d / 8 : d / 8, lines = ld == d ? 1 : rows;
+    const long long per_row = ldt == d ? vocab * d / 8 : d / 8, lines = ldt == d ? 1 : vocab;
     const long long all = lines * per_row, step = (long long)gridDim.x * 256;
     unsigned int best = 0;
 #pragma unroll 8
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
-        const long long at = lines == 1 ? i * 8 : i / per_row * ld + i % per_row * 8;
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(m + at));
-        best = __vmaxu2(best, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
-    }
-    unsigned int top = max(best & 0xffffu, best >> 16) << 16;    // as fp32 bits
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0 && top != 0) atomicMax(reinterpret_cast<unsigned int*>(blockIdx.y == 0 ? max0 : max1), top);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += step)
+        best = max_bits8(table + (lines == 1 ? i * 8 : i / per_row * ldt + i % per_row * 8), best);
+    const unsigned int top = __reduce_max_sync(0xffffffffu, max(best & 0xffffu, best >> 16)) << 16;      // as fp32 bits
+    if (lane == 0 && top != 0) atomicMax(reinterpret_cast<unsigned int*>(table_max), top);
+}
+
+// The two factors that row r of the features is multiplied by (one could leave fp32's range).
+struct FeatureScale { float f, g; };
+__device__ __forceinline__ FeatureScale feature_scale(const float4* factors, const unsigned int* total, long long r) {
+    const int e = __float_as_int(__ldg(&factors[r].w));
+    if (e == ROW_EMPTY) return FeatureScale{0.f, 0.f};       // its coefficients are zero: any finite number will do
+    const int t = max(-200, min(200, total_exponent(total) - e));         // (below -200 all is zero in fp16, above all was zero)
+    return FeatureScale{pow2(t >> 1), pow2(t - (t >> 1))};
 }
 
 // out[c][r] = in[r][c] scaled, as fp16: transpose_bf16_kernel (same tiles, same shared-memory layout) with a conversion.
-// bf16's 8 bits fit fp16's 11; what is below 2^-23 of the largest magnitude loses bits.
+// FEATURES: rows of features, each by its own factor; else a table, by one.  bf16's 8 bits fit fp16's 11; what is far below
+// the largest magnitude loses bits (see OutScale).
+template <typename T, bool FEATURES>
 __global__ void __launch_bounds__(256)
-transpose_scaled_f16_kernel(const __nv_bfloat16* __restrict__ in, long long ld_in, long long rows, int cols,
-                            const float* __restrict__ largest, __half* __restrict__ out, long long ld_out) {
+transpose_scaled_f16_kernel(const T* __restrict__ in, long long ld_in, long long rows, int cols, const float* __restrict__ largest,
+                            const float4* __restrict__ factors, const unsigned int* __restrict__ total,
+                            __half* __restrict__ out, long long ld_out) {
     __shared__ __align__(16) uint32_t tile[64][32];
     const long long r0 = (long long)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64;
     const int t = threadIdx.x;
-    const float scale = pow2(pow2_exponent(largest, OPERAND_TARGET));
     {
         const int k = t & 7, rp = t >> 3;
         const long long r = r0 + 2 * rp;
         const int c = c0 + 8 * k;
         float a[8] = {}, b[8] = {};
+        FeatureScale sa = {1.f, 1.f}, sb = {1.f, 1.f};
+        if (!FEATURES) sa.f = sb.f = pow2(pow2_exponent(largest, OPERAND_TARGET));
         if (c < cols) {
-            if (r < rows) load8(in + r * ld_in + c, a);
-            if (r + 1 < rows) load8(in + (r + 1) * ld_in + c, b);
+            if (r < rows) { load8(in + r * ld_in + c, a); if (FEATURES) sa = feature_scale(factors, total, r); }
+            if (r + 1 < rows) { load8(in + (r + 1) * ld_in + c, b); if (FEATURES) sb = feature_scale(factors, total, r + 1); }
         }
         const int pw = rp ^ (k << 2);
 #pragma unroll
-        for (int m = 0; m < 8; ++m) tile[8 * k + m][pw] = pack_f16x2(a[m] * scale, b[m] * scale);
+        for (int m = 0; m < 8; ++m)
+            tile[8 * k + m][pw] = FEATURES ? pack_f16x2(a[m] * sa.f * sa.g, b[m] * sb.f * sb.g) : pack_f16x2(a[m] * sa.f, b[m] * sb.f);
     }
     __syncthreads();
 #pragma unroll
@@ -994,17 +1021,34 @@ transpose_scaled_f16_kernel(const __nv_bfloat16* __restrict__ in, long long ld_i
     }
 }
 
+// The same without the transposition, for an fp16 problem whose contractions read the operands as they lie: [rows, d].
+__global__ void __launch_bounds__(ROW_KERNEL_THREADS)
+scale_features_f16_kernel(const __half* __restrict__ in, long long ld_in, long long rows, int d, const float4* __restrict__ factors,
+                          const unsigned int* __restrict__ total, __half* __restrict__ out) {
+    const long long row = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const FeatureScale s = feature_scale(factors, total, row);
+    for (int c = (threadIdx.x & 31) * 8; c < d; c += 256) {
+        float v[8];
+        load8(in + row * ld_in + c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * s.f * s.g;
+        *reinterpret_cast<uint4*>(out + row * d + c) =
+            make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
+    }
+}
+
 // Puts the entries' own terms into a coefficient panel: formed in fp32 from the saved log probabilities and rounded once,
 // over what the tile pass stored there.  One warp per row.
 __global__ void __launch_bounds__(ROW_KERNEL_THREADS)
 vocab_entries_kernel(const __grid_constant__ VocabCoef v, const float4* __restrict__ factors, long long r0, long long nr,
                      long long c0, long long nc, __nv_bfloat16* __restrict__ panel, long long rows_alloc, int lo_chunk,
-                     const float* __restrict__ panel_max, int f16) {
+                     int f16) {
     const long long i = (long long)blockIdx.x * (ROW_KERNEL_THREADS / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (i >= nr) return;
     const float4 f = factors[r0 + i];
-    const float g_scale = pow2(pow2_exponent(panel_max, PANEL_TARGET));
+    const float g_scale = pow2(row_exponent(f.w));
     for (int e = lane; e < v.k; e += 32) {
         const long long j = v.tokens[(r0 + i) * v.k + e];
         if (j < c0 || j >= c0 + nc) continue;          // absent, outside the table or in another panel
@@ -1022,13 +1066,13 @@ vocab_entries_kernel(const __grid_constant__ VocabCoef v, const float4* __restri
 }
 
 static int launch_vocab_entries(const VocabGrad& g, long long r0, long long nr, long long c0, long long nc, __nv_bfloat16* panel,
-                                long long rows_alloc, int lo_chunk, const float* panel_max, int f16, cudaStream_t s) {
+                                long long rows_alloc, int lo_chunk, int f16, cudaStream_t s) {
     const VocabCoef& v = g.coef;
     if (v.k == 0 || g.row_entries != nullptr || (!v.distill && v.grad_log_probs == nullptr)) return MECLIP_OK;
     const int wpb = ROW_KERNEL_THREADS / 32;
     ScopedTiming timing(s, TAG_ROW, (double)nr * v.k * 18.0);
     vocab_entries_kernel<<<(unsigned)((nr + wpb - 1) / wpb), ROW_KERNEL_THREADS, 0, s>>>(
-        v, g.row_factors, r0, nr, c0, nc, panel, rows_alloc, lo_chunk, panel_max, f16);
+        v, g.row_factors, r0, nr, c0, nc, panel, rows_alloc, lo_chunk, f16);
     MECLIP_CUDA(cudaGetLastError());
     return MECLIP_OK;
 }

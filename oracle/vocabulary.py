@@ -6,9 +6,9 @@ Bounds count the roundings of the computation, for operands that are exact:
              of a partial sum that stays below |x_i| |y_j|; scale and exponent add a few ulps of the score itself
   p, log p   the error of the scores, plus that of summing V exponentials (a few ulps: the partial sums are positive)
   entropy    sum_j p_j |log p_j + H| <= 2 ln V times the error of the scores
-  gradients  every coefficient is rounded once to fp16 that is scaled so that a bound on all of them comes to 2^14 (half
-             a step, 2^-11 relative, or half of fp16's smallest, 2^-25, over the scale: 2^-39 of that bound) or to two
-             bf16 numbers (less); it carries the error of its p, and the contraction drops up to 2^-23 of a partial sum
+  gradients  every coefficient is rounded once to fp16, its row scaled so that a bound on its coefficients comes to 2^14
+             (half a step, 2^-11 relative, or half of fp16's smallest, 2^-25, over the scale: 2^-39 of that bound, for
+             which the largest of all rows' bounds stands here) or to two bf16 numbers (less); it carries the error of its p, and the contraction drops up to 2^-23 of a partial sum
              every 16 terms; then one rounding to the output's type
 """
 import torch

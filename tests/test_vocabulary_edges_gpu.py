@@ -155,3 +155,97 @@ def test_crowds_of_equal_scores_stay_cheap():
     assert torch.equal(got.top_tokens[::3].cpu(), torch.arange(9).expand(234, 9))
     _inside(got.top_log_probs[::3], torch.full((234, 9), -math.log(20000), dtype=torch.float64),
             torch.full((), 8 * oracle.ULP * math.log(20000), dtype=torch.float64), "top_log_probs")
+
+
+@pytest.mark.parametrize("n,v,d", [(40, 999, 64), (300, 2051, 264), (1100, 2051, 264), (1100, 999, 72)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("frozen", [True, False])
+def test_rows_that_are_not_finite_leave_the_others_alone(n, v, d, dtype, frozen):
+    """An infinite incoming gradient, eight neighbouring rows of NaN: they show in their own rows (and in the table's
+    gradient), the other rows are as exact as without them."""
+    from memoryefficientclip_b200 import token_log_probs
+    x, table, tokens, g = _pair(n, v, d, dtype, n + d, bump=5.0)
+    g_lp, g_h = 1e-4 * torch.randn(n, generator=g), 1e-5 * torch.randn(n, generator=g)
+    bad = torch.zeros(n, dtype=torch.bool)
+    g_lp[3], bad[3] = float("inf"), True
+    g_h[17], bad[17] = float("-inf"), True
+    g_lp[24:32], bad[24:32] = float("nan"), True
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(not frozen)
+    got = token_log_probs(xg, yg, tokens.cuda())
+    torch.autograd.backward([got.log_probs, got.entropy], [g_lp.cuda(), g_h.cuda()])
+    xo, yo = (x, table) if dtype == torch.float16 else (x.bfloat16(), table.bfloat16())
+    wx, _wy, bx, _by = oracle.token_log_probs_grad(xo[~bad], yo, tokens[~bad][:, None], 1.0, g_lp[~bad][:, None], g_h[~bad],
+                                                   (dtype, dtype))
+    _inside(xg.grad[~bad.cuda()], wx, bx, "dx")
+    assert not torch.isfinite(xg.grad[bad.cuda()]).any(1).any()
+    assert frozen or not torch.isfinite(yg.grad).any()
+
+
+@pytest.mark.parametrize("n,v,d", [(40, 999, 64), (300, 2051, 264), (1100, 2051, 264), (1100, 999, 72), (700, 40, 8)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("per_row", [1, 4])
+def test_rows_of_very_different_weights(n, v, d, dtype, per_row):
+    """A row's gradient is as exact as if it were alone, whatever the other rows weigh: 2^0 to 2^-80 and none at all."""
+    from memoryefficientclip_b200 import ops
+    x, table, tokens, g = _pair(n, v, d, dtype, n + v, bump=4.0)
+    many = torch.stack([tokens] + [torch.randint(-1, v, (n,), generator=g) for _ in range(per_row - 1)], 1)
+    weight = 2.0 ** -torch.randint(0, 81, (n,), generator=g).double()
+    weight[::11] = 0
+    weight[5] = 1.0
+    g_lp, g_h = torch.randn(n, per_row, generator=g), torch.randn(n, generator=g) * 0.3
+    xg, yg, tk = x.cuda(), table.cuda(), many.cuda()
+    status = ops.status_word(xg.device)
+    _lp, entropy, _a, _b, saved = ops.token_log_probs(xg, yg, tk, 1.0, 0, True, status)
+    f32 = torch.float32
+    wg, wh = (g_lp.double() * weight[:, None]).float(), (g_h.double() * weight).float()
+    for sides in ((True, True), (True, False), (False, True)):
+        dx, dt = ops.token_log_probs_grad(xg, yg, tk, 1.0, saved, entropy, wg.cuda(), wh.cuda(), f32, f32, *sides, status)
+        wx, _wy, bx, _by = oracle.token_log_probs_grad(x, table, many, 1.0, g_lp, g_h, (f32, f32))
+        if dx is not None:
+            _inside(dx, weight[:, None] * wx, weight[:, None] * bx + torch.finfo(f32).tiny, "dx")
+            assert not dx[::11].any()
+        _wx, wy, _bx, by = oracle.token_log_probs_grad(x, table, many, 1.0, wg, wh, (f32, f32))
+        if dt is not None:
+            _inside(dt, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("n,v,d", [(300, 700, 264), (1100, 700, 264)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_distillation_rows_of_very_different_weights(n, v, d, dtype):
+    """The same with a weight for each row's loss, and features whose lengths differ as much the other way round, so that
+    every row has a say in the table's gradient."""
+    from memoryefficientclip_b200 import ops
+    x, table, _tokens, g = _pair(n, v, d, dtype, 3)
+    shift = torch.randint(0, 11, (n,), generator=g)
+    x = (x.double() * 2.0 ** -shift[:, None].double()).to(dtype)
+    t, logits = _teacher(n, v, 5, g)
+    weight = (2.0 ** shift.double()).float()
+    xg, yg, tg = x.cuda(), table.cuda(), t.cuda()
+    status = ops.status_word(xg.device)
+    _loss, saved = ops.distill_forward(xg, yg, tg, logits.cuda(), 1.0, 1.0, "none", status)
+    dx, dt = ops.distill_backward(xg, yg, tg, 1.0, saved, weight.cuda(), torch.float32, torch.float32, status=status)
+    wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, 1.0, weight, (torch.float32,) * 2)
+    _inside(dx, wx, bx, "dx")
+    _inside(dt, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("size_x,size_g", [(2.0 ** 60, 2.0 ** -50), (2.0 ** -60, 2.0 ** 50), (2.0 ** -110, 1.0),
+                                           (1.0, 2.0 ** -100), (1.0, 2.0 ** 100), (2.0 ** 50, 2.0 ** 50),
+                                           (2.0 ** -50, 2.0 ** -60)])
+@pytest.mark.parametrize("n", [300, 1100])
+def test_magnitudes_at_the_ends_of_the_range(n, size_x, size_g):
+    """Powers of two on the features and the incoming gradients come out again as powers of two."""
+    from memoryefficientclip_b200 import ops
+    v, d, f32 = 500, 264, torch.float32
+    x, table, tokens, g = _pair(n, v, d, torch.bfloat16, 7)
+    g_lp = torch.randn(n, generator=g)
+    grads = []
+    for sx, sg in ((1.0, 1.0), (size_x, size_g)):
+        xg, yg, tk = (x.double() * sx).bfloat16().cuda(), (table.double() / sx).bfloat16().cuda(), tokens.cuda()
+        assert torch.isfinite(yg).all() and (yg.double() * sx).cpu().equal(table.double())
+        _lp, entropy, _a, _b, saved = ops.token_log_probs(xg, yg, tk, 1.0, 0, True, None)
+        dx, dt = ops.token_log_probs_grad(xg, yg, tk, 1.0, saved, entropy, (g_lp.double() * sg).float().cuda(), None, f32, f32)
+        grads.append((dx.double() * sx / sg, dt.double() / sx / sg))
+    for got, want in zip(grads[1], grads[0]):
+        # (the smallest results are fp32's subnormal numbers: half of 2^-149 over 2^-110 for every part of a sum and its scale)
+        assert ((got - want).abs() <= 4 * oracle.ULP * want.abs() + 40 * 2.0 ** -150 / 2.0 ** -110).all()
