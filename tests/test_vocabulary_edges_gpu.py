@@ -249,3 +249,66 @@ def test_magnitudes_at_the_ends_of_the_range(n, size_x, size_g):
     for got, want in zip(grads[1], grads[0]):
         # (the smallest results are fp32's subnormal numbers: half of 2^-149 over 2^-110 for every part of a sum and its scale)
         assert ((got - want).abs() <= 4 * oracle.ULP * want.abs() + 40 * 2.0 ** -150 / 2.0 ** -110).all()
+
+
+@pytest.mark.parametrize("n,v,d", [(1, 40, 64), (5, 1000, 64), (130, 257, 104), (300, 4099, 512), (1100, 2051, 264),
+                                   (64, 9000, 96), (1500, 700, 1152), (2000, 333, 30)])
+def test_fp16_gradients_keep_their_bits(n, v, d):
+    """Two fp16 inputs are contracted as they are: no operand is rounded, and an fp16 coefficient keeps 11 bits."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss, token_log_probs
+    half = torch.float16
+    x, table, tokens, g = _pair(n, v, d, half, n + v, bump=6.0)
+    many = torch.stack([tokens, torch.randint(-1, v, (n,), generator=g), tokens], 1)
+    g_lp, g_h = torch.randn(n, 3, generator=g), torch.randn(n, generator=g) * 0.3
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    got = token_log_probs(xg, yg, many.cuda(), temperature=1.3)
+    dx, dy = torch.autograd.grad([got.log_probs, got.entropy], [xg, yg], [g_lp.cuda(), g_h.cuda()])
+    wx, wy, bx, by = oracle.token_log_probs_grad(x, table, many, 1.3, g_lp, g_h, (half, half))
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+    t, logits = _teacher(n, v, 6, g)
+    loss = MemoryEfficientDistillLoss(0.8, normalized_inputs=True, reduction="none")(xg, yg, t.cuda(), logits.cuda())
+    weight = torch.randn(n, generator=g)
+    dx, dy = torch.autograd.grad(loss, [xg, yg], weight.cuda())
+    wx, wy, bx, by = oracle.distill_grad(x, table, t, logits, 0.8, weight, (half, half))
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
+
+
+@pytest.mark.parametrize("n", [3, 260])
+def test_gradient_of_rows_past_32_bits(n):
+    """A table of 2^31 elements, all but a few rows of which are zero: the gradient of those rows is far above what the
+    comparison allows, so that none at all would be noticed."""
+    from memoryefficientclip_b200 import token_log_probs
+    v, d = 2_100_000, 1024
+    g = torch.Generator().manual_seed(n)
+    where = torch.cat([torch.tensor([0, v - 1, v - 2, 2 ** 31 // d, 2 ** 31 // d - 1]), torch.randint(0, v, (40,), generator=g)]).unique()
+    rows = (torch.randn(len(where), d, generator=g) / math.sqrt(d)).bfloat16()
+    pick = torch.randint(0, len(where), (n,), generator=g)
+    # features that agree on a direction, so that the zero rows' sums do not cancel
+    x = (torch.randn(d, generator=g) + 0.5 * torch.randn(n, d, generator=g)).bfloat16()
+    table = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    table[where.cuda()] = rows.cuda()
+    xg, table = x.cuda().requires_grad_(True), table.requires_grad_(True)
+    got = token_log_probs(xg, table, where[pick].cuda())
+    z, err = oracle.scores(x, rows, 1.0)
+    zeros = torch.full((n, 1), math.log(float(v - len(where))), dtype=torch.float64)
+    lse = torch.logsumexp(torch.cat([z, zeros], 1), 1)
+    _dx, dt = torch.autograd.grad(got.log_probs.sum(), [xg, table])
+    p0 = torch.exp(-lse)[:, None]
+    want = -(p0 * x.double()).sum(0)
+    # a coefficient's 2^-11 (two bf16 panels: less) and its floor, 2^-39 of the bound 2; the score's error; the contraction's
+    # cuts, 2^-23 of a partial sum every 16 of n terms; the output's rounding
+    off = p0 * (2.0 ** -11 + 2 * err[:, None] + 16 * oracle.ULP) + 2.0 ** -39 * 2
+    bound = ((off + oracle.ULP * (n / 16 + 4) * (p0 + off)) * x.double().abs()).sum(0)
+    bound = bound + 2.0 ** -8 * (want.abs() + bound)
+    assert (want.abs() > 8 * bound).double().mean() > 0.9
+    others = torch.cat([torch.tensor([1, v - 3, 2 ** 31 // d + 1, 2 ** 32 // d // 2 + 1, 2 ** 32 // d // 2 - 2]),
+                        torch.randint(0, v, (2000,), generator=g)])
+    others = others[~torch.isin(others, where)]
+    worst = ((dt[others.cuda()].double().cpu() - want).abs() / bound).max().item()
+    assert worst <= 1.0, worst
+    same = dt[others[0].cuda()]
+    alike = (dt == same).all(1)
+    alike[where.cuda()] = True
+    assert alike.all()
