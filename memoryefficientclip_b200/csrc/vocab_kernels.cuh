@@ -800,11 +800,13 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             // q = softmax of the teacher's logits over the entries that are there; KL = sum q (log q - log p)
             auto logit = [&](int e) -> float {
                 const long long at = row * p.k + e;
-                const float v = p.teacher_dtype == 1 ? reinterpret_cast<const float*>(p.teacher_logits)[at]
-                                : p.teacher_dtype == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.teacher_logits)[at])
-                                                       : __half2float(reinterpret_cast<const __half*>(p.teacher_logits)[at]);
-                return v * p.inv_teacher_t;
+                return p.teacher_dtype == 1 ? reinterpret_cast<const float*>(p.teacher_logits)[at]
+                       : p.teacher_dtype == 0 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.teacher_logits)[at])
+                                              : __half2float(reinterpret_cast<const __half*>(p.teacher_logits)[at]);
             };
+            // differences are taken before the temperature divides them: the type's lowest value, which masks carry, stays
+            // finite and so does a row of nothing else
+            auto below = [&](int e, float most) -> float { return (logit(e) - most) * p.inv_teacher_t; };
             auto there = [&](int e) -> bool { return tok[e] >= 0 && !(logit(e) == -INFINITY); };
             float um = -INFINITY, seen = 0.f;
             for (int e = gt; e < p.k; e += G)
@@ -813,7 +815,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
             seen = group_reduce<G, true>(seen, red, gt);
             float sum = 0.f;
             for (int e = gt; e < p.k; e += G)
-                if (there(e)) sum += expf(logit(e) - um);
+                if (there(e)) sum += expf(below(e, um));
             sum = group_reduce<G, false>(sum, red, gt);
             const float inv = 1.f / sum, log_sum = logf(sum);
             double kl = 0.0;
@@ -823,7 +825,7 @@ vocab_rows_kernel(const __grid_constant__ VocabRows p) {
                 // of every entry that names a row, also an impossible one: the backward stores a coefficient at each
                 const double lp2 = vocab_lp2(p, (double)z_of[e], m, r, log2l);
                 if (there(e)) {
-                    const float u = logit(e) - um;
+                    const float u = below(e, um);
                     q = expf(u) * inv;
                     if (tok[e] >= p.vocab) q = NAN;
                     if (q != 0.f) kl += (double)q * ((double)u - (double)log_sum - lp2 * 0.6931471805599453);

@@ -312,3 +312,40 @@ def test_gradient_of_rows_past_32_bits(n):
     alike = (dt == same).all(1)
     alike[where.cuda()] = True
     assert alike.all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("teacher_temperature", [0.25, 1.0, 3.0])
+@pytest.mark.parametrize("n", [10, 400])
+def test_teacher_logits_at_the_ends_of_their_type(n, dtype, teacher_temperature):
+    """The lowest value of a type is a logit like any other, whatever it is divided by: a row of nothing else is spread over its
+    entries, and only -inf says that an entry is not there."""
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss
+    v, d, k = 200, 64, 5
+    x, table, _tokens, g = _pair(n, v, d, torch.bfloat16, n)
+    t, logits = _teacher(n, v, k, g, dtype)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    logits[0], logits[1, 1:], logits[2, :3] = low, low, high
+    logits[3, 0], logits[3, 1], logits[4, 2:] = high, low, float("-inf")
+    logits[4, :2], logits[5, 0], logits[6] = low, float("-inf"), float("-inf")
+    xg, yg = x.cuda().requires_grad_(True), table.cuda().requires_grad_(True)
+    loss = MemoryEfficientDistillLoss(1.0, True, teacher_temperature, "none")(xg, yg, t.cuda(), logits.cuda())
+    kl, has, err = oracle.distill(x, table, t, logits, 1.0, teacher_temperature)
+    assert has[:6].all() and not has[6]
+    # where the logits are the type's ends their differences are 0 or beyond any exponential's range, so that q has no error
+    ends = torch.zeros(n, dtype=torch.bool)
+    ends[[0, 2, 3, 4]] = True
+    _z, score_err = oracle.scores(x, table, 1.0)
+    err = torch.where(ends, 2 * score_err + 16 * oracle.ULP * (kl.abs() + 10), err)
+    _inside(loss, kl, err + 1e-30, "loss")
+    weight = torch.randn(n, generator=g)
+    dx, dy = torch.autograd.grad(loss, [xg, yg], weight.cuda())
+    q, has = oracle.teacher(t, logits, teacher_temperature)
+    w = (weight.double() * has)[:, None]
+    dense = torch.softmax(x.double() @ table.double().T, 1) * w
+    entries = torch.zeros_like(dense).scatter_add_(1, t, -q * w)
+    u = torch.where((q > 0) & ~ends[:, None], logits.double().abs() / teacher_temperature, torch.zeros_like(q)).max()
+    wx, wy, bx, by = oracle._gradients(x, table, 1.0, dense, entries, dense.abs() + entries.abs() * (1 + u),
+                                       (torch.bfloat16,) * 2, 0.0)
+    _inside(dx, wx, bx, "dx")
+    _inside(dy, wy, by, "dtable")
