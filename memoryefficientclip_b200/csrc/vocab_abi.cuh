@@ -89,7 +89,8 @@ static int check_vocab(const char* what, const void* x, const void* table, int d
     if (rows < 1 || vocab < 1 || rows > 0x7fffffffLL || vocab > 0x7fffffffLL || d < 8 || d % 8 != 0 || d > 0x7fffffffLL ||
         ldx < d || ldt < d || ldx % 8 != 0 || ldt % 8 != 0 || !aligned16(x) || !aligned16(table))
         return fail(MECLIP_EINVAL, "%s: need rows, vocab in [1, 2^31), d and pitches multiples of 8, 16-byte alignment", what);
-    if (!(temperature > 0.f) || std::isinf(temperature)) return fail(MECLIP_EINVAL, "%s: temperature must be positive", what);
+    if (!(temperature > 0.f) || std::isinf(temperature) || std::isinf(1.4426950408889634f / temperature))
+        return fail(MECLIP_EINVAL, "%s: temperature must be positive, and its inverse finite", what);
     if (k < 0 || k > VOCAB_MAX_ENTRIES) return fail(MECLIP_EINVAL, "%s: at most %d entries per row", what, VOCAB_MAX_ENTRIES);
     return MECLIP_OK;
 }
@@ -308,7 +309,8 @@ int meclip_distill(const void* x, const void* table, int dtype, int64_t rows, in
         return fail(MECLIP_EINVAL, "distill: null pointer");
     if (teacher_dtype != MECLIP_BF16 && teacher_dtype != MECLIP_F32 && teacher_dtype != MECLIP_F16)
         return fail(MECLIP_EINVAL, "distill: bad teacher dtype %d", teacher_dtype);
-    if (!(teacher_temperature > 0.f) || std::isinf(teacher_temperature)) return fail(MECLIP_EINVAL, "distill: teacher temperature must be positive");
+    if (!(teacher_temperature > 0.f) || std::isinf(teacher_temperature) || std::isinf(1.f / teacher_temperature))
+        return fail(MECLIP_EINVAL, "distill: teacher temperature must be positive, and its inverse finite");
     VocabRows r;
     std::memset(&r, 0, sizeof(r));
     r.x = x; r.y = table; r.ldx = ldx; r.ldy = ldt; r.d = (int)d; r.rows = rows; r.vocab = vocab;

@@ -349,3 +349,15 @@ def test_teacher_logits_at_the_ends_of_their_type(n, dtype, teacher_temperature)
                                        (torch.bfloat16,) * 2, 0.0)
     _inside(dx, wx, bx, "dx")
     _inside(dy, wy, by, "dtable")
+
+
+def test_temperatures_without_a_finite_inverse_are_refused():
+    from memoryefficientclip_b200 import MemoryEfficientDistillLoss, _lib, token_log_probs
+    x, table, tokens, _g = _pair(4, 9, 8, torch.bfloat16, 1)
+    x, table, tokens = x.cuda(), table.cuda(), tokens.cuda()
+    logits = torch.zeros(4, 1, device="cuda")
+    for call in (lambda: token_log_probs(x, table, tokens, temperature=1e-39),
+                 lambda: MemoryEfficientDistillLoss(1e-39, True)(x, table, tokens[:, None], logits),
+                 lambda: MemoryEfficientDistillLoss(1.0, True, 1e-39)(x, table, tokens[:, None], logits)):
+        with pytest.raises(_lib.MeclipError):
+            call()
