@@ -803,10 +803,9 @@ static int launch_pair_t(const CUtensorMap& ta, const CUtensorMap& tb, const CUt
 // 8.94.  Auto: the contractions (K = panel width, thousands) always run as pairs; the sums and coefficient
 // passes (K = D) do from PAIR_MIN_K on.
 static constexpr long long PAIR_MIN_K = 800;
-// The vocabulary's passes have heavier epilogues, which two CTAs with a tile each hide better, up to a longer K (4096 x
-// 32768, under the power cap, statistics and selection: K = 1024 single 307 us, pairs 317; 8192 x 49999 x 1152, a step
-// with its gradients: single 3560 us, pairs 3540).
-static constexpr long long VOCAB_PAIR_MIN_K = 1100;
+// The vocabulary's passes never do: their heavier epilogues hide better behind two CTAs with a tile each.  4096 x 32768,
+// alone, statistics / coefficients in us, single and pairs: K = 512 130 / 150 and 147 / 183, K = 1152 245 / 250 and 258 / 256,
+// K = 2048 394 / 403 and 431 / 431; whole steps under the power cap: K = 2048 2027 and 2041, 8192 x 49999 x 1152 3682 and 3676.
 static int pair_mode() {
     static const int mode = []() {
         const char* v = std::getenv("MECLIP_PAIR");
@@ -863,10 +862,9 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
     // CTA pairs (256 x bn tiles) whenever B is K-major; the single-CTA kernel keeps MN-major B
     const int pmode = pair_mode();
     const bool pair = !b.mn_major && bn % 64 == 0 && g_trace_buf == nullptr &&      // the in-kernel trace is a single-CTA hook
+                      epi != EPI_STATS && epi != EPI_VCOEF &&
                       (f32 || wide || pmode == 1 || ((pmode == 2 || pmode < 0) && epi == EPI_OUT && bn == 256) ||
-                       (pmode < 0 && epi != EPI_OUT && bn == 256 &&
-                        k >= (epi == EPI_STATS || epi == EPI_VCOEF ? VOCAB_PAIR_MIN_K : PAIR_MIN_K))) &&
-                      !(m <= BM && (epi == EPI_STATS || epi == EPI_VCOEF));     // half of every pair would have no rows
+                       (pmode < 0 && epi != EPI_OUT && bn == 256 && k >= PAIR_MIN_K));
     if (b.mn_major) rc = make_tmap(&tb, b.ptr, n, k, b.ld, 64, BK);
     else            rc = make_tmap(&tb, b.ptr, k, n, b.ld, bk, pair ? bn / 2 : bn, f32);
     if (rc) return rc;
@@ -967,8 +965,6 @@ static int launch_gemm(int epi, const Operand& a, const Operand& b, long long m,
         }
         if (epi == EPI_SUMS) return launch_pair_t<EPI_SUMS, 0>(ta, tb, tc, p, pair_smem, stream);
         if (epi == EPI_COEF) return launch_pair_t<EPI_COEF, 0>(ta, tb, tc, p, pair_smem, stream);
-        if (epi == EPI_STATS) return launch_pair_t<EPI_STATS, 0>(ta, tb, tc, p, pair_smem, stream);
-        if (epi == EPI_VCOEF) return launch_pair_t<EPI_VCOEF, 0>(ta, tb, tc, p, pair_smem, stream);
         if (epi == EPI_OUT) return a.mn_major ? launch_pair_t<EPI_OUT, 1>(ta, tb, tc, p, pair_smem, stream)
                                               : launch_pair_t<EPI_OUT, 0>(ta, tb, tc, p, pair_smem, stream);
         return fail(MECLIP_EINVAL, "unknown epilogue %d", epi);
@@ -1752,7 +1748,7 @@ static int grad_impl(int kind, const void* x_bf16, const void* y_bf16, int64_t r
                     if (!use_counters) p.tile_counter = nullptr;
                     p.panel_f16 = panel_f16;
                     a.f16 = b.f16 = vg->f16;
-                    // 256-column tiles beyond one row tile: only those run on CTA pairs
+                    // 256-column tiles beyond one row tile, as in the statistics (pick_stats_bn)
                     rc = launch_gemm(EPI_VCOEF, a, b, nr, nc, d, nr > BM && nc >= 256 ? 256 : pick_bn(nc), p, s0, gpanel[gb], plan.row_block, plan.ldg / 64);
                     if (rc == MECLIP_OK) rc = launch_vocab_entries(*vg, r0, nr, c0, nc, gpanel[gb], plan.row_block, lo_chunk, panel_f16, s0);
                 } else {

@@ -74,7 +74,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
         fence_barrier_init();
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
-        if (epi_is_coef(EPI) || DUAL) tma_prefetch_desc(&tmap_c);
+        if (EPI == EPI_COEF || DUAL) tma_prefetch_desc(&tmap_c);
         if (DUAL) tma_prefetch_desc(&tmap_d);
     }
     if (warp == 1) {

@@ -10,7 +10,7 @@ static constexpr long long VOCAB_ROW_BLOCK = 16384;
 // Column-tile width of the statistics pass.  Up to 128 rows there is one row tile, the pass is bound by reading the table,
 // and what counts is that every SM gets the same share of it: the fewest waves x width, in steps of 32 columns (V = 32768:
 // 147 tiles of 224 columns instead of 128 of 256).  With more rows 256: a narrower tile costs more per column than a
-// fuller last wave brings, and only 256 columns run on CTA pairs.
+// fuller last wave brings.
 static int pick_stats_bn(long long rows, long long vocab) {
     if (rows > BM) return vocab >= 256 ? 256 : (int)((vocab + 63) / 64 * 64);
     int best = 256;
