@@ -33,7 +33,7 @@ def embed_tokens(tokens, table, scale=1.0):
     """scale * table[tokens], of shape tokens.shape + [D] in the table's dtype (rounded once).
 
     tokens: any shape, int64 or int32; a negative token is padding: its row is zero and it gets no gradient.  A token
-    behind the table gives a row of NaN.  table: [V, D] float32, bfloat16 or float16, any D, pitch and alignment.
+    behind the table gives a row of NaN and gets none either.  table: [V, D] float32, bfloat16 or float16, any D, pitch and alignment.
     """
     ops._check_matrix(table, "table")
     assert tokens.get_device() == table.get_device(), "tokens and table must be on one device"
@@ -42,6 +42,6 @@ def embed_tokens(tokens, table, scale=1.0):
     tokens = tokens if tokens.dtype == torch.int64 else tokens.to(torch.int64)
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     table = ops.row_major(table)
-    if ops.differentiated(table):
+    if (table.requires_grad and torch.is_grad_enabled()) or ops.has_tangent(table):
         return _EmbedFn.apply(tokens, table, float(scale))
     return ops.embed(tokens, table, float(scale))

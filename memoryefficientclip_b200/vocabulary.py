@@ -11,9 +11,10 @@ entropy of every row and its top alternatives; gradients flow to the features an
 a teacher that is known by its top logits; ``MemoryEfficientDistillLossFn.apply`` is its autograd node.
 
 Features [N, D] and table [V, D]: float32, bfloat16 or float16 with any D, pitch and alignment.  Two float16 inputs are
-scored as they are; otherwise the operands are bf16 (fp32 inputs are rounded, as in the contrastive losses).  All sums
-are fp32, gradients come back in the inputs' dtypes.  Features and table must be finite: a row of NaN gives NaN for
-that row, and NaN gradients for the table.
+scored as they are; otherwise, and wherever inputs are normalised inside, the operands are bf16 (rounded as in the
+contrastive losses; there is no tf32 route, MECLIP_TF32 does not count here).  All sums are fp32, gradients come back in the
+inputs' dtypes, there are no second or forward-mode derivatives.  Features and table must be finite: a row of NaN gives
+NaN for that row, and NaN gradients for the table.
 """
 from __future__ import annotations
 
@@ -108,8 +109,9 @@ def token_log_probs(features, table, tokens, temperature=1.0, top_k=0) -> TokenL
     """Log probabilities of given tokens under softmax(features @ table^T / temperature).
 
     tokens: [N], or [N, k] with k up to 256 tokens per row, int64 or int32.  A negative token is absent: its log
-    probability is 0 and it gets no gradient.  A token behind the table gives NaN.
+    probability is 0 and it gets no gradient.  A token behind the table gives NaN and gets none either.
     top_k: 0 to 32 alternatives per row, best first; of equal scores the lower token comes first.  They carry no gradient.
+    The order is that of exact scores unless a table row more than twice as long as the best one is among the close ones.
     """
     _check_inputs(features, table, temperature)
     tokens = _check_tokens(tokens, features, "tokens")
@@ -117,7 +119,7 @@ def token_log_probs(features, table, tokens, temperature=1.0, top_k=0) -> TokenL
         f"top_k must be between 0 and {min(MAX_TOP, table.shape[0])}"
     device = features.device
     ops.poll_status(device)
-    if ops.differentiated(features, table):
+    if ((features.requires_grad or table.requires_grad) and torch.is_grad_enabled()) or ops.has_tangent(features, table):
         return TokenLogProbs(*_TokenLogProbsFn.apply(features, table, tokens, float(temperature), top_k))
     x, y = ops.vocab_operands(features, table)
     lp, entropy, top_lp, top, _saved = ops.token_log_probs(x, y, tokens, float(temperature), top_k, False,
@@ -184,9 +186,9 @@ class MemoryEfficientDistillLoss(nn.Module):
     softmax(teacher_logits / teacher_temperature) over the entries that are present in the row.  ``forward(features,
     table, teacher_tokens, teacher_logits)``: teacher_tokens [N, k] (k up to 256, int64 or int32) name rows of the table,
     teacher_logits [N, k] are their logits (float32, bfloat16 or float16; no gradient).  An entry with a negative token or
-    a logit of -inf is absent, whatever else stands in its place; a row without entries adds nothing and gets no gradient;
-    an entry counts by itself where a row names a token twice.  reduction: "mean" over the rows that have entries, "sum", or "none"
-    for the [N] losses.  With normalized_inputs=False features and table are L2-normalised inside, as in the contrastive
+    a logit of -inf is absent, whatever else stands in its place (the lowest finite value is a logit like any other); a row
+    without entries adds nothing and gets no gradient; an entry counts by itself where a row names a token twice.
+    reduction: "mean" over the rows that have entries, "sum", or "none" for the [N] losses.  With normalized_inputs=False features and table are L2-normalised inside, as in the contrastive
     losses: the table is then the other tower's output and the teacher's entries its best pairs.
     """
 
