@@ -478,21 +478,25 @@ int meclip_ring_grad(const meclip_ring_desc* ring, int kind, const void* x_bf16,
  *
  * Operands: x [rows, d], table [vocab, d], both MECLIP_BF16 or both MECLIP_F16, d and pitches multiples of 8, 16-byte
  * aligned (meclip_normalize_fwd with normalize = 0 makes bf16 ones of anything).  Scores must be finite; a row whose
- * scores are not numbers gives NaN for that row.  tokens, teacher_tokens: int64 [rows, per_row], contiguous, 0 <=
- * per_row <= 256.  A negative token is absent (padding); one behind the table gives NaN.  workspace: 256-byte aligned,
- * meclip_vocab_workspace_bytes / meclip_vocab_grad_workspace_bytes.
+ * scores are not numbers gives NaN for that row.  Temperatures need a finite inverse.  tokens, teacher_tokens: int64
+ * [rows, per_row], contiguous, 0 <= per_row <= 256.  A negative token is absent (padding); one behind the table gives NaN
+ * and takes no part in the gradients.  workspace: 256-byte aligned, meclip_vocab_workspace_bytes /
+ * meclip_vocab_grad_workspace_bytes; what it held before does not matter.
  *
  *   meclip_token_log_probs  log_probs [rows, per_row] = z - lse (0 for an absent token); entropy [rows] =
  *                           lse - sum_j p z (may be NULL); the top_k (<= 32, <= vocab) best tokens of each row and
  *                           their log probabilities, larger first and the lower token first among equals (decided on
- *                           fp64 dot products).  row_lse [rows] and token_scores [rows, per_row] (log probabilities), both
+ *                           fp64 dot products, among all columns that the tile pass cannot rule out: its error is bounded
+ *                           with twice the length of the row's best, so the order is certain where no table row in
+ *                           question is longer than that).  row_lse [rows] and token_scores [rows, per_row] (log probabilities), both
  *                           base 2, are saved for the gradient; NULL when there will be none.
  *   meclip_token_log_probs_grad  dx = dz Y / T, dtable = dz^T X / T for
  *                           dz_ij = sum_k g_ik ([j = token_ik] - p_ij) - h_i p_ij (log p_ij + entropy_i),
  *                           g = grad_log_probs, h = grad_entropy (either may be NULL: zero).
  *   meclip_distill          KL(q || p) per row for a teacher that is known by its top logits: q = softmax of
  *                           teacher_logits / teacher_temperature (teacher_dtype, [rows, per_row]) over the row's
- *                           entries that are present (token >= 0 and logit > -inf).  A row without one has loss 0,
+ *                           entries that are present (token >= 0 and logit > -inf; the type's lowest value is a logit
+ *                           like any other).  A row without one has loss 0,
  *                           row_has 0 and no gradient.  An entry counts by itself where a row names a
  *                           token twice.
  *                           loss = sum of row_loss, times inv_count = 1 / (rows with an entry) when `mean` is set
