@@ -361,3 +361,31 @@ def test_temperatures_without_a_finite_inverse_are_refused():
                  lambda: MemoryEfficientDistillLoss(1.0, True, 1e-39)(x, table, tokens[:, None], logits)):
         with pytest.raises(_lib.MeclipError):
             call()
+
+
+@pytest.mark.parametrize("n,v,d", [(700, 1500, 64), (1300, 1500, 264), (200, 1500, 264)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("per_row", [1, 3])
+def test_weights_over_several_blocks(n, v, d, dtype, per_row):
+    """Row factors, entries and scaled features of every block of rows and panel of columns are that block's own."""
+    from memoryefficientclip_b200 import _lib, ops
+    x, table, tokens, g = _pair(n, v, d, dtype, n + per_row, bump=4.0)
+    many = torch.stack([tokens] + [torch.randint(-1, v, (n,), generator=g) for _ in range(per_row - 1)], 1)
+    weight = 2.0 ** -torch.randint(0, 31, (n,), generator=g).double()
+    weight[::13] = 0
+    g_lp, g_h = torch.randn(n, per_row, generator=g), torch.randn(n, generator=g) * 0.3
+    wg, wh = (g_lp.double() * weight[:, None]).float(), (g_h.double() * weight).float()
+    xg, yg, tk = x.cuda(), table.cuda(), many.cuda()
+    f32, status = torch.float32, ops.status_word(xg.device)
+    _lp, entropy, _a, _b, saved = ops.token_log_probs(xg, yg, tk, 1.0, 0, True, status)
+    _lib.check(_lib.load().meclip_debug_set_blocking(128, 128 * 2 * 512))
+    try:
+        dx, dt = ops.token_log_probs_grad(xg, yg, tk, 1.0, saved, entropy, wg.cuda(), wh.cuda(), f32, f32, status=status)
+        torch.cuda.synchronize()
+    finally:
+        _lib.check(_lib.load().meclip_debug_set_blocking(0, 0))
+    wx, _wy, bx, _by = oracle.token_log_probs_grad(x, table, many, 1.0, g_lp, g_h, (f32, f32))
+    # (three panels and eleven blocks of rows: their sums are fewer roundings than the bounds count for the cut contractions)
+    _inside(dx, weight[:, None] * wx, weight[:, None] * bx + torch.finfo(f32).tiny, "dx")
+    _wx, wy, _bx, by = oracle.token_log_probs_grad(x, table, many, 1.0, wg, wh, (f32, f32))
+    _inside(dt, wy, by, "dtable")
